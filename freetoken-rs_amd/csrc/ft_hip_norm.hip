@@ -1,0 +1,296 @@
+// ft_hip_norm.hip -- the residual addition and RMS norm in front of a section,
+// with the q8 blocks that its q4 GEMVs take, in one pass over the rows
+// (ft_hip_add_rmsnorm).
+//
+//   h   = residual + x,  or with the branch's own norm  residual + x / rms(x) * x_w
+//   inv = 1 / sqrt(mean(h * h) + eps),  y = h * inv * w
+//   q8  : u = f32(h * w); per 32 values a = max |u|, q = round half away(127 u / a), d = a * inv / 127
+//
+// The quants are those of u, before the row's scale: 127 u / a is the same
+// quotient for y, and taken from u it depends on 32 values instead of on the
+// last bit of a sum over the row. The quotient is rounded as the real number:
+// u and a have 24 bits, so 127 u / a is either a half exactly or further than
+// 2^-26 from one, and the f64 product with 127 / a (off by less than 2^-45)
+// plus 2^-40 has its floor on the right side either way.
+//
+// Bound by memory: x, the residual, h, y and the blocks each move once; the
+// row stays in registers between its sum and its outputs. Sums and scales are
+// f64 (its rate is f32's here), h and y are rounded to f32 once.
+
+#include "ft_device.hpp"
+#include "ft_runtime.hpp"
+
+#include <cmath>
+
+using namespace ft;
+
+namespace {
+
+struct NormArgs {
+    const void* x;
+    int64_t x_stride;
+    const float* x_w;
+    const float* residual;
+    int64_t r_stride;
+    float* h;
+    int64_t h_stride;
+    const float* w;
+    float* y;
+    int64_t y_stride;
+    uint8_t* q8;
+    int hidden;
+    int64_t n;
+    double eps;
+};
+
+// V consecutive values (V = 4: one aligned vector access, V = 1: any address)
+template <int V>
+struct Vals {
+    float v[V];
+};
+
+template <int V>
+__device__ __forceinline__ Vals<V> load_f32(const float* p) {
+    Vals<V> r;
+    if constexpr (V == 4) {
+        const float4 a = *reinterpret_cast<const float4*>(p);
+        r.v[0] = a.x, r.v[1] = a.y, r.v[2] = a.z, r.v[3] = a.w;
+    } else {
+        r.v[0] = *p;
+    }
+    return r;
+}
+
+template <int V, int TYPE>
+__device__ __forceinline__ Vals<V> load_typed(const void* base, int64_t at) {
+    if constexpr (TYPE == FT_TYPE_F32) {
+        return load_f32<V>(static_cast<const float*>(base) + at);
+    } else {
+        uint16_t b[V];
+        const uint16_t* p = static_cast<const uint16_t*>(base) + at;
+        if constexpr (V == 4) {
+            const uint2 a = *reinterpret_cast<const uint2*>(p);
+            b[0] = (uint16_t)a.x, b[1] = (uint16_t)(a.x >> 16), b[2] = (uint16_t)a.y, b[3] = (uint16_t)(a.y >> 16);
+        } else {
+            b[0] = *p;
+        }
+        Vals<V> r;
+#pragma unroll
+        for (int i = 0; i < V; ++i) r.v[i] = TYPE == FT_TYPE_F16 ? h2f(b[i]) : __uint_as_float((uint32_t)b[i] << 16);
+        return r;
+    }
+}
+
+template <int V>
+__device__ __forceinline__ void store_f32(float* p, const Vals<V>& r) {
+    if constexpr (V == 4)
+        *reinterpret_cast<float4*>(p) = make_float4(r.v[0], r.v[1], r.v[2], r.v[3]);
+    else
+        *p = r.v[0];
+}
+
+__device__ __forceinline__ double shfl_xor_f64(double v, int m) {
+    const long long b = __double_as_longlong(v);
+    const int lo = __shfl_xor((int)b, m), hi = __shfl_xor((int)(b >> 32), m);
+    return __longlong_as_double(((long long)hi << 32) | (uint32_t)lo);
+}
+
+// Sum over the workgroup, the same bits in every thread and on every run:
+// a butterfly in each wave, then the waves in order.
+__device__ __forceinline__ double row_sum(double v, double* red) {
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) v += shfl_xor_f64(v, m);
+    const int waves = blockDim.x >> 6;
+    if (waves == 1) return v;
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double s = 0.0;
+    for (int i = 0; i < waves; ++i) s += red[i];
+    return s;
+}
+
+// One q8 block per group of 32 / V lanes.
+template <int V>
+__device__ __forceinline__ void quantize_u(const Vals<V>& u, double inv, uint8_t* blk, int part) {
+    float a = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) a = fmaxf(a, fabsf(u.v[i]));  // NaN is skipped
+    if constexpr (V == 4) {  // 8 lanes: quad, then the half-row's other quad
+        a = fmaxf(a, quad_xor1(a));
+        a = fmaxf(a, quad_xor2(a));
+        a = fmaxf(a, dpp_f<0x141>(a));
+    } else {
+        a = half_max32(a);
+    }
+    const double r = a > 0.0f ? 127.0 / (double)a : 0.0;
+    int qsum = 0;
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const double t = fabs((double)u.v[i]) * r;  // inf * 0 and NaN give NaN: quant 0
+        const int q = t <= 127.5 ? (int)(t + (0.5 + 0x1p-40)) : 0;
+        const int s = u.v[i] < 0.0f ? -q : q;
+        qsum += s;
+        word |= (uint32_t)(uint8_t)(int8_t)s << (8 * i);
+    }
+    if constexpr (V == 4) {
+        qsum += quad_xor1i(qsum);
+        qsum += quad_xor2i(qsum);
+        qsum += dpp_i<0x141>(qsum);
+        reinterpret_cast<uint32_t*>(blk)[2 + part] = word;
+    } else {
+        qsum = half_sum32(qsum);
+        blk[8 + part] = (uint8_t)word;
+    }
+    if (part == 0) {
+        reinterpret_cast<float*>(blk)[0] = a > 0.0f ? (float)((double)a * inv / 127.0) : 0.0f;
+        reinterpret_cast<int*>(blk)[1] = qsum;
+    }
+}
+
+// A workgroup per row; thread t holds the values (i * threads + t) * V .. + V
+// of it for i < NV. Lanes past the row's end hold zeros; hidden is a multiple
+// of 32 where q8 is written, so that a block's lanes are all inside the row
+// or all outside.
+template <int TYPE, int V, int NV>
+__global__ __launch_bounds__(1024) void k_add_rmsnorm(NormArgs a) {
+    __shared__ double red[2][16];
+    const int64_t row = blockIdx.x;
+    const int t = threadIdx.x, step = blockDim.x * V;
+    Vals<V> h[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = i * step + t * V;
+        if (c < a.hidden) {
+            h[i] = load_typed<V, TYPE>(a.x, row * a.x_stride + c);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) h[i].v[e] = 0.0f;
+        }
+    }
+    if (a.x_w) {
+        double ss = 0.0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < V; ++e) ss = fma((double)h[i].v[e], (double)h[i].v[e], ss);
+        const double inv = 1.0 / sqrt(row_sum(ss, red[0]) / a.hidden + a.eps);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = i * step + t * V;
+            if (c >= a.hidden) continue;
+            const Vals<V> w = load_f32<V>(a.x_w + c);
+            Vals<V> r;
+            if (a.residual) r = load_f32<V>(a.residual + row * a.r_stride + c);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const double n = (double)h[i].v[e] * inv * (double)w.v[e];
+                h[i].v[e] = (float)(a.residual ? n + (double)r.v[e] : n);
+            }
+        }
+    } else if (a.residual) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = i * step + t * V;
+            if (c >= a.hidden) continue;
+            const Vals<V> r = load_f32<V>(a.residual + row * a.r_stride + c);
+#pragma unroll
+            for (int e = 0; e < V; ++e) h[i].v[e] = r.v[e] + h[i].v[e];
+        }
+    }
+    double ss = 0.0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) ss = fma((double)h[i].v[e], (double)h[i].v[e], ss);
+    const double inv = 1.0 / sqrt(row_sum(ss, red[1]) / a.hidden + a.eps);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = i * step + t * V;
+        if (c >= a.hidden) continue;
+        if (a.h) store_f32<V>(a.h + row * a.h_stride + c, h[i]);
+        Vals<V> w;
+        if (a.w) {
+            w = load_f32<V>(a.w + c);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) w.v[e] = 1.0f;
+        }
+        if (a.y) {
+            Vals<V> y;
+#pragma unroll
+            for (int e = 0; e < V; ++e) y.v[e] = (float)((double)h[i].v[e] * inv * (double)w.v[e]);
+            store_f32<V>(a.y + row * a.y_stride + c, y);
+        }
+        if (a.q8) {
+            Vals<V> u;
+#pragma unroll
+            for (int e = 0; e < V; ++e) u.v[e] = h[i].v[e] * w.v[e];
+            quantize_u<V>(u, inv, a.q8 + (row * (a.hidden >> 5) + (c >> 5)) * Q8_BLK, (c & 31) / V);
+        }
+    }
+}
+
+template <int TYPE>
+void launch_norm(const NormArgs& a, bool vec, void* stream) {
+    const dim3 grid((unsigned)a.n);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (!vec) {
+        const int threads = a.hidden >= 1024 ? 1024 : (a.hidden + 63) / 64 * 64;
+        hipLaunchKernelGGL((k_add_rmsnorm<TYPE, 1, 16>), grid, dim3(threads), 0, s, a);
+        return;
+    }
+    const int vecs = a.hidden / 4, threads = vecs >= 1024 ? 1024 : (vecs + 63) / 64 * 64;
+    if (vecs <= threads)
+        hipLaunchKernelGGL((k_add_rmsnorm<TYPE, 4, 1>), grid, dim3(threads), 0, s, a);
+    else
+        hipLaunchKernelGGL((k_add_rmsnorm<TYPE, 4, 4>), grid, dim3(threads), 0, s, a);
+}
+
+bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+
+}  // namespace
+
+extern "C" int ft_hip_add_rmsnorm(ft_hip_ctx* ctx, void* stream, const void* x, int x_type, int64_t x_stride,
+                                  const float* x_w, const float* residual, int64_t residual_stride, float* h,
+                                  int64_t h_stride, const float* w, float eps, float* y, int64_t y_stride, void* q8,
+                                  int64_t hidden, int64_t n) {
+    clear_error();
+    if (hidden <= 0 || hidden > 16384)
+        return fail(FT_HIP_E_SHAPE, "add_rmsnorm: hidden=%lld not in [1, 16384]", (long long)hidden);
+    if (q8 && hidden % 32)
+        return fail(FT_HIP_E_SHAPE, "add_rmsnorm: hidden=%lld must be a multiple of 32 for q8", (long long)hidden);
+    if (n < 0 || n > 4194303)  // a workgroup of up to 1024 threads per row, fewer than 2^32 in all
+        return fail(FT_HIP_E_SHAPE, "add_rmsnorm: n=%lld not in [0, 4194303]", (long long)n);
+    if (x_type != FT_TYPE_F32 && x_type != FT_TYPE_F16 && x_type != FT_TYPE_BF16)
+        return fail(FT_HIP_E_INVALID, "add_rmsnorm: x_type=%d is no FT_TYPE", x_type);
+    if (!(eps >= 0.0f) || std::isinf(eps)) return fail(FT_HIP_E_SHAPE, "add_rmsnorm: eps is not a number >= 0");
+    const int64_t most = INT64_MAX / 4 / (n > 0 ? n : 1);
+    if (x_stride < hidden || x_stride > most) return fail(FT_HIP_E_SHAPE, "add_rmsnorm: x_stride out of range");
+    if (residual && (residual_stride < hidden || residual_stride > most))
+        return fail(FT_HIP_E_SHAPE, "add_rmsnorm: residual_stride out of range");
+    if (h && (h_stride < hidden || h_stride > most)) return fail(FT_HIP_E_SHAPE, "add_rmsnorm: h_stride out of range");
+    if (y && (y_stride < hidden || y_stride > most)) return fail(FT_HIP_E_SHAPE, "add_rmsnorm: y_stride out of range");
+    const unsigned size = x_type == FT_TYPE_F32 ? 4 : 2;
+    if (!aligned(x, size) || !aligned(x_w, 4) || !aligned(residual, 4) || !aligned(h, 4) || !aligned(w, 4) ||
+        !aligned(y, 4) || !aligned(q8, 4))
+        return fail(FT_HIP_E_SHAPE, "add_rmsnorm: a pointer is not aligned to its type (q8: 4 bytes)");
+    if (!ctx || !x) return fail(FT_HIP_E_INVALID, "add_rmsnorm: null argument");
+    if (!h && !y && !q8) return fail(FT_HIP_E_INVALID, "add_rmsnorm: no output (h, y and q8 are null)");
+    if (n == 0) return FT_HIP_OK;
+    const NormArgs a{x, x_stride, x_w, residual, residual_stride, h, h_stride, w, y, y_stride,
+                     static_cast<uint8_t*>(q8), (int)hidden, n, (double)eps};
+    // vectors of 4 where every row starts on one; else value by value
+    const bool vec = hidden % 4 == 0 && aligned(x, 4 * size) && x_stride % 4 == 0 && aligned(x_w, 16) && aligned(w, 16) &&
+                     aligned(residual, 16) && (!residual || residual_stride % 4 == 0) && aligned(h, 16) &&
+                     (!h || h_stride % 4 == 0) && aligned(y, 16) && (!y || y_stride % 4 == 0);
+    DeviceGuard on(ctx->device);
+    if (!on.ok) return fail(FT_HIP_E_DEVICE, "add_rmsnorm: device %d cannot be made current", ctx->device);
+    if (x_type == FT_TYPE_F32)
+        launch_norm<FT_TYPE_F32>(a, vec, stream);
+    else if (x_type == FT_TYPE_F16)
+        launch_norm<FT_TYPE_F16>(a, vec, stream);
+    else
+        launch_norm<FT_TYPE_BF16>(a, vec, stream);
+    return launch_status("add_rmsnorm");
+}

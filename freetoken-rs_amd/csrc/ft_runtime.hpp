@@ -70,6 +70,27 @@ int launch_route_topk(void* stream, const float* w, const float* x, const float*
 int scratch_setup(ft_hip_ctx* ctx);
 // Input RMS norm scale per seq: inv[s] = 1 / sqrt(R-order(x_s . x_s) / dim + 1e-6).
 int launch_rms_inv(void* stream, const float* x, float* inv, int64_t dim, int64_t n_seqs);
+// Makes a context's device current for the launches of one call and gives the
+// caller's back: for entry points that may be called with another device
+// current (the stream then belongs to the context's device).
+struct DeviceGuard {
+    int before = -1;
+    bool ok = false;
+    explicit DeviceGuard(int device) {
+        int now = -1;
+        if (hipGetDevice(&now) != hipSuccess) return;
+        if (now != device) {
+            if (hipSetDevice(device) != hipSuccess) return;
+            before = now;
+        }
+        ok = true;
+    }
+    ~DeviceGuard() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+    DeviceGuard(const DeviceGuard&) = delete;
+    DeviceGuard& operator=(const DeviceGuard&) = delete;
+};
 }  // namespace ft
 
 using ft::clear_error;

@@ -32,6 +32,11 @@ pub const FT_HIP_E_NOT_FOUND: c_int = -8;
 pub const FT_Q8_BLK: usize = 40;
 pub const FT_LAYOUT_Q4_0: c_int = 0;
 pub const FT_LAYOUT_Q4R: c_int = 1;
+pub const FT_TYPE_F32: c_int = 0;
+pub const FT_TYPE_F16: c_int = 1;
+pub const FT_TYPE_BF16: c_int = 2;
+pub const FT_SCORE_SOFTMAX: c_int = 0;
+pub const FT_SCORE_SIGMOID: c_int = 1;
 pub const FT_HIP_NOALLOC_SCRATCH_BYTES: usize = 8 << 20;
 
 #[link(name = "fthip")]
@@ -42,6 +47,7 @@ extern "C" {
     pub fn ft_hip_destroy(ctx: *mut FtHipCtx) -> c_int;
     pub fn ft_hip_row_bytes(layout: c_int, k: i64) -> i64;
     pub fn ft_hip_q4r_scales_bytes(k: i64) -> i64;
+    pub fn ft_hip_add_rmsnorm(ctx: *mut FtHipCtx, stream: *mut c_void, x: *const c_void, x_type: c_int, x_stride: i64, x_w: *const f32, residual: *const f32, residual_stride: i64, h: *mut f32, h_stride: i64, w: *const f32, eps: f32, y: *mut f32, y_stride: i64, q8: *mut c_void, hidden: i64, n: i64) -> c_int;
     pub fn ft_hip_quantize_q8(ctx: *mut FtHipCtx, stream: *mut c_void, x: *const f32, x_stride: i64, q8: *mut c_void, k: i64, n: i64) -> c_int;
     pub fn ft_hip_gemv_q4_grouped_ptr(ctx: *mut FtHipCtx, stream: *mut c_void, bases: *const u64, bank_off: u64, x_idx: *const i32, n_entries: i64, q8: *const c_void, q8_stride_blocks: i64, y: *mut f32, y_stride: i64, n_rows: i64, k: i64, layout: c_int) -> c_int;
     pub fn ft_hip_gemv_q4_grouped_slots(ctx: *mut FtHipCtx, stream: *mut c_void, base: *const c_void, expert_bytes: u64, bank_off: u64, slots: *const i32, x_idx: *const i32, n_entries: i64, q8: *const c_void, q8_stride_blocks: i64, y: *mut f32, y_stride: i64, n_rows: i64, k: i64, layout: c_int) -> c_int;
@@ -55,6 +61,7 @@ extern "C" {
     pub fn ft_hip_gemv_q4r_f32in(ctx: *mut FtHipCtx, stream: *mut c_void, w: *const c_void, x: *const f32, y: *mut f32, act: *mut f32, n_rows: i64, k: i64) -> c_int;
     pub fn ft_hip_router_logits(ctx: *mut FtHipCtx, stream: *mut c_void, w: *const f32, x: *const f32, bias: *const f32, y: *mut f32, dim: i64, n_rows: i64, n_seqs: i64) -> c_int;
     pub fn ft_hip_topk_router(ctx: *mut FtHipCtx, stream: *mut c_void, logits: *const f32, expert_scale: *const f32, ids: *mut i32, wts: *mut f32, e_count: i64, k: i64, n_seqs: i64) -> c_int;
+    pub fn ft_hip_route_experts(ctx: *mut FtHipCtx, stream: *mut c_void, logits: *const f32, logits_stride: i64, bias: *const f32, expert_scale: *const f32, score: c_int, n_groups: i64, top_groups: i64, group_rank: c_int, renorm: c_int, scale: f32, ids: *mut i32, wts: *mut f32, n_experts: i64, top_k: i64, n_seqs: i64) -> c_int;
     pub fn ft_hip_reduce_pairs_weighted(ctx: *mut FtHipCtx, stream: *mut c_void, y: *const f32, wts: *const f32, seq_of: *const i32, out: *mut f32, hidden: i64, n_pairs: i64, n_seqs: i64) -> c_int;
     pub fn ft_hip_repack_rows(ctx: *mut FtHipCtx, stream: *mut c_void, src: *const c_void, src_layout: c_int, dst: *mut c_void, dst_layout: c_int, n_rows: i64, k: i64) -> c_int;
     pub fn ft_hip_gen_values(ctx: *mut FtHipCtx, stream: *mut c_void, key: u64, start: i64, n: i64, scale: f32, out: *mut f32) -> c_int;

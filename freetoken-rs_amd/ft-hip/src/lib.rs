@@ -47,6 +47,46 @@ impl Layout {
     }
 }
 
+/// Element type of an input that may come in 16 bits.
+#[derive(Clone, Copy, Debug, PartialEq, Eq)]
+pub enum Type {
+    F32,
+    F16,
+    Bf16,
+}
+impl Type {
+    fn raw(self) -> i32 {
+        match self {
+            Type::F32 => ffi::FT_TYPE_F32,
+            Type::F16 => ffi::FT_TYPE_F16,
+            Type::Bf16 => ffi::FT_TYPE_BF16,
+        }
+    }
+}
+
+/// Rows in device memory: the address and the values from one row to the next.
+#[derive(Clone, Copy, Debug)]
+pub struct Rows(pub DevPtr, pub usize);
+
+/// How `route_experts` scores experts.
+#[derive(Clone, Copy, Debug, PartialEq, Eq)]
+pub enum Score {
+    Softmax,
+    Sigmoid,
+}
+
+/// The choice `route_experts` makes: `groups` equal groups of which the
+/// `top_groups` best by their `group_rank` best experts stay open.
+#[derive(Clone, Copy, Debug)]
+pub struct Route {
+    pub score: Score,
+    pub groups: usize,
+    pub top_groups: usize,
+    pub group_rank: i32,
+    pub renorm: bool,
+    pub scale: f32,
+}
+
 /// Bytes per 32-element q8 activation block.
 pub const Q8_BLK: usize = ffi::FT_Q8_BLK;
 
@@ -90,6 +130,21 @@ impl Q4Gemv {
     /// `quantize_q8_view` (ft-cuda/src/lib.rs:871-894): the same over a row view.
     pub fn quantize_q8_view(&self, s: Stream, x: DevPtr, x_stride: usize, q8: DevPtr, k: usize, n: usize) -> Result<()> {
         self.quantize_q8(s, x, x_stride, q8, k, n)
+    }
+
+    /// The section's norm (ft-model/src/lib.rs:1358-1367) in one launch: h =
+    /// residual + x (with `x_w`, x normed by it first), y = rmsnorm(h) * w and
+    /// y's q8 blocks; each output or None.
+    #[allow(clippy::too_many_arguments)]
+    pub fn add_rmsnorm(&self, s: Stream, x: Rows, x_type: Type, x_w: Option<DevPtr>, residual: Option<Rows>,
+                       h: Option<Rows>, w: Option<DevPtr>, eps: f32, y: Option<Rows>, q8: Option<DevPtr>,
+                       hidden: usize, n: usize) -> Result<()> {
+        let (r, h, y) = (residual.unwrap_or(Rows(0, 0)), h.unwrap_or(Rows(0, 0)), y.unwrap_or(Rows(0, 0)));
+        check(unsafe {
+            ffi::ft_hip_add_rmsnorm(self.ctx, s.0, p(x.0), x_type.raw(), x.1 as i64, opt(x_w), p(r.0), r.1 as i64,
+                                    pm(h.0), h.1 as i64, opt(w), eps, pm(y.0), y.1 as i64, pm(q8.unwrap_or(0)),
+                                    hidden as i64, n as i64)
+        })
     }
 
     /// `gemv_grouped_q8_ptr` (ft-cuda/src/lib.rs:593-623): y[e] = W_e q8[x_idx[e]]
@@ -212,6 +267,24 @@ impl Q4Gemv {
         check(unsafe {
             ffi::ft_hip_topk_router(self.ctx, s.0, p(logits), opt(expert_scale), pm(ids), pm(wts), e_count as i64,
                                     k as i64, n_seqs as i64)
+        })
+    }
+
+    /// Experts by softmax or sigmoid scores with a selection bias, groups,
+    /// renormalised and scaled weights (no reference counterpart; see the header).
+    #[allow(clippy::too_many_arguments)]
+    pub fn route_experts(&self, s: Stream, logits: Rows, bias: Option<DevPtr>, expert_scale: Option<DevPtr>,
+                         route: Route, ids: DevPtr, wts: DevPtr, n_experts: usize, top_k: usize, n_seqs: usize)
+                         -> Result<()> {
+        let score = match route.score {
+            Score::Softmax => ffi::FT_SCORE_SOFTMAX,
+            Score::Sigmoid => ffi::FT_SCORE_SIGMOID,
+        };
+        check(unsafe {
+            ffi::ft_hip_route_experts(self.ctx, s.0, p(logits.0), logits.1 as i64, opt(bias), opt(expert_scale), score,
+                                      route.groups as i64, route.top_groups as i64, route.group_rank,
+                                      route.renorm as i32, route.scale, pm(ids), pm(wts), n_experts as i64,
+                                      top_k as i64, n_seqs as i64)
         })
     }
 

@@ -20,6 +20,8 @@ E_IO, E_FORMAT, E_NOT_FOUND = -6, -7, -8
 NOALLOC_SCRATCH_BYTES = 8 << 20  # FT_HIP_NOALLOC_SCRATCH_BYTES
 Q8_BLK = 40
 LAYOUT_Q4_0, LAYOUT_Q4R = 0, 1
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 
 _lib = None
 
@@ -34,6 +36,7 @@ SIGNATURES = {
     "ft_hip_row_bytes": (_I64, [_I, _I64]),
     "ft_hip_q4r_scales_bytes": (_I64, [_I64]),
     "ft_hip_quantize_q8": (_I, [_P, _P, _P, _I64, _P, _I64, _I64]),
+    "ft_hip_add_rmsnorm": (_I, [_P, _P, _P, _I, _I64, _P, _P, _I64, _P, _I64, _P, _F, _P, _I64, _P, _I64, _I64]),
     "ft_hip_gemv_q4_grouped_ptr": (_I, [_P, _P, _P, _U64, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I]),
     "ft_hip_gemv_q4_grouped_slots": (_I, [_P, _P, _P, _U64, _U64, _P, _P, _I64, _P, _I64, _P, _I64, _I64,
                                           _I64, _I]),
@@ -47,6 +50,7 @@ SIGNATURES = {
     "ft_hip_gemv_q4r_f32in": (_I, [_P, _P, _P, _P, _P, _P, _I64, _I64]),
     "ft_hip_router_logits": (_I, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64]),
     "ft_hip_topk_router": (_I, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64]),
+    "ft_hip_route_experts": (_I, [_P, _P, _P, _I64, _P, _P, _I, _I64, _I64, _I, _I, _F, _P, _P, _I64, _I64, _I64]),
     "ft_hip_reduce_pairs_weighted": (_I, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64]),
     "ft_hip_repack_rows": (_I, [_P, _P, _P, _I, _P, _I, _I64, _I64]),
     "ft_hip_gen_values": (_I, [_P, _P, _U64, _I64, _I64, _F, _P]),
@@ -161,6 +165,38 @@ def _stream(stream):
     return ctypes.c_void_p(stream.cuda_stream)
 
 
+_TYPES = {}  # torch dtype -> FT_TYPE_*
+
+
+def _type(t):
+    """FT_TYPE_* of a tensor of the types an input may come in."""
+    if not _TYPES:
+        import torch
+        _TYPES.update({torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16})
+    if t.dtype not in _TYPES:
+        raise FtHipError(E_INVALID, f"{t.dtype} is none of float32, float16, bfloat16")
+    return _TYPES[t.dtype]
+
+
+def _rows(t, n, width, size, what):
+    """(pointer, row stride) of n rows of `width` values of `size` bytes in t: a
+    [rows, values] tensor with a row stride of its own, or a contiguous one of
+    any shape; (NULL, 0) for None. Raises where t cannot hold them."""
+    if t is None:
+        return None, 0
+    if t.element_size() != size:
+        raise FtHipError(E_INVALID, f"{what}: {t.dtype} has not {size} bytes a value")
+    if t.dim() == 2:
+        rows, cols = t.shape
+        stride = t.stride(0) if rows > 1 else max(cols, width)
+        ok = rows >= n and cols >= width and (cols == 1 or t.stride(1) == 1)
+    else:
+        stride, ok = width, t.is_contiguous() and t.numel() >= n * width
+    if n > 0 and not ok:
+        raise FtHipError(E_SHAPE, f"{what}: {tuple(t.shape)} does not hold {n} rows of {width} consecutive values")
+    return ctypes.c_void_p(t.data_ptr()), stride
+
+
 class Q4Gemv:
     """Counterpart of ft_cuda::Q4Gemv on one gfx950 device."""
 
@@ -183,6 +219,27 @@ class Q4Gemv:
     # -- ft-cuda/src/lib.rs:898-921 --
     def quantize_q8(self, x, x_stride, q8, k, n, stream=None):
         check(lib().ft_hip_quantize_q8(self._ctx, _stream(stream), _ptr(x), x_stride, _ptr(q8), k, n))
+
+    def _on(self, stream):
+        """The stream's handle; None: the current stream of this handle's device."""
+        if stream is None:
+            import torch
+            stream = torch.cuda.current_stream(self.device)
+        return ctypes.c_void_p(stream.cuda_stream)
+
+    # -- ft-model/src/lib.rs:1358-1367: the section's norm, with the addition before and the q8 after it --
+    def add_rmsnorm(self, x, w, hidden, n, eps, residual=None, h=None, y=None, q8=None, x_w=None, stream=None):
+        """h = residual + x (x_w given: x normed by x_w first), y = rmsnorm(h) * w and y's q8 blocks, each output
+        or None. x: f32, f16 or bf16 rows; the others f32. A 2-D tensor's row stride is taken as it is."""
+        xp, xs = _rows(x, n, hidden, x.element_size(), "add_rmsnorm: x")
+        rp, rs = _rows(residual, n, hidden, 4, "add_rmsnorm: residual")
+        hp, hs = _rows(h, n, hidden, 4, "add_rmsnorm: h")
+        yp, ys = _rows(y, n, hidden, 4, "add_rmsnorm: y")
+        wp, xwp = _rows(w, 1, hidden, 4, "add_rmsnorm: w")[0], _rows(x_w, 1, hidden, 4, "add_rmsnorm: x_w")[0]
+        if q8 is not None and not (q8.is_contiguous() and q8.numel() * q8.element_size() >= n * (hidden // 32) * Q8_BLK):
+            raise FtHipError(E_SHAPE, f"add_rmsnorm: q8 does not hold {n} rows of {hidden} values")
+        check(lib().ft_hip_add_rmsnorm(self._ctx, self._on(stream), xp, _type(x), xs, xwp, rp, rs, hp, hs, wp, eps, yp,
+                                       ys, _ptr(q8), hidden, n))
 
     # -- ft-cuda/src/lib.rs:593-623 (q4_0) and :736-767 (q4r) --
     def gemv_grouped_ptr(self, bases, bank_off, x_idx, n_entries, q8, q8_stride_blocks, y, y_stride,
@@ -270,6 +327,21 @@ class Q4Gemv:
     def topk_router_dev(self, logits, expert_scale, ids, wts, e_count, k, n_seqs, stream=None):
         check(lib().ft_hip_topk_router(self._ctx, _stream(stream), _ptr(logits), _ptr(expert_scale), _ptr(ids),
                                        _ptr(wts), e_count, k, n_seqs))
+
+    # -- no reference counterpart: routing beyond the softmax over the top-k --
+    def route_experts(self, logits, ids, wts, n_experts, top_k, n_seqs, score=SCORE_SOFTMAX, bias=None, n_groups=1,
+                      top_groups=1, group_rank=1, renorm=True, scale=1.0, expert_scale=None, stream=None):
+        """ids/wts of the top_k experts per row of logits: scores by softmax or sigmoid, chosen with `bias` added
+        among the top_groups best of n_groups groups, weights renormalised and scaled (see the header)."""
+        lp, ls = _rows(logits, n_seqs, n_experts, 4, "route_experts: logits")
+        bp = _rows(bias, 1, n_experts, 4, "route_experts: bias")[0]
+        ep = _rows(expert_scale, 1, n_experts, 4, "route_experts: expert_scale")[0]
+        for t, what in ((ids, "ids"), (wts, "wts")):
+            if t.element_size() != 4 or not t.is_contiguous() or t.numel() < n_seqs * top_k:
+                raise FtHipError(E_SHAPE, f"route_experts: {what} does not hold {n_seqs} x {top_k} values of 4 bytes")
+        check(lib().ft_hip_route_experts(self._ctx, self._on(stream), lp, ls, bp, ep, score, n_groups, top_groups,
+                                         group_rank, int(renorm), scale, _ptr(ids), _ptr(wts), n_experts, top_k,
+                                         n_seqs))
 
     # -- ft-cuda/src/lib.rs:808-829 --
     def reduce_pairs_weighted(self, y, wts, seq_of, out, hidden, n_pairs, n_seqs, stream=None):

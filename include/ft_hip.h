@@ -55,6 +55,15 @@ extern "C" {
 #define FT_LAYOUT_Q4_0 0
 #define FT_LAYOUT_Q4R 1
 
+/* element types of the inputs that may come in 16 bits */
+#define FT_TYPE_F32 0
+#define FT_TYPE_F16 1
+#define FT_TYPE_BF16 2
+
+/* how ft_hip_route_experts scores experts */
+#define FT_SCORE_SOFTMAX 0
+#define FT_SCORE_SIGMOID 1
+
 typedef struct ft_hip_ctx ft_hip_ctx;
 
 /* Library version (major*10000 + minor*100 + patch). */
@@ -79,6 +88,34 @@ int64_t ft_hip_q4r_scales_bytes(int64_t k);
  * x: [n, x_stride] f32 (x_stride 0 shares one vector), q8: [n, k/32] blocks. */
 int ft_hip_quantize_q8(ft_hip_ctx* ctx, void* stream, const float* x, int64_t x_stride,
                        void* q8, int64_t k, int64_t n);
+
+/* Residual addition, RMS norm and q8 of n rows in one launch: what stands in
+ * front of each section (the reference's add_rows and rmsnorm_rows followed by
+ * quantize_q8, ft-model/src/lib.rs:1358-1367). Per row of `hidden` values:
+ *   b   = x, or with x_w (the branch's own norm, before the addition)
+ *         x / sqrt(mean(x*x) + eps) * x_w
+ *   h   = residual + b (b without a residual), rounded to f32
+ *   inv = 1 / sqrt(mean(h*h) + eps)
+ *   y   = h * inv * w (w NULL: 1)
+ *   q8  = blocks {d, qsum, qs} with qs = round half away from zero of
+ *         127 * u / a, u = f32(h * w), a = max |u| of the block's 32 values,
+ *         and d = a * inv / 127.
+ * The quants are the real quotients' roundings and do not depend on inv, so
+ * that a sum's last bit moves none of them; they are within one of
+ * ft_hip_quantize_q8's on y, which rounds y and 1/d first. Sums are f64; h, y
+ * and d are each rounded once. A block's NaN values get quant 0 and are
+ * skipped by its maximum, a block with inf has all quants 0, and a row with
+ * either has NaN or 0 in its y and d.
+ * x: [n] rows of x_type (FT_TYPE_*) x_stride values apart; x_w, w: [hidden]
+ * or NULL; residual, h, y: f32 rows their own stride apart, each or NULL (not
+ * all three outputs); q8: [n][hidden/32] blocks or NULL, 4-byte aligned. h may
+ * be residual itself, and h or y may be x where it is f32 (same stride); other
+ * buffers may not overlap an output. hidden <= 16384, a multiple of 32 where
+ * q8 is written; rows that all start on 4 values (16 bytes of f32) are read
+ * four values at a time. */
+int ft_hip_add_rmsnorm(ft_hip_ctx* ctx, void* stream, const void* x, int x_type, int64_t x_stride, const float* x_w,
+                       const float* residual, int64_t residual_stride, float* h, int64_t h_stride, const float* w,
+                       float eps, float* y, int64_t y_stride, void* q8, int64_t hidden, int64_t n);
 
 /* Grouped q4 x q8 GEMV over per-entry weight pointers. Replaces
  * gemv_grouped_q8_ptr (ft-cuda/src/lib.rs:593-623, layout q4_0) and
@@ -199,6 +236,32 @@ int ft_hip_router_logits(ft_hip_ctx* ctx, void* stream, const float* w, const fl
 int ft_hip_topk_router(ft_hip_ctx* ctx, void* stream, const float* logits,
                        const float* expert_scale, int32_t* ids, float* wts, int64_t e_count,
                        int64_t k, int64_t n_seqs);
+
+/* Experts chosen from router logits for models that route otherwise than
+ * ft_hip_topk_router (no reference counterpart; the reference's one model
+ * takes the softmax over its top-k). Per token, over the n_experts logits l:
+ *   s = softmax(l) or sigmoid(l) (score: FT_SCORE_*),  c = s + bias (NULL: 0)
+ *   n_groups > 1: the experts lie in n_groups equal consecutive groups, a
+ *     group's score is its largest c (group_rank 1) or the sum of its two
+ *     largest (2), and only the top_groups best groups stay open
+ *   ids = the top_k open experts by c, largest first; equal c (equal groups):
+ *     the lower index first
+ *   wts = s of the chosen; renorm 1: over their sum (0 where the sum is 0);
+ *     times scale, times expert_scale[e] (NULL: 1)
+ * Scores and sums are f64, wts are rounded once; the bias decides the choice
+ * and is no part of the weight. With softmax, renorm 1, no bias and no groups
+ * the ids are ft_hip_topk_router's where all logits are finite, and the
+ * weights agree to rounding.
+ * An expert whose logit or c is NaN, or whose logit or bias is -inf, is never
+ * chosen (several +inf logits share the softmax). Where fewer than top_k are
+ * left, the other entries are expert 0 with weight 0, so that launches over the
+ * pairs stay inside the bank and add nothing.
+ * logits: [n_seqs] rows logits_stride values apart; ids/wts [n_seqs][top_k].
+ * n_experts <= 1024, n_groups <= 64 dividing it, top_k <= 32. */
+int ft_hip_route_experts(ft_hip_ctx* ctx, void* stream, const float* logits, int64_t logits_stride,
+                         const float* bias, const float* expert_scale, int score, int64_t n_groups,
+                         int64_t top_groups, int group_rank, int renorm, float scale, int32_t* ids, float* wts,
+                         int64_t n_experts, int64_t top_k, int64_t n_seqs);
 
 /* Replaces reduce_pairs_weighted (ft-cuda/src/lib.rs:808-829):
  * out[s][i] += sum over pairs p with seq_of[p] == s, in p order, of
