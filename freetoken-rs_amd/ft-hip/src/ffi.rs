@@ -63,6 +63,8 @@ extern "C" {
     pub fn ft_hip_topk_router(ctx: *mut FtHipCtx, stream: *mut c_void, logits: *const f32, expert_scale: *const f32, ids: *mut i32, wts: *mut f32, e_count: i64, k: i64, n_seqs: i64) -> c_int;
     pub fn ft_hip_route_experts(ctx: *mut FtHipCtx, stream: *mut c_void, logits: *const f32, logits_stride: i64, bias: *const f32, expert_scale: *const f32, score: c_int, n_groups: i64, top_groups: i64, group_rank: c_int, renorm: c_int, scale: f32, ids: *mut i32, wts: *mut f32, n_experts: i64, top_k: i64, n_seqs: i64) -> c_int;
     pub fn ft_hip_reduce_pairs_weighted(ctx: *mut FtHipCtx, stream: *mut c_void, y: *const f32, wts: *const f32, seq_of: *const i32, out: *mut f32, hidden: i64, n_pairs: i64, n_seqs: i64) -> c_int;
+    pub fn ft_hip_sample_tokens_workspace_bytes(vocab: i64, n: i64) -> usize;
+    pub fn ft_hip_sample_tokens(ctx: *mut FtHipCtx, stream: *mut c_void, logits: *const c_void, logits_type: c_int, logits_stride: i64, vocab: i64, n: i64, temperature: *const f32, top_k: *const i32, top_p: *const f32, min_p: *const f32, u: *const f32, tokens: *mut i32, logprobs: *mut f32, workspace: *mut c_void, workspace_bytes: usize) -> c_int;
     pub fn ft_hip_repack_rows(ctx: *mut FtHipCtx, stream: *mut c_void, src: *const c_void, src_layout: c_int, dst: *mut c_void, dst_layout: c_int, n_rows: i64, k: i64) -> c_int;
     pub fn ft_hip_gen_values(ctx: *mut FtHipCtx, stream: *mut c_void, key: u64, start: i64, n: i64, scale: f32, out: *mut f32) -> c_int;
     pub fn ft_hip_gen_q4_rows(ctx: *mut FtHipCtx, stream: *mut c_void, key: u64, row0: i64, n_rows: i64, k: i64, scale: f32, out: *mut c_void, layout: c_int) -> c_int;

@@ -288,6 +288,25 @@ impl Q4Gemv {
         })
     }
 
+    /// Bytes of `sample_tokens`' workspace (0: a shape it refuses).
+    pub fn sample_tokens_workspace_bytes(vocab: usize, n: usize) -> usize {
+        unsafe { ffi::ft_hip_sample_tokens_workspace_bytes(vocab as i64, n as i64) }
+    }
+
+    /// A token per row of logits (the reference kernel: ft-cuda/src/q4.cu:1246-1291)
+    /// from the random numbers `u` and the rows' settings, None: off (see the header).
+    #[allow(clippy::too_many_arguments)]
+    pub fn sample_tokens(&self, s: Stream, logits: Rows, logits_type: Type, vocab: usize, n: usize,
+                         temperature: Option<DevPtr>, top_k: Option<DevPtr>, top_p: Option<DevPtr>,
+                         min_p: Option<DevPtr>, u: DevPtr, tokens: DevPtr, logprobs: Option<DevPtr>,
+                         workspace: DevPtr, workspace_bytes: usize) -> Result<()> {
+        check(unsafe {
+            ffi::ft_hip_sample_tokens(self.ctx, s.0, p(logits.0), logits_type.raw(), logits.1 as i64, vocab as i64,
+                                      n as i64, opt(temperature), opt(top_k), opt(top_p), opt(min_p), p(u),
+                                      pm(tokens), pm(logprobs.unwrap_or(0)), pm(workspace), workspace_bytes)
+        })
+    }
+
     /// `reduce_pairs_weighted` (ft-cuda/src/lib.rs:808-829).
     #[allow(clippy::too_many_arguments)]
     pub fn reduce_pairs_weighted(&self, s: Stream, y: DevPtr, wts: DevPtr, seq_of: DevPtr, out: DevPtr,

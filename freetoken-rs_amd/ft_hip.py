@@ -52,6 +52,8 @@ SIGNATURES = {
     "ft_hip_topk_router": (_I, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64]),
     "ft_hip_route_experts": (_I, [_P, _P, _P, _I64, _P, _P, _I, _I64, _I64, _I, _I, _F, _P, _P, _I64, _I64, _I64]),
     "ft_hip_reduce_pairs_weighted": (_I, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64]),
+    "ft_hip_sample_tokens_workspace_bytes": (_SZ, [_I64, _I64]),
+    "ft_hip_sample_tokens": (_I, [_P, _P, _P, _I, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _SZ]),
     "ft_hip_repack_rows": (_I, [_P, _P, _P, _I, _P, _I, _I64, _I64]),
     "ft_hip_gen_values": (_I, [_P, _P, _U64, _I64, _I64, _F, _P]),
     "ft_hip_gen_q4_rows": (_I, [_P, _P, _U64, _I64, _I64, _I64, _F, _P, _I]),
@@ -347,6 +349,29 @@ class Q4Gemv:
     def reduce_pairs_weighted(self, y, wts, seq_of, out, hidden, n_pairs, n_seqs, stream=None):
         check(lib().ft_hip_reduce_pairs_weighted(self._ctx, _stream(stream), _ptr(y), _ptr(wts), _ptr(seq_of),
                                                  _ptr(out), hidden, n_pairs, n_seqs))
+
+    # -- ft-cuda/src/q4.cu:1246-1291, with settings per row --
+    @staticmethod
+    def sample_tokens_workspace_bytes(vocab, n):
+        return lib().ft_hip_sample_tokens_workspace_bytes(vocab, n)
+
+    def sample_tokens(self, logits, vocab, n, u, tokens, workspace, temperature=None, top_k=None, top_p=None,
+                      min_p=None, logprobs=None, stream=None):
+        """tokens[n] drawn from rows of f32, f16 or bf16 logits with the random numbers u[n] and each row's settings
+        (f32 tensors [n], top_k int32; None: off), logprobs[n] their log probabilities among the kept (see the header)."""
+        lp, ls = _rows(logits, n, vocab, logits.element_size(), "sample_tokens: logits")
+        ptrs = []
+        for t, what in ((temperature, "temperature"), (top_k, "top_k"), (top_p, "top_p"), (min_p, "min_p"), (u, "u"),
+                        (tokens, "tokens"), (logprobs, "logprobs")):
+            if t is None:
+                ptrs.append(None)
+                continue
+            whole = t.dtype.is_floating_point is (what in ("top_k", "tokens"))
+            if t.element_size() != 4 or whole or not t.is_contiguous() or t.numel() < n:
+                raise FtHipError(E_SHAPE, f"sample_tokens: {what} does not hold {n} values of its 4-byte type")
+            ptrs.append(_ptr(t))
+        check(lib().ft_hip_sample_tokens(self._ctx, self._on(stream), lp, _type(logits), ls, vocab, n, *ptrs,
+                                         _ptr(workspace), workspace.numel() * workspace.element_size()))
 
     # -- setup: ft-core/src/q4_0.rs:248-258 on the device --
     def repack_rows(self, src, src_layout, dst, dst_layout, n_rows, k, stream=None):

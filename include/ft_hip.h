@@ -271,6 +271,35 @@ int ft_hip_reduce_pairs_weighted(ft_hip_ctx* ctx, void* stream, const float* y,
                                  const float* wts, const int32_t* seq_of, float* out,
                                  int64_t hidden, int64_t n_pairs, int64_t n_seqs);
 
+/* A token per row of logits, drawn with the row's settings from its given
+ * random number: what follows the vocabulary head (the reference's
+ * sample_tokens, ft-cuda/src/q4.cu:1246-1291, with per-row settings). Per row,
+ * M its largest logit, e_i = exp((l_i - M) / temperature):
+ *   order  logits falling, equal ones by rising index
+ *   kept   its first top_k; of these the shortest prefix whose e sum to at
+ *          least top_p of theirs; of these the e_i >= min_p
+ *   token  the first kept index, in index order, at which the running sum of
+ *          kept e passes u * S, S their sum; logprob = log(e / S) of it
+ * temperature, top_k, top_p, min_p: device arrays [n], or NULL for 1, off, off
+ * and off. temperature <= 0 or NaN: the largest logit (the lowest index),
+ * logprob 0. top_k <= 0 or >= vocab, top_p >= 1 or NaN, min_p <= 0 or NaN: off;
+ * the first of the order is always kept (top_p 0: alone; min_p over 1: as 1).
+ * u: [n], in [0, 1); less or NaN as 0, 1 and more as the last kept index.
+ * Logits of NaN and -inf are never drawn; +inf ones share the draw; a row
+ * without any other gets token -1 and logprob NaN. Weights and sums are f64,
+ * in a fixed order: the same call gives the same bits.
+ * logits: [n] rows of logits_type (FT_TYPE_*) logits_stride values apart, read
+ * only; tokens [n]; logprobs [n] or NULL. workspace: device scratch of
+ * ft_hip_sample_tokens_workspace_bytes() bytes (0 for a bad shape), 16-byte
+ * aligned, any content, for one call at a time. */
+#define FT_SAMPLE_MAX_VOCAB 2097152
+#define FT_SAMPLE_MAX_ROWS 65535
+size_t ft_hip_sample_tokens_workspace_bytes(int64_t vocab, int64_t n);
+int ft_hip_sample_tokens(ft_hip_ctx* ctx, void* stream, const void* logits, int logits_type, int64_t logits_stride,
+                         int64_t vocab, int64_t n, const float* temperature, const int32_t* top_k,
+                         const float* top_p, const float* min_p, const float* u, int32_t* tokens, float* logprobs,
+                         void* workspace, size_t workspace_bytes);
+
 /* Row layout conversion on the device (setup, not the hot path): the
  * reference repacks q4_0 banks to q4r at load (ft-model/src/lib.rs:570-609,
  * ft-core/src/q4_0.rs:248-258). src and dst hold n_rows rows of k weights. */

@@ -61,3 +61,31 @@ def test_route_experts(change, code, word):
     rc, msg = _err(ft_hip.lib().ft_hip_route_experts(*{**ROUTE, **change}.values()))
     assert rc == getattr(ft_hip, "E_" + code), msg
     assert word in msg, msg
+
+
+SAMPLE = dict(ctx=None, stream=None, logits=P, logits_type=0, stride=1000, vocab=1000, n=4, temperature=None,
+              top_k=None, top_p=None, min_p=None, u=P, tokens=P, logprobs=None, workspace=P, workspace_bytes=1 << 40)
+
+
+@pytest.mark.parametrize("change,code,word", [
+    (dict(vocab=0), "SHAPE", "vocab"), (dict(vocab=(1 << 21) + 1), "SHAPE", "vocab"), (dict(vocab=BIG), "SHAPE", "vocab"),
+    (dict(n=-1), "SHAPE", "n="), (dict(n=65536), "SHAPE", "n="), (dict(n=BIG), "SHAPE", "n="),
+    (dict(logits_type=3), "INVALID", "logits_type"), (dict(stride=999), "SHAPE", "stride"),
+    (dict(stride=BIG), "SHAPE", "stride"), (dict(logits=ODD), "SHAPE", "aligned"),
+    (dict(logits_type=1, logits=ctypes.c_void_p(0x1001)), "SHAPE", "aligned"),
+    (dict(workspace=ctypes.c_void_p(0x1008)), "SHAPE", "workspace"), (dict(workspace_bytes=0), "SHAPE", "workspace"),
+    (dict(u=None), "INVALID", "null"), (dict(tokens=None), "INVALID", "null"), (dict(logits=None), "INVALID", "null"),
+    (dict(workspace=None), "INVALID", "null"), (dict(), "INVALID", "null"),
+])
+def test_sample_tokens(change, code, word):
+    rc, msg = _err(ft_hip.lib().ft_hip_sample_tokens(*{**SAMPLE, **change}.values()))
+    assert rc == getattr(ft_hip, "E_" + code), msg
+    assert word in msg, msg
+
+
+def test_sample_tokens_workspace():
+    f = ft_hip.lib().ft_hip_sample_tokens_workspace_bytes
+    assert f(0, 1) == f(1, -1) == f((1 << 21) + 1, 1) == f(1, 65536) == 0
+    assert 0 < f(1, 1) <= f(262144, 1) <= f(262144, 256) <= f(1 << 21, 65535)
+    rc, msg = _err(ft_hip.lib().ft_hip_sample_tokens(*{**SAMPLE, "workspace_bytes": f(1000, 4) - 1}.values()))
+    assert rc == ft_hip.E_SHAPE and "needed" in msg
