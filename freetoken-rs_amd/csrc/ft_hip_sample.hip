@@ -23,7 +23,21 @@ using namespace ft;
 namespace {
 
 constexpr int ROW_THREADS = 1024, ROW_WAVES = ROW_THREADS / 64;
-constexpr int FIX = 42;  // fraction bits of a weight <= 1: 2^21 of them stay below 2^63
+constexpr int FIX = 42;     // fraction bits of a weight <= 1: 2^21 of them stay below 2^63
+constexpr int LIST = 8192;  // values of a row that a workgroup keeps in LDS
+constexpr int FEW = 256;    // values that are ranked by comparing all with all
+constexpr int SEG = 64;     // values whose maximum the scan leaves
+constexpr int MAX_SEGS = FT_SAMPLE_MAX_VOCAB / SEG;
+constexpr int MAX_CHUNKS = FT_SAMPLE_MAX_VOCAB / 8192;
+
+// e is counted in steps of 2^(1/8): BINS of them reach 2^-64 below a chunk's
+// largest. A value's e over its step's middle is in [2^-1/16, 2^1/16); a bin's
+// word holds the number of values above bit 47 and below it their sum over
+// OFFSET in units of 2^-FRAC (8192 times 0.107 * 2^35 is far below 2^47). The
+// chunk's largest value itself is in no bin: how often it occurs is counted
+// apart, so that equal largest logits weigh the same whole number everywhere.
+constexpr int BINS = 512, FRAC = 35;
+constexpr double OFFSET = 0.9375;
 
 struct SampleArgs {
     const void* logits;
@@ -112,36 +126,62 @@ __device__ __forceinline__ int wave_scan_i(int v) {
     return v;
 }
 
+// What a workgroup that finishes a row keeps in LDS.
 struct RowLds {
     uint64_t w[1024];
     uint32_t n[1024];
     double part[ROW_WAVES];
+    double part2[ROW_WAVES];
     int parti[ROW_WAVES];
     int pick;
-    double at, at_w;
+    double at;
     int at_n;
+    float v[LIST];  // values taken from the row, by rising index
+    int i[LIST];
 };
 
-// Where the order is cut: the first `ties` values equal to key and all above.
+template <int TYPE>
+__device__ __forceinline__ const void* row_at(const SampleArgs& a, int64_t r) {
+    return static_cast<const char*>(a.logits) + r * a.stride * (TYPE == FT_TYPE_F32 ? 4 : 2);
+}
+
+// The values that a step of a row's work goes through, by rising index.
+template <int TYPE>
+struct WholeRow {
+    const void* row;
+    int V;
+    __device__ __forceinline__ int size() const { return V; }
+    __device__ __forceinline__ float value(int at) const { return logit<TYPE>(row, at); }
+    __device__ __forceinline__ int index(int at) const { return at; }
+};
+struct List {
+    const float* v;
+    const int* i;
+    int n;
+    __device__ __forceinline__ int size() const { return n; }
+    __device__ __forceinline__ float value(int at) const { return v[at]; }
+    __device__ __forceinline__ int index(int at) const { return i[at]; }
+};
+
+// Where the order is cut: kept are all keys above `key` and the values equal to it up to index `end`.
 struct Cut {
     uint32_t key;
-    int ties, of;   // of: how many values equal key
-    double before;  // their sum above key
+    int ties, of;   // of the `of` values equal to key the first `ties` are kept
+    int end;        // index of the last of these
+    double before;  // sum of e above key
     double e;       // one of key's
 };
 
 // First place of the order at which the count (by_count) or the sum reaches
-// the target: the key range [lo, hi] is counted into up to 1024 equal pieces,
-// the piece that reaches it is the next range, until a piece is one key. A
+// the target, among the source's keys in [lo, hi]; base_n values of sum base_w
+// are ahead of them. The range is counted into up to 1024 equal pieces, the
+// piece that reaches the target is the next range, until a piece is one key. A
 // piece's weights are summed as whole numbers relative to its upper edge, so
 // that the sum has about FIX bits wherever it lies.
-template <int TYPE>
-__device__ Cut find_cut(const void* row, int V, const Row& s, float M, bool by_count, bool sums, double target,
-                        RowLds& l) {
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    uint32_t hi = key_of(M), lo = M == INFINITY ? hi : key_of(-INFINITY) + 1;
-    int base_n = 0;
-    double base_w = 0.0;
+template <typename SRC>
+__device__ Cut find_cut(const SRC& src, uint32_t lo, uint32_t hi, int base_n, double base_w, const Row& s, float M,
+                        bool by_count, bool sums, double target, RowLds& l) {
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, size = src.size();
     for (;;) {
         const uint32_t width = hi - lo;
         const int shift = width < 1024u ? 0 : 22 - __clz(width);
@@ -149,8 +189,8 @@ __device__ Cut find_cut(const void* row, int V, const Row& s, float M, bool by_c
         l.w[t] = 0;
         if (t == 0) l.pick = 1024;
         __syncthreads();
-        for (int i = t; i < V; i += ROW_THREADS) {
-            const float v = logit<TYPE>(row, i);
+        for (int i = t; i < size; i += ROW_THREADS) {
+            const float v = src.value(i);
             const uint32_t k = key_of(v);
             if (!(v > -INFINITY) || k < lo || k > hi) continue;
             const uint32_t b = (hi - k) >> shift;
@@ -186,7 +226,7 @@ __device__ Cut find_cut(const void* row, int V, const Row& s, float M, bool by_c
         const bool there = own_n && (by_count ? (double)cum_n >= target : cum_w >= target);
         if (there) atomicMin(&l.pick, t);
         __syncthreads();
-        if (l.pick == 1024) {  // a rounding below the target: the last piece that holds anything
+        if (l.pick == 1024) {  // fewer values than asked for, or a rounding below the target: the last piece that holds any
             __syncthreads();
             if (t == 0) l.pick = -1;
             __syncthreads();
@@ -194,18 +234,25 @@ __device__ Cut find_cut(const void* row, int V, const Row& s, float M, bool by_c
             __syncthreads();
         }
         const int b = l.pick;
+        if (b < 0) return Cut{0, 1, 1, 0x7FFFFFFF, 0.0, 0.0};  // no value in the range: no cut
         if (t == b) {
             l.at = prev_w;
-            l.at_w = own_w;
             l.at_n = prev_n;
+            l.part2[0] = own_w;
         }
         __syncthreads();
         base_w = l.at;
         base_n = l.at_n;
         const int here = (int)l.n[b];
         hi -= (uint32_t)b << shift;
+        if (here == 1 && shift) {  // the only value of its piece: kept, and all above the piece's end
+            const uint32_t span = (1u << shift) - 1;
+            const Cut c{hi - lo > span ? hi - span : lo, 1, 1, 0x7FFFFFFF, base_w, l.part2[0]};
+            __syncthreads();
+            return c;
+        }
         if (shift == 0) {
-            Cut c{hi, here, here, base_w, weight(of_key(hi), M, s.inv_t)};
+            Cut c{hi, here, here, 0x7FFFFFFF, base_w, weight(of_key(hi), M, s.inv_t)};
             if (by_count) {
                 c.ties = min(here, max(1, (int)target - base_n));
             } else if (c.e > 0.0) {  // the fewest with before + ties * e >= target
@@ -223,110 +270,60 @@ __device__ Cut find_cut(const void* row, int V, const Row& s, float M, bool by_c
     }
 }
 
-// One workgroup takes a row from memory as often as it needs it: right for
-// every case, for any number of kept or equal values.
-template <int TYPE>
-__device__ void sample_streaming(const SampleArgs& a, int64_t r, const Row& s, RowLds& l) {
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, V = a.V;
-    const void* row = static_cast<const char*>(a.logits) + r * a.stride * (TYPE == FT_TYPE_F32 ? 4 : 2);
-    float M = -INFINITY;
-    for (int i = t; i < V; i += ROW_THREADS) M = fmaxf(M, logit<TYPE>(row, i));  // NaN is skipped
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o));
-    if (lane == 0) l.part[wave] = M;
-    if (t == 0) l.pick = 0x7FFFFFFF;
-    __syncthreads();
-    for (int i = 0; i < ROW_WAVES; ++i) M = fmaxf(M, (float)l.part[i]);
-    __syncthreads();
-    if (M == -INFINITY) {  // nothing can be drawn
-        if (t == 0) {
-            a.tokens[r] = -1;
-            if (a.logprobs) a.logprobs[r] = NAN;
-        }
-        return;
-    }
-    if (s.greedy) {
-        for (int i = t; i < V; i += ROW_THREADS)
-            if (logit<TYPE>(row, i) == M) {
-                atomicMin(&l.pick, i);
-                break;
-            }
+// The index of the last value equal to the cut's key that is kept.
+template <typename SRC>
+__device__ void find_end(const SRC& src, Cut& cut, RowLds& l) {
+    if (cut.ties >= cut.of) return;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, size = src.size();
+    int seen = 0;
+    for (int base = 0; base < size && seen < cut.ties; base += ROW_THREADS) {
+        const float v = base + t < size ? src.value(base + t) : -INFINITY;
+        const bool tie = v > -INFINITY && key_of(v) == cut.key;
+        const uint64_t set = __ballot(tie);
+        if (lane == 0) l.parti[wave] = __popcll(set);
         __syncthreads();
-        if (t == 0) {
-            a.tokens[r] = l.pick;
-            if (a.logprobs) a.logprobs[r] = 0.0f;
+        int rank = seen;
+        for (int w = 0; w < ROW_WAVES; ++w) {
+            if (w < wave) rank += l.parti[w];
+            seen += l.parti[w];
         }
-        return;
-    }
-    Cut cut{0, 0x7FFFFFFF, 0x7FFFFFFF, 0.0, 0.0};
-    const bool by_p = s.p < 1.0;
-    if (s.k < V) cut = find_cut<TYPE>(row, V, s, M, true, by_p, (double)s.k, l);
-    if (by_p) {
-        double z;
-        if (s.k < V) {
-            z = cut.before + cut.ties * cut.e;
-        } else {
-            z = 0.0;
-            for (int i = t; i < V; i += ROW_THREADS) {
-                const float v = logit<TYPE>(row, i);
-                if (v > -INFINITY) z += weight(v, M, s.inv_t);
-            }
-            z = wave_sum(z);
-            if (lane == 0) l.part[wave] = z;
-            __syncthreads();
-            z = 0.0;
-            for (int i = 0; i < ROW_WAVES; ++i) z += l.part[i];
-            __syncthreads();
-        }
-        const Cut c = find_cut<TYPE>(row, V, s, M, false, true, s.p * z, l);
-        if (c.key > cut.key || (c.key == cut.key && c.ties < cut.ties)) cut = c;
-    }
-    // of the values equal to the cut's key, those up to index tie_end are kept
-    int tie_end = V;
-    if (cut.ties < cut.of) {
-        int seen = 0;
-        for (int base = 0; base < V; base += ROW_THREADS) {
-            const int i = base + t;
-            const float v = i < V ? logit<TYPE>(row, i) : -INFINITY;
-            const bool tie = v > -INFINITY && key_of(v) == cut.key;
-            const uint64_t set = __ballot(tie);
-            if (lane == 0) l.parti[wave] = __popcll(set);
-            __syncthreads();
-            int rank = seen;
-            for (int w = 0; w < ROW_WAVES; ++w) {
-                if (w < wave) rank += l.parti[w];
-                seen += l.parti[w];
-            }
-            if (tie && rank + __popcll(set & ((2ull << lane) - 1)) == cut.ties) l.pick = i;
-            __syncthreads();
-            if (seen >= cut.ties) break;
-        }
-        tie_end = l.pick;
+        if (tie && rank + __popcll(set & ((2ull << lane) - 1)) == cut.ties) l.pick = src.index(base + t);
         __syncthreads();
     }
-    const auto kept = [&](int i) {
-        const float v = logit<TYPE>(row, i);
-        if (!(v > -INFINITY)) return 0.0;
-        const uint32_t k = key_of(v);
-        if (k < cut.key || (k == cut.key && i > tie_end)) return 0.0;
-        const double e = weight(v, M, s.inv_t);
-        return e >= s.m ? e : 0.0;
-    };
-    // the range that holds the token, a sixteenth of the last each time
-    int lo = 0, len = V;
-    double before = 0.0, total = 0.0, goal = 0.0;
+    cut.end = l.pick;
+    __syncthreads();
+}
+
+// e of a value if it is kept, else 0.
+__device__ __forceinline__ double kept(float v, int index, const Cut& cut, const Row& s, float M) {
+    if (!(v > -INFINITY)) return 0.0;
+    const uint32_t k = key_of(v);
+    if (k < cut.key || (k == cut.key && index > cut.end)) return 0.0;
+    const double e = weight(v, M, s.inv_t);
+    return e >= s.m ? e : 0.0;
+}
+
+// The draw among the source's places [lo, lo + len), ahead of which the kept
+// sum is `before`; total < 0: [lo, lo + len) is all, and its sum the total.
+// Sixteenths of the range are summed, the one that holds the token is the next
+// range, down to a wave's 64 places.
+template <typename SRC>
+__device__ void draw(const SampleArgs& a, int64_t r, const SRC& src, int lo, int len, double before, double total,
+                     const Cut& cut, const Row& s, float M, RowLds& l) {
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     while (len > 64) {
         const int piece = ((len + ROW_WAVES - 1) / ROW_WAVES + 63) / 64 * 64;
         const int b0 = lo + wave * piece, b1 = min(lo + len, b0 + piece);
         double z = 0.0;
-        for (int i = b0 + lane; i < b1; i += 64) z += kept(i);
+        for (int i = b0 + lane; i < b1; i += 64) z += kept(src.value(i), src.index(i), cut, s, M);
         z = wave_sum(z);
         if (lane == 0) l.part[wave] = z;
         __syncthreads();
-        if (len == V) {
+        if (total < 0.0) {
+            total = 0.0;
             for (int i = 0; i < ROW_WAVES; ++i) total += l.part[i];
-            goal = s.u * total;
         }
+        const double goal = s.u * total;
         int at = -1, some = 0;
         double cum = before, at_before = before, some_before = before;
         for (int i = 0; i < ROW_WAVES; ++i) {
@@ -335,7 +332,7 @@ __device__ void sample_streaming(const SampleArgs& a, int64_t r, const Row& s, R
                 some = i;
                 some_before = cum;
             }
-            if (at < 0 && cum + z > goal) {
+            if (at < 0 && z > 0.0 && cum + z > goal) {
                 at = i;
                 at_before = cum;
             }
@@ -346,37 +343,814 @@ __device__ void sample_streaming(const SampleArgs& a, int64_t r, const Row& s, R
             at_before = some_before;
         }
         before = at_before;
-        len = min(piece, lo + len - (lo + at * piece));
+        len = min(piece, len - at * piece);
         lo += at * piece;
         __syncthreads();
     }
     if (wave) return;
-    const double e = lane < len ? kept(lo + lane) : 0.0;
+    const int i = lo + lane;
+    const double e = lane < len ? kept(src.value(i), src.index(i), cut, s, M) : 0.0;
     const double cum = wave_scan(e);
-    if (V <= 64) {
-        total = shfl_f64(cum, 63);
-        goal = s.u * total;
-    }
-    const uint64_t over = __ballot(e > 0.0 && before + cum > goal), any = __ballot(e > 0.0);
+    if (total < 0.0) total = shfl_f64(cum, 63);
+    const uint64_t over = __ballot(e > 0.0 && before + cum > s.u * total), any = __ballot(e > 0.0);
     const int at = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)any);
     if (lane == at) {
-        a.tokens[r] = lo + lane;
+        a.tokens[r] = src.index(i);
         if (a.logprobs) a.logprobs[r] = (float)log(e / total);
     }
 }
 
+// Sum and maximum over the workgroup, the same in every thread.
+__device__ __forceinline__ double block_sum(double z, RowLds& l) {
+    z = wave_sum(z);
+    if ((threadIdx.x & 63) == 0) l.part[threadIdx.x >> 6] = z;
+    __syncthreads();
+    z = 0.0;
+    for (int i = 0; i < ROW_WAVES; ++i) z += l.part[i];
+    __syncthreads();
+    return z;
+}
+__device__ __forceinline__ float wave_max(float m) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+    return m;
+}
+__device__ __forceinline__ float block_max(float m, RowLds& l) {
+    m = wave_max(m);
+    if ((threadIdx.x & 63) == 0) l.part[threadIdx.x >> 6] = m;
+    __syncthreads();
+    for (int i = 0; i < ROW_WAVES; ++i) m = fmaxf(m, (float)l.part[i]);
+    __syncthreads();
+    return m;
+}
+
+__device__ __forceinline__ void answer(const SampleArgs& a, int64_t r, int token, float logprob) {
+    if (threadIdx.x == 0) {
+        a.tokens[r] = token;
+        if (a.logprobs) a.logprobs[r] = logprob;
+    }
+}
+
+// The largest and the smallest value above -inf over the workgroup.
+__device__ __forceinline__ void block_range(float& hi, float& lo, RowLds& l) {
+    hi = wave_max(hi);
+    lo = -wave_max(-lo);
+    if ((threadIdx.x & 63) == 0) {
+        l.part[threadIdx.x >> 6] = hi;
+        l.part2[threadIdx.x >> 6] = lo;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ROW_WAVES; ++i) {
+        hi = fmaxf(hi, (float)l.part[i]);
+        lo = fminf(lo, (float)l.part2[i]);
+    }
+    __syncthreads();
+}
+
+// A row from all of its values, streamed: right for every case, with any
+// number of kept or equal values. M > -inf.
+template <int TYPE>
+__device__ __attribute__((noinline)) void sample_streaming(const SampleArgs& a, int64_t r, const Row& s, float M,
+                                                           RowLds& l) {
+    const WholeRow<TYPE> src{row_at<TYPE>(a, r), a.V};
+    const int t = threadIdx.x;
+    const uint32_t hi = key_of(M), lo = M == INFINITY ? hi : key_of(-INFINITY) + 1;
+    const bool by_p = s.p < 1.0;
+    Cut cut{0, 1, 1, 0x7FFFFFFF, 0.0, 0.0};
+    double z = 0.0;
+    if (s.k < a.V) {
+        cut = find_cut(src, lo, hi, 0, 0.0, s, M, true, by_p, (double)s.k, l);
+        z = cut.before + cut.ties * cut.e;
+    } else if (by_p) {
+        for (int i = t; i < a.V; i += ROW_THREADS) {
+            const float v = src.value(i);
+            if (v > -INFINITY) z += weight(v, M, s.inv_t);
+        }
+        z = block_sum(z, l);
+    }
+    if (by_p) {
+        const Cut c = find_cut(src, lo, hi, 0, 0.0, s, M, false, true, s.p * z, l);
+        if (c.key > cut.key || (c.key == cut.key && c.ties < cut.ties)) cut = c;
+    }
+    find_end(src, cut, l);
+    draw(a, r, src, 0, a.V, 0.0, -1.0, cut, s, M, l);
+}
+
+// A row whose kept values are all in the list, of at most FEW values: each is
+// ranked by comparing it with all others, the sums run over the ranks and then
+// over the indices. rest: the sum of e outside the list that top_p is also a
+// share of (without top-k).
+__device__ __forceinline__ void sample_few(const SampleArgs& a, int64_t r, int n, double rest, const Row& s, float M,
+                                           RowLds& l) {
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, at = t & (FEW - 1);
+    const float v = at < n ? l.v[at] : -INFINITY;
+    const bool ok = v > -INFINITY;
+    const uint64_t key = ((uint64_t)(ok ? key_of(v) : 0u) << 32) | (uint32_t)~at;
+    if (t < FEW) {
+        l.w[t] = key;
+        l.n[t] = 0;
+        l.n[FEW + t] = 0x7FFFFFFF;
+    }
+    if (t == 0) l.pick = 0x7FFFFFFF;
+    __syncthreads();
+    int ahead = 0;
+    const int j0 = wave / (FEW / 64) * (FEW * FEW / ROW_THREADS);  // a quarter of the others
+#pragma unroll 8
+    for (int j = 0; j < FEW * FEW / ROW_THREADS; ++j) ahead += l.w[j0 + j] > key;
+    atomicAdd(&l.n[at], (uint32_t)ahead);
+    const double e = ok ? weight(v, M, s.inv_t) : 0.0;
+    __syncthreads();
+    const int rank = (int)l.n[at];
+    double* by_rank = reinterpret_cast<double*>(l.w);
+    if (t < FEW) by_rank[rank] = e;
+    __syncthreads();
+    // the sums over the ranks, by the first waves
+    const bool in = t < FEW && t < s.k;
+    const double scan = wave_scan(in ? by_rank[at] : 0.0);
+    if (lane == 63) l.part[wave] = scan;
+    __syncthreads();
+    double cum = scan, z = 0.0;
+#pragma unroll
+    for (int i = 0; i < FEW / 64; ++i) {
+        if (i < wave) cum += l.part[i];
+        z += l.part[i];
+    }
+    const double own = by_rank[at];
+    if (t < FEW) by_rank[FEW + t] = cum;
+    __syncthreads();
+    const double goal = s.p * (z + rest);
+    const bool keep = in && own > 0.0 && own >= s.m && (t == 0 || s.p >= 1.0 || by_rank[FEW + at - 1] < goal);
+    const uint64_t set = __ballot(keep);
+    if (lane == 0) l.parti[wave] = __popcll(set);
+    __syncthreads();
+    int kept_n = 0;
+#pragma unroll
+    for (int i = 0; i < FEW / 64; ++i) kept_n += l.parti[i];
+    // and over the indices
+    const double w = t < FEW && rank < kept_n ? e : 0.0;
+    const double scan2 = wave_scan(w);
+    if (lane == 63) l.part2[wave] = scan2;
+    __syncthreads();
+    double cum2 = 0.0, total = 0.0;
+#pragma unroll
+    for (int i = 0; i < FEW / 64; ++i) {
+        if (i < wave) cum2 += l.part2[i];
+        total += l.part2[i];
+    }
+    cum2 += scan2;
+    if (w > 0.0) {
+        if (cum2 > s.u * total) atomicMin(&l.pick, t);
+        atomicMin(&l.n[FEW], (uint32_t)(FEW - 1 - t));  // the last
+    }
+    __syncthreads();
+    const int pick = l.pick < FEW ? l.pick : FEW - 1 - (int)l.n[FEW];
+    if (t == pick) {
+        a.tokens[r] = l.i[t];
+        if (a.logprobs) a.logprobs[r] = (float)log(e / total);
+    }
+}
+
+// A row whose kept values are all in the list.
+__device__ __forceinline__ void sample_list(const SampleArgs& a, int64_t r, int n, double rest, const Row& s, float M,
+                                            RowLds& l) {
+    if (n <= FEW) return sample_few(a, r, n, rest, s, M, l);
+    const int t = threadIdx.x;
+    const List list{l.v, l.i, n};
+    float x = -INFINITY, y = INFINITY;
+    for (int i = t; i < n; i += ROW_THREADS)
+        if (l.v[i] > -INFINITY) {
+            x = fmaxf(x, l.v[i]);
+            y = fminf(y, l.v[i]);
+        }
+    block_range(x, y, l);
+    const uint32_t hi = key_of(x), lo = x == INFINITY ? hi : key_of(y);
+    const bool by_k = s.k < n, by_p = s.p < 1.0;
+    Cut cut{0, 1, 1, 0x7FFFFFFF, 0.0, 0.0};
+    double z = 0.0;
+    if (by_p && !by_k) {
+        for (int i = t; i < n; i += ROW_THREADS)
+            if (l.v[i] > -INFINITY) z += weight(l.v[i], M, s.inv_t);
+        z = block_sum(z, l) + rest;
+    }
+#pragma unroll 1
+    for (int step = by_k ? 0 : 1; step < (by_p ? 2 : 1); ++step) {
+        const Cut c = find_cut(list, lo, hi, 0, 0.0, s, M, step == 0, by_p, step == 0 ? (double)s.k : s.p * z, l);
+        if (step == 0) z = c.before + c.ties * c.e;
+        if (c.key > cut.key || (c.key == cut.key && c.ties < cut.ties)) cut = c;
+    }
+    find_end(list, cut, l);
+    draw(a, r, list, 0, n, 0.0, -1.0, cut, s, M, l);
+}
+
+// Rows of at most LIST values: all of them in LDS, one launch.
 template <int TYPE>
 __global__ __launch_bounds__(ROW_THREADS) void k_sample_rows(SampleArgs a) {
     __shared__ RowLds l;
     const int64_t r = blockIdx.x;
-    sample_streaming<TYPE>(a, r, row_of(a, r), l);
+    const Row s = row_of(a, r);
+    const void* row = row_at<TYPE>(a, r);
+    float m = -INFINITY, lowest = INFINITY;
+    for (int i = threadIdx.x; i < a.V; i += ROW_THREADS) {
+        const float v = logit<TYPE>(row, i);
+        l.v[i] = v;
+        l.i[i] = i;
+        m = fmaxf(m, v);  // NaN is skipped
+    }
+    if (threadIdx.x == 0) l.pick = 0x7FFFFFFF;
+    block_range(m, lowest, l);
+    if (m == -INFINITY) return answer(a, r, -1, NAN);
+    if (s.greedy) {
+        for (int i = threadIdx.x; i < a.V; i += ROW_THREADS)
+            if (l.v[i] == m) {
+                atomicMin(&l.pick, i);
+                break;
+            }
+        __syncthreads();
+        return answer(a, r, l.pick, 0.0f);
+    }
+    sample_list(a, r, a.V, 0.0, s, m, l);
+}
+
+// ---- longer rows: a scan by many workgroups, then one that finishes the row ----
+
+// What the scan says of a chunk (a workgroup's values).
+struct Chunk {
+    double sum;    // of the binned e, over the middle of the largest's step
+    double far;    // of e further than the bins below the largest, over the largest's
+    float max;
+    uint32_t top;  // how many values equal it
+};
+
+// The scan's results, per row: every segment's maximum, the chunks, their bins.
+struct Scan {
+    char* base;
+    int64_t row_bytes;
+    int chunk, chunks, segs;
+    __host__ __device__ static int64_t up16(int64_t v) { return (v + 15) / 16 * 16; }
+    __host__ __device__ int64_t at_info() const { return up16((int64_t)segs * 4); }
+    __host__ __device__ int64_t at_bins() const { return at_info() + up16((int64_t)chunks * sizeof(Chunk)); }
+    __host__ __device__ int64_t bytes() const { return at_bins() + (int64_t)chunks * BINS * 8; }
+    __device__ float* seg(int i) const { return reinterpret_cast<float*>(base + i * row_bytes); }
+    __device__ Chunk* info(int i) const { return reinterpret_cast<Chunk*>(base + i * row_bytes + at_info()); }
+    __device__ uint64_t* bins(int i) const { return reinterpret_cast<uint64_t*>(base + i * row_bytes + at_bins()); }
+};
+
+// Whether a row is decided by its segments' maxima: the largest value alone,
+// or a top-k that the segments bound (a larger one with top_p is streamed).
+__device__ __forceinline__ bool by_maxima(const Row& s, int V, int segs) {
+    return s.greedy || (s.k < V && (s.p < 1.0 || s.k <= segs));
+}
+
+// A value's place in steps of e, and its step; v1: the step of 2^(1/8) per
+// unit of the logit.
+__device__ __forceinline__ double per_unit(const Row& s) { return s.inv_t * (8.0 * 1.4426950408889634074); }
+__device__ __forceinline__ double step_of(float v, double unit) { return rint((double)v * unit); }
+// Steps below the largest's (g: step_of(M)); BINS: that or more.
+__device__ __forceinline__ int bin_of(float v, float M, double g, double unit) {
+    if (v == M) return 0;
+    const double d = g - step_of(v, unit);
+    return d < (double)BINS ? (int)d : BINS;
+}
+// The largest's place over the middle of its step, in steps.
+__device__ __forceinline__ double over_step(float M, double g, double unit) {
+    const double d = (double)M * unit - g;
+    return fabs(d) <= 0.5 ? d : 0.0;  // inf - inf: 0
+}
+__device__ __forceinline__ double bin_sum(uint64_t word) {
+    return (double)(uint32_t)(word >> 47) * OFFSET +
+           (double)(word & ((1ull << 47) - 1)) * (1.0 / (double)(1ull << FRAC));
+}
+
+template <int TYPE>
+__device__ __forceinline__ void load4(const void* row, int i, int V, bool vec, float v[4]) {
+    if (vec && i + 4 <= V) {
+        if constexpr (TYPE == FT_TYPE_F32) {
+            const float4 x = *reinterpret_cast<const float4*>(static_cast<const float*>(row) + i);
+            v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+        } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(row) + i);
+            const uint16_t b[4] = {(uint16_t)x.x, (uint16_t)(x.x >> 16), (uint16_t)x.y, (uint16_t)(x.y >> 16)};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = TYPE == FT_TYPE_F16 ? h2f(b[e]) : __uint_as_float((uint32_t)b[e] << 16);
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = i + e < V ? logit<TYPE>(row, i + e) : -INFINITY;
+}
+template <int TYPE>
+__device__ __forceinline__ bool vec_row(const void* row) {
+    return (reinterpret_cast<uintptr_t>(row) & (TYPE == FT_TYPE_F32 ? 15 : 7)) == 0;
+}
+
+// Workgroup (c, row): chunk c of the row in registers, VECS times four values
+// a thread; one pass over memory.
+template <int TYPE, int VECS>
+__global__ __launch_bounds__(1024) void k_sample_scan(SampleArgs a, Scan w, int64_t row0) {
+    __shared__ uint64_t bins[BINS];
+    __shared__ double part[16], part2[16];
+    __shared__ uint32_t top_n;
+    const int t = threadIdx.x, T = blockDim.x, lane = t & 63, wave = t >> 6, waves = T >> 6, c = blockIdx.x;
+    const int64_t r = row0 + blockIdx.y;
+    const void* row = row_at<TYPE>(a, r);
+    const bool vec = vec_row<TYPE>(row);
+    float v[VECS][4];
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) load4<TYPE>(row, c * w.chunk + (i * T + t) * 4, a.V, vec, v[i]);
+    const Row s = row_of(a, r);
+    float m = -INFINITY;
+    float* seg = w.seg(blockIdx.y);
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) {
+        float x = fmaxf(fmaxf(fmaxf(v[i][0], v[i][1]), fmaxf(v[i][2], v[i][3])), -INFINITY);  // NaN is skipped
+        x = fmaxf(x, quad_xor1(x));
+        x = fmaxf(x, quad_xor2(x));
+        x = fmaxf(x, dpp_f<0x141>(x));
+        x = fmaxf(x, dpp_f<0x140>(x));
+        const int at = (c * w.chunk + (i * T + t) * 4) / SEG;
+        if ((lane & 15) == 0 && at < w.segs) seg[at] = x;
+        m = fmaxf(m, x);
+    }
+    if (by_maxima(s, a.V, w.segs)) return;
+    m = wave_max(m);
+    if (lane == 0) part[wave] = m;
+    for (int b = t; b < BINS; b += T) bins[b] = 0;
+    if (t == 0) top_n = 0;
+    __syncthreads();
+    for (int i = 0; i < waves; ++i) m = fmaxf(m, (float)part[i]);
+    __syncthreads();
+    const double unit = per_unit(s), g = step_of(m, unit);
+    double far = 0.0;
+    int top = 0;
+#pragma unroll
+    for (int i = 0; i < VECS; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top += __popcll(__ballot(v[i][e] == m));
+#pragma unroll
+    for (int i = 0; i < VECS; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float x = v[i][e];
+            if (!(x > -INFINITY) || x == m) continue;
+            const double y = (double)x * unit, n = rint(y), d = g - n;
+            if (d < (double)BINS) {
+                // 2^((y - n) / 8) by its series: |q| <= ln 2 / 16, so that q^7 / 5040 is below 2^-44
+                const double q = (y - n) * 0.08664339756999316;
+                const double p =
+                    fma(fma(fma(fma(fma(q, 1.0 / 720, 1.0 / 120), q, 1.0 / 24), q, 1.0 / 6), q, 0.5), q, 1.0);
+                const uint32_t f = (uint32_t)fma(fma(p, q, 1.0 - OFFSET), (double)(1ull << FRAC), 0.5);
+                atomicAdd((unsigned long long*)&bins[(int)d], (1ull << 47) + f);
+            } else {
+                far += weight(x, m, s.inv_t);
+            }
+        }
+    if (lane == 0) atomicAdd(&top_n, (uint32_t)top);
+    __syncthreads();
+    // the chunk's sums, its bins in their order
+    double z = 0.0;
+    uint64_t* out = w.bins(blockIdx.y) + (int64_t)c * BINS;
+    for (int b = t; b < BINS; b += T) {
+        const uint64_t word = bins[b];
+        out[b] = word;
+        if (word) z += bin_sum(word) * exp2(b * -0.125);
+    }
+    z = wave_sum(z);
+    far = wave_sum(far);
+    if (lane == 0) {
+        part[wave] = z;
+        part2[wave] = far;
+    }
+    __syncthreads();
+    if (t == 0) {
+        Chunk k{0.0, 0.0, m, m > -INFINITY ? top_n : 0};
+        for (int i = 0; i < waves; ++i) {
+            k.sum += part[i];
+            k.far += part2[i];
+        }
+        w.info(blockIdx.y)[c] = k;
+    }
+}
+
+// What k_sample_finish keeps beside RowLds.
+struct FinishLds {
+    double cum_w[BINS], scale[BINS];
+    int cum_n[BINS];
+    double sums[MAX_CHUNKS], top_w[MAX_CHUNKS];  // the chunks' kept e, and that of their largest values
+    int top[MAX_CHUNKS], off[MAX_CHUNKS];        // how many these are, and their bin
+    uint16_t open[MAX_SEGS];
+    int cut_lo, cut_hi;
+};
+
+constexpr int SEGS_HELD = 4;  // segments' maxima that a thread keeps
+
+// A wave's segments: a run of `per`, 64 at a time; the first SEGS_HELD times are in registers.
+struct Segs {
+    const float* p;
+    int segs, per, s0;
+    float held[SEGS_HELD];
+    __device__ __forceinline__ void load(const float* seg, int n) {
+        p = seg;
+        segs = n;
+        per = ((n + ROW_WAVES - 1) / ROW_WAVES + 63) / 64 * 64;
+        s0 = (threadIdx.x >> 6) * per + (threadIdx.x & 63);
+#pragma unroll
+        for (int j = 0; j < SEGS_HELD; ++j) held[j] = j * 64 < per && s0 + j * 64 < segs ? p[s0 + j * 64] : -INFINITY;
+    }
+    // fn(segment's maximum (-inf past the end), its number) for each of the thread's, all of a wave's lanes together
+    template <typename F>
+    __device__ __forceinline__ void each(const F& fn) const {
+#pragma unroll
+        for (int j = 0; j < SEGS_HELD; ++j)
+            if (j * 64 < per) fn(held[j], s0 + j * 64);
+        for (int j = SEGS_HELD; j * 64 < per; ++j) fn(s0 + j * 64 < segs ? p[s0 + j * 64] : -INFINITY, s0 + j * 64);
+    }
+};
+
+// The row's values in [from, to], by rising index, into the list, from the
+// segments whose maximum is at least `from`. Returns how many there are; more
+// than LIST: not all were taken.
+template <int TYPE>
+__device__ __forceinline__ int gather(const void* row, int V, const Segs& segs, float from, float to, RowLds& l,
+                                      FinishLds& f) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const bool vec = vec_row<TYPE>(row);
+    const uint64_t below = (1ull << lane) - 1;
+    // the open segments' numbers, in order
+    int mine = 0;
+    segs.each([&](float m, int) { mine += __popcll(__ballot(m > -INFINITY && m >= from)); });
+    if (lane == 0) l.parti[wave] = mine;
+    __syncthreads();
+    int at = 0, count = 0;
+#pragma unroll
+    for (int w = 0; w < ROW_WAVES; ++w) {
+        if (w < wave) at += l.parti[w];
+        count += l.parti[w];
+    }
+    segs.each([&](float m, int k) {
+        const bool in = m > -INFINITY && m >= from;
+        const uint64_t set = __ballot(in);
+        if (in) f.open[at + __popcll(set & below)] = (uint16_t)k;
+        at += __popcll(set);
+    });
+    __syncthreads();
+    // rounds of up to 8 times 4 segments a wave: the waves' runs of a round lie one after the other
+    int n = 0;
+    for (int base = 0; base < count && n <= LIST; base += ROW_WAVES * 32) {
+        const int now = min(count - base, ROW_WAVES * 32), per = (now + ROW_WAVES * 4 - 1) / (ROW_WAVES * 4);
+        float v[8][4];
+        int first[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int k = (wave * per + u) * 4 + (lane >> 4);
+            const bool in = u < per && k < now;
+            first[u] = in ? f.open[base + k] * SEG + (lane & 15) * 4 : 0;
+            if (in) {
+                load4<TYPE>(row, first[u], V, vec, v[u]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[u][e] = -INFINITY;
+            }
+        }
+        int got = 0;
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (!(v[u][e] > -INFINITY && v[u][e] >= from && v[u][e] <= to)) v[u][e] = -INFINITY;
+                got += __popcll(__ballot(v[u][e] > -INFINITY));
+            }
+        __syncthreads();  // the last round's counts are read
+        if (lane == 0) l.parti[wave] = got;
+        __syncthreads();
+        int put = n;
+#pragma unroll
+        for (int w = 0; w < ROW_WAVES; ++w) {
+            if (w < wave) put += l.parti[w];
+            n += l.parti[w];
+        }
+        if (got == 0) continue;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            uint64_t set[4];
+            int before = 0, all = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                set[e] = __ballot(v[u][e] > -INFINITY);
+                before += __popcll(set[e] & below);
+                all += __popcll(set[e]);
+            }
+            int to_at = put + before;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (v[u][e] > -INFINITY) {
+                    if (to_at < LIST) {
+                        l.v[to_at] = v[u][e];
+                        l.i[to_at] = first[u] + e;
+                    }
+                    ++to_at;
+                }
+            put += all;
+        }
+    }
+    __syncthreads();
+    return n;
+}
+
+// A value that at least k of the row's values reach, from the segments' maxima
+// (lowest: the smallest above -inf): k segments have one each. -inf if fewer
+// than k segments hold any.
+__device__ __forceinline__ float reached_by(int k, const Segs& segs, float lowest, float M, RowLds& l) {
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const uint32_t hi = key_of(M), lo = key_of(lowest), width = hi - lo;
+    const int shift = width < 1024u ? 0 : 22 - __clz(width);
+    l.n[t] = 0;
+    if (t == 0) l.pick = 1024;
+    __syncthreads();
+    segs.each([&](float m, int) {
+        if (m > -INFINITY) atomicAdd(&l.n[(hi - key_of(m)) >> shift], 1u);
+    });
+    __syncthreads();
+    int scan = wave_scan_i((int)l.n[t]);
+    if (lane == 63) l.parti[wave] = scan;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < ROW_WAVES; ++w)
+        if (w < wave) scan += l.parti[w];
+    if (scan >= k) atomicMin(&l.pick, t);
+    __syncthreads();
+    const int b = l.pick;
+    __syncthreads();
+    if (b == 1024) return -INFINITY;
+    const uint64_t under = (((uint64_t)b + 1) << shift) - 1;
+    return under >= width ? lowest : of_key(hi - (uint32_t)under);
+}
+
+// The smallest value whose bin is at most b (b < BINS), found 64 keys at a time.
+__device__ __forceinline__ float lowest_in(int b, float M, double g, double unit) {
+    if (M == INFINITY) return M;
+    const int lane = threadIdx.x & 63;
+    uint32_t lo = key_of(-INFINITY) + 1, hi = key_of(M);  // hi is in; the answer is in [lo, hi]
+    while (lo < hi) {
+        const uint32_t step = (hi - lo) / 64 + 1;
+        const uint64_t k = (uint64_t)lo + (uint64_t)lane * step;
+        const bool in = k >= hi || bin_of(of_key((uint32_t)k), M, g, unit) <= b;
+        const uint64_t set = __ballot(in);  // a run of lanes to the last, or none
+        const int first = set ? __ffsll((unsigned long long)set) - 1 : 64;
+        const uint64_t up = (uint64_t)lo + (uint64_t)first * step;
+        if (first > 0) lo = lo + (uint32_t)(first - 1) * step + 1;
+        if (up < hi) hi = (uint32_t)up;
+        if (first == 0) break;
+    }
+    return of_key(hi);
+}
+
+// The chunk that holds the token, among `n` kept sums.
+__device__ __forceinline__ int pick_chunk(const double* sums, int n, double u, double* before, double* total) {
+    double z = 0.0;
+    for (int i = 0; i < n; ++i) z += sums[i];
+    const double goal = u * z;
+    int at = -1, some = 0;
+    double cum = 0.0, some_before = 0.0;
+    for (int i = 0; i < n && at < 0; ++i) {
+        if (sums[i] > 0.0) {
+            some = i;
+            some_before = cum;
+            if (cum + sums[i] > goal) at = i;
+        }
+        cum += sums[i];
+    }
+    *total = z;
+    *before = some_before;
+    return some;
+}
+
+// The rest of a row after the scan, by one workgroup:
+//  - top_k up to the number of segments: the values that k segments' maxima
+//    reach are few and contain the top k; they go into the list, which decides
+//    alone.
+//  - else the bins say on which step of e the order is cut. If all from there
+//    up fit the list, it decides alone; if not, the list holds the steps on
+//    which the cut lies, the bins what is above, and the token's chunk is read
+//    again for the draw.
+//  - where neither fits the list (thousands of equal values, say), or top_k of
+//    thousands meets top_p, the row is streamed.
+template <int TYPE>
+__global__ __launch_bounds__(ROW_THREADS) void k_sample_finish(SampleArgs a, Scan w, int64_t row0) {
+    __shared__ RowLds l;
+    __shared__ FinishLds f;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, V = a.V, chunks = w.chunks;
+    const int64_t r = row0 + blockIdx.x;
+    Segs segs;
+    segs.load(w.seg(blockIdx.x), w.segs);
+    const Row s = row_of(a, r);
+    const void* row = row_at<TYPE>(a, r);
+    float M = -INFINITY, lowest = INFINITY;
+    segs.each([&](float m, int) {
+        M = fmaxf(M, m);
+        if (m > -INFINITY) lowest = fminf(lowest, m);
+    });
+    if (t == 0) l.pick = 0x7FFFFFFF;
+    block_range(M, lowest, l);
+    if (M == -INFINITY) return answer(a, r, -1, NAN);
+    if (s.greedy) {
+        segs.each([&](float m, int k) {
+            if (m == M) atomicMin(&l.pick, k);
+        });
+        __syncthreads();
+        if (wave) return;
+        const int i = l.pick * SEG + lane;
+        const uint64_t set = __ballot(i < V && logit<TYPE>(row, i) == M);
+        return answer(a, r, l.pick * SEG + __ffsll((unsigned long long)set) - 1, 0.0f);
+    }
+    const bool by_k = s.k < V, by_p = s.p < 1.0;
+    float from, to = INFINITY;
+    int first = 0, last = BINS;  // the bins in the list
+    bool all = true;             // the list holds all from the largest on
+    bool too_many = false;       // for the list
+    double rest = 0.0, goal = 0.0;
+    const double unit = per_unit(s), g = step_of(M, unit), ref = over_step(M, g, unit);
+    const uint64_t* bins = w.bins(blockIdx.x);
+    if (by_maxima(s, V, w.segs)) {
+        too_many = s.k > w.segs;
+        from = too_many ? M : reached_by(s.k, segs, lowest, M, l);
+        if (s.m > 0.0 && !by_p) {  // values that min_p may keep; without top_p no sum needs the others
+            const double d = log(s.m) / s.inv_t, x = (double)M + d - 1e-6 * (fabs((double)M) + fabs(d));
+            if (x > (double)from) from = (float)x;
+        }
+    } else {
+        double far = 0.0;
+        for (int c = t; c < chunks; c += ROW_THREADS) {
+            const Chunk k = w.info(blockIdx.x)[c];
+            const bool some = k.max > -INFINITY;
+            const double e = some ? weight(k.max, M, s.inv_t) : 0.0;
+            const double below = k.max == M ? 0.0 : g - step_of(k.max, unit);  // of its step under the largest's
+            f.off[c] = some ? bin_of(k.max, M, g, unit) : BINS;
+            f.top[c] = (int)k.top;
+            f.top_w[c] = k.top * e;
+            f.sums[c] = e > 0.0 ? f.top_w[c] + k.far * e + k.sum * exp2((below + ref) * -0.125) : 0.0;
+            far += k.far * e;
+        }
+        __syncthreads();
+        if (!by_k && !by_p && s.m == 0.0) {
+            double before, total;
+            const int c = pick_chunk(f.sums, chunks, s.u, &before, &total);
+            return draw(a, r, WholeRow<TYPE>{row, V}, c * w.chunk, min(w.chunk, V - c * w.chunk), before, total,
+                        Cut{0, 1, 1, 0x7FFFFFFF, 0.0, 0.0}, s, M, l);
+        }
+        // the chunks' bins as the row's: whole numbers, in any order
+        {
+            const int b = t & (BINS - 1);
+            uint64_t frac = 0;
+            uint32_t n = 0;
+#pragma unroll 8
+            for (int c = t / BINS; c < chunks; c += ROW_THREADS / BINS) {
+                const int j = b - f.off[c];
+                const uint64_t x = j >= 0 ? bins[(int64_t)c * BINS + j] : 0;
+                n += (uint32_t)(x >> 47);
+                frac += x & ((1ull << 47) - 1);
+            }
+            l.n[t] = n;
+            l.w[t] = frac;
+        }
+        if (t == 0) f.cut_lo = f.cut_hi = BINS;
+        __syncthreads();
+        double own_w = 0.0, own_scale = 0.0;
+        int own_n = 0;
+        if (t < BINS) {
+            own_scale = exp2((t + ref) * -0.125);  // the step's middle over the largest e
+            own_n = (int)(l.n[t] + l.n[t + BINS]);
+            own_w = (own_n * OFFSET + (double)(l.w[t] + l.w[t + BINS]) * (1.0 / (double)(1ull << FRAC))) * own_scale;
+            for (int c = 0; c < chunks; ++c)
+                if (f.off[c] == t) {
+                    own_n += f.top[c];
+                    own_w += f.top_w[c];
+                }
+        }
+        const double scan_w = wave_scan(own_w);
+        const int scan_n = wave_scan_i(own_n);
+        if (lane == 63) {
+            l.part[wave] = scan_w;
+            l.parti[wave] = scan_n;
+        }
+        double z = 0.0;
+        for (int c = 0; c < chunks; ++c) z += f.sums[c];
+        __syncthreads();
+        // the steps on which top_k or top_p may cut (sums are right to 1e-9)
+        goal = s.p * z;
+        if (t < BINS) {
+            double x = scan_w;
+            int n = scan_n;
+#pragma unroll
+            for (int i = 0; i < BINS / 64; ++i)
+                if (i < wave) {
+                    x += l.part[i];
+                    n += l.parti[i];
+                }
+            f.cum_w[t] = x;
+            f.cum_n[t] = n;
+            f.scale[t] = own_scale;
+            if (by_p ? x >= goal * (1.0 - 1e-9) : by_k && n >= s.k) atomicMin(&f.cut_lo, t);
+            if (by_p ? x >= goal * (1.0 + 1e-9) : by_k && n >= s.k) atomicMin(&f.cut_hi, t);
+        }
+        __syncthreads();
+        // and min_p: its place below the largest's step, in steps
+        int min_lo = BINS, min_hi = BINS;
+        if (s.m > 0.0) {
+            const double x = log(s.m) * (-8.0 * 1.4426950408889634074) - ref;
+            if (x < (double)BINS - 2) {
+                min_lo = (int)fmax(0.0, rint(x - 1e-6));
+                min_hi = (int)fmax(0.0, rint(x + 1e-6));
+            }
+        }
+        last = min(f.cut_hi, min_hi);
+        all = last >= BINS || f.cum_n[last] <= LIST;
+        first = all ? 0 : min(f.cut_lo, min_lo);
+        if (last >= BINS || f.cum_n[last] - (first ? f.cum_n[first - 1] : 0) > LIST) too_many = true;
+        if (by_p && all) rest = block_sum((t > last ? own_w : 0.0) + far, l);
+        from = too_many ? M : lowest_in(last, M, g, unit);
+        if (first && !too_many) {
+            const uint32_t k = key_of(lowest_in(first - 1, M, g, unit));
+            to = of_key(k == key_of(0.0f) ? k - 2 : k - 1);  // below 0 comes no -0
+        }
+    }
+    const int n = too_many ? LIST + 1 : gather<TYPE>(row, V, segs, from, to, l, f);
+    if (n > LIST) return sample_streaming<TYPE>(a, r, s, M, l);
+    if (all) return sample_list(a, r, n, rest, s, M, l);
+    Cut cut{0, 1, 1, 0x7FFFFFFF, 0.0, 0.0};
+    if (n > 0 && f.cut_lo <= last) {
+        float x = -INFINITY, y = INFINITY;
+        for (int i = t; i < n; i += ROW_THREADS) {
+            x = fmaxf(x, l.v[i]);
+            y = fminf(y, l.v[i]);
+        }
+        block_range(x, y, l);
+        cut = find_cut(List{l.v, l.i, n}, key_of(y), key_of(x), first ? f.cum_n[first - 1] : 0,
+                       first ? f.cum_w[first - 1] : 0.0, s, M, by_k, by_p, by_k ? (double)s.k : goal, l);
+        find_end(List{l.v, l.i, n}, cut, l);
+    }
+    __syncthreads();
+    for (int c = wave; c < chunks; c += ROW_WAVES) {  // the chunks' kept sums
+        double x = 0.0;
+        for (int b = lane; b < first; b += 64) {
+            const int j = b - f.off[c];
+            if (j >= 0) x += bin_sum(bins[(int64_t)c * BINS + j]) * f.scale[b];
+        }
+        if (lane == 0 && f.off[c] < first) x += f.top_w[c];
+        const int i0 = c * w.chunk, i1 = i0 + w.chunk;
+        for (int i = lane; i < n; i += 64)
+            if (l.i[i] >= i0 && l.i[i] < i1) x += kept(l.v[i], l.i[i], cut, s, M);
+        x = wave_sum(x);
+        if (lane == 0) f.sums[c] = x;
+    }
+    __syncthreads();
+    double before, total;
+    const int c = pick_chunk(f.sums, chunks, s.u, &before, &total);
+    draw(a, r, WholeRow<TYPE>{row, V}, c * w.chunk, min(w.chunk, V - c * w.chunk), before, total, cut, s, M, l);
+}
+
+constexpr int SCAN_ROWS = 512;  // rows whose scan the workspace holds
+
+// Values a workgroup of the scan takes: 8192 by 1024 threads where there are
+// few rows, by 256 once such workgroups fill the device.
+bool wide_scan(int64_t vocab, int64_t n) { return vocab * n < (int64_t)1024 * 8192; }
+
+Scan scan_of(int64_t vocab, int64_t n, void* workspace) {
+    Scan w;
+    w.base = static_cast<char*>(workspace);
+    w.chunk = 8192;
+    w.chunks = (int)((vocab + w.chunk - 1) / w.chunk);
+    w.segs = (int)((vocab + SEG - 1) / SEG);
+    w.row_bytes = Scan::up16(w.bytes());
+    return w;
+}
+
+template <int TYPE>
+void launch_sample(const SampleArgs& a, int64_t n, void* workspace, void* stream) {
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (a.V <= LIST) {
+        hipLaunchKernelGGL(k_sample_rows<TYPE>, dim3((unsigned)n), dim3(ROW_THREADS), 0, s, a);
+        return;
+    }
+    const int64_t rows = n < SCAN_ROWS ? n : SCAN_ROWS;
+    const Scan w = scan_of(a.V, rows, workspace);
+    for (int64_t r = 0; r < n; r += rows) {
+        const unsigned now = (unsigned)(n - r < rows ? n - r : rows);
+        const dim3 grid((unsigned)w.chunks, now);
+        if (wide_scan(a.V, rows))
+            hipLaunchKernelGGL((k_sample_scan<TYPE, 2>), grid, dim3(1024), 0, s, a, w, r);
+        else
+            hipLaunchKernelGGL((k_sample_scan<TYPE, 8>), grid, dim3(256), 0, s, a, w, r);
+        hipLaunchKernelGGL(k_sample_finish<TYPE>, dim3(now), dim3(ROW_THREADS), 0, s, a, w, r);
+    }
 }
 
 }  // namespace
 
 extern "C" size_t ft_hip_sample_tokens_workspace_bytes(int64_t vocab, int64_t n) {
     if (vocab <= 0 || vocab > FT_SAMPLE_MAX_VOCAB || n < 0 || n > FT_SAMPLE_MAX_ROWS) return 0;
-    return 256;
+    const int64_t rows = n < SCAN_ROWS ? n : SCAN_ROWS;
+    return vocab <= LIST || n == 0 ? 256 : (size_t)(rows * scan_of(vocab, rows, nullptr).row_bytes);
 }
 
 extern "C" int ft_hip_sample_tokens(ft_hip_ctx* ctx, void* stream, const void* logits, int logits_type,
@@ -404,13 +1178,11 @@ extern "C" int ft_hip_sample_tokens(ft_hip_ctx* ctx, void* stream, const void* l
     const SampleArgs a{logits, logits_stride, (int)vocab, temperature, top_k, top_p, min_p, u, tokens, logprobs};
     DeviceGuard on(ctx->device);
     if (!on.ok) return fail(FT_HIP_E_DEVICE, "sample_tokens: device %d cannot be made current", ctx->device);
-    const dim3 grid((unsigned)n), block(ROW_THREADS);
-    hipStream_t s = static_cast<hipStream_t>(stream);
     if (logits_type == FT_TYPE_F32)
-        hipLaunchKernelGGL(k_sample_rows<FT_TYPE_F32>, grid, block, 0, s, a);
+        launch_sample<FT_TYPE_F32>(a, n, workspace, stream);
     else if (logits_type == FT_TYPE_F16)
-        hipLaunchKernelGGL(k_sample_rows<FT_TYPE_F16>, grid, block, 0, s, a);
+        launch_sample<FT_TYPE_F16>(a, n, workspace, stream);
     else
-        hipLaunchKernelGGL(k_sample_rows<FT_TYPE_BF16>, grid, block, 0, s, a);
+        launch_sample<FT_TYPE_BF16>(a, n, workspace, stream);
     return launch_status("sample_tokens");
 }
