@@ -15,6 +15,7 @@
 
 #include "ft_device.hpp"
 #include "ft_runtime.hpp"
+#include "ft_wave.hpp"
 
 #include <cmath>
 
@@ -94,36 +95,6 @@ __device__ __forceinline__ float of_key(uint32_t k) {
 // exp((l - at) / T) for l <= at; one of several +inf is as good as another.
 __device__ __forceinline__ double weight(float l, float at, double inv_t) {
     return l == at ? 1.0 : at == INFINITY ? 0.0 : exp(((double)l - (double)at) * inv_t);
-}
-
-__device__ __forceinline__ double shfl_f64(double v, int l) {
-    const long long b = __double_as_longlong(v);
-    const int lo = __shfl((int)b, l), hi = __shfl((int)(b >> 32), l);
-    return __longlong_as_double(((long long)hi << 32) | (uint32_t)lo);
-}
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v += shfl_f64(v, (threadIdx.x & 63) ^ o);
-    return v;
-}
-// Sum of lanes 0..lane.
-__device__ __forceinline__ double wave_scan(double v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double x = shfl_f64(v, lane >= o ? lane - o : lane);
-        if (lane >= o) v += x;
-    }
-    return v;
-}
-__device__ __forceinline__ int wave_scan_i(int v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int x = __shfl(v, lane >= o ? lane - o : lane);
-        if (lane >= o) v += x;
-    }
-    return v;
 }
 
 // What a workgroup that finishes a row keeps in LDS.
@@ -207,7 +178,7 @@ __device__ Cut find_cut(const SRC& src, uint32_t lo, uint32_t hi, int base_n, do
                                                  weight(of_key(hi - (uint32_t)last), M, s.inv_t)
                                            : 0.0;
         const double scan_w = wave_scan(own_w);
-        const int scan_n = wave_scan_i(own_n);
+        const int scan_n = wave_scan(own_n);
         if (lane == 63) {
             l.part[wave] = scan_w;
             l.parti[wave] = scan_n;
@@ -287,7 +258,7 @@ __device__ void find_end(const SRC& src, Cut& cut, RowLds& l) {
             if (w < wave) rank += l.parti[w];
             seen += l.parti[w];
         }
-        if (tie && rank + __popcll(set & ((2ull << lane) - 1)) == cut.ties) l.pick = src.index(base + t);
+        if (tie && rank + wave_below(set) + 1 == cut.ties) l.pick = src.index(base + t);
         __syncthreads();
     }
     cut.end = l.pick;
@@ -351,7 +322,7 @@ __device__ void draw(const SampleArgs& a, int64_t r, const SRC& src, int lo, int
     const int i = lo + lane;
     const double e = lane < len ? kept(src.value(i), src.index(i), cut, s, M) : 0.0;
     const double cum = wave_scan(e);
-    if (total < 0.0) total = shfl_f64(cum, 63);
+    if (total < 0.0) total = wave_lane(cum, 63);
     const uint64_t over = __ballot(e > 0.0 && before + cum > s.u * total), any = __ballot(e > 0.0);
     const int at = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)any);
     if (lane == at) {
@@ -360,7 +331,7 @@ __device__ void draw(const SampleArgs& a, int64_t r, const SRC& src, int lo, int
     }
 }
 
-// Sum and maximum over the workgroup, the same in every thread.
+// Sum over the workgroup, the same in every thread.
 __device__ __forceinline__ double block_sum(double z, RowLds& l) {
     z = wave_sum(z);
     if ((threadIdx.x & 63) == 0) l.part[threadIdx.x >> 6] = z;
@@ -370,20 +341,6 @@ __device__ __forceinline__ double block_sum(double z, RowLds& l) {
     __syncthreads();
     return z;
 }
-__device__ __forceinline__ float wave_max(float m) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
-    return m;
-}
-__device__ __forceinline__ float block_max(float m, RowLds& l) {
-    m = wave_max(m);
-    if ((threadIdx.x & 63) == 0) l.part[threadIdx.x >> 6] = m;
-    __syncthreads();
-    for (int i = 0; i < ROW_WAVES; ++i) m = fmaxf(m, (float)l.part[i]);
-    __syncthreads();
-    return m;
-}
-
 __device__ __forceinline__ void answer(const SampleArgs& a, int64_t r, int token, float logprob) {
     if (threadIdx.x == 0) {
         a.tokens[r] = token;
@@ -775,7 +732,6 @@ __device__ __forceinline__ int gather(const void* row, int V, const Segs& segs, 
                                       FinishLds& f) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const bool vec = vec_row<TYPE>(row);
-    const uint64_t below = (1ull << lane) - 1;
     // the open segments' numbers, in order
     int mine = 0;
     segs.each([&](float m, int) { mine += __popcll(__ballot(m > -INFINITY && m >= from)); });
@@ -790,7 +746,7 @@ __device__ __forceinline__ int gather(const void* row, int V, const Segs& segs, 
     segs.each([&](float m, int k) {
         const bool in = m > -INFINITY && m >= from;
         const uint64_t set = __ballot(in);
-        if (in) f.open[at + __popcll(set & below)] = (uint16_t)k;
+        if (in) f.open[at + wave_below(set)] = (uint16_t)k;
         at += __popcll(set);
     });
     __syncthreads();
@@ -802,24 +758,23 @@ __device__ __forceinline__ int gather(const void* row, int V, const Segs& segs, 
         int first[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
+            if (u >= per) break;
             const int k = (wave * per + u) * 4 + (lane >> 4);
-            const bool in = u < per && k < now;
-            first[u] = in ? f.open[base + k] * SEG + (lane & 15) * 4 : 0;
-            if (in) {
-                load4<TYPE>(row, first[u], V, vec, v[u]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[u][e] = -INFINITY;
-            }
+            first[u] = k < now ? f.open[base + k] * SEG + (lane & 15) * 4 : V;
+            load4<TYPE>(row, first[u], V, vec, v[u]);
         }
         int got = 0;
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
+        for (int u = 0; u < 8; ++u) {
+            if (u >= per) break;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                if (!(v[u][e] > -INFINITY && v[u][e] >= from && v[u][e] <= to)) v[u][e] = -INFINITY;
-                got += __popcll(__ballot(v[u][e] > -INFINITY));
+                const bool in = v[u][e] > -INFINITY && v[u][e] >= from && v[u][e] <= to;
+                v[u][e] = in ? v[u][e] : -INFINITY;
+                got += in;
             }
+        }
+        got = wave_sum(got);
         __syncthreads();  // the last round's counts are read
         if (lane == 0) l.parti[wave] = got;
         __syncthreads();
@@ -832,25 +787,24 @@ __device__ __forceinline__ int gather(const void* row, int V, const Segs& segs, 
         if (got == 0) continue;
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
+            if (u >= per) break;
             uint64_t set[4];
-            int before = 0, all = 0;
+            int before = put;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 set[e] = __ballot(v[u][e] > -INFINITY);
-                before += __popcll(set[e] & below);
-                all += __popcll(set[e]);
+                before += wave_below(set[e]);
+                put += __popcll(set[e]);
             }
-            int to_at = put + before;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 if (v[u][e] > -INFINITY) {
-                    if (to_at < LIST) {
-                        l.v[to_at] = v[u][e];
-                        l.i[to_at] = first[u] + e;
+                    if (before < LIST) {
+                        l.v[before] = v[u][e];
+                        l.i[before] = first[u] + e;
                     }
-                    ++to_at;
+                    ++before;
                 }
-            put += all;
         }
     }
     __syncthreads();
@@ -871,7 +825,7 @@ __device__ __forceinline__ float reached_by(int k, const Segs& segs, float lowes
         if (m > -INFINITY) atomicAdd(&l.n[(hi - key_of(m)) >> shift], 1u);
     });
     __syncthreads();
-    int scan = wave_scan_i((int)l.n[t]);
+    int scan = wave_scan((int)l.n[t]);
     if (lane == 63) l.parti[wave] = scan;
     __syncthreads();
 #pragma unroll
@@ -905,23 +859,32 @@ __device__ __forceinline__ float lowest_in(int b, float M, double g, double unit
     return of_key(hi);
 }
 
-// The chunk that holds the token, among `n` kept sums.
-__device__ __forceinline__ int pick_chunk(const double* sums, int n, double u, double* before, double* total) {
+// Sum of `n` values in LDS, the same in every wave.
+__device__ __forceinline__ double sum_of(const double* v, int n) {
     double z = 0.0;
-    for (int i = 0; i < n; ++i) z += sums[i];
-    const double goal = u * z;
-    int at = -1, some = 0;
-    double cum = 0.0, some_before = 0.0;
-    for (int i = 0; i < n && at < 0; ++i) {
-        if (sums[i] > 0.0) {
-            some = i;
-            some_before = cum;
-            if (cum + sums[i] > goal) at = i;
+    for (int i = threadIdx.x & 63; i < n; i += 64) z += v[i];
+    return wave_sum(z);
+}
+
+// The chunk that holds the token, among `n` kept sums; the same in every wave.
+__device__ __forceinline__ int pick_chunk(const double* sums, int n, double u, double* before, double* total) {
+    const int lane = threadIdx.x & 63;
+    const double z = sum_of(sums, n), goal = u * z;
+    double base = 0.0;
+    int some = 0;
+    for (int i = 0; i < n; i += 64) {
+        const double own = i + lane < n ? sums[i + lane] : 0.0;
+        const double cum = base + wave_scan(own), prev = wave_lane_before(cum, base);
+        const uint64_t over = __ballot(own > 0.0 && cum > goal), any = __ballot(own > 0.0);
+        if (any) {
+            const int at = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)any);
+            some = i + at;
+            *before = wave_lane(prev, at);
         }
-        cum += sums[i];
+        if (over) break;
+        base = wave_lane(cum, 63);
     }
     *total = z;
-    *before = some_before;
     return some;
 }
 
@@ -1015,26 +978,28 @@ __global__ __launch_bounds__(ROW_THREADS) void k_sample_finish(SampleArgs a, Sca
         }
         if (t == 0) f.cut_lo = f.cut_hi = BINS;
         __syncthreads();
+        for (int c = t; c < chunks; c += ROW_THREADS)  // and the chunks' largest values
+            if (f.off[c] < BINS) {
+                const double e = f.top_w[c] / f.top[c] * exp2((f.off[c] + ref) * 0.125) - OFFSET;
+                atomicAdd(&l.n[f.off[c]], (uint32_t)f.top[c]);
+                atomicAdd((unsigned long long*)&l.w[f.off[c]],
+                          (uint64_t)f.top[c] * (uint64_t)fma(fmax(e, 0.0), (double)(1ull << FRAC), 0.5));
+            }
+        __syncthreads();
         double own_w = 0.0, own_scale = 0.0;
         int own_n = 0;
         if (t < BINS) {
             own_scale = exp2((t + ref) * -0.125);  // the step's middle over the largest e
             own_n = (int)(l.n[t] + l.n[t + BINS]);
             own_w = (own_n * OFFSET + (double)(l.w[t] + l.w[t + BINS]) * (1.0 / (double)(1ull << FRAC))) * own_scale;
-            for (int c = 0; c < chunks; ++c)
-                if (f.off[c] == t) {
-                    own_n += f.top[c];
-                    own_w += f.top_w[c];
-                }
         }
         const double scan_w = wave_scan(own_w);
-        const int scan_n = wave_scan_i(own_n);
+        const int scan_n = wave_scan(own_n);
         if (lane == 63) {
             l.part[wave] = scan_w;
             l.parti[wave] = scan_n;
         }
-        double z = 0.0;
-        for (int c = 0; c < chunks; ++c) z += f.sums[c];
+        const double z = sum_of(f.sums, chunks);
         __syncthreads();
         // the steps on which top_k or top_p may cut (sums are right to 1e-9)
         goal = s.p * z;
