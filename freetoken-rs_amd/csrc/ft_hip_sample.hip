@@ -17,6 +17,7 @@
 #include "ft_runtime.hpp"
 #include "ft_wave.hpp"
 
+#include <cfloat>
 #include <cmath>
 
 using namespace ft;
@@ -102,10 +103,10 @@ struct RowLds {
     uint64_t w[1024];
     uint32_t n[1024];
     double part[ROW_WAVES];
-    double part2[ROW_WAVES];
     int parti[ROW_WAVES];
     int pick;
-    double at;
+    uint32_t key_hi, key_lo;  // init_range
+    double at, at_w;
     int at_n;
     float v[LIST];  // values taken from the row, by rising index
     int i[LIST];
@@ -209,7 +210,7 @@ __device__ Cut find_cut(const SRC& src, uint32_t lo, uint32_t hi, int base_n, do
         if (t == b) {
             l.at = prev_w;
             l.at_n = prev_n;
-            l.part2[0] = own_w;
+            l.at_w = own_w;
         }
         __syncthreads();
         base_w = l.at;
@@ -218,7 +219,7 @@ __device__ Cut find_cut(const SRC& src, uint32_t lo, uint32_t hi, int base_n, do
         hi -= (uint32_t)b << shift;
         if (here == 1 && shift) {  // the only value of its piece: kept, and all above the piece's end
             const uint32_t span = (1u << shift) - 1;
-            const Cut c{hi - lo > span ? hi - span : lo, 1, 1, 0x7FFFFFFF, base_w, l.part2[0]};
+            const Cut c{hi - lo > span ? hi - span : lo, 1, 1, 0x7FFFFFFF, base_w, l.at_w};
             __syncthreads();
             return c;
         }
@@ -274,6 +275,21 @@ __device__ __forceinline__ double kept(float v, int index, const Cut& cut, const
     return e >= s.m ? e : 0.0;
 }
 
+// Place of the first sum that passes `goal`, `base` before them, and the sum
+// before it; where none does the last place that adds anything. A wave's work:
+// v, its lanes' sums in order. -1: none adds anything.
+__device__ __forceinline__ int pick_lane(double own, double base, double goal, double* before, bool* passed,
+                                         double* after) {
+    const double scan = wave_scan(own), cum = base + scan;
+    const uint64_t over = __ballot(own > 0.0 && cum > goal), any = __ballot(own > 0.0);
+    *after = wave_lane(cum, 63);
+    *passed = over != 0;
+    if (!any) return -1;
+    const int at = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)any);
+    *before = at ? wave_lane(cum, at - 1) : base;
+    return at;
+}
+
 // The draw among the source's places [lo, lo + len), ahead of which the kept
 // sum is `before`; total < 0: [lo, lo + len) is all, and its sum the total.
 // Sixteenths of the range are summed, the one that holds the token is the next
@@ -294,26 +310,10 @@ __device__ void draw(const SampleArgs& a, int64_t r, const SRC& src, int lo, int
             total = 0.0;
             for (int i = 0; i < ROW_WAVES; ++i) total += l.part[i];
         }
-        const double goal = s.u * total;
-        int at = -1, some = 0;
-        double cum = before, at_before = before, some_before = before;
-        for (int i = 0; i < ROW_WAVES; ++i) {
-            const double z = l.part[i];
-            if (z > 0.0) {
-                some = i;
-                some_before = cum;
-            }
-            if (at < 0 && z > 0.0 && cum + z > goal) {
-                at = i;
-                at_before = cum;
-            }
-            cum += z;
-        }
-        if (at < 0) {  // u at 1, or a rounding: the last that holds anything
-            at = some;
-            at_before = some_before;
-        }
-        before = at_before;
+        double here = before, after;
+        bool passed;
+        const int at = max(0, pick_lane(lane < ROW_WAVES ? l.part[lane] : 0.0, before, s.u * total, &here, &passed, &after));
+        before = here;
         len = min(piece, len - at * piece);
         lo += at * piece;
         __syncthreads();
@@ -348,20 +348,24 @@ __device__ __forceinline__ void answer(const SampleArgs& a, int64_t r, int token
     }
 }
 
-// The largest and the smallest value above -inf over the workgroup.
+// The largest and the smallest value above -inf over the workgroup (-inf and
+// anything where there is none). init_range before, and a barrier between.
+__device__ __forceinline__ void init_range(RowLds& l) {
+    if (threadIdx.x == 0) {
+        l.key_hi = 0;
+        l.key_lo = 0xFFFFFFFFu;
+    }
+}
 __device__ __forceinline__ void block_range(float& hi, float& lo, RowLds& l) {
     hi = wave_max(hi);
     lo = -wave_max(-lo);
-    if ((threadIdx.x & 63) == 0) {
-        l.part[threadIdx.x >> 6] = hi;
-        l.part2[threadIdx.x >> 6] = lo;
+    if ((threadIdx.x & 63) == 0 && hi > -INFINITY) {
+        atomicMax(&l.key_hi, key_of(hi));
+        atomicMin(&l.key_lo, key_of(lo));
     }
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < ROW_WAVES; ++i) {
-        hi = fmaxf(hi, (float)l.part[i]);
-        lo = fminf(lo, (float)l.part2[i]);
-    }
+    hi = l.key_hi ? of_key(l.key_hi) : -INFINITY;
+    lo = of_key(l.key_lo);
     __syncthreads();
 }
 
@@ -395,9 +399,9 @@ __device__ __attribute__((noinline)) void sample_streaming(const SampleArgs& a, 
 }
 
 // A row whose kept values are all in the list, of at most FEW values: each is
-// ranked by comparing it with all others, the sums run over the ranks and then
-// over the indices. rest: the sum of e outside the list that top_p is also a
-// share of (without top-k).
+// ranked by comparing it with all others; a wave then sums e over the ranks for
+// the cuts and over the indices for the draw, four places a lane. rest: the sum
+// of e outside the list that top_p is also a share of (without top-k).
 __device__ __forceinline__ void sample_few(const SampleArgs& a, int64_t r, int n, double rest, const Row& s, float M,
                                            RowLds& l) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, at = t & (FEW - 1);
@@ -407,65 +411,61 @@ __device__ __forceinline__ void sample_few(const SampleArgs& a, int64_t r, int n
     if (t < FEW) {
         l.w[t] = key;
         l.n[t] = 0;
-        l.n[FEW + t] = 0x7FFFFFFF;
     }
-    if (t == 0) l.pick = 0x7FFFFFFF;
     __syncthreads();
     int ahead = 0;
     const int j0 = wave / (FEW / 64) * (FEW * FEW / ROW_THREADS);  // a quarter of the others
 #pragma unroll 8
     for (int j = 0; j < FEW * FEW / ROW_THREADS; ++j) ahead += l.w[j0 + j] > key;
     atomicAdd(&l.n[at], (uint32_t)ahead);
-    const double e = ok ? weight(v, M, s.inv_t) : 0.0;
     __syncthreads();
-    const int rank = (int)l.n[at];
     double* by_rank = reinterpret_cast<double*>(l.w);
-    if (t < FEW) by_rank[rank] = e;
-    __syncthreads();
-    // the sums over the ranks, by the first waves
-    const bool in = t < FEW && t < s.k;
-    const double scan = wave_scan(in ? by_rank[at] : 0.0);
-    if (lane == 63) l.part[wave] = scan;
-    __syncthreads();
-    double cum = scan, z = 0.0;
-#pragma unroll
-    for (int i = 0; i < FEW / 64; ++i) {
-        if (i < wave) cum += l.part[i];
-        z += l.part[i];
+    double* by_index = by_rank + FEW;
+    if (t < FEW) {
+        const double e = ok ? weight(v, M, s.inv_t) : 0.0;
+        by_rank[l.n[t]] = e;
+        by_index[t] = e;
     }
-    const double own = by_rank[at];
-    if (t < FEW) by_rank[FEW + t] = cum;
     __syncthreads();
-    const double goal = s.p * (z + rest);
-    const bool keep = in && own > 0.0 && own >= s.m && (t == 0 || s.p >= 1.0 || by_rank[FEW + at - 1] < goal);
-    const uint64_t set = __ballot(keep);
-    if (lane == 0) l.parti[wave] = __popcll(set);
-    __syncthreads();
+    if (wave) return;
+    double e[4], z = 0.0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        e[i] = 4 * lane + i < s.k ? by_rank[4 * lane + i] : 0.0;
+        z += e[i];
+    }
+    const double scan = wave_scan(z), goal = s.p * (wave_lane(scan, 63) + rest);
+    double cum = wave_lane_before(scan, 0.0);
     int kept_n = 0;
 #pragma unroll
-    for (int i = 0; i < FEW / 64; ++i) kept_n += l.parti[i];
-    // and over the indices
-    const double w = t < FEW && rank < kept_n ? e : 0.0;
-    const double scan2 = wave_scan(w);
-    if (lane == 63) l.part2[wave] = scan2;
-    __syncthreads();
-    double cum2 = 0.0, total = 0.0;
+    for (int i = 0; i < 4; ++i) {  // cum: the sum before this one
+        kept_n += e[i] > 0.0 && e[i] >= s.m && (4 * lane + i == 0 || s.p >= 1.0 || cum < goal);
+        cum += e[i];
+    }
+    kept_n = wave_sum(kept_n);
+    double own = 0.0;
 #pragma unroll
-    for (int i = 0; i < FEW / 64; ++i) {
-        if (i < wave) cum2 += l.part2[i];
-        total += l.part2[i];
+    for (int i = 0; i < 4; ++i) {
+        e[i] = (int)l.n[4 * lane + i] < kept_n ? by_index[4 * lane + i] : 0.0;
+        own += e[i];
     }
-    cum2 += scan2;
-    if (w > 0.0) {
-        if (cum2 > s.u * total) atomicMin(&l.pick, t);
-        atomicMin(&l.n[FEW], (uint32_t)(FEW - 1 - t));  // the last
+    const double total = wave_sum(own), draw = s.u * total;
+    double before, after;
+    bool passed;
+    const int p = pick_lane(own, 0.0, draw, &before, &passed, &after);
+    if (lane != p) return;
+    int i = -1;
+    double had = 0.0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (e[j] > 0.0 && (i < 0 || !(before > draw))) {  // to the first that passes, or the last
+            i = j;
+            had = e[j];
+        }
+        before += e[j];
     }
-    __syncthreads();
-    const int pick = l.pick < FEW ? l.pick : FEW - 1 - (int)l.n[FEW];
-    if (t == pick) {
-        a.tokens[r] = l.i[t];
-        if (a.logprobs) a.logprobs[r] = (float)log(e / total);
-    }
+    a.tokens[r] = l.i[4 * lane + i];
+    if (a.logprobs) a.logprobs[r] = (float)log(had / total);
 }
 
 // A row whose kept values are all in the list.
@@ -474,7 +474,9 @@ __device__ __forceinline__ void sample_list(const SampleArgs& a, int64_t r, int 
     if (n <= FEW) return sample_few(a, r, n, rest, s, M, l);
     const int t = threadIdx.x;
     const List list{l.v, l.i, n};
+    init_range(l);
     float x = -INFINITY, y = INFINITY;
+    __syncthreads();
     for (int i = t; i < n; i += ROW_THREADS)
         if (l.v[i] > -INFINITY) {
             x = fmaxf(x, l.v[i]);
@@ -507,12 +509,15 @@ __global__ __launch_bounds__(ROW_THREADS) void k_sample_rows(SampleArgs a) {
     const int64_t r = blockIdx.x;
     const Row s = row_of(a, r);
     const void* row = row_at<TYPE>(a, r);
+    init_range(l);
+    __syncthreads();
     float m = -INFINITY, lowest = INFINITY;
     for (int i = threadIdx.x; i < a.V; i += ROW_THREADS) {
         const float v = logit<TYPE>(row, i);
         l.v[i] = v;
         l.i[i] = i;
         m = fmaxf(m, v);  // NaN is skipped
+        if (v > -INFINITY) lowest = fminf(lowest, v);
     }
     if (threadIdx.x == 0) l.pick = 0x7FFFFFFF;
     block_range(m, lowest, l);
@@ -694,7 +699,9 @@ struct FinishLds {
     double cum_w[BINS], scale[BINS];
     int cum_n[BINS];
     double sums[MAX_CHUNKS], top_w[MAX_CHUNKS];  // the chunks' kept e, and that of their largest values
-    int top[MAX_CHUNKS], off[MAX_CHUNKS];        // how many these are, and their bin
+    uint64_t top_f[MAX_CHUNKS];                  // one such e as a bin holds it
+    uint32_t top[MAX_CHUNKS];                    // how many these are
+    int off[MAX_CHUNKS];                         // and their bin
     uint16_t open[MAX_SEGS];
     int cut_lo, cut_hi;
 };
@@ -724,6 +731,14 @@ struct Segs {
     }
 };
 
+// The sum of the waves' counts before this wave's, and of all.
+__device__ __forceinline__ void waves_before(const int* counts, int& before, int& all) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int own = lane < ROW_WAVES ? counts[lane] : 0, scan = wave_scan(own);
+    before = wave_lane(scan - own, wave);
+    all = wave_lane(scan, 63);
+}
+
 // The row's values in [from, to], by rising index, into the list, from the
 // segments whose maximum is at least `from`. Returns how many there are; more
 // than LIST: not all were taken.
@@ -732,19 +747,16 @@ __device__ __forceinline__ int gather(const void* row, int V, const Segs& segs, 
                                       FinishLds& f) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const bool vec = vec_row<TYPE>(row);
+    from = fmaxf(from, -FLT_MAX);
     // the open segments' numbers, in order
     int mine = 0;
-    segs.each([&](float m, int) { mine += __popcll(__ballot(m > -INFINITY && m >= from)); });
+    segs.each([&](float m, int) { mine += __popcll(__ballot(m >= from)); });
     if (lane == 0) l.parti[wave] = mine;
     __syncthreads();
-    int at = 0, count = 0;
-#pragma unroll
-    for (int w = 0; w < ROW_WAVES; ++w) {
-        if (w < wave) at += l.parti[w];
-        count += l.parti[w];
-    }
+    int at, count;
+    waves_before(l.parti, at, count);
     segs.each([&](float m, int k) {
-        const bool in = m > -INFINITY && m >= from;
+        const bool in = m >= from;
         const uint64_t set = __ballot(in);
         if (in) f.open[at + wave_below(set)] = (uint16_t)k;
         at += __popcll(set);
@@ -763,47 +775,45 @@ __device__ __forceinline__ int gather(const void* row, int V, const Segs& segs, 
             first[u] = k < now ? f.open[base + k] * SEG + (lane & 15) * 4 : V;
             load4<TYPE>(row, first[u], V, vec, v[u]);
         }
-        int got = 0;
+        uint32_t mask = 0;  // bit 4 u + e
+        int own[3] = {0, 0, 0};  // how many by u, 10 bits each
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             if (u >= per) break;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const bool in = v[u][e] > -INFINITY && v[u][e] >= from && v[u][e] <= to;
-                v[u][e] = in ? v[u][e] : -INFINITY;
-                got += in;
-            }
+            for (int e = 0; e < 4; ++e)
+                mask |= v[u][e] == __builtin_amdgcn_fmed3f(v[u][e], from, to) ? 1u << (4 * u + e) : 0u;
+            own[u / 3] |= __popc(mask >> (4 * u)) << (10 * (u % 3));
         }
-        got = wave_sum(got);
+        int lower[3], all[3], got = 0;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            const int scan = wave_scan(own[i]);
+            lower[i] = scan - own[i];
+            all[i] = wave_lane(scan, 63);
+            got += (all[i] & 1023) + (all[i] >> 10 & 1023) + (all[i] >> 20);
+        }
         __syncthreads();  // the last round's counts are read
         if (lane == 0) l.parti[wave] = got;
         __syncthreads();
-        int put = n;
-#pragma unroll
-        for (int w = 0; w < ROW_WAVES; ++w) {
-            if (w < wave) put += l.parti[w];
-            n += l.parti[w];
-        }
+        int put, more;
+        waves_before(l.parti, put, more);
+        put += n;
+        n += more;
         if (got == 0) continue;
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             if (u >= per) break;
-            uint64_t set[4];
-            int before = put;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                set[e] = __ballot(v[u][e] > -INFINITY);
-                before += wave_below(set[e]);
-                put += __popcll(set[e]);
-            }
+            int to_at = put + (lower[u / 3] >> (10 * (u % 3)) & 1023);
+            put += all[u / 3] >> (10 * (u % 3)) & 1023;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (v[u][e] > -INFINITY) {
-                    if (before < LIST) {
-                        l.v[before] = v[u][e];
-                        l.i[before] = first[u] + e;
+                if (mask >> (4 * u + e) & 1) {
+                    if (to_at < LIST) {
+                        l.v[to_at] = v[u][e];
+                        l.i[to_at] = first[u] + e;
                     }
-                    ++before;
+                    ++to_at;
                 }
         }
     }
@@ -813,29 +823,26 @@ __device__ __forceinline__ int gather(const void* row, int V, const Segs& segs, 
 
 // A value that at least k of the row's values reach, from the segments' maxima
 // (lowest: the smallest above -inf): k segments have one each. -inf if fewer
-// than k segments hold any.
+// than k segments hold any. l.n[0..256) is 0 on entry.
 __device__ __forceinline__ float reached_by(int k, const Segs& segs, float lowest, float M, RowLds& l) {
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const uint32_t hi = key_of(M), lo = key_of(lowest), width = hi - lo;
-    const int shift = width < 1024u ? 0 : 22 - __clz(width);
-    l.n[t] = 0;
-    if (t == 0) l.pick = 1024;
-    __syncthreads();
+    const int lane = threadIdx.x & 63;
+    const uint32_t hi = key_of(M), width = hi - key_of(lowest);
+    const int shift = width < 256u ? 0 : 24 - __clz(width);
     segs.each([&](float m, int) {
         if (m > -INFINITY) atomicAdd(&l.n[(hi - key_of(m)) >> shift], 1u);
     });
     __syncthreads();
-    int scan = wave_scan((int)l.n[t]);
-    if (lane == 63) l.parti[wave] = scan;
-    __syncthreads();
+    int own[4], sum = 0;  // bins 4 lane ..
 #pragma unroll
-    for (int w = 0; w < ROW_WAVES; ++w)
-        if (w < wave) scan += l.parti[w];
-    if (scan >= k) atomicMin(&l.pick, t);
-    __syncthreads();
-    const int b = l.pick;
-    __syncthreads();
-    if (b == 1024) return -INFINITY;
+    for (int i = 0; i < 4; ++i) sum += own[i] = (int)l.n[4 * lane + i];
+    const int scan = wave_scan(sum);
+    const uint64_t set = __ballot(scan >= k);
+    if (!set) return -INFINITY;
+    const int at = __ffsll((unsigned long long)set) - 1;
+    int cum = scan - sum, b = 0;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) b += (cum += own[i]) < k;
+    b = 4 * at + wave_lane(b, at);
     const uint64_t under = (((uint64_t)b + 1) << shift) - 1;
     return under >= width ? lowest : of_key(hi - (uint32_t)under);
 }
@@ -869,22 +876,19 @@ __device__ __forceinline__ double sum_of(const double* v, int n) {
 // The chunk that holds the token, among `n` kept sums; the same in every wave.
 __device__ __forceinline__ int pick_chunk(const double* sums, int n, double u, double* before, double* total) {
     const int lane = threadIdx.x & 63;
-    const double z = sum_of(sums, n), goal = u * z;
+    *total = sum_of(sums, n);
     double base = 0.0;
     int some = 0;
-    for (int i = 0; i < n; i += 64) {
-        const double own = i + lane < n ? sums[i + lane] : 0.0;
-        const double cum = base + wave_scan(own), prev = wave_lane_before(cum, base);
-        const uint64_t over = __ballot(own > 0.0 && cum > goal), any = __ballot(own > 0.0);
-        if (any) {
-            const int at = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)any);
+    bool passed = false;
+    for (int i = 0; i < n && !passed; i += 64) {
+        double here, after;
+        const int at = pick_lane(i + lane < n ? sums[i + lane] : 0.0, base, u * *total, &here, &passed, &after);
+        if (at >= 0) {
             some = i + at;
-            *before = wave_lane(prev, at);
+            *before = here;
         }
-        if (over) break;
-        base = wave_lane(cum, 63);
+        base = after;
     }
-    *total = z;
     return some;
 }
 
@@ -906,14 +910,17 @@ __global__ __launch_bounds__(ROW_THREADS) void k_sample_finish(SampleArgs a, Sca
     const int64_t r = row0 + blockIdx.x;
     Segs segs;
     segs.load(w.seg(blockIdx.x), w.segs);
+    init_range(l);
+    if (t == 0) l.pick = 0x7FFFFFFF;
+    if (t < 256) l.n[t] = 0;
     const Row s = row_of(a, r);
+    __syncthreads();
     const void* row = row_at<TYPE>(a, r);
     float M = -INFINITY, lowest = INFINITY;
     segs.each([&](float m, int) {
         M = fmaxf(M, m);
         if (m > -INFINITY) lowest = fminf(lowest, m);
     });
-    if (t == 0) l.pick = 0x7FFFFFFF;
     block_range(M, lowest, l);
     if (M == -INFINITY) return answer(a, r, -1, NAN);
     if (s.greedy) {
@@ -949,7 +956,10 @@ __global__ __launch_bounds__(ROW_THREADS) void k_sample_finish(SampleArgs a, Sca
             const double e = some ? weight(k.max, M, s.inv_t) : 0.0;
             const double below = k.max == M ? 0.0 : g - step_of(k.max, unit);  // of its step under the largest's
             f.off[c] = some ? bin_of(k.max, M, g, unit) : BINS;
-            f.top[c] = (int)k.top;
+            f.top[c] = k.top;
+            f.top_f[c] = some && k.max < INFINITY && f.off[c] < BINS
+                             ? (uint64_t)fma(fmax(e * exp2((f.off[c] + ref) * 0.125) - OFFSET, 0.0), (double)(1ull << FRAC), 0.5)
+                             : 0;
             f.top_w[c] = k.top * e;
             f.sums[c] = e > 0.0 ? f.top_w[c] + k.far * e + k.sum * exp2((below + ref) * -0.125) : 0.0;
             far += k.far * e;
@@ -970,53 +980,41 @@ __global__ __launch_bounds__(ROW_THREADS) void k_sample_finish(SampleArgs a, Sca
             for (int c = t / BINS; c < chunks; c += ROW_THREADS / BINS) {
                 const int j = b - f.off[c];
                 const uint64_t x = j >= 0 ? bins[(int64_t)c * BINS + j] : 0;
-                n += (uint32_t)(x >> 47);
-                frac += x & ((1ull << 47) - 1);
+                n += (uint32_t)(x >> 47) + (j == 0 ? f.top[c] : 0);
+                frac += (x & ((1ull << 47) - 1)) + (j == 0 ? f.top[c] * f.top_f[c] : 0);
             }
             l.n[t] = n;
             l.w[t] = frac;
         }
         if (t == 0) f.cut_lo = f.cut_hi = BINS;
         __syncthreads();
-        for (int c = t; c < chunks; c += ROW_THREADS)  // and the chunks' largest values
-            if (f.off[c] < BINS) {
-                const double e = f.top_w[c] / f.top[c] * exp2((f.off[c] + ref) * 0.125) - OFFSET;
-                atomicAdd(&l.n[f.off[c]], (uint32_t)f.top[c]);
-                atomicAdd((unsigned long long*)&l.w[f.off[c]],
-                          (uint64_t)f.top[c] * (uint64_t)fma(fmax(e, 0.0), (double)(1ull << FRAC), 0.5));
-            }
-        __syncthreads();
-        double own_w = 0.0, own_scale = 0.0;
-        int own_n = 0;
-        if (t < BINS) {
-            own_scale = exp2((t + ref) * -0.125);  // the step's middle over the largest e
-            own_n = (int)(l.n[t] + l.n[t + BINS]);
-            own_w = (own_n * OFFSET + (double)(l.w[t] + l.w[t + BINS]) * (1.0 / (double)(1ull << FRAC))) * own_scale;
-        }
-        const double scan_w = wave_scan(own_w);
-        const int scan_n = wave_scan(own_n);
-        if (lane == 63) {
-            l.part[wave] = scan_w;
-            l.parti[wave] = scan_n;
-        }
         const double z = sum_of(f.sums, chunks);
-        __syncthreads();
-        // the steps on which top_k or top_p may cut (sums are right to 1e-9)
         goal = s.p * z;
-        if (t < BINS) {
-            double x = scan_w;
-            int n = scan_n;
+        if (wave == 0) {  // the bins' running sums, 8 to a lane, and the steps on which top_k or top_p may cut
+            double x[8], sum = 0.0, scale = exp2((8 * lane + ref) * -0.125);  // a step's middle over the largest e
+            int n[8], count = 0;
 #pragma unroll
-            for (int i = 0; i < BINS / 64; ++i)
-                if (i < wave) {
-                    x += l.part[i];
-                    n += l.parti[i];
-                }
-            f.cum_w[t] = x;
-            f.cum_n[t] = n;
-            f.scale[t] = own_scale;
-            if (by_p ? x >= goal * (1.0 - 1e-9) : by_k && n >= s.k) atomicMin(&f.cut_lo, t);
-            if (by_p ? x >= goal * (1.0 + 1e-9) : by_k && n >= s.k) atomicMin(&f.cut_hi, t);
+            for (int i = 0; i < 8; ++i) {
+                const int b = 8 * lane + i;
+                n[i] = (int)(l.n[b] + l.n[b + BINS]);
+                x[i] = (n[i] * OFFSET + (double)(l.w[b] + l.w[b + BINS]) * (1.0 / (double)(1ull << FRAC))) * scale;
+                f.scale[b] = scale;
+                scale *= 0.91700404320467123;  // 2^(-1/8)
+                sum += x[i];
+                count += n[i];
+            }
+            double cum = wave_lane_before(wave_scan(sum), 0.0);
+            int cum_n = wave_scan(count) - count, lo = BINS, hi = BINS;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {  // (sums are right to 1e-9)
+                const int b = 8 * lane + i;
+                f.cum_w[b] = cum += x[i];
+                f.cum_n[b] = cum_n += n[i];
+                if (lo == BINS && (by_p ? cum >= goal * (1.0 - 1e-9) : by_k && cum_n >= s.k)) lo = b;
+                if (hi == BINS && (by_p ? cum >= goal * (1.0 + 1e-9) : by_k && cum_n >= s.k)) hi = b;
+            }
+            if (lo < BINS) atomicMin(&f.cut_lo, lo);
+            if (hi < BINS) atomicMin(&f.cut_hi, hi);
         }
         __syncthreads();
         // and min_p: its place below the largest's step, in steps
@@ -1032,7 +1030,13 @@ __global__ __launch_bounds__(ROW_THREADS) void k_sample_finish(SampleArgs a, Sca
         all = last >= BINS || f.cum_n[last] <= LIST;
         first = all ? 0 : min(f.cut_lo, min_lo);
         if (last >= BINS || f.cum_n[last] - (first ? f.cum_n[first - 1] : 0) > LIST) too_many = true;
-        if (by_p && all) rest = block_sum((t > last ? own_w : 0.0) + far, l);
+        if (by_p && all) {
+            double x = far;
+            if (t > last && t < BINS)
+                x += ((l.n[t] + l.n[t + BINS]) * OFFSET +
+                      (double)(l.w[t] + l.w[t + BINS]) * (1.0 / (double)(1ull << FRAC))) * f.scale[t];
+            rest = block_sum(x, l);
+        }
         from = too_many ? M : lowest_in(last, M, g, unit);
         if (first && !too_many) {
             const uint32_t k = key_of(lowest_in(first - 1, M, g, unit));
@@ -1044,6 +1048,8 @@ __global__ __launch_bounds__(ROW_THREADS) void k_sample_finish(SampleArgs a, Sca
     if (all) return sample_list(a, r, n, rest, s, M, l);
     Cut cut{0, 1, 1, 0x7FFFFFFF, 0.0, 0.0};
     if (n > 0 && f.cut_lo <= last) {
+        init_range(l);
+        __syncthreads();
         float x = -INFINITY, y = INFINITY;
         for (int i = t; i < n; i += ROW_THREADS) {
             x = fmaxf(x, l.v[i]);
