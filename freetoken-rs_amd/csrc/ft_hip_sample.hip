@@ -52,7 +52,9 @@ struct SampleArgs {
     const float* u;
     int32_t* tokens;
     float* logprobs;
+    int given;  // HAS_*
 };
+enum { HAS_T = 1, HAS_K = 2, HAS_P = 4, HAS_M = 8 };
 
 // A row's settings, with what is out of range brought into it.
 struct Row {
@@ -61,18 +63,18 @@ struct Row {
     bool greedy;
 };
 
+// The settings that are not given come as `u`, so that all are loaded at once.
 __device__ __forceinline__ Row row_of(const SampleArgs& a, int64_t r) {
+    const float t_in = a.temperature[r], p_in = a.top_p[r], m_in = a.min_p[r], u = a.u[r];
+    const int k_in = a.top_k[r];
+    const float t = a.given & HAS_T ? t_in : 1.0f, p = a.given & HAS_P ? p_in : 1.0f, m = a.given & HAS_M ? m_in : 0.0f;
+    const int k = a.given & HAS_K ? k_in : 0;
     Row s;
-    const float t = a.temperature ? a.temperature[r] : 1.0f;
     s.greedy = !(t > 0.0f);
     s.inv_t = s.greedy ? 1.0 : 1.0 / (double)t;
-    const int k = a.top_k ? a.top_k[r] : 0;
     s.k = k > 0 && k < a.V ? k : a.V;
-    const float p = a.top_p ? a.top_p[r] : 1.0f;
     s.p = p < 1.0f ? fmax((double)p, 0.0) : 1.0;  // NaN: off
-    const float m = a.min_p ? a.min_p[r] : 0.0f;
     s.m = m > 0.0f ? fmin((double)m, 1.0) : 0.0;  // NaN: off
-    const float u = a.u[r];
     s.u = u > 0.0f ? fmin((double)u, 1.0) : 0.0;
     return s;
 }
@@ -644,6 +646,7 @@ __global__ __launch_bounds__(1024) void k_sample_scan(SampleArgs a, Scan w, int6
     __syncthreads();
     const double unit = per_unit(s), g = step_of(m, unit);
     double far = 0.0;
+    bool beyond = false;
     int top = 0;
 #pragma unroll
     for (int i = 0; i < VECS; ++i)
@@ -654,19 +657,26 @@ __global__ __launch_bounds__(1024) void k_sample_scan(SampleArgs a, Scan w, int6
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float x = v[i][e];
-            if (!(x > -INFINITY) || x == m) continue;
             const double y = (double)x * unit, n = rint(y), d = g - n;
-            if (d < (double)BINS) {
-                // 2^((y - n) / 8) by its series: |q| <= ln 2 / 16, so that q^7 / 5040 is below 2^-44
-                const double q = (y - n) * 0.08664339756999316;
-                const double p =
-                    fma(fma(fma(fma(fma(q, 1.0 / 720, 1.0 / 120), q, 1.0 / 24), q, 1.0 / 6), q, 0.5), q, 1.0);
+            // 2^((y - n) / 8) by its series: |q| <= ln 2 / 16, so that q^7 / 5040 is below 2^-44
+            const double q = (y - n) * 0.08664339756999316;
+            const double p = fma(fma(fma(fma(fma(q, 1.0 / 720, 1.0 / 120), q, 1.0 / 24), q, 1.0 / 6), q, 0.5), q, 1.0);
+            if (x < m && d < (double)BINS) {  // false for NaN and -inf
                 const uint32_t f = (uint32_t)fma(fma(p, q, 1.0 - OFFSET), (double)(1ull << FRAC), 0.5);
                 atomicAdd((unsigned long long*)&bins[(int)d], (1ull << 47) + f);
             } else {
-                far += weight(x, m, s.inv_t);
+                beyond |= x < m && x > -INFINITY;
             }
         }
+    if (__ballot(beyond)) {  // few in most rows
+#pragma unroll
+        for (int i = 0; i < VECS; ++i)
+#pragma unroll 1
+            for (int e = 0; e < 4; ++e) {
+                const float x = e == 0 ? v[i][0] : e == 1 ? v[i][1] : e == 2 ? v[i][2] : v[i][3];
+                if (x < m && x > -INFINITY && !(g - step_of(x, unit) < (double)BINS)) far += weight(x, m, s.inv_t);
+            }
+    }
     if (lane == 0) atomicAdd(&top_n, (uint32_t)top);
     __syncthreads();
     // the chunk's sums, its bins in their order
@@ -762,19 +772,34 @@ __device__ __forceinline__ int gather(const void* row, int V, const Segs& segs, 
         at += __popcll(set);
     });
     __syncthreads();
-    // rounds of up to 8 times 4 segments a wave: the waves' runs of a round lie one after the other
-    int n = 0;
-    for (int base = 0; base < count && n <= LIST; base += ROW_WAVES * 32) {
+    // rounds of up to 8 times 4 segments a wave, the next round's loads ahead: the waves' runs of a round lie one after
+    // the other
+    float ahead[8][4];
+    int ahead_i[8];
+    const auto load = [&](int base) {
         const int now = min(count - base, ROW_WAVES * 32), per = (now + ROW_WAVES * 4 - 1) / (ROW_WAVES * 4);
-        float v[8][4];
-        int first[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             if (u >= per) break;
             const int k = (wave * per + u) * 4 + (lane >> 4);
-            first[u] = k < now ? f.open[base + k] * SEG + (lane & 15) * 4 : V;
-            load4<TYPE>(row, first[u], V, vec, v[u]);
+            ahead_i[u] = k < now ? f.open[base + k] * SEG + (lane & 15) * 4 : V;
+            load4<TYPE>(row, ahead_i[u], V, vec, ahead[u]);
         }
+        return per;
+    };
+    int n = 0, next = load(0);
+    for (int base = 0; base < count && n <= LIST; base += ROW_WAVES * 32) {
+        float v[8][4];
+        int first[8];
+        const int per = next;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            if (u >= per) break;
+            first[u] = ahead_i[u];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[u][e] = ahead[u][e];
+        }
+        if (base + ROW_WAVES * 32 < count) next = load(base + ROW_WAVES * 32);
         uint32_t mask = 0;  // bit 4 u + e
         int own[3] = {0, 0, 0};  // how many by u, 10 bits each
 #pragma unroll
@@ -804,16 +829,16 @@ __device__ __forceinline__ int gather(const void* row, int V, const Segs& segs, 
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             if (u >= per) break;
-            int to_at = put + (lower[u / 3] >> (10 * (u % 3)) & 1023);
+            int at = put + (lower[u / 3] >> (10 * (u % 3)) & 1023);
             put += all[u / 3] >> (10 * (u % 3)) & 1023;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 if (mask >> (4 * u + e) & 1) {
-                    if (to_at < LIST) {
-                        l.v[to_at] = v[u][e];
-                        l.i[to_at] = first[u] + e;
+                    if (at < LIST) {
+                        l.v[at] = v[u][e];
+                        l.i[at] = first[u] + e;
                     }
-                    ++to_at;
+                    ++at;
                 }
         }
     }
@@ -890,6 +915,20 @@ __device__ __forceinline__ int pick_chunk(const double* sums, int n, double u, d
         base = after;
     }
     return some;
+}
+
+// How many of the n rising numbers are below x, found 64 places at a time.
+__device__ __forceinline__ int run_end(const int* v, int n, int x) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, hi = n;  // the answer is in [lo, hi]
+    while (lo < hi) {
+        const int step = (hi - lo) / 64 + 1, at = lo + lane * step;
+        const uint64_t below = __ballot(at < hi && v[at] < x);  // a run from lane 0, or none
+        const int many = __popcll(below);
+        hi = min(hi, lo + many * step);
+        if (many) lo += (many - 1) * step + 1;
+    }
+    return lo;
 }
 
 // The rest of a row after the scan, by one workgroup:
@@ -988,33 +1027,36 @@ __global__ __launch_bounds__(ROW_THREADS) void k_sample_finish(SampleArgs a, Sca
         }
         if (t == 0) f.cut_lo = f.cut_hi = BINS;
         __syncthreads();
+        // the bins' running sums, and the steps on which top_k or top_p may cut (sums are right to 1e-9)
+        double own_w = 0.0;
+        int own_n = 0;
+        if (t < BINS) {
+            f.scale[t] = exp2((t + ref) * -0.125);  // a step's middle over the largest e
+            own_n = (int)(l.n[t] + l.n[t + BINS]);
+            own_w = (own_n * OFFSET + (double)(l.w[t] + l.w[t + BINS]) * (1.0 / (double)(1ull << FRAC))) * f.scale[t];
+        }
+        const double scan_w = wave_scan(own_w);
+        const int scan_n = wave_scan(own_n);
+        if (lane == 63) {
+            l.part[wave] = scan_w;
+            l.parti[wave] = scan_n;
+        }
         const double z = sum_of(f.sums, chunks);
         goal = s.p * z;
-        if (wave == 0) {  // the bins' running sums, 8 to a lane, and the steps on which top_k or top_p may cut
-            double x[8], sum = 0.0, scale = exp2((8 * lane + ref) * -0.125);  // a step's middle over the largest e
-            int n[8], count = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int b = 8 * lane + i;
-                n[i] = (int)(l.n[b] + l.n[b + BINS]);
-                x[i] = (n[i] * OFFSET + (double)(l.w[b] + l.w[b + BINS]) * (1.0 / (double)(1ull << FRAC))) * scale;
-                f.scale[b] = scale;
-                scale *= 0.91700404320467123;  // 2^(-1/8)
-                sum += x[i];
-                count += n[i];
-            }
-            double cum = wave_lane_before(wave_scan(sum), 0.0);
-            int cum_n = wave_scan(count) - count, lo = BINS, hi = BINS;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {  // (sums are right to 1e-9)
-                const int b = 8 * lane + i;
-                f.cum_w[b] = cum += x[i];
-                f.cum_n[b] = cum_n += n[i];
-                if (lo == BINS && (by_p ? cum >= goal * (1.0 - 1e-9) : by_k && cum_n >= s.k)) lo = b;
-                if (hi == BINS && (by_p ? cum >= goal * (1.0 + 1e-9) : by_k && cum_n >= s.k)) hi = b;
-            }
-            if (lo < BINS) atomicMin(&f.cut_lo, lo);
-            if (hi < BINS) atomicMin(&f.cut_hi, hi);
+        __syncthreads();
+        if (t < BINS) {
+            int n, every;
+            waves_before(l.parti, n, every);
+            const double part = lane < ROW_WAVES ? l.part[lane] : 0.0, parts = wave_scan(part);
+            const int up = __builtin_amdgcn_readfirstlane(wave);
+            const double c = scan_w + (up ? wave_lane(parts, up - 1) : 0.0);
+            n += scan_n;
+            f.cum_w[t] = c;
+            f.cum_n[t] = n;
+            const uint64_t lo = __ballot(by_p ? c >= goal * (1.0 - 1e-9) : by_k && n >= s.k);
+            const uint64_t hi = __ballot(by_p ? c >= goal * (1.0 + 1e-9) : by_k && n >= s.k);
+            if (lane == 0 && lo) atomicMin(&f.cut_lo, t + __ffsll((unsigned long long)lo) - 1);
+            if (lane == 0 && hi) atomicMin(&f.cut_hi, t + __ffsll((unsigned long long)hi) - 1);
         }
         __syncthreads();
         // and min_p: its place below the largest's step, in steps
@@ -1032,9 +1074,7 @@ __global__ __launch_bounds__(ROW_THREADS) void k_sample_finish(SampleArgs a, Sca
         if (last >= BINS || f.cum_n[last] - (first ? f.cum_n[first - 1] : 0) > LIST) too_many = true;
         if (by_p && all) {
             double x = far;
-            if (t > last && t < BINS)
-                x += ((l.n[t] + l.n[t + BINS]) * OFFSET +
-                      (double)(l.w[t] + l.w[t + BINS]) * (1.0 / (double)(1ull << FRAC))) * f.scale[t];
+            if (t > last) x += own_w;
             rest = block_sum(x, l);
         }
         from = too_many ? M : lowest_in(last, M, g, unit);
@@ -1068,9 +1108,8 @@ __global__ __launch_bounds__(ROW_THREADS) void k_sample_finish(SampleArgs a, Sca
             if (j >= 0) x += bin_sum(bins[(int64_t)c * BINS + j]) * f.scale[b];
         }
         if (lane == 0 && f.off[c] < first) x += f.top_w[c];
-        const int i0 = c * w.chunk, i1 = i0 + w.chunk;
-        for (int i = lane; i < n; i += 64)
-            if (l.i[i] >= i0 && l.i[i] < i1) x += kept(l.v[i], l.i[i], cut, s, M);
+        const int i1 = run_end(l.i, n, (c + 1) * w.chunk);
+        for (int i = run_end(l.i, n, c * w.chunk) + lane; i < i1; i += 64) x += kept(l.v[i], l.i[i], cut, s, M);
         x = wave_sum(x);
         if (lane == 0) f.sums[c] = x;
     }
@@ -1146,7 +1185,10 @@ extern "C" int ft_hip_sample_tokens(ft_hip_ctx* ctx, void* stream, const void* l
         return fail(FT_HIP_E_SHAPE, "sample_tokens: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     if (!ctx || !logits || !u || !tokens || !workspace) return fail(FT_HIP_E_INVALID, "sample_tokens: null argument");
     if (n == 0) return FT_HIP_OK;
-    const SampleArgs a{logits, logits_stride, (int)vocab, temperature, top_k, top_p, min_p, u, tokens, logprobs};
+    const int given = (temperature ? HAS_T : 0) | (top_k ? HAS_K : 0) | (top_p ? HAS_P : 0) | (min_p ? HAS_M : 0);
+    const SampleArgs a{logits, logits_stride, (int)vocab, temperature ? temperature : u,
+                       top_k ? top_k : reinterpret_cast<const int32_t*>(u), top_p ? top_p : u, min_p ? min_p : u, u,
+                       tokens, logprobs, given};
     DeviceGuard on(ctx->device);
     if (!on.ok) return fail(FT_HIP_E_DEVICE, "sample_tokens: device %d cannot be made current", ctx->device);
     if (logits_type == FT_TYPE_F32)
