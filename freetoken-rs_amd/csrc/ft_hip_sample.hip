@@ -71,7 +71,8 @@ __device__ __forceinline__ Row row_of(const SampleArgs& a, int64_t r) {
     const int k = a.given & HAS_K ? k_in : 0;
     Row s;
     s.greedy = !(t > 0.0f);
-    s.inv_t = s.greedy ? 1.0 : 1.0 / (double)t;
+    // T = inf as 2^200: exp of any two f32 values' distance over it is 1, and -inf over it is -inf
+    s.inv_t = s.greedy ? 1.0 : fmax(1.0 / (double)t, 0x1p-200);
     s.k = k > 0 && k < a.V ? k : a.V;
     s.p = p < 1.0f ? fmax((double)p, 0.0) : 1.0;  // NaN: off
     s.m = m > 0.0f ? fmin((double)m, 1.0) : 0.0;  // NaN: off
@@ -608,6 +609,12 @@ __device__ __forceinline__ bool vec_row(const void* row) {
     return (reinterpret_cast<uintptr_t>(row) & (TYPE == FT_TYPE_F32 ? 15 : 7)) == 0;
 }
 
+// The value in scalar registers, whatever the compiler knows of it.
+__device__ __forceinline__ double scalar(double v) {
+    asm("" : "+s"(v));
+    return v;
+}
+
 // Workgroup (c, row): chunk c of the row in registers, VECS times four values
 // a thread; one pass over memory.
 template <int TYPE, int VECS>
@@ -646,36 +653,49 @@ __global__ __launch_bounds__(1024) void k_sample_scan(SampleArgs a, Scan w, int6
     __syncthreads();
     const double unit = per_unit(s), g = step_of(m, unit);
     double far = 0.0;
+    // no value above `last` is beyond the bins
+    const double end = (g - (BINS - 1)) / unit;
+    const float last = (float)(end + fabs(end) * 1e-6);
     bool beyond = false;
     int top = 0;
 #pragma unroll
     for (int i = 0; i < VECS; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) top += __popcll(__ballot(v[i][e] == m));
+    // a value's word: (2^(q / 8) - OFFSET) 2^FRAC + 1/2 by the series to q^5 (|q| <= 1/2: what is left is under a third
+    // of a unit). The constants are kept in scalar registers: as literals each would cost two moves per use.
+    const double L = 0.08664339756999316, U = (double)(1ull << FRAC);  // ln 2 / 8
+    const double c0 = scalar((1.0 - OFFSET) * U + 0.5), c1 = scalar(L * U), c2 = scalar(L * L / 2 * U),
+                 c3 = scalar(L * L * L / 6 * U), c4 = scalar(L * L * L * L / 24 * U),
+                 c5 = scalar(L * L * L * L * L / 120 * U);
 #pragma unroll
-    for (int i = 0; i < VECS; ++i)
+    for (int i = 0; i < VECS; ++i) {
+        uint32_t word[4];
+        int bin[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const double y = (double)v[i][e] * unit, n = rint(y), q = y - n;
+            word[e] = (uint32_t)fma(fma(fma(fma(fma(q, c5, c4), q, c3), q, c2), q, c1), q, c0);
+            bin[e] = (int)(g - n);  // saturates; NaN and -inf are out below
+            asm("" : "+v"(word[e]), "+v"(bin[e]));  // four chains side by side, not each under its mask
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float x = v[i][e];
-            const double y = (double)x * unit, n = rint(y), d = g - n;
-            // 2^((y - n) / 8) by its series: |q| <= ln 2 / 16, so that q^7 / 5040 is below 2^-44
-            const double q = (y - n) * 0.08664339756999316;
-            const double p = fma(fma(fma(fma(fma(q, 1.0 / 720, 1.0 / 120), q, 1.0 / 24), q, 1.0 / 6), q, 0.5), q, 1.0);
-            if (x < m && d < (double)BINS) {  // false for NaN and -inf
-                const uint32_t f = (uint32_t)fma(fma(p, q, 1.0 - OFFSET), (double)(1ull << FRAC), 0.5);
-                atomicAdd((unsigned long long*)&bins[(int)d], (1ull << 47) + f);
-            } else {
-                beyond |= x < m && x > -INFINITY;
-            }
+            if (x < m && (uint32_t)bin[e] < BINS)
+                atomicAdd((unsigned long long*)&bins[bin[e]], (1ull << 47) + word[e]);
+            beyond |= x == __builtin_amdgcn_fmed3f(x, -FLT_MAX, last);
         }
-    if (__ballot(beyond)) {  // few in most rows
-#pragma unroll
-        for (int i = 0; i < VECS; ++i)
+    }
+    if (__ballot(beyond)) {  // far below the largest: few in most rows, from the caches again
 #pragma unroll 1
-            for (int e = 0; e < 4; ++e) {
-                const float x = e == 0 ? v[i][0] : e == 1 ? v[i][1] : e == 2 ? v[i][2] : v[i][3];
-                if (x < m && x > -INFINITY && !(g - step_of(x, unit) < (double)BINS)) far += weight(x, m, s.inv_t);
-            }
+        for (int i = 0; i < VECS; ++i) {
+            float x[4];
+            load4<TYPE>(row, c * w.chunk + (i * T + t) * 4, a.V, vec, x);
+            for (int e = 0; e < 4; ++e)
+                if (x[e] < m && x[e] > -INFINITY && !(g - step_of(x[e], unit) < (double)BINS))
+                    far += weight(x[e], m, s.inv_t);
+        }
     }
     if (lane == 0) atomicAdd(&top_n, (uint32_t)top);
     __syncthreads();
