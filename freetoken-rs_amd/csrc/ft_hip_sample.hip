@@ -567,10 +567,15 @@ __device__ __forceinline__ bool by_maxima(const Row& s, int V, int segs) {
     return s.greedy || (s.k < V && (s.p < 1.0 || s.k <= segs));
 }
 
-// A value's place in steps of e, and its step; v1: the step of 2^(1/8) per
-// unit of the logit.
+// A value's place in steps of e (per_unit: the step of 2^(1/8) per unit of the
+// logit), and its step, the nearest whole number: by the sum with MAGIC, whose
+// last bit is 1; further out, where the steps of f32 are many of these, by rint.
+constexpr double MAGIC = 0x1.8p52, NEAR = 0x1p50;
 __device__ __forceinline__ double per_unit(const Row& s) { return s.inv_t * (8.0 * 1.4426950408889634074); }
-__device__ __forceinline__ double step_of(float v, double unit) { return rint((double)v * unit); }
+__device__ __forceinline__ double step_of(float v, double unit) {
+    const double y = (double)v * unit;
+    return fabs(y) < NEAR ? fma((double)v, unit, MAGIC) - MAGIC : rint(y);
+}
 // Steps below the largest's (g: step_of(M)); BINS: that or more.
 __device__ __forceinline__ int bin_of(float v, float M, double g, double unit) {
     if (v == M) return 0;
@@ -579,7 +584,7 @@ __device__ __forceinline__ int bin_of(float v, float M, double g, double unit) {
 }
 // The largest's place over the middle of its step, in steps.
 __device__ __forceinline__ double over_step(float M, double g, double unit) {
-    const double d = (double)M * unit - g;
+    const double d = fma((double)M, unit, -g);
     return fabs(d) <= 0.5 ? d : 0.0;  // inf - inf: 0
 }
 __device__ __forceinline__ double bin_sum(uint64_t word) {
@@ -587,20 +592,23 @@ __device__ __forceinline__ double bin_sum(uint64_t word) {
            (double)(word & ((1ull << 47) - 1)) * (1.0 / (double)(1ull << FRAC));
 }
 
+// Four values from an aligned place of a row.
+template <int TYPE>
+__device__ __forceinline__ void load4(const void* row, int i, float v[4]) {
+    if constexpr (TYPE == FT_TYPE_F32) {
+        const float4 x = *reinterpret_cast<const float4*>(static_cast<const float*>(row) + i);
+        v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+    } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(row) + i);
+        const uint16_t b[4] = {(uint16_t)x.x, (uint16_t)(x.x >> 16), (uint16_t)x.y, (uint16_t)(x.y >> 16)};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = TYPE == FT_TYPE_F16 ? h2f(b[e]) : __uint_as_float((uint32_t)b[e] << 16);
+    }
+}
+// From any place; -inf past the end.
 template <int TYPE>
 __device__ __forceinline__ void load4(const void* row, int i, int V, bool vec, float v[4]) {
-    if (vec && i + 4 <= V) {
-        if constexpr (TYPE == FT_TYPE_F32) {
-            const float4 x = *reinterpret_cast<const float4*>(static_cast<const float*>(row) + i);
-            v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
-        } else {
-            const uint2 x = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(row) + i);
-            const uint16_t b[4] = {(uint16_t)x.x, (uint16_t)(x.x >> 16), (uint16_t)x.y, (uint16_t)(x.y >> 16)};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = TYPE == FT_TYPE_F16 ? h2f(b[e]) : __uint_as_float((uint32_t)b[e] << 16);
-        }
-        return;
-    }
+    if (vec && i + 4 <= V) return load4<TYPE>(row, i, v);
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = i + e < V ? logit<TYPE>(row, i + e) : -INFINITY;
 }
@@ -627,18 +635,19 @@ __global__ __launch_bounds__(1024) void k_sample_scan(SampleArgs a, Scan w, int6
     const void* row = row_at<TYPE>(a, r);
     const bool vec = vec_row<TYPE>(row);
     float v[VECS][4];
+    if (vec && (c + 1) * w.chunk <= a.V) {  // one branch for all loads: a branch at each would wait for each
 #pragma unroll
-    for (int i = 0; i < VECS; ++i) load4<TYPE>(row, c * w.chunk + (i * T + t) * 4, a.V, vec, v[i]);
+        for (int i = 0; i < VECS; ++i) load4<TYPE>(row, c * w.chunk + (i * T + t) * 4, v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VECS; ++i) load4<TYPE>(row, c * w.chunk + (i * T + t) * 4, a.V, vec, v[i]);
+    }
     const Row s = row_of(a, r);
     float m = -INFINITY;
     float* seg = w.seg(blockIdx.y);
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
-        float x = fmaxf(fmaxf(fmaxf(v[i][0], v[i][1]), fmaxf(v[i][2], v[i][3])), -INFINITY);  // NaN is skipped
-        x = fmaxf(x, quad_xor1(x));
-        x = fmaxf(x, quad_xor2(x));
-        x = fmaxf(x, dpp_f<0x141>(x));
-        x = fmaxf(x, dpp_f<0x140>(x));
+        const float x = row_max16(fmaxf(fmaxf(fmaxf(v[i][0], v[i][1]), fmaxf(v[i][2], v[i][3])), -INFINITY));
         const int at = (c * w.chunk + (i * T + t) * 4) / SEG;
         if ((lane & 15) == 0 && at < w.segs) seg[at] = x;
         m = fmaxf(m, x);
@@ -653,38 +662,46 @@ __global__ __launch_bounds__(1024) void k_sample_scan(SampleArgs a, Scan w, int6
     __syncthreads();
     const double unit = per_unit(s), g = step_of(m, unit);
     double far = 0.0;
-    // no value above `last` is beyond the bins
-    const double end = (g - (BINS - 1)) / unit;
-    const float last = (float)(end + fabs(end) * 1e-6);
+    // the bins hold the values from `low` on: the smallest on one of the first BINS steps
+    float low = m;
+    if (fabs(g) < NEAR) {
+        low = (float)fmax((g - BINS + 0.5) / unit, -(double)FLT_MAX);
+        if (step_of(low, unit) <= g - BINS) low = of_key(key_of(low) + 1);
+        const float less = of_key(key_of(low) - 1);
+        if (less >= -FLT_MAX && step_of(less, unit) > g - BINS) low = less;
+    }
+    const float under = of_key(key_of(low) - 1);  // what is up to here is beyond them
     bool beyond = false;
     int top = 0;
 #pragma unroll
     for (int i = 0; i < VECS; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) top += __popcll(__ballot(v[i][e] == m));
-    // a value's word: (2^(q / 8) - OFFSET) 2^FRAC + 1/2 by the series to q^5 (|q| <= 1/2: what is left is under a third
-    // of a unit). The constants are kept in scalar registers: as literals each would cost two moves per use.
+    // a value's word: (2^(q / 8) - OFFSET) 2^FRAC by the series to q^5 (|q| <= 1/2: what is left is under a third of a
+    // unit), whose sum with 2^52 has it in its low half, as the sum with MAGIC has the step: conversions of f64 are
+    // slow. The constants are kept in scalar registers: as literals each would cost two moves per use.
     const double L = 0.08664339756999316, U = (double)(1ull << FRAC);  // ln 2 / 8
-    const double c0 = scalar((1.0 - OFFSET) * U + 0.5), c1 = scalar(L * U), c2 = scalar(L * L / 2 * U),
+    const double c0 = scalar((1.0 - OFFSET) * U + 0x1p52), c1 = scalar(L * U), c2 = scalar(L * L / 2 * U),
                  c3 = scalar(L * L * L / 6 * U), c4 = scalar(L * L * L * L / 24 * U),
                  c5 = scalar(L * L * L * L * L / 120 * U);
+    const int g_low = (int)__double_as_longlong(g + MAGIC);
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
         uint32_t word[4];
         int bin[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const double y = (double)v[i][e] * unit, n = rint(y), q = y - n;
-            word[e] = (uint32_t)fma(fma(fma(fma(fma(q, c5, c4), q, c3), q, c2), q, c1), q, c0);
-            bin[e] = (int)(g - n);  // saturates; NaN and -inf are out below
+            const double x = v[i][e], n = fma(x, unit, MAGIC), q = fma(x, unit, -(n - MAGIC));
+            word[e] = (uint32_t)__double_as_longlong(
+                fma(fma(fma(fma(fma(q, c5, c4), q, c3), q, c2), q, c1), q, c0));
+            bin[e] = g_low - (int)__double_as_longlong(n);
             asm("" : "+v"(word[e]), "+v"(bin[e]));  // four chains side by side, not each under its mask
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float x = v[i][e];
-            if (x < m && (uint32_t)bin[e] < BINS)
-                atomicAdd((unsigned long long*)&bins[bin[e]], (1ull << 47) + word[e]);
-            beyond |= x == __builtin_amdgcn_fmed3f(x, -FLT_MAX, last);
+            if (x >= low && x < m) atomicAdd((unsigned long long*)&bins[bin[e]], (1ull << 47) + word[e]);
+            beyond |= x == __builtin_amdgcn_fmed3f(x, -FLT_MAX, under);
         }
     }
     if (__ballot(beyond)) {  // far below the largest: few in most rows, from the caches again
@@ -693,8 +710,7 @@ __global__ __launch_bounds__(1024) void k_sample_scan(SampleArgs a, Scan w, int6
             float x[4];
             load4<TYPE>(row, c * w.chunk + (i * T + t) * 4, a.V, vec, x);
             for (int e = 0; e < 4; ++e)
-                if (x[e] < m && x[e] > -INFINITY && !(g - step_of(x[e], unit) < (double)BINS))
-                    far += weight(x[e], m, s.inv_t);
+                if (x[e] < low && x[e] > -INFINITY) far += weight(x[e], m, s.inv_t);
         }
     }
     if (lane == 0) atomicAdd(&top_n, (uint32_t)top);
@@ -702,10 +718,12 @@ __global__ __launch_bounds__(1024) void k_sample_scan(SampleArgs a, Scan w, int6
     // the chunk's sums, its bins in their order
     double z = 0.0;
     uint64_t* out = w.bins(blockIdx.y) + (int64_t)c * BINS;
+    double scale = exp2(t * -0.125);
     for (int b = t; b < BINS; b += T) {
         const uint64_t word = bins[b];
         out[b] = word;
-        if (word) z += bin_sum(word) * exp2(b * -0.125);
+        z += bin_sum(word) * scale;
+        scale = ldexp(scale, -T / 8);
     }
     z = wave_sum(z);
     far = wave_sum(far);

@@ -61,6 +61,19 @@ __device__ __forceinline__ float wave_move(float v) {  // v itself where nothing
     return __int_as_float(__builtin_amdgcn_update_dpp(b, b, CTRL, ROWS, 0xF, false));
 }
 
+// Largest of a row's 16 lanes, in each of them, of a value that is no NaN: a
+// step is one instruction, where fmaxf on a moved value takes three (the move
+// and a maximum with itself, for signalling NaNs). A DPP operand may be read
+// two wait states after it is written.
+__device__ __forceinline__ float row_max16(float v) {
+    asm("s_nop 1\n\tv_max_f32_dpp %0, %0, %0 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n\t"
+        "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n\t"
+        "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_half_mirror row_mask:0xf bank_mask:0xf\n\t"
+        "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_mirror row_mask:0xf bank_mask:0xf"
+        : "+v"(v));
+    return v;
+}
+
 // Largest of all lanes, in every lane; NaN is skipped.
 __device__ __forceinline__ float wave_max(float v) {
     v = fmaxf(v, wave_move<0x111>(v));
