@@ -10,8 +10,9 @@
 // quotient for y, and taken from u it depends on 32 values instead of on the
 // last bit of a sum over the row. The quotient is rounded as the real number:
 // u and a have 24 bits, so 127 u / a is either a half exactly or further than
-// 2^-26 from one, and the f64 product with 127 / a (off by less than 2^-45)
-// plus 2^-40 has its floor on the right side either way.
+// 2^-26 from one. It is taken as u times 127 / a * (1 + 2^-44), in f64 off by
+// less than 2^-45 of itself besides: a half comes out above the half, any
+// other stays on its side, and the nearest whole number is the one sought.
 //
 // Bound by memory: x, the residual, h, y and the blocks each move once; the
 // row stays in registers between its sum and its outputs. Sums and scales are
@@ -19,7 +20,9 @@
 
 #include "ft_device.hpp"
 #include "ft_runtime.hpp"
+#include "ft_wave.hpp"
 
+#include <cfloat>
 #include <cmath>
 
 using namespace ft;
@@ -39,8 +42,7 @@ struct NormArgs {
     int64_t y_stride;
     uint8_t* q8;
     int hidden;
-    int64_t n;
-    double eps;
+    double eps, per_value;  // per_value: 1 / hidden
 };
 
 // V consecutive values (V = 4: one aligned vector access, V = 1: any address)
@@ -89,24 +91,30 @@ __device__ __forceinline__ void store_f32(float* p, const Vals<V>& r) {
         *p = r.v[0];
 }
 
-__device__ __forceinline__ double shfl_xor_f64(double v, int m) {
-    const long long b = __double_as_longlong(v);
-    const int lo = __shfl_xor((int)b, m), hi = __shfl_xor((int)(b >> 32), m);
-    return __longlong_as_double(((long long)hi << 32) | (uint32_t)lo);
+// Sum over the workgroup, the same bits in every thread and on every run: the
+// waves' sums in order.
+__device__ __forceinline__ double row_sum(double v, double* red) {
+    v = wave_sum(v);
+    const int waves = blockDim.x >> 6, lane = threadIdx.x & 63;
+    if (waves == 1) return v;
+    if (lane == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return wave_sum(lane < waves ? red[lane] : 0.0);
 }
 
-// Sum over the workgroup, the same bits in every thread and on every run:
-// a butterfly in each wave, then the waves in order.
-__device__ __forceinline__ double row_sum(double v, double* red) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) v += shfl_xor_f64(v, m);
-    const int waves = blockDim.x >> 6;
-    if (waves == 1) return v;
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    double s = 0.0;
-    for (int i = 0; i < waves; ++i) s += red[i];
-    return s;
+// 1 / x and 1 / sqrt(x) to an ulp or two of f64: the instruction's 24 bits and
+// two Newton steps (IEEE division and square root take about 60 instructions
+// between them). x positive, and for rsqrt 0 gives inf or NaN, inf gives 0.
+__device__ __forceinline__ double recip(double x) {
+    double y = __builtin_amdgcn_rcp(x);
+    y = fma(fma(-x, y, 1.0), y, y);
+    return fma(fma(-x, y, 1.0), y, y);
+}
+__device__ __forceinline__ double rsqrt_of(double x) {
+    if (x > 0x1p1000) return 0.0;  // of f32 values: inf
+    double y = __builtin_amdgcn_rsq(x);
+    y = fma(fma(-x * y, y, 1.0), 0.5 * y, y);
+    return fma(fma(-x * y, y, 1.0), 0.5 * y, y);
 }
 
 // One q8 block per group of 32 / V lanes.
@@ -122,17 +130,17 @@ __device__ __forceinline__ void quantize_u(const Vals<V>& u, double inv, uint8_t
     } else {
         a = half_max32(a);
     }
-    const double r = a > 0.0f ? 127.0 / (double)a : 0.0;
-    int qsum = 0;
+    const double r = a > 0.0f && a < INFINITY ? recip((double)a) * (127.0 * (1.0 + 0x1p-44)) : 0.0;
+    const float most = fminf(a, FLT_MAX);
     uint32_t word = 0;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const double t = fabs((double)u.v[i]) * r;  // inf * 0 and NaN give NaN: quant 0
-        const int q = t <= 127.5 ? (int)(t + (0.5 + 0x1p-40)) : 0;
-        const int s = u.v[i] < 0.0f ? -q : q;
-        qsum += s;
-        word |= (uint32_t)(uint8_t)(int8_t)s << (8 * i);
+        const float v = fabsf(u.v[i]) <= most ? u.v[i] : 0.0f;  // NaN and inf: quant 0
+        // the sum's last bit is 1: its low half is the nearest whole number
+        const int q = (int)__double_as_longlong(fma((double)v, r, 0x1.8p52));
+        word |= (uint32_t)(uint8_t)q << (8 * i);
     }
+    int qsum = V == 4 ? __builtin_amdgcn_sdot4((int)word, 0x01010101, 0, false) : (int)(int8_t)word;
     if constexpr (V == 4) {
         qsum += quad_xor1i(qsum);
         qsum += quad_xor2i(qsum);
@@ -143,7 +151,7 @@ __device__ __forceinline__ void quantize_u(const Vals<V>& u, double inv, uint8_t
         blk[8 + part] = (uint8_t)word;
     }
     if (part == 0) {
-        reinterpret_cast<float*>(blk)[0] = a > 0.0f ? (float)((double)a * inv / 127.0) : 0.0f;
+        reinterpret_cast<float*>(blk)[0] = a > 0.0f ? (float)((double)a * inv * (1.0 / 127.0)) : 0.0f;
         reinterpret_cast<int*>(blk)[1] = qsum;
     }
 }
@@ -157,16 +165,23 @@ __global__ __launch_bounds__(1024) void k_add_rmsnorm(NormArgs a) {
     __shared__ double red[2][16];
     const int64_t row = blockIdx.x;
     const int t = threadIdx.x, step = blockDim.x * V;
-    Vals<V> h[NV];
+    const auto zero = [](Vals<V>& r) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) r.v[e] = 0.0f;
+    };
+    // all that the row's sums do not decide is loaded at once
+    Vals<V> h[NV], r[NV], xw[NV], w[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = i * step + t * V;
-        if (c < a.hidden) {
-            h[i] = load_typed<V, TYPE>(a.x, row * a.x_stride + c);
-        } else {
-#pragma unroll
-            for (int e = 0; e < V; ++e) h[i].v[e] = 0.0f;
+        if (c >= a.hidden) {
+            zero(h[i]);
+            continue;
         }
+        h[i] = load_typed<V, TYPE>(a.x, row * a.x_stride + c);
+        if (a.residual) r[i] = load_f32<V>(a.residual + row * a.r_stride + c);
+        if (a.x_w) xw[i] = load_f32<V>(a.x_w + c);
+        if (a.w) w[i] = load_f32<V>(a.w + c);
     }
     if (a.x_w) {
         double ss = 0.0;
@@ -174,28 +189,20 @@ __global__ __launch_bounds__(1024) void k_add_rmsnorm(NormArgs a) {
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int e = 0; e < V; ++e) ss = fma((double)h[i].v[e], (double)h[i].v[e], ss);
-        const double inv = 1.0 / sqrt(row_sum(ss, red[0]) / a.hidden + a.eps);
+        const double inv = rsqrt_of(fma(row_sum(ss, red[0]), a.per_value, a.eps));
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = i * step + t * V;
-            if (c >= a.hidden) continue;
-            const Vals<V> w = load_f32<V>(a.x_w + c);
-            Vals<V> r;
-            if (a.residual) r = load_f32<V>(a.residual + row * a.r_stride + c);
+            if (i * step + t * V >= a.hidden) continue;
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const double n = (double)h[i].v[e] * inv * (double)w.v[e];
-                h[i].v[e] = (float)(a.residual ? n + (double)r.v[e] : n);
-            }
+            for (int e = 0; e < V; ++e)
+                h[i].v[e] = (float)fma((double)h[i].v[e] * inv, (double)xw[i].v[e], a.residual ? (double)r[i].v[e] : 0.0);
         }
     } else if (a.residual) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = i * step + t * V;
-            if (c >= a.hidden) continue;
-            const Vals<V> r = load_f32<V>(a.residual + row * a.r_stride + c);
+            if (i * step + t * V >= a.hidden) continue;
 #pragma unroll
-            for (int e = 0; e < V; ++e) h[i].v[e] = r.v[e] + h[i].v[e];
+            for (int e = 0; e < V; ++e) h[i].v[e] = r[i].v[e] + h[i].v[e];
         }
     }
     double ss = 0.0;
@@ -203,48 +210,47 @@ __global__ __launch_bounds__(1024) void k_add_rmsnorm(NormArgs a) {
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int e = 0; e < V; ++e) ss = fma((double)h[i].v[e], (double)h[i].v[e], ss);
-    const double inv = 1.0 / sqrt(row_sum(ss, red[1]) / a.hidden + a.eps);
+    const double inv = rsqrt_of(fma(row_sum(ss, red[1]), a.per_value, a.eps));
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = i * step + t * V;
         if (c >= a.hidden) continue;
         if (a.h) store_f32<V>(a.h + row * a.h_stride + c, h[i]);
-        Vals<V> w;
-        if (a.w) {
-            w = load_f32<V>(a.w + c);
-        } else {
+        if (!a.w) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) w.v[e] = 1.0f;
+            for (int e = 0; e < V; ++e) w[i].v[e] = 1.0f;
         }
         if (a.y) {
             Vals<V> y;
 #pragma unroll
-            for (int e = 0; e < V; ++e) y.v[e] = (float)((double)h[i].v[e] * inv * (double)w.v[e]);
+            for (int e = 0; e < V; ++e) y.v[e] = (float)((double)h[i].v[e] * inv * (double)w[i].v[e]);
             store_f32<V>(a.y + row * a.y_stride + c, y);
         }
         if (a.q8) {
             Vals<V> u;
 #pragma unroll
-            for (int e = 0; e < V; ++e) u.v[e] = h[i].v[e] * w.v[e];
+            for (int e = 0; e < V; ++e) u.v[e] = h[i].v[e] * w[i].v[e];
             quantize_u<V>(u, inv, a.q8 + (row * (a.hidden >> 5) + (c >> 5)) * Q8_BLK, (c & 31) / V);
         }
     }
 }
 
 template <int TYPE>
-void launch_norm(const NormArgs& a, bool vec, void* stream) {
-    const dim3 grid((unsigned)a.n);
+void launch_norm(const NormArgs& a, int64_t n, int64_t few, bool vec, void* stream) {
+    const dim3 grid((unsigned)n);
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (!vec) {
         const int threads = a.hidden >= 1024 ? 1024 : (a.hidden + 63) / 64 * 64;
         hipLaunchKernelGGL((k_add_rmsnorm<TYPE, 1, 16>), grid, dim3(threads), 0, s, a);
         return;
     }
-    const int vecs = a.hidden / 4, threads = vecs >= 1024 ? 1024 : (vecs + 63) / 64 * 64;
-    if (vecs <= threads)
-        hipLaunchKernelGGL((k_add_rmsnorm<TYPE, 4, 1>), grid, dim3(threads), 0, s, a);
+    // few rows: as many threads on a row as it has vectors; many: four vectors a thread, so that what a wave does once
+    // a row (two sums, two square roots) is shared by more values
+    const int vecs = a.hidden / 4, wide = (vecs + 63) / 64 * 64;
+    if (n <= few && vecs <= 1024)
+        hipLaunchKernelGGL((k_add_rmsnorm<TYPE, 4, 1>), grid, dim3(wide), 0, s, a);
     else
-        hipLaunchKernelGGL((k_add_rmsnorm<TYPE, 4, 4>), grid, dim3(threads), 0, s, a);
+        hipLaunchKernelGGL((k_add_rmsnorm<TYPE, 4, 4>), grid, dim3((vecs + 255) / 256 * 64), 0, s, a);
 }
 
 bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
@@ -279,7 +285,7 @@ extern "C" int ft_hip_add_rmsnorm(ft_hip_ctx* ctx, void* stream, const void* x, 
     if (!h && !y && !q8) return fail(FT_HIP_E_INVALID, "add_rmsnorm: no output (h, y and q8 are null)");
     if (n == 0) return FT_HIP_OK;
     const NormArgs a{x, x_stride, x_w, residual, residual_stride, h, h_stride, w, y, y_stride,
-                     static_cast<uint8_t*>(q8), (int)hidden, n, (double)eps};
+                     static_cast<uint8_t*>(q8), (int)hidden, (double)eps, 1.0 / (double)hidden};
     // vectors of 4 where every row starts on one; else value by value
     const bool vec = hidden % 4 == 0 && aligned(x, 4 * size) && x_stride % 4 == 0 && aligned(x_w, 16) && aligned(w, 16) &&
                      aligned(residual, 16) && (!residual || residual_stride % 4 == 0) && aligned(h, 16) &&
@@ -287,10 +293,10 @@ extern "C" int ft_hip_add_rmsnorm(ft_hip_ctx* ctx, void* stream, const void* x, 
     DeviceGuard on(ctx->device);
     if (!on.ok) return fail(FT_HIP_E_DEVICE, "add_rmsnorm: device %d cannot be made current", ctx->device);
     if (x_type == FT_TYPE_F32)
-        launch_norm<FT_TYPE_F32>(a, vec, stream);
+        launch_norm<FT_TYPE_F32>(a, n, ctx->num_cus, vec, stream);
     else if (x_type == FT_TYPE_F16)
-        launch_norm<FT_TYPE_F16>(a, vec, stream);
+        launch_norm<FT_TYPE_F16>(a, n, ctx->num_cus, vec, stream);
     else
-        launch_norm<FT_TYPE_BF16>(a, vec, stream);
+        launch_norm<FT_TYPE_BF16>(a, n, ctx->num_cus, vec, stream);
     return launch_status("add_rmsnorm");
 }
