@@ -11,12 +11,19 @@
 // f32's rate here): an f32 exp's last bit would swap near-equal experts in
 // some of a prompt's thousands of tokens.
 //
-// A token's experts lie over the 64 lanes of a wave, expert lane + 64 j in
-// slot j; every selection is a maximum over the wave.
+// SUB lanes of a wave share a token (64 / SUB tokens a wave), each with VPL
+// consecutive experts, sorted in registers once; the next expert is then the
+// largest of the lanes' first ones, and its lane moves up its next. Lanes hold
+// rising experts, so that among equal ones the lowest lane has the lowest.
+//
+// Bound by instructions: about 350 a wave for 64 * VPL logits, where memory
+// would allow about 60.
 
 #include "ft_device.hpp"
 #include "ft_runtime.hpp"
+#include "ft_wave.hpp"
 
+#include <algorithm>
 #include <cmath>
 
 using namespace ft;
@@ -35,141 +42,265 @@ struct RouteArgs {
     int sigmoid, n_groups, group_size, top_groups, group_rank, renorm;
     double scale;
     int E, k;
-    int64_t n;
+    int n;
+    bool vec;  // rows start on 16 bytes and E is a multiple of 4
 };
 
-__device__ __forceinline__ double shfl_xor_f64(double v, int m) {
-    const long long b = __double_as_longlong(v);
-    const int lo = __shfl_xor((int)b, m), hi = __shfl_xor((int)(b >> 32), m);
-    return __longlong_as_double(((long long)hi << 32) | (uint32_t)lo);
+// Exchanges within the SUB lanes of a token: step 0..log2(SUB)-1 of a
+// butterfly, in which mirrors stand for the wider exchanges inside a row.
+template <int STEP>
+__device__ __forceinline__ void partner(int v, int& a, int& b) {
+    if constexpr (STEP < 4) {
+        a = v;
+        b = dpp_i<STEP == 0 ? 0xB1 : STEP == 1 ? 0x4E : STEP == 2 ? 0x141 : 0x140>(v);
+    } else {
+        const auto s = STEP == 4 ? __builtin_amdgcn_permlane16_swap(v, v, false, false)
+                                 : __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        a = s[0];
+        b = s[1];
+    }
 }
-__device__ __forceinline__ double shfl_f64(double v, int l) {
-    const long long b = __double_as_longlong(v);
-    const int lo = __shfl((int)b, l), hi = __shfl((int)(b >> 32), l);
-    return __longlong_as_double(((long long)hi << 32) | (uint32_t)lo);
+template <int STEP>
+__device__ __forceinline__ void partner(double v, double& a, double& b) {
+    const long long x = __double_as_longlong(v);
+    int al, bl, ah, bh;
+    partner<STEP>((int)x, al, bl);
+    partner<STEP>((int)(x >> 32), ah, bh);
+    a = __longlong_as_double(((long long)ah << 32) | (uint32_t)al);
+    b = __longlong_as_double(((long long)bh << 32) | (uint32_t)bl);
+}
+template <int SUB, int STEP = 0>
+__device__ __forceinline__ double sub_sum(double v) {
+    if constexpr (1 << STEP < SUB) {
+        double a, b;
+        partner<STEP>(v, a, b);
+        return sub_sum<SUB, STEP + 1>(a + b);
+    }
+    return v;
+}
+template <int SUB, int STEP = 0>
+__device__ __forceinline__ float sub_max(float v) {
+    if constexpr (1 << STEP < SUB) {
+        int a, b;
+        partner<STEP>(__float_as_int(v), a, b);
+        return sub_max<SUB, STEP + 1>(fmaxf(__int_as_float(a), __int_as_float(b)));
+    }
+    return v;
+}
+template <int SUB, int STEP = 0>
+__device__ __forceinline__ uint32_t sub_max(uint32_t v) {
+    if constexpr (1 << STEP < SUB) {
+        int a, b;
+        partner<STEP>((int)v, a, b);
+        return sub_max<SUB, STEP + 1>(max((uint32_t)a, (uint32_t)b));
+    }
+    return v;
+}
+// The two largest of P lanes' pairs (P a power of two up to SUB).
+template <int SUB, int STEP = 0>
+__device__ __forceinline__ void sub_top2(double& b1, double& b2, int P) {
+    if constexpr (1 << STEP < SUB) {
+        if (1 << STEP < P) {
+            double a1, c1, a2, c2;
+            partner<STEP>(b1, a1, c1);
+            partner<STEP>(b2, a2, c2);
+            b1 = fmax(a1, c1);
+            b2 = fmax(fmin(a1, c1), fmax(a2, c2));
+        }
+        sub_top2<SUB, STEP + 1>(b1, b2, P);
+    }
 }
 
-// LDS written by a wave is read by its other lanes after this.
-__device__ __forceinline__ void wave_lds_fence() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-    __builtin_amdgcn_wave_barrier();
+// exp(x) for x in [-745, 700], to 2^-51: x = n ln 2 + r by the sum with
+// 1.5 * 2^52, whose low half is n; the series of exp(r), |r| <= ln 2 / 2, to
+// r^12 (the next term is below 2^-52).
+__device__ __forceinline__ double exp_series(double x) {
+    const double t = fma(x, 1.4426950408889634074, 0x1.8p52), n = t - 0x1.8p52;
+    double r = fma(n, -0x1.62e42fefap-1, x);  // ln 2 to 34 bits: n times it is exact
+    r = fma(n, -0x1.cf79abc9e3b3ap-40, r);    // and the rest of it
+    double p = scalar(1.0 / 479001600);
+    p = fma(p, r, scalar(1.0 / 39916800));
+    p = fma(p, r, scalar(1.0 / 3628800));
+    p = fma(p, r, scalar(1.0 / 362880));
+    p = fma(p, r, scalar(1.0 / 40320));
+    p = fma(p, r, scalar(1.0 / 5040));
+    p = fma(p, r, scalar(1.0 / 720));
+    p = fma(p, r, scalar(1.0 / 120));
+    p = fma(p, r, scalar(1.0 / 24));
+    p = fma(p, r, scalar(1.0 / 6));
+    p = fma(fma(fma(p, r, 0.5), r, 1.0), r, 1.0);
+    return ldexp(p, (int)__double_as_longlong(t));
+}
+__device__ __forceinline__ double recip(double x) {  // of finite x >= 1
+    double y = __builtin_amdgcn_rcp(x);
+    y = fma(fma(-x, y, 1.0), y, y);
+    return fma(fma(-x, y, 1.0), y, y);
 }
 
-template <int VPL>
+// A key that rises with c; 0: not to be chosen.
+__device__ __forceinline__ uint64_t key_of(double c, bool ok) {
+    const uint64_t b = (uint64_t)__double_as_longlong(c);
+    const uint64_t key = b ^ ((uint64_t)((int64_t)b >> 63) | 0x8000000000000000ull);
+    return ok ? key : 0;
+}
+
+template <int SUB, int VPL>
 __global__ __launch_bounds__(256) void k_route_experts(RouteArgs a) {
-    extern __shared__ double lds[];  // with groups: per wave its token's c
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t token = (int64_t)blockIdx.x * 4 + wave;
-    if (token >= a.n) return;  // whole waves; no workgroup barrier below
+    extern __shared__ double lds[];  // with groups: per wave its tokens' c
+    __shared__ int chosen[256];
+    constexpr int TOKENS = 64 / SUB;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane & (SUB - 1), first = lane & ~(SUB - 1);
+    const int wanted = ((int)blockIdx.x * 4 + wave) * TOKENS + lane / SUB;
+    const int token = min(wanted, a.n - 1);  // past the last: computed again, not stored
     const float* row = a.logits + token * a.stride;
     const double none = -(double)INFINITY;
 
     float l[VPL];
-    float m = -INFINITY;
+    if (a.vec) {
 #pragma unroll
-    for (int j = 0; j < VPL; ++j) {
-        const int e = lane + 64 * j;
-        l[j] = e < a.E ? row[e] : -INFINITY;
-        m = fmaxf(m, l[j]);  // NaN is skipped
-    }
-    double s[VPL], c[VPL];
-    if (a.sigmoid) {
-#pragma unroll
-        for (int j = 0; j < VPL; ++j) s[j] = 1.0 / (1.0 + exp(-(double)l[j]));
+        for (int j = 0; j < VPL; j += 4) {
+            const int e = sub * VPL + j;
+            const float4 x = *reinterpret_cast<const float4*>(row + (e < a.E ? e : 0));
+            const bool in = e < a.E;
+            l[j] = in ? x.x : -INFINITY, l[j + 1] = in ? x.y : -INFINITY;
+            l[j + 2] = in ? x.z : -INFINITY, l[j + 3] = in ? x.w : -INFINITY;
+        }
     } else {
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
-        double sum = 0.0;
+        for (int j = 0; j < VPL; ++j) {
+            const int e = sub * VPL + j;
+            const float x = row[e < a.E ? e : 0];
+            l[j] = e < a.E ? x : -INFINITY;
+        }
+    }
+    float bias[VPL];
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) bias[j] = a.bias ? a.bias[min(sub * VPL + j, a.E - 1)] : 0.0f;
+    double s[VPL], sum = 0.0;
+    float m = -INFINITY;
+    if (a.sigmoid) {
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) s[j] = recip(1.0 + exp_series(fmin(fmax(-(double)l[j], -700.0), 700.0)));
+    } else {
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) m = fmaxf(m, l[j]);  // NaN is skipped
+        m = sub_max<SUB>(m);
 #pragma unroll
         for (int j = 0; j < VPL; ++j) {
-            s[j] = l[j] == m ? 1.0 : exp((double)l[j] - (double)m);  // several +inf share
+            s[j] = l[j] == m ? 1.0 : exp_series(fmax((double)l[j] - (double)m, -745.0));  // several +inf share
             sum += l[j] > -INFINITY ? s[j] : 0.0;
         }
+        sum = sub_sum<SUB>(sum);
+        const double per = recip(fmax(sum, 1.0));
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) sum += shfl_xor_f64(sum, o);
-#pragma unroll
-        for (int j = 0; j < VPL; ++j) s[j] = s[j] / sum;
+        for (int j = 0; j < VPL; ++j) s[j] *= per;
     }
+    uint64_t key[VPL];
+    uint32_t id[VPL];
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
-        const int e = lane + 64 * j;
-        c[j] = s[j] + (a.bias && e < a.E ? (double)a.bias[e] : 0.0);
-        if (!(l[j] > -INFINITY) || !(c[j] == c[j])) c[j] = none;  // -inf, NaN: never chosen
+        const double c = s[j] + (double)bias[j];
+        const bool ok = l[j] > -INFINITY && c > none;  // -inf, NaN: never chosen
+        key[j] = key_of(c, ok);
+        id[j] = sub * VPL + j;
+        s[j] = ok ? c : none;
     }
 
     if (a.n_groups > 1) {
-        double* w = lds + wave * a.E;
+        double* w = lds + (wave * 64 + first) * VPL;
 #pragma unroll
-        for (int j = 0; j < VPL; ++j)
-            if (lane + 64 * j < a.E) w[lane + 64 * j] = c[j];
-        wave_lds_fence();
-        // the group's two best, by lane g < n_groups
+        for (int j = 0; j < VPL; ++j) w[sub * VPL + j] = s[j];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");  // read by the wave's other lanes below
+        __builtin_amdgcn_wave_barrier();
+        // P lanes to a group: its two best
+        const int P = SUB >> (32 - __clz(a.n_groups - 1)), g = sub / P;
         double b1 = none, b2 = none;
-        if (lane < a.n_groups)
-            for (int i = 0; i < a.group_size; ++i) {
-                const double v = w[lane * a.group_size + i];
+        if (g < a.n_groups)
+            for (int i = sub & (P - 1); i < a.group_size; i += P) {
+                const double v = w[g * a.group_size + i];
                 b2 = fmax(b2, fmin(b1, v));
                 b1 = fmax(b1, v);
             }
+        sub_top2<SUB>(b1, b2, P);
         const double gs = a.group_rank == 2 && b2 > none ? b1 + b2 : b1;
         // open: fewer than top_groups groups are ahead of it
         int ahead = 0;
-        for (int g = 0; g < a.n_groups; ++g) {
-            const double o = shfl_f64(gs, g);
-            ahead += o > gs || (o == gs && g < lane);
+        for (int o = 0; o < a.n_groups; ++o) {
+            const long long x = __double_as_longlong(gs);
+            const int from = first + o * P, lo = __shfl((int)x, from), hi = __shfl((int)(x >> 32), from);
+            const double v = __longlong_as_double(((long long)hi << 32) | (uint32_t)lo);
+            ahead += v > gs || (v == gs && o < g);
         }
-        const uint64_t open = __ballot(lane < a.n_groups && ahead < a.top_groups);
+        const uint64_t open = __ballot(ahead < a.top_groups) >> first;
+        const uint32_t per = ((1u << 20) + a.group_size - 1) / a.group_size;  // e / group_size, for e * group_size < 2^20
 #pragma unroll
         for (int j = 0; j < VPL; ++j) {
-            const int e = lane + 64 * j;
-            if (e < a.E && !((open >> (e / a.group_size)) & 1)) c[j] = none;
+            const uint32_t of = (sub * VPL + j) * per >> 20;
+            if (!((open >> min(of * P, 63u)) & 1)) key[j] = 0;
         }
     }
 
-    int id = 0;
-    double wt = 0.0;  // lane r holds the r-th chosen
+    // the lane's experts by falling key; neighbours change only where the second is larger, so that equal ones keep their order
+#pragma unroll
+    for (int i = VPL - 1; i > 0; --i)
+#pragma unroll
+        for (int j = 0; j < i; ++j) {
+            const bool swap = key[j + 1] > key[j];
+            const uint64_t k0 = key[j], k1 = key[j + 1];
+            const uint32_t i0 = id[j], i1 = id[j + 1];
+            key[j] = swap ? k1 : k0;
+            key[j + 1] = swap ? k0 : k1;
+            id[j] = swap ? i1 : i0;
+            id[j + 1] = swap ? i0 : i1;
+        }
+
+    int* out = chosen + wave * 64 + first;
+    int found = 0;
     for (int r = 0; r < a.k; ++r) {
-        double bc = none;
-        int bi = 0x7FFFFFFF;
-#pragma unroll
-        for (int j = 0; j < VPL; ++j)
-            if (c[j] > bc) {
-                bc = c[j];
-                bi = lane + 64 * j;
-            }
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const double oc = shfl_xor_f64(bc, o);
-            const int oi = __shfl_xor(bi, o);
-            if (oc > bc || (oc == bc && oi < bi)) {
-                bc = oc;
-                bi = oi;
-            }
+        const uint32_t top = sub_max<SUB>((uint32_t)(key[0] >> 32));
+        const bool here = (uint32_t)(key[0] >> 32) == top && top;
+        constexpr uint64_t MINE = ~0ull >> (64 - SUB);
+        uint64_t set = __ballot(here) >> first & MINE;
+        if (__ballot(__popcll(set) > 1)) {  // equal upper halves: rare
+            const uint32_t low = sub_max<SUB>(here ? (uint32_t)key[0] : 0u);
+            set = __ballot(here && (uint32_t)key[0] == low) >> first & MINE;
         }
-        if (bi == 0x7FFFFFFF) break;  // none left (uniform)
-        double sv = 0.0;
+        found += set != 0;  // 0: none left for this token
+        if (sub == __ffsll((unsigned long long)set) - 1) {
+            out[r] = (int)id[0];
 #pragma unroll
-        for (int j = 0; j < VPL; ++j)
-            if (bi == lane + 64 * j) {
-                c[j] = none;
-                sv = s[j];
+            for (int j = 0; j + 1 < VPL; ++j) {
+                key[j] = key[j + 1];
+                id[j] = id[j + 1];
             }
-        sv = shfl_f64(sv, bi & 63);
-        if (lane == r) {
-            id = bi;
-            wt = sv;
+            key[VPL - 1] = 0;
         }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+    int e = 0;
+    double wt = 0.0;  // lane r holds the r-th chosen
+    if (sub < found) {
+        e = out[sub];
+        const double x = row[e];
+        wt = a.sigmoid ? 1.0 / (1.0 + exp(-x)) : (x == (double)m ? 1.0 : exp(x - (double)m)) / sum;
     }
     if (a.renorm) {
-        double sum = wt;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) sum += shfl_xor_f64(sum, o);
-        wt = sum > 0.0 ? wt / sum : 0.0;
+        const double total = sub_sum<SUB>(wt);
+        wt = total > 0.0 ? wt / total : 0.0;
     }
-    if (lane < a.k) {
-        a.ids[token * a.k + lane] = id;
-        a.wts[token * a.k + lane] = (float)(wt * a.scale * (a.escale ? (double)a.escale[id] : 1.0));
+    if (sub < a.k && wanted < a.n) {
+        a.ids[(int64_t)token * a.k + sub] = e;
+        a.wts[(int64_t)token * a.k + sub] = (float)(wt * a.scale * (a.escale ? (double)a.escale[e] : 1.0));
     }
+}
+
+template <int SUB, int VPL>
+void launch_route(const RouteArgs& a, void* stream) {
+    constexpr int TOKENS = 4 * (64 / SUB);
+    const size_t lds = a.n_groups > 1 ? 256 * VPL * sizeof(double) : 0;
+    hipLaunchKernelGGL((k_route_experts<SUB, VPL>), dim3((unsigned)((a.n + TOKENS - 1) / TOKENS)), dim3(256), lds,
+                       static_cast<hipStream_t>(stream), a);
 }
 
 }  // namespace
@@ -200,21 +331,23 @@ extern "C" int ft_hip_route_experts(ft_hip_ctx* ctx, void* stream, const float* 
     if (!ctx || !logits || !ids || !wts) return fail(FT_HIP_E_INVALID, "route_experts: null argument");
     if (n_seqs == 0) return FT_HIP_OK;
     const RouteArgs a{logits, logits_stride, bias, expert_scale, ids, wts, score == FT_SCORE_SIGMOID, (int)G,
-                      (int)(E / G), (int)top_groups, group_rank, renorm, (double)scale, (int)E, (int)top_k, n_seqs};
+                      (int)(E / G), (int)top_groups, group_rank, renorm, (double)scale, (int)E, (int)top_k, (int)n_seqs,
+                      reinterpret_cast<uintptr_t>(logits) % 16 == 0 && logits_stride % 4 == 0 && E % 4 == 0};
     DeviceGuard on(ctx->device);
     if (!on.ok) return fail(FT_HIP_E_DEVICE, "route_experts: device %d cannot be made current", ctx->device);
-    const dim3 grid((unsigned)((n_seqs + 3) / 4)), block(256);
-    const size_t lds = G > 1 ? 4 * (size_t)E * sizeof(double) : 0;
-    hipStream_t s = static_cast<hipStream_t>(stream);
-    if (E <= 64)
-        hipLaunchKernelGGL(k_route_experts<1>, grid, block, lds, s, a);
-    else if (E <= 128)
-        hipLaunchKernelGGL(k_route_experts<2>, grid, block, lds, s, a);
+    // as few lanes to a token as hold its experts four to a lane, and one lane each for its groups and its choices
+    const int64_t lanes = std::max({(E + 3) / 4, (long long)G, (long long)top_k});
+    if (lanes <= 8)
+        launch_route<8, 4>(a, stream);
+    else if (lanes <= 16)
+        launch_route<16, 4>(a, stream);
+    else if (lanes <= 32)
+        launch_route<32, 4>(a, stream);
     else if (E <= 256)
-        hipLaunchKernelGGL(k_route_experts<4>, grid, block, lds, s, a);
+        launch_route<64, 4>(a, stream);
     else if (E <= 512)
-        hipLaunchKernelGGL(k_route_experts<8>, grid, block, lds, s, a);
+        launch_route<64, 8>(a, stream);
     else
-        hipLaunchKernelGGL(k_route_experts<16>, grid, block, lds, s, a);
+        launch_route<64, 16>(a, stream);
     return launch_status("route_experts");
 }

@@ -617,12 +617,6 @@ __device__ __forceinline__ bool vec_row(const void* row) {
     return (reinterpret_cast<uintptr_t>(row) & (TYPE == FT_TYPE_F32 ? 15 : 7)) == 0;
 }
 
-// The value in scalar registers, whatever the compiler knows of it.
-__device__ __forceinline__ double scalar(double v) {
-    asm("" : "+s"(v));
-    return v;
-}
-
 // Workgroup (c, row): chunk c of the row in registers, VECS times four values
 // a thread; one pass over memory.
 template <int TYPE, int VECS>

@@ -90,4 +90,11 @@ __device__ __forceinline__ int wave_below(uint64_t set) {
     return __builtin_amdgcn_mbcnt_hi((uint32_t)(set >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)set, 0));
 }
 
+// The value in scalar registers, whatever the compiler knows of it (as a
+// literal, a constant of f64 costs two moves where it is used).
+__device__ __forceinline__ double scalar(double v) {
+    asm("" : "+s"(v));
+    return v;
+}
+
 }  // namespace ft
