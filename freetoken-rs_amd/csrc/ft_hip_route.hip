@@ -69,12 +69,17 @@ __device__ __forceinline__ void partner(double v, double& a, double& b) {
     a = __longlong_as_double(((long long)ah << 32) | (uint32_t)al);
     b = __longlong_as_double(((long long)bh << 32) | (uint32_t)bl);
 }
-template <int SUB, int STEP = 0>
-__device__ __forceinline__ double sub_sum(double v) {
+// Sum over the first P of a token's lanes (the others hold 0) or over aligned
+// runs of P, P a power of two up to SUB.
+template <int SUB, int STEP = 0, typename T>
+__device__ __forceinline__ T sub_sum(T v, int P = SUB) {
     if constexpr (1 << STEP < SUB) {
-        double a, b;
-        partner<STEP>(v, a, b);
-        return sub_sum<SUB, STEP + 1>(a + b);
+        if (1 << STEP < P) {
+            T a, b;
+            partner<STEP>(v, a, b);
+            v = a + b;
+        }
+        return sub_sum<SUB, STEP + 1>(v, P);
     }
     return v;
 }
@@ -87,14 +92,32 @@ __device__ __forceinline__ float sub_max(float v) {
     }
     return v;
 }
-template <int SUB, int STEP = 0>
+template <int SUB>
 __device__ __forceinline__ uint32_t sub_max(uint32_t v) {
-    if constexpr (1 << STEP < SUB) {
+    v = row_max16<(SUB < 16)>(v);
+    if constexpr (SUB >= 32) {
         int a, b;
-        partner<STEP>((int)v, a, b);
-        return sub_max<SUB, STEP + 1>(max((uint32_t)a, (uint32_t)b));
+        partner<4>((int)v, a, b);
+        v = max((uint32_t)a, (uint32_t)b);
+    }
+    if constexpr (SUB >= 64) {
+        int a, b;
+        partner<5>((int)v, a, b);
+        v = max((uint32_t)a, (uint32_t)b);
     }
     return v;
+}
+// Of values that are no NaN: without the maximum with itself that fmax takes
+// first of a value from memory. The wait is for a DPP move of the result.
+__device__ __forceinline__ double max_of(double a, double b) {
+    double r;
+    asm("v_max_f64 %0, %1, %2\n\ts_nop 1" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+__device__ __forceinline__ double min_of(double a, double b) {
+    double r;
+    asm("v_min_f64 %0, %1, %2\n\ts_nop 1" : "=v"(r) : "v"(a), "v"(b));
+    return r;
 }
 // The two largest of P lanes' pairs (P a power of two up to SUB).
 template <int SUB, int STEP = 0>
@@ -104,8 +127,8 @@ __device__ __forceinline__ void sub_top2(double& b1, double& b2, int P) {
             double a1, c1, a2, c2;
             partner<STEP>(b1, a1, c1);
             partner<STEP>(b2, a2, c2);
-            b1 = fmax(a1, c1);
-            b2 = fmax(fmin(a1, c1), fmax(a2, c2));
+            b1 = max_of(a1, c1);
+            b2 = max_of(min_of(a1, c1), max_of(a2, c2));
         }
         sub_top2<SUB, STEP + 1>(b1, b2, P);
     }
@@ -131,17 +154,35 @@ __device__ __forceinline__ double exp_series(double x) {
     p = fma(fma(fma(p, r, 0.5), r, 1.0), r, 1.0);
     return ldexp(p, (int)__double_as_longlong(t));
 }
-__device__ __forceinline__ double recip(double x) {  // of finite x >= 1
+__device__ __forceinline__ double recip(double x) {  // of x in [1e-290, 1e305]
     double y = __builtin_amdgcn_rcp(x);
     y = fma(fma(-x, y, 1.0), y, y);
     return fma(fma(-x, y, 1.0), y, y);
 }
 
-// A key that rises with c; 0: not to be chosen.
-__device__ __forceinline__ uint64_t key_of(double c, bool ok) {
+// A key that rises with c, its last bits (`bits`) replaced by `place`; 0: not to be chosen.
+__device__ __forceinline__ uint64_t key_of(double c, bool ok, uint32_t bits, uint32_t place) {
     const uint64_t b = (uint64_t)__double_as_longlong(c);
-    const uint64_t key = b ^ ((uint64_t)((int64_t)b >> 63) | 0x8000000000000000ull);
+    const uint64_t key = ((b ^ ((uint64_t)((int64_t)b >> 63) | 0x8000000000000000ull)) & ~(uint64_t)bits) | place;
     return ok ? key : 0;
+}
+
+// N keys by falling size (odd-even merge sort).
+template <int N>
+__device__ __forceinline__ void sort_falling(uint64_t key[N]) {
+#pragma unroll
+    for (int p = 1; p < N; p <<= 1)
+#pragma unroll
+        for (int k = p; k >= 1; k >>= 1)
+#pragma unroll
+            for (int j = k % p; j + k < N; j += 2 * k)
+#pragma unroll
+                for (int i = 0; i < k; ++i)
+                    if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+                        const uint64_t x = key[i + j], y = key[i + j + k];
+                        key[i + j] = y > x ? y : x;
+                        key[i + j + k] = y > x ? x : y;
+                    }
 }
 
 template <int SUB, int VPL>
@@ -195,14 +236,14 @@ __global__ __launch_bounds__(256) void k_route_experts(RouteArgs a) {
 #pragma unroll
         for (int j = 0; j < VPL; ++j) s[j] *= per;
     }
+    // a key's last bits are the expert's place in its lane, the first the largest: c of a lane that differ by less than
+    // 2^-48 of themselves count as equal
     uint64_t key[VPL];
-    uint32_t id[VPL];
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
         const double c = s[j] + (double)bias[j];
         const bool ok = l[j] > -INFINITY && c > none;  // -inf, NaN: never chosen
-        key[j] = key_of(c, ok);
-        id[j] = sub * VPL + j;
+        key[j] = key_of(c, ok, VPL - 1, VPL - 1 - j);
         s[j] = ok ? c : none;
     }
 
@@ -218,42 +259,30 @@ __global__ __launch_bounds__(256) void k_route_experts(RouteArgs a) {
         if (g < a.n_groups)
             for (int i = sub & (P - 1); i < a.group_size; i += P) {
                 const double v = w[g * a.group_size + i];
-                b2 = fmax(b2, fmin(b1, v));
-                b1 = fmax(b1, v);
+                b2 = max_of(b2, min_of(b1, v));
+                b1 = max_of(b1, v);
             }
         sub_top2<SUB>(b1, b2, P);
         const double gs = a.group_rank == 2 && b2 > none ? b1 + b2 : b1;
-        // open: fewer than top_groups groups are ahead of it
+        // open: fewer than top_groups groups are ahead of it; its lanes ask a part of the others each
         int ahead = 0;
-        for (int o = 0; o < a.n_groups; ++o) {
+        for (int o = sub & (P - 1); o - (sub & (P - 1)) < a.n_groups; o += P) {
             const long long x = __double_as_longlong(gs);
-            const int from = first + o * P, lo = __shfl((int)x, from), hi = __shfl((int)(x >> 32), from);
+            const int from = first + min(o, a.n_groups - 1) * P, lo = __shfl((int)x, from), hi = __shfl((int)(x >> 32), from);
             const double v = __longlong_as_double(((long long)hi << 32) | (uint32_t)lo);
-            ahead += v > gs || (v == gs && o < g);
+            ahead += o < a.n_groups && (v > gs || (v == gs && o < g));
         }
+        ahead = sub_sum<SUB>(ahead, P);
         const uint64_t open = __ballot(ahead < a.top_groups) >> first;
         const uint32_t per = ((1u << 20) + a.group_size - 1) / a.group_size;  // e / group_size, for e * group_size < 2^20
 #pragma unroll
         for (int j = 0; j < VPL; ++j) {
-            const uint32_t of = (sub * VPL + j) * per >> 20;
+            const uint32_t of = __umul24(sub * VPL + j, per) >> 20;
             if (!((open >> min(of * P, 63u)) & 1)) key[j] = 0;
         }
     }
 
-    // the lane's experts by falling key; neighbours change only where the second is larger, so that equal ones keep their order
-#pragma unroll
-    for (int i = VPL - 1; i > 0; --i)
-#pragma unroll
-        for (int j = 0; j < i; ++j) {
-            const bool swap = key[j + 1] > key[j];
-            const uint64_t k0 = key[j], k1 = key[j + 1];
-            const uint32_t i0 = id[j], i1 = id[j + 1];
-            key[j] = swap ? k1 : k0;
-            key[j + 1] = swap ? k0 : k1;
-            id[j] = swap ? i1 : i0;
-            id[j + 1] = swap ? i0 : i1;
-        }
-
+    sort_falling<VPL>(key);
     int* out = chosen + wave * 64 + first;
     int found = 0;
     for (int r = 0; r < a.k; ++r) {
@@ -262,17 +291,14 @@ __global__ __launch_bounds__(256) void k_route_experts(RouteArgs a) {
         constexpr uint64_t MINE = ~0ull >> (64 - SUB);
         uint64_t set = __ballot(here) >> first & MINE;
         if (__ballot(__popcll(set) > 1)) {  // equal upper halves: rare
-            const uint32_t low = sub_max<SUB>(here ? (uint32_t)key[0] : 0u);
-            set = __ballot(here && (uint32_t)key[0] == low) >> first & MINE;
+            const uint32_t own = here ? (uint32_t)key[0] | (VPL - 1) : 0u, low = sub_max<SUB>(own);
+            set = __ballot(here && own == low) >> first & MINE;  // of equal c the lowest lane's
         }
         found += set != 0;  // 0: none left for this token
         if (sub == __ffsll((unsigned long long)set) - 1) {
-            out[r] = (int)id[0];
+            out[r] = sub * VPL + (VPL - 1) - (int)((uint32_t)key[0] & (VPL - 1));
 #pragma unroll
-            for (int j = 0; j + 1 < VPL; ++j) {
-                key[j] = key[j + 1];
-                id[j] = id[j + 1];
-            }
+            for (int j = 0; j + 1 < VPL; ++j) key[j] = key[j + 1];
             key[VPL - 1] = 0;
         }
     }
@@ -283,11 +309,15 @@ __global__ __launch_bounds__(256) void k_route_experts(RouteArgs a) {
     if (sub < found) {
         e = out[sub];
         const double x = row[e];
-        wt = a.sigmoid ? 1.0 / (1.0 + exp(-x)) : (x == (double)m ? 1.0 : exp(x - (double)m)) / sum;
+        // as above; where that is far out, by the full functions, which end in 0
+        if (a.sigmoid)
+            wt = x > -700.0 ? recip(1.0 + exp_series(fmax(-x, -700.0))) : 1.0 / (1.0 + exp(-x));
+        else
+            wt = x == (double)m ? 1.0 / sum : (x - (double)m > -700.0 ? exp_series(x - (double)m) : exp(x - (double)m)) * recip(sum);
     }
     if (a.renorm) {
-        const double total = sub_sum<SUB>(wt);
-        wt = total > 0.0 ? wt / total : 0.0;
+        const double total = sub_sum<SUB>(wt, 1 << (32 - __clz(max(a.k - 1, 0))));
+        wt = total > 1e-290 ? wt * recip(total) : total > 0.0 ? wt / total : 0.0;
     }
     if (sub < a.k && wanted < a.n) {
         a.ids[(int64_t)token * a.k + sub] = e;
@@ -335,8 +365,10 @@ extern "C" int ft_hip_route_experts(ft_hip_ctx* ctx, void* stream, const float* 
                       reinterpret_cast<uintptr_t>(logits) % 16 == 0 && logits_stride % 4 == 0 && E % 4 == 0};
     DeviceGuard on(ctx->device);
     if (!on.ok) return fail(FT_HIP_E_DEVICE, "route_experts: device %d cannot be made current", ctx->device);
-    // as few lanes to a token as hold its experts four to a lane, and one lane each for its groups and its choices
-    const int64_t lanes = std::max({(E + 3) / 4, (long long)G, (long long)top_k});
+    // As few lanes to a token as hold its experts four to a lane, and one lane each for its groups and its choices.
+    // (Eight to a lane need a fifth fewer instructions, but each wave's chain of selections is longer: 16384 tokens over
+    // 256 experts 24.9 us against 23.5, 5003 over 128 8.6 against 7.4.)
+    const int64_t lanes = std::max({(E + 3) / 4, G, (long long)top_k});
     if (lanes <= 8)
         launch_route<8, 4>(a, stream);
     else if (lanes <= 16)

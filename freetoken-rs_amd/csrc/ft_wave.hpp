@@ -64,13 +64,25 @@ __device__ __forceinline__ float wave_move(float v) {  // v itself where nothing
 // Largest of a row's 16 lanes, in each of them, of a value that is no NaN: a
 // step is one instruction, where fmaxf on a moved value takes three (the move
 // and a maximum with itself, for signalling NaNs). A DPP operand may be read
-// two wait states after it is written.
+// two wait states after it is written, also by what follows the asm, which the
+// compiler does not look into.
 __device__ __forceinline__ float row_max16(float v) {
     asm("s_nop 1\n\tv_max_f32_dpp %0, %0, %0 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n\t"
         "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n\t"
         "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_half_mirror row_mask:0xf bank_mask:0xf\n\t"
-        "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_mirror row_mask:0xf bank_mask:0xf"
+        "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_mirror row_mask:0xf bank_mask:0xf\n\ts_nop 1"
         : "+v"(v));
+    return v;
+}
+
+// The same of whole numbers; EIGHT: of 8 lanes.
+template <bool EIGHT>
+__device__ __forceinline__ uint32_t row_max16(uint32_t v) {
+    asm("s_nop 1\n\tv_max_u32_dpp %0, %0, %0 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n\t"
+        "s_nop 1\n\tv_max_u32_dpp %0, %0, %0 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n\t"
+        "s_nop 1\n\tv_max_u32_dpp %0, %0, %0 row_half_mirror row_mask:0xf bank_mask:0xf\n\ts_nop 1"
+        : "+v"(v));
+    if (!EIGHT) asm("s_nop 1\n\tv_max_u32_dpp %0, %0, %0 row_mirror row_mask:0xf bank_mask:0xf\n\ts_nop 1" : "+v"(v));
     return v;
 }
 

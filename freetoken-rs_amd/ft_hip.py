@@ -188,15 +188,19 @@ def _rows(t, n, width, size, what):
         return None, 0
     if t.element_size() != size:
         raise FtHipError(E_INVALID, f"{what}: {t.dtype} has not {size} bytes a value")
-    if t.dim() == 2:
-        rows, cols = t.shape
-        stride = t.stride(0) if rows > 1 else max(cols, width)
-        ok = rows >= n and cols >= width and (cols == 1 or t.stride(1) == 1)
+    shape = t.shape
+    if len(shape) == 2:
+        rows, stride = shape
+        ok = rows >= n and stride >= width
+        if ok and not t.is_contiguous():
+            ok = stride == 1 or t.stride(1) == 1
+            if rows > 1:
+                stride = t.stride(0)
     else:
-        stride, ok = width, t.is_contiguous() and t.numel() >= n * width
-    if n > 0 and not ok:
-        raise FtHipError(E_SHAPE, f"{what}: {tuple(t.shape)} does not hold {n} rows of {width} consecutive values")
-    return ctypes.c_void_p(t.data_ptr()), stride
+        stride, ok = width, t.numel() >= n * width and t.is_contiguous()
+    if not ok and n > 0:
+        raise FtHipError(E_SHAPE, f"{what}: {tuple(shape)} does not hold {n} rows of {width} consecutive values")
+    return t.data_ptr(), stride
 
 
 class Q4Gemv:
@@ -227,7 +231,7 @@ class Q4Gemv:
         if stream is None:
             import torch
             stream = torch.cuda.current_stream(self.device)
-        return ctypes.c_void_p(stream.cuda_stream)
+        return stream.cuda_stream
 
     # -- ft-model/src/lib.rs:1358-1367: the section's norm, with the addition before and the q8 after it --
     def add_rmsnorm(self, x, w, hidden, n, eps, residual=None, h=None, y=None, q8=None, x_w=None, stream=None):
