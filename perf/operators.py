@@ -245,8 +245,9 @@ def run(st):
         if case["kind"] == "norm":
             g.add_rmsnorm(st["x"], st["w"], case["hidden"], case["n"], EPS, residual=st["residual"], h=st["h"],
                           y=st["y"], q8=st["q8"], x_w=st["x_w"])
-            out = _blocks(st["q8"], case["n"], case["hidden"])
-            out["h"] = st["h"]
+            if "blocks" not in st:  # views of the buffer that it keeps
+                st["blocks"] = _blocks(st["q8"], case["n"], case["hidden"])
+            out = dict(st["blocks"], h=st["h"])
             if case["y"]:
                 out["y"] = st["y"]
             return out
