@@ -203,7 +203,9 @@ def bench_dense(args, g):
     GELU*up and the q8, and two (ft_hip_gemv_q4r_f32in: the gate|up GEMV with
     the q8 of x in its launch and GELU*up as its f32 second output, the down
     GEMV with the q8 of that in its launch) (config.shared_mlp_chain_us; the
-    token with the fastest chain: config.us_per_token_with_shared_chain)."""
+    token with the fastest chain: config.us_per_token_with_shared_chain), and
+    the chain behind the last layer: its norm with the q8 of the result, lm_head
+    and the draw of a token (config.head_chain_us)."""
     import numpy as np
     import torch
     import ft_hip
@@ -321,6 +323,28 @@ def bench_dense(args, g):
     torch.cuda.synchronize()
     floor_us = ev0.elapsed_time(ev1) * 1000.0 / args.steps
     log(f"[dense] launch floor (1 x 32 matrix): {floor_us:.2f} us/launch")
+    # from the residual stream to the next token: the last norm with its q8, lm_head, the draw (top-k 64, top-p 0.95)
+    V, H = moe_synth.DENSE["lm_head"]
+    head = moe_synth.VocabHead(g, moe_synth.dense_weights(g, "lm_head", device=dev), torch.ones(H, device=dev), V, H, 1)
+    rng = np.random.default_rng(11)
+    branch, residual = (torch.from_numpy(rng.standard_normal((1, H)).astype(np.float32)).to(dev) for _ in range(2))
+    draw = {"u": torch.full((1,), 0.5, device=dev), "temperature": torch.full((1,), 0.8, device=dev),
+            "top_k": torch.full((1,), 64, dtype=torch.int32, device=dev), "top_p": torch.full((1,), 0.95, device=dev)}
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        head.run(branch, residual, 1, stream=stream, **draw)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            for _ in range(args.steps):
+                head.run(branch, residual, 1, stream=stream, **draw)
+        graph.replay()
+        ev0, ev1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        ev0.record(stream)
+        graph.replay()
+        ev1.record(stream)
+    torch.cuda.synchronize()
+    head_us = ev0.elapsed_time(ev1) * 1000.0 / args.steps
+    log(f"[dense] last norm, lm_head and the draw: {head_us:.2f} us")
     L = moe_synth.GEMMA.n_layers
     layer = ["qkv", "o_proj", "shared_gate_up", "shared_down"]
     tok_us = L * sum(per[n]["us"] for n in layer) + per["lm_head"]["us"]
@@ -339,6 +363,7 @@ def bench_dense(args, g):
         "config": {"workload": "dense q4r GEMVs of the Gemma-4-26B-A4B-shaped decode step, batch 1",
                    "name": "dense", "gemvs": per, "layers": L, "gemv_lanes": args.gemv_lanes or "auto",
                    "launch_floor_us": round(floor_us, 3), "shared_mlp_chain_us": chains,
+                   "head_chain_us": round(head_us, 2),
                    "us_per_token_with_shared_chain": round(tok_chain_us, 2)},
         "achieved_GBps": round(tok_bytes / (tok_us * 1e-6) / 1e9, 1),
         "hbm_frac": round(tok_bytes / (tok_us * 1e-6) / 1e9 / HBM_PEAK_GBPS, 4),

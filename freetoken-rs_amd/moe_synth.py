@@ -355,3 +355,71 @@ class BatchedStack:
         self.g.moe_stack_grouped(x_in, x_out, n_seqs, self.max_seqs, s.hidden, s.inter, s.n_experts, s.top_k,
                                  self.m.L, self.f.banks, self.m.routers, self.m.bias, None, ids, wts, self.ws,
                                  stream)
+
+
+class VocabHead:
+    """From the residual stream to the next tokens: the last norm with its q8
+    blocks, the vocabulary head's q4r GEMV (one row set for every sequence) and
+    the draw, for up to max_seqs sequences. weights: [vocab] q4r rows of hidden."""
+
+    def __init__(self, gemv, weights, norm_w, vocab, hidden, max_seqs, eps=1e-6):
+        self.g, self.weights, self.norm_w, self.vocab, self.H, self.eps = gemv, weights, norm_w, vocab, hidden, eps
+        dev = weights.device
+        self.q8 = torch.empty(max_seqs * hidden // 32 * ft_hip.Q8_BLK, dtype=torch.uint8, device=dev)
+        self.logits = torch.empty((max_seqs, vocab), dtype=torch.float32, device=dev)
+        self.slots = torch.zeros(max_seqs, dtype=torch.int32, device=dev)
+        self.tokens = torch.empty(max_seqs, dtype=torch.int32, device=dev)
+        self.logprobs = torch.empty(max_seqs, dtype=torch.float32, device=dev)
+        self.ws = torch.empty(gemv.sample_tokens_workspace_bytes(vocab, max_seqs), dtype=torch.uint8, device=dev)
+
+    def run(self, branch, residual, n_seqs, u, temperature=None, top_k=None, top_p=None, min_p=None, stream=None):
+        """tokens (and log probabilities) of n_seqs sequences from residual + branch (residual None: branch alone)."""
+        self.g.add_rmsnorm(branch, self.norm_w, self.H, n_seqs, self.eps, residual=residual, q8=self.q8, stream=stream)
+        self.g.gemv_q4r_idx(self.weights, 0, 0, self.slots, None, n_seqs, self.q8, self.H // 32, self.logits,
+                            self.vocab, self.vocab, self.H, stream=stream)
+        self.g.sample_tokens(self.logits, self.vocab, n_seqs, u, self.tokens, self.ws, temperature, top_k, top_p, min_p,
+                             self.logprobs, stream=stream)
+        return self.tokens[:n_seqs], self.logprobs[:n_seqs]
+
+
+class RoutedStack:
+    """A batch through a SyntheticMoE's layers with the routing of route_experts
+    (`route`: its keyword arguments) in place of the layer entry points' softmax
+    over the top-k. Per layer: the addition and norm (f32 row for the router, q8
+    for the experts), router logits, routing, the pairs' gate|up and down GEMVs
+    and their weighted sum, which is the next layer's branch."""
+
+    def __init__(self, model, max_seqs, norm_w=None, eps=1e-6, **route):
+        s, dev = model.shape, model.device
+        self.m, self.g, self.eps, self.route, self.norm_w = model, model.g, eps, route, norm_w
+        p = max_seqs * s.top_k
+        f32 = lambda *shape: torch.empty(shape, dtype=torch.float32, device=dev)  # noqa: E731
+        u8 = lambda n: torch.empty(n, dtype=torch.uint8, device=dev)  # noqa: E731
+        self.h, self.y, self.branch = f32(max_seqs, s.hidden), f32(max_seqs, s.hidden), f32(max_seqs, s.hidden)
+        self.logits, self.wts = f32(max_seqs, s.n_experts), f32(max_seqs, s.top_k)
+        self.ids = torch.empty((max_seqs, s.top_k), dtype=torch.int32, device=dev)
+        self.seq_of = torch.arange(p, dtype=torch.int32, device=dev) // s.top_k
+        self.q8x, self.q8a = u8(max_seqs * s.hidden // 32 * ft_hip.Q8_BLK), u8(p * s.inter // 32 * ft_hip.Q8_BLK)
+        self.down = f32(p, s.hidden)
+
+    def layer(self, l, branch, residual, n_seqs, stream=None):
+        """h = residual + branch; self.branch = the routed experts of norm(h)."""
+        g, m, s = self.g, self.m, self.m.shape
+        H, E, K, p = s.hidden, s.n_experts, s.top_k, n_seqs * s.top_k
+        bank = m.banks[l * E * m.expert_bytes:(l + 1) * E * m.expert_bytes]
+        g.add_rmsnorm(branch, None if self.norm_w is None else self.norm_w[l], H, n_seqs, self.eps, residual=residual,
+                      h=self.h, y=self.y, q8=self.q8x, stream=stream)
+        g.gemv_f32_rows_dev(m.routers[l], self.y, self.logits, H, E, n_seqs, stream=stream)
+        g.route_experts(self.logits, self.ids, self.wts, E, K, n_seqs, stream=stream, **self.route)
+        g.gemv_gate_up_act(bank, m.expert_bytes, self.ids, p, K, self.q8x, H, s.inter, self.q8a, m.layout, stream=stream)
+        g.gemv_grouped_slots(bank, m.expert_bytes, m.gu_bytes, self.ids, None, p, self.q8a, s.inter // 32, self.down, H,
+                             H, s.inter, m.layout, stream=stream)
+        self.branch[:n_seqs].zero_()
+        g.reduce_pairs_weighted(self.down, self.wts, self.seq_of, self.branch, H, p, n_seqs, stream=stream)
+
+    def run(self, x, n_seqs, stream=None):
+        """All layers: returns (branch, residual) of the last, what the next norm adds. A given stream has to be current
+        (the branch is cleared on it)."""
+        for l in range(self.m.L):
+            self.layer(l, x if l == 0 else self.branch, None if l == 0 else self.h, n_seqs, stream)
+        return self.branch, self.h
