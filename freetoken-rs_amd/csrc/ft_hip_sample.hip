@@ -505,36 +505,142 @@ __device__ __forceinline__ void sample_list(const SampleArgs& a, int64_t r, int 
     draw(a, r, list, 0, n, 0.0, -1.0, cut, s, M, l);
 }
 
-// Rows of at most LIST values: all of them in LDS, one launch.
+// The sum of the waves' counts before this wave's, and of all.
+__device__ __forceinline__ void waves_before(const int* counts, int& before, int& all) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int own = lane < ROW_WAVES ? counts[lane] : 0, scan = wave_scan(own);
+    before = wave_lane(scan - own, wave);
+    all = wave_lane(scan, 63);
+}
+
+// A value that at least k of the row's values reach, from the maxima of parts
+// of it (lowest: the smallest of these above -inf, or less): k parts have one
+// each. -inf if fewer than k parts hold any. Counted in 256 pieces of the key
+// range, and again in the piece that reaches k while that holds many more: a
+// range that goes below 0 has pieces of whole binades. l.n is 0 on entry.
+template <typename PARTS>
+__device__ __forceinline__ float reached_by(int k, const PARTS& parts, float lowest, float M, RowLds& l) {
+    const int lane = threadIdx.x & 63;
+    uint32_t hi = key_of(M), lo = key_of(lowest);
+    int base = 0;
+#pragma unroll 1
+    for (uint32_t* counts = l.n;; counts += 256) {
+        const uint32_t width = hi - lo;
+        const int shift = width < 256u ? 0 : 24 - __clz(width);
+        parts.each([&](float m, int) {
+            const uint32_t q = key_of(m);
+            if (m > -INFINITY && q >= lo && q <= hi) atomicAdd(&counts[(hi - q) >> shift], 1u);
+        });
+        __syncthreads();
+        int own[4], sum = 0;  // bins 4 lane ..
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum += own[i] = (int)counts[4 * lane + i];
+        const int scan = base + wave_scan(sum);
+        const uint64_t set = __ballot(scan >= k);
+        if (!set) return -INFINITY;
+        const int at = __ffsll((unsigned long long)set) - 1;
+        int b = 0, before = scan - sum;
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            if (b == i && before + own[i] < k) {
+                before += own[i];
+                ++b;
+            }
+        const int here = b == 0 ? own[0] : b == 1 ? own[1] : b == 2 ? own[2] : own[3];
+        b = 4 * at + wave_lane(b, at);
+        base = wave_lane(before, at);
+        const int through = base + wave_lane(here, at);
+        const uint64_t under = (((uint64_t)b + 1) << shift) - 1;
+        lo = under >= width ? lo : hi - (uint32_t)under;
+        hi -= (uint32_t)b << shift;
+        if (shift == 0 || through <= k + k / 2 + 32 || counts == l.n + 768) return of_key(lo);
+    }
+}
+
+// A thread's part of a row, by its maximum.
+struct Part {
+    float max;
+    template <typename F>
+    __device__ __forceinline__ void each(const F& fn) const {
+        fn(max, 0);
+    }
+};
+
+// A little less than the value whose e is x: what is below has less for sure.
+__device__ __forceinline__ float value_below(double x, const Row& s, float M) {
+    const double d = log(x) / s.inv_t, v = (double)M + d - 1e-6 * (fabs((double)M) + fabs(d));
+    return v > -(double)FLT_MAX ? (float)v : -INFINITY;  // also where inf meets -inf
+}
+
+// Rows of at most LIST values, one launch: in registers, a run of 512 to a
+// wave; those that may be kept go into the list.
 template <int TYPE>
 __global__ __launch_bounds__(ROW_THREADS) void k_sample_rows(SampleArgs a) {
     __shared__ RowLds l;
+    constexpr int N = LIST / ROW_THREADS;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, first = wave * 64 * N + lane;
     const int64_t r = blockIdx.x;
-    const Row s = row_of(a, r);
     const void* row = row_at<TYPE>(a, r);
-    init_range(l);
-    __syncthreads();
-    float m = -INFINITY, lowest = INFINITY;
-    for (int i = threadIdx.x; i < a.V; i += ROW_THREADS) {
-        const float v = logit<TYPE>(row, i);
-        l.v[i] = v;
-        l.i[i] = i;
-        m = fmaxf(m, v);  // NaN is skipped
-        if (v > -INFINITY) lowest = fminf(lowest, v);
+    float v[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const int i = first + 64 * j;
+        const float x = logit<TYPE>(row, i < a.V ? i : 0);
+        v[j] = i < a.V && x > -INFINITY ? x : -INFINITY;  // NaN too
     }
-    if (threadIdx.x == 0) l.pick = 0x7FFFFFFF;
-    block_range(m, lowest, l);
-    if (m == -INFINITY) return answer(a, r, -1, NAN);
+    init_range(l);
+    if (t == 0) l.pick = 0x7FFFFFFF;
+    l.n[t] = 0;
+    const Row s = row_of(a, r);
+    __syncthreads();
+    float top = -INFINITY;  // of the thread's
+#pragma unroll
+    for (int j = 0; j < N; ++j) top = fmaxf(top, v[j]);
+    float M = top, lowest = top > -INFINITY ? top : INFINITY;
+    block_range(M, lowest, l);
+    if (M == -INFINITY) return answer(a, r, -1, NAN);
     if (s.greedy) {
-        for (int i = threadIdx.x; i < a.V; i += ROW_THREADS)
-            if (l.v[i] == m) {
-                atomicMin(&l.pick, i);
-                break;
-            }
+#pragma unroll
+        for (int j = N - 1; j >= 0; --j)
+            if (v[j] == M) atomicMin(&l.pick, first + 64 * j);
         __syncthreads();
         return answer(a, r, l.pick, 0.0f);
     }
-    sample_list(a, r, a.V, 0.0, s, m, l);
+    const bool by_k = s.k < a.V, by_p = s.p < 1.0;
+    float from = -INFINITY;
+    if (by_k && s.k <= ROW_THREADS) from = reached_by(s.k, Part{top}, lowest, M, l);
+    if (by_p && !by_k) {  // values of less than (1 - p) z / V are together less than the (1 - p) z that top_p leaves out
+        double z = 0.0;
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (v[j] > -INFINITY) z += weight(v[j], M, s.inv_t);
+        from = value_below((1.0 - s.p) * (1.0 - 1e-9) * block_sum(z, l) / a.V, s, M);
+    }
+    if (s.m > 0.0 && !by_p) from = fmaxf(from, value_below(s.m, s, M));
+    from = fmaxf(from, -FLT_MAX);
+    double rest = 0.0;
+    int got = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        got += __popcll(__ballot(v[j] >= from));
+        if (by_p && !by_k && v[j] > -INFINITY && v[j] < from) rest += weight(v[j], M, s.inv_t);
+    }
+    if (lane == 0) l.parti[wave] = got;
+    __syncthreads();
+    int at, n;
+    waves_before(l.parti, at, n);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const uint64_t set = __ballot(v[j] >= from);
+        const int to = at + wave_below(set);
+        if (v[j] >= from) {
+            l.v[to] = v[j];
+            l.i[to] = first + 64 * j;
+        }
+        at += __popcll(set);
+    }
+    rest = block_sum(rest, l);  // its barriers also close the list
+    sample_list(a, r, n, rest, s, M, l);
 }
 
 // ---- longer rows: a scan by many workgroups, then one that finishes the row ----
@@ -773,14 +879,6 @@ struct Segs {
     }
 };
 
-// The sum of the waves' counts before this wave's, and of all.
-__device__ __forceinline__ void waves_before(const int* counts, int& before, int& all) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int own = lane < ROW_WAVES ? counts[lane] : 0, scan = wave_scan(own);
-    before = wave_lane(scan - own, wave);
-    all = wave_lane(scan, 63);
-}
-
 // The row's values in [from, to], by rising index, into the list, from the
 // segments whose maximum is at least `from`. Returns how many there are; more
 // than LIST: not all were taken.
@@ -878,32 +976,6 @@ __device__ __forceinline__ int gather(const void* row, int V, const Segs& segs, 
     return n;
 }
 
-// A value that at least k of the row's values reach, from the segments' maxima
-// (lowest: the smallest above -inf): k segments have one each. -inf if fewer
-// than k segments hold any. l.n[0..256) is 0 on entry.
-__device__ __forceinline__ float reached_by(int k, const Segs& segs, float lowest, float M, RowLds& l) {
-    const int lane = threadIdx.x & 63;
-    const uint32_t hi = key_of(M), width = hi - key_of(lowest);
-    const int shift = width < 256u ? 0 : 24 - __clz(width);
-    segs.each([&](float m, int) {
-        if (m > -INFINITY) atomicAdd(&l.n[(hi - key_of(m)) >> shift], 1u);
-    });
-    __syncthreads();
-    int own[4], sum = 0;  // bins 4 lane ..
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sum += own[i] = (int)l.n[4 * lane + i];
-    const int scan = wave_scan(sum);
-    const uint64_t set = __ballot(scan >= k);
-    if (!set) return -INFINITY;
-    const int at = __ffsll((unsigned long long)set) - 1;
-    int cum = scan - sum, b = 0;
-#pragma unroll
-    for (int i = 0; i < 3; ++i) b += (cum += own[i]) < k;
-    b = 4 * at + wave_lane(b, at);
-    const uint64_t under = (((uint64_t)b + 1) << shift) - 1;
-    return under >= width ? lowest : of_key(hi - (uint32_t)under);
-}
-
 // The smallest value whose bin is at most b (b < BINS), found 64 keys at a time.
 __device__ __forceinline__ float lowest_in(int b, float M, double g, double unit) {
     if (M == INFINITY) return M;
@@ -983,7 +1055,7 @@ __global__ __launch_bounds__(ROW_THREADS) void k_sample_finish(SampleArgs a, Sca
     segs.load(w.seg(blockIdx.x), w.segs);
     init_range(l);
     if (t == 0) l.pick = 0x7FFFFFFF;
-    if (t < 256) l.n[t] = 0;
+    l.n[t] = 0;
     const Row s = row_of(a, r);
     __syncthreads();
     const void* row = row_at<TYPE>(a, r);
@@ -1015,10 +1087,7 @@ __global__ __launch_bounds__(ROW_THREADS) void k_sample_finish(SampleArgs a, Sca
     if (by_maxima(s, V, w.segs)) {
         too_many = s.k > w.segs;
         from = too_many ? M : reached_by(s.k, segs, lowest, M, l);
-        if (s.m > 0.0 && !by_p) {  // values that min_p may keep; without top_p no sum needs the others
-            const double d = log(s.m) / s.inv_t, x = (double)M + d - 1e-6 * (fabs((double)M) + fabs(d));
-            if (x > (double)from) from = (float)x;
-        }
+        if (s.m > 0.0 && !by_p) from = fmaxf(from, value_below(s.m, s, M));  // without top_p no sum needs the others
     } else {
         double far = 0.0;
         for (int c = t; c < chunks; c += ROW_THREADS) {
