@@ -17,6 +17,10 @@
 // Bound by memory: x, the residual, h, y and the blocks each move once; the
 // row stays in registers between its sum and its outputs. Sums and scales are
 // f64 (its rate is f32's here), h and y are rounded to f32 once.
+//
+// Measured, kernel alone, hidden 2816, f32 in, h and q8 out: 1 row 2.4 us, 64
+// rows 3.4, 777 rows 7.2, 16384 rows 104 (5.9 TB/s; a copy of 256 MiB runs at
+// 5.0). Up to some hundred rows the time is a launch and one round trip.
 
 #include "ft_device.hpp"
 #include "ft_runtime.hpp"
@@ -195,7 +199,8 @@ __global__ __launch_bounds__(1024) void k_add_rmsnorm(NormArgs a) {
             if (i * step + t * V >= a.hidden) continue;
 #pragma unroll
             for (int e = 0; e < V; ++e)
-                h[i].v[e] = (float)fma((double)h[i].v[e] * inv, (double)xw[i].v[e], a.residual ? (double)r[i].v[e] : 0.0);
+                h[i].v[e] = (float)fma((double)h[i].v[e] * inv, (double)xw[i].v[e],
+                                       a.residual ? (double)r[i].v[e] : 0.0);
         }
     } else if (a.residual) {
 #pragma unroll
@@ -245,7 +250,8 @@ void launch_norm(const NormArgs& a, int64_t n, int64_t few, bool vec, void* stre
         return;
     }
     // few rows: as many threads on a row as it has vectors; many: four vectors a thread, so that what a wave does once
-    // a row (two sums, two square roots) is shared by more values
+    // a row (two sums, two square roots) is shared by more values. Hidden 2816: 64 rows 3.4 us against 4.0, 256 rows
+    // 4.0 against 4.5; 777 rows 7.7 against 7.0, 16384 rows 115 against 104.
     const int vecs = a.hidden / 4, wide = (vecs + 63) / 64 * 64;
     if (n <= few && vecs <= 1024)
         hipLaunchKernelGGL((k_add_rmsnorm<TYPE, 4, 1>), grid, dim3(wide), 0, s, a);
@@ -283,12 +289,19 @@ extern "C" int ft_hip_add_rmsnorm(ft_hip_ctx* ctx, void* stream, const void* x, 
         return fail(FT_HIP_E_SHAPE, "add_rmsnorm: a pointer is not aligned to its type (q8: 4 bytes)");
     if (!ctx || !x) return fail(FT_HIP_E_INVALID, "add_rmsnorm: null argument");
     if (!h && !y && !q8) return fail(FT_HIP_E_INVALID, "add_rmsnorm: no output (h, y and q8 are null)");
+    // a thread writes the places that it has read, and no others: an output may lie on an input's rows, not beside them
+    const auto beside = [&](const float* out, int64_t out_stride) {
+        return out && ((out == residual && n > 1 && out_stride != residual_stride) ||
+                       (out == x && (x_type != FT_TYPE_F32 || (n > 1 && out_stride != x_stride))));
+    };
+    if (beside(h, h_stride) || beside(y, y_stride) || (h && h == y))
+        return fail(FT_HIP_E_SHAPE, "add_rmsnorm: an output on an input of another stride or type, or on the other output");
     if (n == 0) return FT_HIP_OK;
     const NormArgs a{x, x_stride, x_w, residual, residual_stride, h, h_stride, w, y, y_stride,
                      static_cast<uint8_t*>(q8), (int)hidden, (double)eps, 1.0 / (double)hidden};
     // vectors of 4 where every row starts on one; else value by value
-    const bool vec = hidden % 4 == 0 && aligned(x, 4 * size) && x_stride % 4 == 0 && aligned(x_w, 16) && aligned(w, 16) &&
-                     aligned(residual, 16) && (!residual || residual_stride % 4 == 0) && aligned(h, 16) &&
+    const bool vec = hidden % 4 == 0 && aligned(x, 4 * size) && x_stride % 4 == 0 && aligned(x_w, 16) &&
+                     aligned(w, 16) && aligned(residual, 16) && (!residual || residual_stride % 4 == 0) && aligned(h, 16) &&
                      (!h || h_stride % 4 == 0) && aligned(y, 16) && (!y || y_stride % 4 == 0);
     DeviceGuard on(ctx->device);
     if (!on.ok) return fail(FT_HIP_E_DEVICE, "add_rmsnorm: device %d cannot be made current", ctx->device);

@@ -180,14 +180,17 @@ def _type(t):
     return _TYPES[t.dtype]
 
 
-def _rows(t, n, width, size, what):
+def _rows(t, n, width, size, what, device):
     """(pointer, row stride) of n rows of `width` values of `size` bytes in t: a
     [rows, values] tensor with a row stride of its own, or a contiguous one of
-    any shape; (NULL, 0) for None. Raises where t cannot hold them."""
+    any shape; (NULL, 0) for None. Raises where t cannot hold them or is on
+    another device (a host pointer would end the process)."""
     if t is None:
         return None, 0
-    if t.element_size() != size:
-        raise FtHipError(E_INVALID, f"{what}: {t.dtype} has not {size} bytes a value")
+    if t.get_device() != device:
+        raise FtHipError(E_INVALID, f"{what}: on {t.device}, the handle's device is {device}")
+    if t.element_size() != size or not t.dtype.is_floating_point:
+        raise FtHipError(E_INVALID, f"{what}: {t.dtype} is no float of {size} bytes")
     shape = t.shape
     if len(shape) == 2:
         rows, stride = shape
@@ -237,13 +240,16 @@ class Q4Gemv:
     def add_rmsnorm(self, x, w, hidden, n, eps, residual=None, h=None, y=None, q8=None, x_w=None, stream=None):
         """h = residual + x (x_w given: x normed by x_w first), y = rmsnorm(h) * w and y's q8 blocks, each output
         or None. x: f32, f16 or bf16 rows; the others f32. A 2-D tensor's row stride is taken as it is."""
-        xp, xs = _rows(x, n, hidden, x.element_size(), "add_rmsnorm: x")
-        rp, rs = _rows(residual, n, hidden, 4, "add_rmsnorm: residual")
-        hp, hs = _rows(h, n, hidden, 4, "add_rmsnorm: h")
-        yp, ys = _rows(y, n, hidden, 4, "add_rmsnorm: y")
-        wp, xwp = _rows(w, 1, hidden, 4, "add_rmsnorm: w")[0], _rows(x_w, 1, hidden, 4, "add_rmsnorm: x_w")[0]
-        if q8 is not None and not (q8.is_contiguous() and q8.numel() * q8.element_size() >= n * (hidden // 32) * Q8_BLK):
-            raise FtHipError(E_SHAPE, f"add_rmsnorm: q8 does not hold {n} rows of {hidden} values")
+        xp, xs = _rows(x, n, hidden, x.element_size(), "add_rmsnorm: x", self.device)
+        rp, rs = _rows(residual, n, hidden, 4, "add_rmsnorm: residual", self.device)
+        hp, hs = _rows(h, n, hidden, 4, "add_rmsnorm: h", self.device)
+        yp, ys = _rows(y, n, hidden, 4, "add_rmsnorm: y", self.device)
+        wp = _rows(w, 1, hidden, 4, "add_rmsnorm: w", self.device)[0]
+        xwp = _rows(x_w, 1, hidden, 4, "add_rmsnorm: x_w", self.device)[0]
+        if q8 is not None and not (q8.get_device() == self.device and q8.is_contiguous()
+                                   and q8.numel() * q8.element_size() >= n * (hidden // 32) * Q8_BLK):
+            raise FtHipError(E_SHAPE, f"add_rmsnorm: q8 does not hold {n} rows of {hidden} values on device "
+                                      f"{self.device}")
         check(lib().ft_hip_add_rmsnorm(self._ctx, self._on(stream), xp, _type(x), xs, xwp, rp, rs, hp, hs, wp, eps, yp,
                                        ys, _ptr(q8), hidden, n))
 
@@ -339,12 +345,15 @@ class Q4Gemv:
                       top_groups=1, group_rank=1, renorm=True, scale=1.0, expert_scale=None, stream=None):
         """ids/wts of the top_k experts per row of logits: scores by softmax or sigmoid, chosen with `bias` added
         among the top_groups best of n_groups groups, weights renormalised and scaled (see the header)."""
-        lp, ls = _rows(logits, n_seqs, n_experts, 4, "route_experts: logits")
-        bp = _rows(bias, 1, n_experts, 4, "route_experts: bias")[0]
-        ep = _rows(expert_scale, 1, n_experts, 4, "route_experts: expert_scale")[0]
+        lp, ls = _rows(logits, n_seqs, n_experts, 4, "route_experts: logits", self.device)
+        bp = _rows(bias, 1, n_experts, 4, "route_experts: bias", self.device)[0]
+        ep = _rows(expert_scale, 1, n_experts, 4, "route_experts: expert_scale", self.device)[0]
         for t, what in ((ids, "ids"), (wts, "wts")):
-            if t.element_size() != 4 or not t.is_contiguous() or t.numel() < n_seqs * top_k:
-                raise FtHipError(E_SHAPE, f"route_experts: {what} does not hold {n_seqs} x {top_k} values of 4 bytes")
+            whole = t.dtype.is_floating_point is (what == "ids")
+            if (t.get_device() != self.device or t.element_size() != 4 or whole or not t.is_contiguous()
+                    or t.numel() < n_seqs * top_k):
+                raise FtHipError(E_SHAPE, f"route_experts: {what} does not hold {n_seqs} x {top_k} values of its 4-byte "
+                                          f"type on device {self.device}")
         check(lib().ft_hip_route_experts(self._ctx, self._on(stream), lp, ls, bp, ep, score, n_groups, top_groups,
                                          group_rank, int(renorm), scale, _ptr(ids), _ptr(wts), n_experts, top_k,
                                          n_seqs))
@@ -362,8 +371,9 @@ class Q4Gemv:
     def sample_tokens(self, logits, vocab, n, u, tokens, workspace, temperature=None, top_k=None, top_p=None,
                       min_p=None, logprobs=None, stream=None):
         """tokens[n] drawn from rows of f32, f16 or bf16 logits with the random numbers u[n] and each row's settings
-        (f32 tensors [n], top_k int32; None: off), logprobs[n] their log probabilities among the kept (see the header)."""
-        lp, ls = _rows(logits, n, vocab, logits.element_size(), "sample_tokens: logits")
+        (f32 tensors [n], top_k int32; None: off), logprobs[n] their log probabilities among the kept (see the
+        header)."""
+        lp, ls = _rows(logits, n, vocab, logits.element_size(), "sample_tokens: logits", self.device)
         ptrs = []
         for t, what in ((temperature, "temperature"), (top_k, "top_k"), (top_p, "top_p"), (min_p, "min_p"), (u, "u"),
                         (tokens, "tokens"), (logprobs, "logprobs")):
@@ -371,9 +381,13 @@ class Q4Gemv:
                 ptrs.append(None)
                 continue
             whole = t.dtype.is_floating_point is (what in ("top_k", "tokens"))
-            if t.element_size() != 4 or whole or not t.is_contiguous() or t.numel() < n:
-                raise FtHipError(E_SHAPE, f"sample_tokens: {what} does not hold {n} values of its 4-byte type")
-            ptrs.append(_ptr(t))
+            if (t.get_device() != self.device or t.element_size() != 4 or whole or not t.is_contiguous()
+                    or t.numel() < n):
+                raise FtHipError(E_SHAPE, f"sample_tokens: {what} does not hold {n} values of its 4-byte type on device "
+                                          f"{self.device}")
+            ptrs.append(t.data_ptr())
+        if workspace.get_device() != self.device:
+            raise FtHipError(E_INVALID, f"sample_tokens: workspace on {workspace.device}, not device {self.device}")
         check(lib().ft_hip_sample_tokens(self._ctx, self._on(stream), lp, _type(logits), ls, vocab, n, *ptrs,
                                          _ptr(workspace), workspace.numel() * workspace.element_size()))
 

@@ -108,9 +108,9 @@ int ft_hip_quantize_q8(ft_hip_ctx* ctx, void* stream, const float* x, int64_t x_
  * either has NaN or 0 in its y and d.
  * x: [n] rows of x_type (FT_TYPE_*) x_stride values apart; x_w, w: [hidden]
  * or NULL; residual, h, y: f32 rows their own stride apart, each or NULL (not
- * all three outputs); q8: [n][hidden/32] blocks or NULL, 4-byte aligned. h may
- * be residual itself, and h or y may be x where it is f32 (same stride); other
- * buffers may not overlap an output. hidden <= 16384, a multiple of 32 where
+ * all three outputs); q8: [n][hidden/32] blocks or NULL, 4-byte aligned. h
+ * or y may be residual itself, or x itself where that is f32 (same stride);
+ * nothing else may overlap an output. hidden <= 16384, a multiple of 32 where
  * q8 is written; rows that all start on 4 values (16 bytes of f32) are read
  * four values at a time. */
 int ft_hip_add_rmsnorm(ft_hip_ctx* ctx, void* stream, const void* x, int x_type, int64_t x_stride, const float* x_w,
@@ -248,10 +248,14 @@ int ft_hip_topk_router(ft_hip_ctx* ctx, void* stream, const float* logits,
  *     the lower index first
  *   wts = s of the chosen; renorm 1: over their sum (0 where the sum is 0);
  *     times scale, times expert_scale[e] (NULL: 1)
- * Scores and sums are f64, wts are rounded once; the bias decides the choice
- * and is no part of the weight. With softmax, renorm 1, no bias and no groups
- * the ids are ft_hip_topk_router's where all logits are finite, and the
- * weights agree to rounding.
+ * A group of one expert has that one's c in place of the sum. Scores and sums
+ * are f64: c that differ by less than 2^-47 of themselves may count as equal,
+ * and so do softmax scores of logits more than 700 below the largest and
+ * sigmoids of logits below -700. wts are rounded once; the bias decides the
+ * choice and is no part of the weight. With softmax, renorm 1, no bias and no
+ * groups the ids are ft_hip_topk_router's where the logits are finite, less
+ * than 700 and, if not equal, more than 2^-46 apart, and the weights agree to
+ * rounding.
  * An expert whose logit or c is NaN, or whose logit or bias is -inf, is never
  * chosen (several +inf logits share the softmax). Where fewer than top_k are
  * left, the other entries are expert 0 with weight 0, so that launches over the

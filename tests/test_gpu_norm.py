@@ -278,3 +278,43 @@ def test_refused_by_the_python_side(gemv):
         with pytest.raises(ft_hip.FtHipError) as e:
             gemv.add_rmsnorm(kw.pop("x"), kw.pop("w"), 64, 4, EPS, **kw)
         assert e.value.code in (ft_hip.E_SHAPE, ft_hip.E_INVALID), change
+
+
+def test_outputs_beside_an_input_are_refused(gemv):
+    """An output may lie on an input's rows, not across them: another stride or type would mix rows; nor on the other
+    output."""
+    n, hidden = 4, 64
+    x, r, w, _ = inputs(n, hidden, 2)
+    xd, rd, wd = x.to(DEV), dev(r), dev(w)
+    wide = torch.zeros((n, 96), device=DEV)
+    wide[:, :hidden] = rd
+    across = wide.flatten()[:n * hidden].view(n, hidden)  # the same start, rows 64 apart
+    x16 = torch.zeros((n, 2 * hidden), dtype=torch.float16, device=DEV)
+    on_x16 = x16.view(torch.float32)
+    before = wide.clone()
+    for kw in (dict(residual=wide[:, :hidden], h=across), dict(residual=wide[:, :hidden], y=across),
+               dict(x=wide[:, :hidden], h=across), dict(x=wide[:, :hidden], y=across), dict(h=wide, y=wide),
+               dict(x=x16, h=on_x16), dict(x=x16, y=on_x16)):
+        kw = dict(dict(x=xd, residual=rd), **kw)
+        with pytest.raises(ft_hip.FtHipError) as e:
+            gemv.add_rmsnorm(kw.pop("x"), wd, hidden, n, EPS, **kw)
+        assert e.value.code == ft_hip.E_SHAPE
+    torch.cuda.synchronize()
+    assert torch.equal(before, wide)
+    # a single row has no stride to differ in
+    h = torch.empty((1, hidden), device=DEV)
+    gemv.add_rmsnorm(xd, wd, hidden, 1, EPS, residual=rd, h=h)
+    gemv.add_rmsnorm(xd, wd, hidden, 1, EPS, residual=wide[:, :hidden], h=across)
+    assert torch.equal(across[:1], h)
+
+
+def test_tensors_of_another_device_or_kind_are_refused(gemv):
+    x, r, w, _ = inputs(4, 64, 3)
+    xd, rd, wd = x.to(DEV), dev(r), dev(w)
+    q8 = torch.zeros(4 * 2 * 40, dtype=torch.uint8)
+    for change in (dict(x=x), dict(residual=rd.cpu()), dict(h=rd.cpu()), dict(y=rd.cpu()), dict(w=wd.cpu()),
+                   dict(x_w=wd.cpu()), dict(q8=q8), dict(x=xd.int()), dict(residual=rd.int()), dict(w=wd.int())):
+        kw = dict(dict(x=xd, w=wd, residual=rd, h=torch.zeros_like(rd)), **change)
+        with pytest.raises((ft_hip.FtHipError)) as e:
+            gemv.add_rmsnorm(kw.pop("x"), kw.pop("w"), 64, 4, EPS, **kw)
+        assert e.value.code in (ft_hip.E_SHAPE, ft_hip.E_INVALID), change

@@ -206,3 +206,30 @@ def test_refused_by_the_python_side(gemv):
         with pytest.raises(ft_hip.FtHipError) as e:
             gemv.route_experts(kw.pop("logits"), kw.pop("ids"), kw.pop("wts"), 16, 2, 4, **kw)
         assert e.value.code in (ft_hip.E_SHAPE, ft_hip.E_INVALID), change
+
+
+@pytest.mark.parametrize("score", [ft_hip.SCORE_SOFTMAX, ft_hip.SCORE_SIGMOID])
+@pytest.mark.parametrize("E", [6, 40, 300])
+def test_scores_that_vanish(gemv, score, E):
+    """Scores below the smallest number of f64 are equal (0 in 64 bits): the lower index first, weight 0."""
+    l = np.full((3, E), -1000.0, np.float32)
+    l[0, E - 1], l[0, 3] = 2.0, -900.0
+    l[1, E // 2], l[1, 0] = 300.0, -1100.0
+    l[2] = -3.0e38
+    l[2, 1:3] = 3.0e38
+    ids, wts = torch.zeros((3, 3), dtype=torch.int32, device=DEV), torch.zeros((3, 3), device=DEV)
+    gemv.route_experts(dev(l), ids, wts, E, 3, 3, score=score)
+    assert ids.tolist() == [[E - 1, 0, 1], [E // 2, 0, 1], [1, 2, 0]]
+    assert wts.tolist() == [[1.0, 0.0, 0.0], [1.0, 0.0, 0.0], [0.5, 0.5, 0.0]]
+
+
+def test_tensors_of_another_device_or_kind_are_refused(gemv):
+    l = torch.zeros((4, 16), device=DEV)
+    ids, wts = torch.zeros((4, 2), dtype=torch.int32, device=DEV), torch.zeros((4, 2), device=DEV)
+    for change in (dict(logits=l.cpu()), dict(logits=l.int()), dict(ids=ids.cpu()), dict(wts=wts.cpu()),
+                   dict(ids=wts), dict(wts=ids), dict(bias=l[0].cpu()), dict(bias=l[0].int()),
+                   dict(expert_scale=l[0].cpu())):
+        kw = dict(dict(logits=l, ids=ids, wts=wts), **change)
+        with pytest.raises(ft_hip.FtHipError) as e:
+            gemv.route_experts(kw.pop("logits"), kw.pop("ids"), kw.pop("wts"), 16, 2, 4, **kw)
+        assert e.value.code in (ft_hip.E_SHAPE, ft_hip.E_INVALID), change
