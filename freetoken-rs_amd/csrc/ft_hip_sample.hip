@@ -201,7 +201,7 @@ __device__ Cut find_cut(const SRC& src, uint32_t lo, uint32_t hi, int base_n, do
         const bool there = own_n && (by_count ? (double)cum_n >= target : cum_w >= target);
         if (there) atomicMin(&l.pick, t);
         __syncthreads();
-        if (l.pick == 1024) {  // fewer values than asked for, or a rounding below the target: the last piece that holds any
+        if (l.pick == 1024) {  // fewer values than asked for, or a rounding below the target: the last that holds any
             __syncthreads();
             if (t == 0) l.pick = -1;
             __syncthreads();
@@ -315,7 +315,8 @@ __device__ void draw(const SampleArgs& a, int64_t r, const SRC& src, int lo, int
         }
         double here = before, after;
         bool passed;
-        const int at = max(0, pick_lane(lane < ROW_WAVES ? l.part[lane] : 0.0, before, s.u * total, &here, &passed, &after));
+        const double part = lane < ROW_WAVES ? l.part[lane] : 0.0;
+        const int at = max(0, pick_lane(part, before, s.u * total, &here, &passed, &after));
         before = here;
         len = min(piece, len - at * piece);
         lo += at * piece;
@@ -609,7 +610,7 @@ __global__ __launch_bounds__(ROW_THREADS) void k_sample_rows(SampleArgs a) {
     const bool by_k = s.k < a.V, by_p = s.p < 1.0;
     float from = -INFINITY;
     if (by_k && s.k <= ROW_THREADS) from = reached_by(s.k, Part{top}, lowest, M, l);
-    if (by_p && !by_k) {  // values of less than (1 - p) z / V are together less than the (1 - p) z that top_p leaves out
+    if (by_p && !by_k) {  // those of less than (1 - p) z / V are together less than the (1 - p) z that top_p leaves out
         double z = 0.0;
 #pragma unroll
         for (int j = 0; j < N; ++j)
@@ -668,10 +669,8 @@ struct Scan {
 };
 
 // Whether a row is decided by its segments' maxima: the largest value alone,
-// or a top-k that the segments bound (a larger one with top_p is streamed).
-__device__ __forceinline__ bool by_maxima(const Row& s, int V, int segs) {
-    return s.greedy || (s.k < V && (s.p < 1.0 || s.k <= segs));
-}
+// or a top-k that the segments bound.
+__device__ __forceinline__ bool by_maxima(const Row& s, int segs) { return s.greedy || s.k <= segs; }
 
 // A value's place in steps of e (per_unit: the step of 2^(1/8) per unit of the
 // logit), and its step, the nearest whole number: by the sum with MAGIC, whose
@@ -752,7 +751,7 @@ __global__ __launch_bounds__(1024) void k_sample_scan(SampleArgs a, Scan w, int6
         if ((lane & 15) == 0 && at < w.segs) seg[at] = x;
         m = fmaxf(m, x);
     }
-    if (by_maxima(s, a.V, w.segs)) return;
+    if (by_maxima(s, w.segs)) return;
     m = wave_max(m);
     if (lane == 0) part[wave] = m;
     for (int b = t; b < BINS; b += T) bins[b] = 0;
@@ -1044,7 +1043,7 @@ __device__ __forceinline__ int run_end(const int* v, int n, int x) {
 //    which the cut lies, the bins what is above, and the token's chunk is read
 //    again for the draw.
 //  - where neither fits the list (thousands of equal values, say), or top_k of
-//    thousands meets top_p, the row is streamed.
+//    more than the list meets top_p, the row is streamed.
 template <int TYPE>
 __global__ __launch_bounds__(ROW_THREADS) void k_sample_finish(SampleArgs a, Scan w, int64_t row0) {
     __shared__ RowLds l;
@@ -1084,9 +1083,8 @@ __global__ __launch_bounds__(ROW_THREADS) void k_sample_finish(SampleArgs a, Sca
     double rest = 0.0, goal = 0.0;
     const double unit = per_unit(s), g = step_of(M, unit), ref = over_step(M, g, unit);
     const uint64_t* bins = w.bins(blockIdx.x);
-    if (by_maxima(s, V, w.segs)) {
-        too_many = s.k > w.segs;
-        from = too_many ? M : reached_by(s.k, segs, lowest, M, l);
+    if (by_maxima(s, w.segs)) {
+        from = reached_by(s.k, segs, lowest, M, l);
         if (s.m > 0.0 && !by_p) from = fmaxf(from, value_below(s.m, s, M));  // without top_p no sum needs the others
     } else {
         double far = 0.0;
@@ -1097,8 +1095,9 @@ __global__ __launch_bounds__(ROW_THREADS) void k_sample_finish(SampleArgs a, Sca
             const double below = k.max == M ? 0.0 : g - step_of(k.max, unit);  // of its step under the largest's
             f.off[c] = some ? bin_of(k.max, M, g, unit) : BINS;
             f.top[c] = k.top;
+            const double over = fmax(e * exp2((f.off[c] + ref) * 0.125) - OFFSET, 0.0);
             f.top_f[c] = some && k.max < INFINITY && f.off[c] < BINS
-                             ? (uint64_t)fma(fmax(e * exp2((f.off[c] + ref) * 0.125) - OFFSET, 0.0), (double)(1ull << FRAC), 0.5)
+                             ? (uint64_t)fma(over, (double)(1ull << FRAC), 0.5)
                              : 0;
             f.top_w[c] = k.top * e;
             f.sums[c] = e > 0.0 ? f.top_w[c] + k.far * e + k.sum * exp2((below + ref) * -0.125) : 0.0;
@@ -1154,15 +1153,15 @@ __global__ __launch_bounds__(ROW_THREADS) void k_sample_finish(SampleArgs a, Sca
             n += scan_n;
             f.cum_w[t] = c;
             f.cum_n[t] = n;
-            const uint64_t lo = __ballot(by_p ? c >= goal * (1.0 - 1e-9) : by_k && n >= s.k);
-            const uint64_t hi = __ballot(by_p ? c >= goal * (1.0 + 1e-9) : by_k && n >= s.k);
+            const uint64_t lo = __ballot(by_k ? n >= s.k : by_p && c >= goal * (1.0 - 1e-9));
+            const uint64_t hi = __ballot(by_k ? n >= s.k : by_p && c >= goal * (1.0 + 1e-9));
             if (lane == 0 && lo) atomicMin(&f.cut_lo, t + __ffsll((unsigned long long)lo) - 1);
             if (lane == 0 && hi) atomicMin(&f.cut_hi, t + __ffsll((unsigned long long)hi) - 1);
         }
         __syncthreads();
         // and min_p: its place below the largest's step, in steps
         int min_lo = BINS, min_hi = BINS;
-        if (s.m > 0.0) {
+        if (s.m > 0.0 && !(by_k && by_p)) {  // top_p's share is of all the top k
             const double x = log(s.m) * (-8.0 * 1.4426950408889634074) - ref;
             if (x < (double)BINS - 2) {
                 min_lo = (int)fmax(0.0, rint(x - 1e-6));
@@ -1173,7 +1172,8 @@ __global__ __launch_bounds__(ROW_THREADS) void k_sample_finish(SampleArgs a, Sca
         all = last >= BINS || f.cum_n[last] <= LIST;
         first = all ? 0 : min(f.cut_lo, min_lo);
         if (last >= BINS || f.cum_n[last] - (first ? f.cum_n[first - 1] : 0) > LIST) too_many = true;
-        if (by_p && all) {
+        if (by_k && by_p && !all) too_many = true;  // two cuts: only the list decides both
+        if (by_p && !by_k && all) {
             double x = far;
             if (t > last) x += own_w;
             rest = block_sum(x, l);

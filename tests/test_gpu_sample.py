@@ -305,3 +305,54 @@ def test_refused_by_the_python_side(gemv):
         with pytest.raises(ft_hip.FtHipError) as e:
             gemv.sample_tokens(kw.pop("logits"), 100, 4, kw.pop("u"), kw.pop("tokens"), kw.pop("workspace"), **kw)
         assert e.value.code in (ft_hip.E_SHAPE, ft_hip.E_INVALID), change
+
+
+@pytest.mark.parametrize("settings", list(SETTINGS))
+@pytest.mark.parametrize("V", [8191, 8192])
+def test_longest_rows_of_one_launch(gemv, settings, V):
+    rng = np.random.default_rng(V + 1000 * list(SETTINGS).index(settings))
+    n = 5
+    check(gemv, torch.from_numpy(model_logits(rng, n, V)).half(), rng.random(n), **SETTINGS[settings](rng, n))
+
+
+def test_more_rows_than_the_workspace_holds(gemv):
+    """Rows that share the workspace one batch after the other: as each alone."""
+    rng = np.random.default_rng(21)
+    n, V = 1030, 8201
+    l = torch.from_numpy(model_logits(rng, n, V)).to(DEV)
+    u = rng.random(n)
+    s = dict(temperature=rng.uniform(0, 2, n), top_k=rng.integers(-50, 100, n), top_p=rng.uniform(0.5, 1.2, n),
+             min_p=rng.uniform(-0.1, 0.1, n))
+    assert gemv.sample_tokens_workspace_bytes(V, n) == gemv.sample_tokens_workspace_bytes(V, 512)
+    tok, lp = draw(gemv, l, n, V, u, **s)
+    for a, b in ((0, 3), (510, 515), (1000, 1030)):
+        part = draw(gemv, l[a:b], b - a, V, u[a:b], **{k: v[a:b] for k, v in s.items()})
+        assert np.array_equal(tok[a:b], part[0]) and np.array_equal(lp[a:b], part[1])
+
+
+def test_one_row_of_logits_for_several_draws(gemv):
+    """A batch that is the same row again and again, and one that rises in u: as a call each."""
+    rng = np.random.default_rng(8)
+    for V in (700, 30000):
+        l = torch.from_numpy(model_logits(rng, 1, V)).to(DEV)
+        u = [0.3, 0.3, 0.9, 0.3]
+        tok, lp = draw(gemv, l.repeat(4, 1), 4, V, u, top_p=[0.9] * 4)
+        assert tok[0] == tok[1] == tok[3] and lp[0] == lp[1] == lp[3]
+        for i in range(4):
+            one = draw(gemv, l, 1, V, u[i:i + 1], top_p=[0.9])
+            assert one[0][0] == tok[i] and one[1][0] == lp[i]
+
+
+def test_tensors_of_another_device_are_refused(gemv):
+    l = torch.zeros((4, 100), device=DEV)
+    one = torch.ones(4, device=DEV)
+    tokens = torch.zeros(4, dtype=torch.int32, device=DEV)
+    ws = torch.zeros(gemv.sample_tokens_workspace_bytes(100, 4), dtype=torch.uint8, device=DEV)
+    for change in (dict(logits=l.cpu()), dict(logits=l.int()), dict(u=one.cpu()), dict(tokens=tokens.cpu()),
+                   dict(workspace=ws.cpu()), dict(temperature=one.cpu()), dict(top_k=tokens.cpu()),
+                   dict(top_p=one.cpu()), dict(min_p=one.cpu()), dict(logprobs=one.cpu()),
+                   dict(u=one[:1].expand(4))):
+        kw = dict(dict(logits=l, u=one, tokens=tokens, workspace=ws), **change)
+        with pytest.raises(ft_hip.FtHipError) as e:
+            gemv.sample_tokens(kw.pop("logits"), 100, 4, kw.pop("u"), kw.pop("tokens"), kw.pop("workspace"), **kw)
+        assert e.value.code in (ft_hip.E_SHAPE, ft_hip.E_INVALID), change
