@@ -12,6 +12,10 @@
 // hundreds of thousands of terms f32 sums would move the border by whole
 // tokens. Sums are made in a fixed order, and where many threads add to one
 // counter it holds whole numbers, so a row's result is the same on every run.
+//
+// Rows of up to 8192 logits are one launch, longer ones a scan by many
+// workgroups and a finish by one per row; what bounds each, and its times
+// (kernels alone, f32 logits), stand beside it.
 
 #include "ft_device.hpp"
 #include "ft_runtime.hpp"
@@ -574,7 +578,11 @@ __device__ __forceinline__ float value_below(double x, const Row& s, float M) {
 }
 
 // Rows of at most LIST values, one launch: in registers, a run of 512 to a
-// wave; those that may be kept go into the list.
+// wave; those that may be kept go into the list. Bound by the chain of steps of
+// one workgroup, most of them the instructions' first fetch and a barrier: 64
+// rows of 8000 take 10.9 us with top-k 64 and top-p, 22.7 with top-p, 12.9 with
+// neither, where scan and finish take 19.5, 25.9 and 21.5; a row of 2000 9.2,
+// 11.7 and 8.5.
 template <int TYPE>
 __global__ __launch_bounds__(ROW_THREADS) void k_sample_rows(SampleArgs a) {
     __shared__ RowLds l;
@@ -723,7 +731,10 @@ __device__ __forceinline__ bool vec_row(const void* row) {
 }
 
 // Workgroup (c, row): chunk c of the row in registers, VECS times four values
-// a thread; one pass over memory.
+// a thread; one pass over memory. With bins to fill it is bound by instructions,
+// about 36 a value, most in f64, and an LDS atomic: 256 rows of 262144 take 71 us
+// (3.8 TB/s), 64 rows 25, one 6.2. Where the segments' maxima decide, by memory:
+// 64 rows 11.7 us (5.7 TB/s, in part from the caches), one 3.2.
 template <int TYPE, int VECS>
 __global__ __launch_bounds__(1024) void k_sample_scan(SampleArgs a, Scan w, int64_t row0) {
     __shared__ uint64_t bins[BINS];
@@ -1044,6 +1055,11 @@ __device__ __forceinline__ int run_end(const int* v, int n, int x) {
 //    again for the draw.
 //  - where neither fits the list (thousands of equal values, say), or top_k of
 //    more than the list meets top_p, the row is streamed.
+// Bound by the chain of one workgroup's steps: about 4 us until the first data
+// is there, then the list's making and its cuts. A row of 262144: 14.5 us with
+// top-k 64 and top-p; 57 with top-p alone where the cut lies among thousands
+// (64 rows 71, 256 rows 87), of which reading the row's open segments again is
+// some 36; streamed about 1 ms.
 template <int TYPE>
 __global__ __launch_bounds__(ROW_THREADS) void k_sample_finish(SampleArgs a, Scan w, int64_t row0) {
     __shared__ RowLds l;
@@ -1222,8 +1238,11 @@ __global__ __launch_bounds__(ROW_THREADS) void k_sample_finish(SampleArgs a, Sca
 
 constexpr int SCAN_ROWS = 512;  // rows whose scan the workspace holds
 
-// Values a workgroup of the scan takes: 8192 by 1024 threads where there are
-// few rows, by 256 once such workgroups fill the device.
+// A chunk of 8192 values by 1024 threads, where all chunks at once leave the
+// device half empty, or by 256 threads with four times the values each, which
+// share a chunk's fixed steps: a row of 262144 6.2 us against 7.2, 8 rows of
+// 151936 6.3 against 7.4; 32 rows of 262144 18.4 against 15.7, 256 rows 114
+// against 71.
 bool wide_scan(int64_t vocab, int64_t n) { return vocab * n < (int64_t)1024 * 8192; }
 
 Scan scan_of(int64_t vocab, int64_t n, void* workspace) {
