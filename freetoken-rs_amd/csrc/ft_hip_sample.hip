@@ -1058,8 +1058,8 @@ __device__ __forceinline__ int run_end(const int* v, int n, int x) {
 // Bound by the chain of one workgroup's steps: about 4 us until the first data
 // is there, then the list's making and its cuts. A row of 262144: 14.5 us with
 // top-k 64 and top-p; 57 with top-p alone where the cut lies among thousands
-// (64 rows 71, 256 rows 87), of which reading the row's open segments again is
-// some 36; streamed about 1 ms.
+// (64 rows 71, 256 rows 87), of which reading its open segments again is 25 to
+// 36; streamed about 1 ms.
 template <int TYPE>
 __global__ __launch_bounds__(ROW_THREADS) void k_sample_finish(SampleArgs a, Scan w, int64_t row0) {
     __shared__ RowLds l;
