@@ -176,3 +176,82 @@ def test_routing_of_the_layer_entry_point(gemv):
     assert torch.equal(ids, r.ids)
     assert float(((wts - r.wts).abs() / wts).max()) < 2.0 ** -20
     assert np.array_equal(blocks(r.q8x, 8, shape.hidden)[2].shape, (8, shape.hidden // 32, 32))
+
+
+def far(n, width, stride, dtype):
+    """n rows of width values, `stride` values apart, in a buffer that is nothing else."""
+    return torch.empty((n - 1) * stride + width, dtype=dtype, device=DEV).as_strided((n, width), (stride, 1))
+
+
+def test_rows_further_apart_than_32_bits(gemv):
+    """Row offsets past 2^32 bytes and 2^31 values: as on rows one after the other."""
+    rng = np.random.default_rng(5)
+    H, E, V = 320, 64, 9000
+    x, w = batch(2, H, 1).half(), batch(1, H, 2)[0]
+    xf, yf = far(2, H, (1 << 31) + 8, torch.float16), far(2, H, (1 << 30) + 64, torch.float32)
+    xf.copy_(x)
+    y, q8, q8f = torch.empty((2, H), device=DEV), *(torch.zeros(2 * 400, dtype=torch.uint8, device=DEV) for _ in "ab")
+    gemv.add_rmsnorm(x, w, H, 2, 1e-6, y=y, q8=q8)
+    gemv.add_rmsnorm(xf, w, H, 2, 1e-6, y=yf, q8=q8f)
+    assert torch.equal(y, yf) and torch.equal(q8, q8f)
+    del xf, yf
+    l = batch(3, E, 3)
+    lf = far(3, E, (1 << 30) + 4, torch.float32)
+    lf.copy_(l)
+    out = [(torch.zeros((3, 4), dtype=torch.int32, device=DEV), torch.zeros((3, 4), device=DEV)) for _ in "ab"]
+    for logits, (ids, wts) in zip((l, lf), out):
+        gemv.route_experts(logits, ids, wts, E, 4, 3, score=ft_hip.SCORE_SIGMOID)
+    assert torch.equal(out[0][0], out[1][0]) and torch.equal(out[0][1], out[1][1])
+    del lf
+    l = torch.from_numpy((3 * rng.standard_normal((2, V))).astype(np.float32)).to(DEV).bfloat16()
+    lf = far(2, V, (1 << 31) + 8, torch.bfloat16)
+    lf.copy_(l)
+    ws = torch.empty(gemv.sample_tokens_workspace_bytes(V, 2), dtype=torch.uint8, device=DEV)
+    out = [(torch.zeros(2, dtype=torch.int32, device=DEV), torch.zeros(2, device=DEV)) for _ in "ab"]
+    for logits, (tokens, lp) in zip((l, lf), out):
+        gemv.sample_tokens(logits, V, 2, torch.full((2,), 0.7, device=DEV), tokens, ws,
+                           top_p=torch.full((2,), 0.9, device=DEV), logprobs=lp)
+    assert torch.equal(out[0][0], out[1][0]) and torch.equal(out[0][1], out[1][1])
+
+
+def test_most_rows_of_the_norm(gemv):
+    """2^22 - 1 rows of one value: y = x / sqrt(x x + eps), each rounded once."""
+    n = (1 << 22) - 1
+    x = torch.from_numpy(np.random.default_rng(3).standard_normal((n, 1)).astype(np.float32)).to(DEV)
+    y = torch.empty_like(x)
+    gemv.add_rmsnorm(x, None, 1, n, 1e-6, y=y)
+    want = x.double() / torch.sqrt(x.double() ** 2 + float(np.float32(1e-6)))
+    assert float(((y.double() - want).abs() / want.abs().clamp_min(1e-30)).max()) <= 2.0 ** -24 * (1 + 1e-6)
+
+
+def test_two_threads_on_one_handle(gemv):
+    """Calls of two host threads at once, each on a stream, buffers and workspace of its own, as one after the other."""
+    import threading
+    H = SMALL.hidden
+    parts = [(stack_of(gemv, 4), head_of(gemv, H, VOCAB, 4), batch(4, H, 80 + i), settings(4, 80 + i)) for i in range(2)]
+    want = []
+    for r, head, x, s in parts:
+        want.append([t.clone() for t in head.run(*r.run(x, 4), 4, **s)])
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(part, w):
+        try:
+            r, head, x, s = part
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(10):
+                    got = head.run(*r.run(x, 4), 4, **s)
+                    with pytest.raises(ft_hip.FtHipError, match="n_groups"):
+                        gemv.route_experts(r.logits, r.ids, r.wts, SMALL.n_experts, 4, 4, n_groups=3)
+                stream.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, w))
+        except BaseException as e:  # noqa: BLE001 - handed to the test's own thread
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=p) for p in zip(parts, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
