@@ -182,9 +182,12 @@ def _type(t):
 
 def _rows(t, n, width, size, what, device):
     """(pointer, row stride) of n rows of `width` values of `size` bytes in t: a
-    [rows, values] tensor with a row stride of its own, or a contiguous one of
-    any shape; (NULL, 0) for None. Raises where t cannot hold them or is on
-    another device (a host pointer would end the process)."""
+    [rows, values] tensor with a row stride of its own, a contiguous one of more
+    dimensions, whose rows are its last dimensions that hold `width` values
+    ([batch, 1, padded vocabulary]: the last, [rows, heads, values]: the last
+    two), or a contiguous one of one dimension, rows one after the other;
+    (NULL, 0) for None. Raises where t cannot hold them or is on another device
+    (a host pointer would end the process)."""
     if t is None:
         return None, 0
     if t.get_device() != device:
@@ -200,7 +203,13 @@ def _rows(t, n, width, size, what, device):
             if rows > 1:
                 stride = t.stride(0)
     else:
-        stride, ok = width, t.numel() >= n * width and t.is_contiguous()
+        stride, ok = width, t.is_contiguous()
+        if len(shape) > 2 and t.numel() != n * width:  # equal: no value is between two rows
+            stride, dims = 1, list(shape)
+            while dims and stride < width:
+                stride *= dims.pop()
+            ok = ok and stride >= width
+        ok = ok and t.numel() >= n * stride
     if not ok and n > 0:
         raise FtHipError(E_SHAPE, f"{what}: {tuple(shape)} does not hold {n} rows of {width} consecutive values")
     return t.data_ptr(), stride

@@ -1,0 +1,81 @@
+"""The norm, the routing and the draw on rows inside tensors of three
+dimensions, padded as a head or a router leaves them: the same bits as on rows
+one after the other, and what lies between the rows stays as it was."""
+import numpy as np
+import pytest
+import torch
+
+import ft_hip
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def rows(n, width, seed, scale=1.0):
+    return torch.from_numpy((scale * np.random.default_rng(seed).standard_normal((n, width))).astype(np.float32)).to(DEV)
+
+
+def padded(a, pad, shape=None, dtype=torch.float32):
+    """a [n, width] inside [n, 1, width + pad] (seen as `shape`), 60 in between."""
+    n, width = a.shape
+    t = torch.full((n, 1, width + pad), 60.0, dtype=dtype, device=DEV)
+    t[:, 0, :width] = a
+    return t if shape is None else t.view(shape)
+
+
+@pytest.mark.parametrize("pad", [0, 1, 64])
+@pytest.mark.parametrize("n", [1, 3])
+def test_draw(gemv, n, pad):
+    for V, dtype in ((9000, torch.float32), (700, torch.bfloat16)):
+        l = rows(n, V, V + n, 3.0)
+        u = torch.linspace(0.1, 0.9, n, device=DEV)
+        ws = torch.empty(gemv.sample_tokens_workspace_bytes(V, n), dtype=torch.uint8, device=DEV)
+        got = []
+        for logits in (l.to(dtype), padded(l, pad, dtype=dtype), padded(l, pad, (1, n, V + pad), dtype)):
+            tokens, lp = torch.zeros(n, dtype=torch.int32, device=DEV), torch.zeros(n, device=DEV)
+            gemv.sample_tokens(logits, V, n, u, tokens, ws, logprobs=lp)
+            got.append((tokens, lp))
+        torch.cuda.synchronize()
+        for tokens, lp in got[1:]:
+            assert torch.equal(tokens, got[0][0]) and torch.equal(lp, got[0][1])
+
+
+@pytest.mark.parametrize("pad", [0, 1, 64])
+def test_routing(gemv, pad):
+    n, E = 5, 96
+    l = rows(n, E, pad)
+    got = []
+    for logits in (l, padded(l, pad), padded(l, pad, (n, 1, 1, E + pad))):
+        ids, wts = torch.zeros((n, 6), dtype=torch.int32, device=DEV), torch.zeros((n, 6), device=DEV)
+        gemv.route_experts(logits, ids, wts, E, 6, n, score=ft_hip.SCORE_SIGMOID)
+        got.append((ids, wts))
+    torch.cuda.synchronize()
+    for ids, wts in got[1:]:
+        assert torch.equal(ids, got[0][0]) and torch.equal(wts, got[0][1])
+
+
+@pytest.mark.parametrize("pad", [0, 1, 64])
+def test_norm(gemv, pad):
+    n, H = 4, 320
+    x, r, w = rows(n, H, 1), rows(n, H, 2), rows(1, H, 3)[0]
+    h, y, q8 = torch.zeros((n, H), device=DEV), torch.zeros((n, H), device=DEV), torch.zeros(n * 400, dtype=torch.uint8,
+                                                                                             device=DEV)
+    gemv.add_rmsnorm(x, w, H, n, 1e-6, residual=r, h=h, y=y, q8=q8)
+    xp, rp, hp, yp = (padded(a, pad) for a in (x, r, r, r))
+    qp = torch.zeros_like(q8)
+    gemv.add_rmsnorm(xp, w, H, n, 1e-6, residual=rp, h=hp, y=yp, q8=qp)
+    torch.cuda.synchronize()
+    assert torch.equal(hp[:, 0, :H], h) and torch.equal(yp[:, 0, :H], y) and torch.equal(qp, q8)
+    for t in (hp, yp):
+        assert bool((t[:, 0, H:] == 60.0).all())
+
+
+def test_norm_of_heads(gemv):
+    """A branch as attention leaves it, [rows, heads, values]: a row is all of its heads."""
+    n, H = 3, 256
+    x = rows(n, H, 5)
+    y, yh = torch.zeros((n, H), device=DEV), torch.zeros((n, 4, 64), device=DEV)
+    gemv.add_rmsnorm(x, None, H, n, 1e-6, y=y)
+    gemv.add_rmsnorm(x.view(n, 4, 64), None, H, n, 1e-6, y=yh)
+    torch.cuda.synchronize()
+    assert torch.equal(yh.view(n, H), y)
