@@ -409,7 +409,7 @@ class RoutedStack:
         bank = m.banks[l * E * m.expert_bytes:(l + 1) * E * m.expert_bytes]
         g.add_rmsnorm(branch, None if self.norm_w is None else self.norm_w[l], H, n_seqs, self.eps, residual=residual,
                       h=self.h, y=self.y, q8=self.q8x, stream=stream)
-        g.gemv_f32_rows_dev(m.routers[l], self.y, self.logits, H, E, n_seqs, stream=stream)
+        g.gemv_f32_rows_dev(m.routers[l], self.y, self.logits, H, E, n_seqs, bias=m.layer_bias(l), stream=stream)
         g.route_experts(self.logits, self.ids, self.wts, E, K, n_seqs, stream=stream, **self.route)
         g.gemv_gate_up_act(bank, m.expert_bytes, self.ids, p, K, self.q8x, H, s.inter, self.q8a, m.layout, stream=stream)
         g.gemv_grouped_slots(bank, m.expert_bytes, m.gu_bytes, self.ids, None, p, self.q8a, s.inter // 32, self.down, H,
