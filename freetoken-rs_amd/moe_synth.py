@@ -357,6 +357,12 @@ class BatchedStack:
                                  stream)
 
 
+def _current(g, stream):
+    """Makes the stream (None: the current one of the handle's device) the current one, and its device: what torch and
+    every method of the handle that is given no stream then run on."""
+    return torch.cuda.stream(torch.cuda.current_stream(g.device) if stream is None else stream)
+
+
 class VocabHead:
     """From the residual stream to the next tokens: the last norm with its q8
     blocks, the vocabulary head's q4r GEMV (one row set for every sequence) and
@@ -374,11 +380,12 @@ class VocabHead:
 
     def run(self, branch, residual, n_seqs, u, temperature=None, top_k=None, top_p=None, min_p=None, stream=None):
         """tokens (and log probabilities) of n_seqs sequences from residual + branch (residual None: branch alone)."""
-        self.g.add_rmsnorm(branch, self.norm_w, self.H, n_seqs, self.eps, residual=residual, q8=self.q8, stream=stream)
-        self.g.gemv_q4r_idx(self.weights, 0, 0, self.slots, None, n_seqs, self.q8, self.H // 32, self.logits,
-                            self.vocab, self.vocab, self.H, stream=stream)
-        self.g.sample_tokens(self.logits, self.vocab, n_seqs, u, self.tokens, self.ws, temperature, top_k, top_p, min_p,
-                             self.logprobs, stream=stream)
+        with _current(self.g, stream):
+            self.g.add_rmsnorm(branch, self.norm_w, self.H, n_seqs, self.eps, residual=residual, q8=self.q8)
+            self.g.gemv_q4r_idx(self.weights, 0, 0, self.slots, None, n_seqs, self.q8, self.H // 32, self.logits,
+                                self.vocab, self.vocab, self.H)
+            self.g.sample_tokens(self.logits, self.vocab, n_seqs, u, self.tokens, self.ws, temperature, top_k, top_p,
+                                 min_p, self.logprobs)
         return self.tokens[:n_seqs], self.logprobs[:n_seqs]
 
 
@@ -407,19 +414,19 @@ class RoutedStack:
         g, m, s = self.g, self.m, self.m.shape
         H, E, K, p = s.hidden, s.n_experts, s.top_k, n_seqs * s.top_k
         bank = m.banks[l * E * m.expert_bytes:(l + 1) * E * m.expert_bytes]
-        g.add_rmsnorm(branch, None if self.norm_w is None else self.norm_w[l], H, n_seqs, self.eps, residual=residual,
-                      h=self.h, y=self.y, q8=self.q8x, stream=stream)
-        g.gemv_f32_rows_dev(m.routers[l], self.y, self.logits, H, E, n_seqs, bias=m.layer_bias(l), stream=stream)
-        g.route_experts(self.logits, self.ids, self.wts, E, K, n_seqs, stream=stream, **self.route)
-        g.gemv_gate_up_act(bank, m.expert_bytes, self.ids, p, K, self.q8x, H, s.inter, self.q8a, m.layout, stream=stream)
-        g.gemv_grouped_slots(bank, m.expert_bytes, m.gu_bytes, self.ids, None, p, self.q8a, s.inter // 32, self.down, H,
-                             H, s.inter, m.layout, stream=stream)
-        self.branch[:n_seqs].zero_()
-        g.reduce_pairs_weighted(self.down, self.wts, self.seq_of, self.branch, H, p, n_seqs, stream=stream)
+        with _current(g, stream):
+            g.add_rmsnorm(branch, None if self.norm_w is None else self.norm_w[l], H, n_seqs, self.eps,
+                          residual=residual, h=self.h, y=self.y, q8=self.q8x)
+            g.gemv_f32_rows_dev(m.routers[l], self.y, self.logits, H, E, n_seqs, bias=m.layer_bias(l))
+            g.route_experts(self.logits, self.ids, self.wts, E, K, n_seqs, **self.route)
+            g.gemv_gate_up_act(bank, m.expert_bytes, self.ids, p, K, self.q8x, H, s.inter, self.q8a, m.layout)
+            g.gemv_grouped_slots(bank, m.expert_bytes, m.gu_bytes, self.ids, None, p, self.q8a, s.inter // 32,
+                                 self.down, H, H, s.inter, m.layout)
+            self.branch[:n_seqs].zero_()
+            g.reduce_pairs_weighted(self.down, self.wts, self.seq_of, self.branch, H, p, n_seqs)
 
     def run(self, x, n_seqs, stream=None):
-        """All layers: returns (branch, residual) of the last, what the next norm adds. A given stream has to be current
-        (the branch is cleared on it)."""
+        """All layers: returns (branch, residual) of the last, what the next norm adds."""
         for l in range(self.m.L):
             self.layer(l, x if l == 0 else self.branch, None if l == 0 else self.h, n_seqs, stream)
         return self.branch, self.h
