@@ -259,8 +259,6 @@ void launch_norm(const NormArgs& a, int64_t n, int64_t few, bool vec, void* stre
         hipLaunchKernelGGL((k_add_rmsnorm<TYPE, 4, 4>), grid, dim3((vecs + 255) / 256 * 64), 0, s, a);
 }
 
-bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
-
 }  // namespace
 
 extern "C" int ft_hip_add_rmsnorm(ft_hip_ctx* ctx, void* stream, const void* x, int x_type, int64_t x_stride,

@@ -366,11 +366,13 @@ extern "C" int ft_hip_route_experts(ft_hip_ctx* ctx, void* stream, const float* 
         return fail(FT_HIP_E_SHAPE, "route_experts: n_seqs=%lld not in [0, 2^24]", (long long)n_seqs);
     if (logits_stride < E || logits_stride > (int64_t)1 << 36)
         return fail(FT_HIP_E_SHAPE, "route_experts: logits_stride out of range");
+    if (!aligned(logits, 4) || !aligned(bias, 4) || !aligned(expert_scale, 4) || !aligned(ids, 4) || !aligned(wts, 4))
+        return fail(FT_HIP_E_SHAPE, "route_experts: a pointer is not aligned to 4 bytes");
     if (!ctx || !logits || !ids || !wts) return fail(FT_HIP_E_INVALID, "route_experts: null argument");
     if (n_seqs == 0) return FT_HIP_OK;
     const RouteArgs a{logits, logits_stride, bias, expert_scale, ids, wts, score == FT_SCORE_SIGMOID, (int)G,
                       (int)(E / G), (int)top_groups, group_rank, renorm, (double)scale, (int)E, (int)top_k, (int)n_seqs,
-                      reinterpret_cast<uintptr_t>(logits) % 16 == 0 && logits_stride % 4 == 0 && E % 4 == 0};
+                      aligned(logits, 16) && logits_stride % 4 == 0 && E % 4 == 0};
     DeviceGuard on(ctx->device);
     if (!on.ok) return fail(FT_HIP_E_DEVICE, "route_experts: device %d cannot be made current", ctx->device);
     // As few lanes to a token as hold its experts four to a lane, and one lane each for its groups and its choices.

@@ -1296,9 +1296,12 @@ extern "C" int ft_hip_sample_tokens(ft_hip_ctx* ctx, void* stream, const void* l
         return fail(FT_HIP_E_INVALID, "sample_tokens: logits_type=%d is no FT_TYPE", logits_type);
     if (logits_stride < vocab || logits_stride > (int64_t)1 << 40)
         return fail(FT_HIP_E_SHAPE, "sample_tokens: logits_stride out of range");
-    if (reinterpret_cast<uintptr_t>(logits) % (logits_type == FT_TYPE_F32 ? 4 : 2))
+    if (!aligned(logits, logits_type == FT_TYPE_F32 ? 4 : 2))
         return fail(FT_HIP_E_SHAPE, "sample_tokens: logits are not aligned to their type");
-    if (reinterpret_cast<uintptr_t>(workspace) % 16)
+    if (!aligned(temperature, 4) || !aligned(top_k, 4) || !aligned(top_p, 4) || !aligned(min_p, 4) || !aligned(u, 4) ||
+        !aligned(tokens, 4) || !aligned(logprobs, 4))
+        return fail(FT_HIP_E_SHAPE, "sample_tokens: a row's settings or outputs are not aligned to 4 bytes");
+    if (!aligned(workspace, 16))
         return fail(FT_HIP_E_SHAPE, "sample_tokens: workspace must be 16-byte aligned");
     const size_t need = ft_hip_sample_tokens_workspace_bytes(vocab, n);
     if (workspace_bytes < need)

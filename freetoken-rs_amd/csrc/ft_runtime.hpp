@@ -70,6 +70,7 @@ int launch_route_topk(void* stream, const float* w, const float* x, const float*
 int scratch_setup(ft_hip_ctx* ctx);
 // Input RMS norm scale per seq: inv[s] = 1 / sqrt(R-order(x_s . x_s) / dim + 1e-6).
 int launch_rms_inv(void* stream, const float* x, float* inv, int64_t dim, int64_t n_seqs);
+inline bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 // Makes a context's device current for the launches of one call and gives the
 // caller's back: for entry points that may be called with another device
 // current (the stream then belongs to the context's device).
