@@ -397,6 +397,8 @@ class Q4Gemv:
             ptrs.append(t.data_ptr())
         if workspace.get_device() != self.device:
             raise FtHipError(E_INVALID, f"sample_tokens: workspace on {workspace.device}, not device {self.device}")
+        if not workspace.is_contiguous():  # its size is what the values take side by side
+            raise FtHipError(E_SHAPE, f"sample_tokens: workspace of strides {workspace.stride()} is not contiguous")
         check(lib().ft_hip_sample_tokens(self._ctx, self._on(stream), lp, _type(logits), ls, vocab, n, *ptrs,
                                          _ptr(workspace), workspace.numel() * workspace.element_size()))
 

@@ -92,3 +92,15 @@ def test_views_of_more_dimensions_that_are_not_contiguous_are_refused(noted):
     for call in (norm, route, sample):
         with pytest.raises(ft_hip.FtHipError):
             call(*noted, t, 64, 3)
+
+
+def test_a_workspace_with_gaps_is_refused(noted):
+    """Its count says nothing of the memory behind it: bytes between would be overwritten, or bytes past its end."""
+    logits = torch.zeros(2, 9000)
+    for ws in (torch.zeros(1 << 11, dtype=torch.uint8)[::2], torch.zeros(1, dtype=torch.uint8).expand(1 << 20),
+               torch.zeros((8, 64), dtype=torch.uint8).t(), torch.zeros((4, 64), dtype=torch.uint8)[:, :32]):
+        with pytest.raises(ft_hip.FtHipError, match="workspace") as e:
+            sample(*noted, logits, 9000, 2, ws)
+        assert e.value.code == ft_hip.E_SHAPE
+    sample(*noted, logits, 9000, 2, torch.zeros((8, 64), dtype=torch.uint8)[4:])  # a run of rows has none
+    assert noted[1]["ft_hip_sample_tokens"][14] == 4 * 64
