@@ -103,4 +103,4 @@ def test_a_workspace_with_gaps_is_refused(noted):
             sample(*noted, logits, 9000, 2, ws)
         assert e.value.code == ft_hip.E_SHAPE
     sample(*noted, logits, 9000, 2, torch.zeros((8, 64), dtype=torch.uint8)[4:])  # a run of rows has none
-    assert noted[1]["ft_hip_sample_tokens"][14] == 4 * 64
+    assert noted[1]["ft_hip_sample_tokens"][15] == 4 * 64
