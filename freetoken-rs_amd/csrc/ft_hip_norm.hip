@@ -23,6 +23,7 @@
 // 5.0). Up to some hundred rows the time is a launch and one round trip.
 
 #include "ft_device.hpp"
+#include "ft_overlap.hpp"
 #include "ft_runtime.hpp"
 #include "ft_wave.hpp"
 
@@ -287,13 +288,20 @@ extern "C" int ft_hip_add_rmsnorm(ft_hip_ctx* ctx, void* stream, const void* x, 
         return fail(FT_HIP_E_SHAPE, "add_rmsnorm: a pointer is not aligned to its type (q8: 4 bytes)");
     if (!ctx || !x) return fail(FT_HIP_E_INVALID, "add_rmsnorm: null argument");
     if (!h && !y && !q8) return fail(FT_HIP_E_INVALID, "add_rmsnorm: no output (h, y and q8 are null)");
-    // a thread writes the places that it has read, and no others: an output may lie on an input's rows, not beside them
-    const auto beside = [&](const float* out, int64_t out_stride) {
-        return out && ((out == residual && n > 1 && out_stride != residual_stride) ||
-                       (out == x && (x_type != FT_TYPE_F32 || (n > 1 && out_stride != x_stride))));
+    // A thread writes the places that it has read, and no others: h or y may lie on an input's rows, on all of them with
+    // the same stride; any other overlap would mix rows, or blocks with what they are made of.
+    const auto f32 = [&](const float* p, int64_t stride) { return Span{p, n, stride * 4, hidden * 4}; };
+    const Span sx{x, n, x_stride * size, hidden * size}, sr = f32(residual, residual_stride), sh = f32(h, h_stride),
+        sy = f32(y, y_stride), sq{q8, 1, 0, n * (hidden / 32) * Q8_BLK}, sw{w, 1, 0, hidden * 4}, sxw{x_w, 1, 0, hidden * 4};
+    const auto mixes = [&](const Span& out, const Span& in) {
+        return overlap(out, in) && !(out.at == in.at && out.bytes == in.bytes && (n == 1 || out.stride == in.stride));
     };
-    if (beside(h, h_stride) || beside(y, y_stride) || (h && h == y))
-        return fail(FT_HIP_E_SHAPE, "add_rmsnorm: an output on an input of another stride or type, or on the other output");
+    for (const Span& out : {sh, sy})
+        if (mixes(out, sx) || mixes(out, sr) || overlap(out, sw) || overlap(out, sxw) || overlap(out, sq))
+            return fail(FT_HIP_E_SHAPE, "add_rmsnorm: h or y overlaps an input other than row on row, a weight or q8");
+    if (overlap(sh, sy)) return fail(FT_HIP_E_SHAPE, "add_rmsnorm: h and y overlap");
+    if (overlap(sq, sx) || overlap(sq, sr) || overlap(sq, sw) || overlap(sq, sxw))
+        return fail(FT_HIP_E_SHAPE, "add_rmsnorm: q8 overlaps an input");
     if (n == 0) return FT_HIP_OK;
     const NormArgs a{x, x_stride, x_w, residual, residual_stride, h, h_stride, w, y, y_stride,
                      static_cast<uint8_t*>(q8), (int)hidden, (double)eps, 1.0 / (double)hidden};

@@ -110,7 +110,8 @@ int ft_hip_quantize_q8(ft_hip_ctx* ctx, void* stream, const float* x, int64_t x_
  * or NULL; residual, h, y: f32 rows their own stride apart, each or NULL (not
  * all three outputs); q8: [n][hidden/32] blocks or NULL, 4-byte aligned. h
  * or y may be residual itself, or x itself where that is f32 (same stride);
- * nothing else may overlap an output. hidden <= 16384, a multiple of 32 where
+ * any other overlap of an output with an input or the other outputs is refused
+ * (rows side by side in one buffer overlap nowhere). hidden <= 16384, a multiple of 32 where
  * q8 is written; rows that all start on 4 values (16 bytes of f32) are read
  * four values at a time. */
 int ft_hip_add_rmsnorm(ft_hip_ctx* ctx, void* stream, const void* x, int x_type, int64_t x_stride, const float* x_w,

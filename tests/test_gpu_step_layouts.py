@@ -79,3 +79,33 @@ def test_norm_of_heads(gemv):
     gemv.add_rmsnorm(x.view(n, 4, 64), None, H, n, 1e-6, y=yh)
     torch.cuda.synchronize()
     assert torch.equal(yh.view(n, H), y)
+
+
+def test_norm_of_rows_side_by_side(gemv):
+    """x, residual, h and y as columns of one buffer, and with strides of their own in one: no row overlaps another."""
+    n, H = 5, 64
+    x, r, w = rows(n, H, 7), rows(n, H, 8), rows(1, H, 9)[0]
+    h, y, q8 = torch.zeros((n, H), device=DEV), torch.zeros((n, H), device=DEV), torch.zeros(n * 80, dtype=torch.uint8,
+                                                                                             device=DEV)
+    gemv.add_rmsnorm(x, w, H, n, 1e-6, residual=r, h=h, y=y, q8=q8)
+    one = torch.zeros((n, 4 * H), device=DEV)
+    xs, rs, hs, ys = (one[:, i * H:(i + 1) * H] for i in range(4))
+    xs.copy_(x)
+    rs.copy_(r)
+    qs = torch.zeros_like(q8)
+    gemv.add_rmsnorm(xs, w, H, n, 1e-6, residual=rs, h=hs, y=ys, q8=qs)
+    torch.cuda.synchronize()
+    assert torch.equal(hs, h) and torch.equal(ys, y) and torch.equal(qs, q8)
+    assert torch.equal(xs, x) and torch.equal(rs, r)
+    # x in steps of 3 H from 0, h in steps of 6 H from H: never the same place
+    one = torch.zeros(2 * 3 * H * n, device=DEV)
+    xs, hs = one.as_strided((n, H), (3 * H, 1)), one.as_strided((n, H), (6 * H, 1), H)
+    xs.copy_(x)
+    gemv.add_rmsnorm(xs, w, H, n, 1e-6, residual=r, h=hs)
+    torch.cuda.synchronize()
+    assert torch.equal(hs, h) and torch.equal(xs, x)
+    # h on the residual and y on x, with q8: rows on rows
+    xi, ri, qi = x.clone(), r.clone(), torch.zeros_like(q8)
+    gemv.add_rmsnorm(xi, w, H, n, 1e-6, residual=ri, h=ri, y=xi, q8=qi)
+    torch.cuda.synchronize()
+    assert torch.equal(ri, h) and torch.equal(xi, y) and torch.equal(qi, q8)

@@ -1,7 +1,10 @@
 """CPU tests: what the norm, the routing and the draw refuse of the memory they
 are given, before any GPU call (no pointer below is ever dereferenced)."""
 import ctypes
+import os
+import subprocess
 
+import numpy as np
 import pytest
 
 import ft_hip
@@ -25,3 +28,67 @@ def call(name, **change):
 def test_pointers_that_are_not_aligned(name, argument, at):
     rc, msg = call(name, **{argument: ctypes.c_void_p(at)})
     assert rc == ft_hip.E_SHAPE and "aligned" in msg, msg
+
+
+@pytest.fixture(scope="module")
+def overlap():
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    subprocess.run(["make", "-s", "-C", os.path.join(root, "oracle")], check=True)
+    f = ctypes.CDLL(os.path.join(root, "oracle", "_build", "liboverlapcheck.so")).oc_overlap
+    f.argtypes = [ctypes.c_uint64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64] * 2
+    return f
+
+
+def test_rows_that_overlap(overlap):
+    """Against the bytes themselves, for rows of the same and of other strides, side by side and interleaved."""
+    rng = np.random.default_rng(4)
+    met = [0, 0]
+    for i in range(20000):
+        spans = []
+        for _ in "ab":
+            n, size = int(rng.integers(1, 7)), int(rng.integers(1, 9))
+            spans.append([int(rng.integers(100, 140)), n, size + int(rng.integers(0, 12)), size])
+        if i % 2:
+            spans[1][2] = max(spans[0][2], spans[1][3])
+            spans[0][2] = max(spans[1][2], spans[0][3])
+        sets = [{at + r * stride + j for r in range(n) for j in range(size)} for at, n, stride, size in spans]
+        want = bool(sets[0] & sets[1])
+        assert overlap(*spans[0], *spans[1]) == overlap(*spans[1], *spans[0]) == want, spans
+        met[want] += 1
+    assert min(met) > 3000
+
+
+def test_rows_that_overlap_far_apart(overlap):
+    """Strides and addresses at the limits of what the entry points take."""
+    top, far = (1 << 57) - 4096, (1 << 63) // 8
+    assert not overlap(0, 2, 8, 8, 4096, 2, 8, 8)  # no pointer: no rows
+    assert not overlap(4096, 0, 8, 8, 4096, 1, 8, 8) and not overlap(4096, 1, 8, 8, 4096, 1, 8, 0)
+    assert overlap(top, 2, far, 64, top, 1, 64, 64) and not overlap(top, 2, far, 64, top + 64, 1, 64, 64)
+    assert overlap(top, 2, far, 64, top + far + 63, 1, 64, 1) and not overlap(top, 2, far, 64, top + far + 64, 1, 64, 1)
+    assert not overlap(top, 4194303, 1 << 39, 64, top + 64, 4194303, 1 << 39, (1 << 39) - 64)
+    assert overlap(top, 4194303, 1 << 39, 64, top + 64, 4194303, 1 << 39, (1 << 39) - 63)
+
+
+ROOM = ctypes.create_string_buffer(4096)  # stands for a context, which no refused call reads
+CTX = ctypes.cast(ROOM, ctypes.c_void_p)
+
+# x, residual, h, y: 2 rows of 64 f32 (256 bytes) a KiB apart in one buffer, weights and blocks (160 bytes) behind it
+LAID = dict(NORM, ctx=CTX, x=ctypes.c_void_p(0x10000), residual=ctypes.c_void_p(0x10100),
+            h=ctypes.c_void_p(0x10200), y=ctypes.c_void_p(0x10300), x_stride=256, residual_stride=256, h_stride=256,
+            y_stride=256, w=ctypes.c_void_p(0x20000), x_w=ctypes.c_void_p(0x20100), q8=ctypes.c_void_p(0x20200))
+
+
+@pytest.mark.parametrize("change", [
+    dict(h=0x10004), dict(h=0x100fc), dict(h=0x10104), dict(h=0x10500), dict(y=0x10504), dict(h=0x10304),
+    dict(y=0x10204), dict(h=0x10300), dict(y=0x20004), dict(h=0x200fc), dict(y=0x20100), dict(h=0x20204),
+    dict(h=0x10000, h_stride=64), dict(y=0x10100, y_stride=128), dict(h=0x10000, x_type=1), dict(y=0x10040, x_type=2),
+    dict(q8=0x10040), dict(q8=0x10440), dict(q8=0x10300), dict(q8=0x2009c), dict(q8=0x20180), dict(q8=0x10000),
+    dict(w=0x10300), dict(x_w=0x10200), dict(n=1, y=0x10080), dict(n=1, h=0x101fc),
+])
+def test_add_rmsnorm_refuses_outputs_that_overlap(change):
+    """Every case is refused before any GPU call."""
+    change = {k: ctypes.c_void_p(v) if k in ("x", "residual", "h", "y", "w", "x_w", "q8") else v
+              for k, v in change.items()}
+    rc = ft_hip.lib().ft_hip_add_rmsnorm(*{**LAID, **change}.values())
+    msg = ft_hip.lib().ft_hip_last_error().decode()
+    assert rc == ft_hip.E_SHAPE and "overlap" in msg, msg
