@@ -18,6 +18,7 @@
 // (kernels alone, f32 logits), stand beside it.
 
 #include "ft_device.hpp"
+#include "ft_overlap.hpp"
 #include "ft_runtime.hpp"
 #include "ft_wave.hpp"
 
@@ -1307,6 +1308,19 @@ extern "C" int ft_hip_sample_tokens(ft_hip_ctx* ctx, void* stream, const void* l
     if (workspace_bytes < need)
         return fail(FT_HIP_E_SHAPE, "sample_tokens: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     if (!ctx || !logits || !u || !tokens || !workspace) return fail(FT_HIP_E_INVALID, "sample_tokens: null argument");
+    // a row's settings are read before its outputs are written, and no other row's are: an output may be one of them
+    const int64_t size = logits_type == FT_TYPE_F32 ? 4 : 2;
+    const auto row4 = [&](const void* p) { return Span{p, 1, 0, n * 4}; };
+    const Span rows{logits, n, logits_stride * size, vocab * size}, ws{workspace, 1, 0, (int64_t)need},
+        tok = row4(tokens), lp = row4(logprobs), settings[] = {row4(temperature), row4(top_k), row4(top_p), row4(min_p),
+                                                               row4(u)};
+    if (overlap(tok, rows) || overlap(lp, rows) || overlap(tok, lp))
+        return fail(FT_HIP_E_SHAPE, "sample_tokens: tokens or logprobs overlap the logits or each other");
+    if (overlap(ws, rows) || overlap(ws, tok) || overlap(ws, lp))
+        return fail(FT_HIP_E_SHAPE, "sample_tokens: the workspace overlaps the logits or an output");
+    for (const Span& in : settings)
+        if (overlap(ws, in) || (overlap(tok, in) && tok.at != in.at) || (overlap(lp, in) && lp.at != in.at))
+            return fail(FT_HIP_E_SHAPE, "sample_tokens: the workspace or an output overlaps a row's settings");
     if (n == 0) return FT_HIP_OK;
     const int given = (temperature ? HAS_T : 0) | (top_k ? HAS_K : 0) | (top_p ? HAS_P : 0) | (min_p ? HAS_M : 0);
     const SampleArgs a{logits, logits_stride, (int)vocab, temperature ? temperature : u,

@@ -262,7 +262,8 @@ int ft_hip_topk_router(ft_hip_ctx* ctx, void* stream, const float* logits,
  * left, the other entries are expert 0 with weight 0, so that launches over the
  * pairs stay inside the bank and add nothing.
  * logits: [n_seqs] rows logits_stride values apart; ids/wts [n_seqs][top_k];
- * all pointers 4-byte aligned. n_experts <= 1024, n_groups <= 64 dividing it, top_k <= 32. */
+ * all pointers 4-byte aligned; ids and wts that overlap each other or an input
+ * are refused. n_experts <= 1024, n_groups <= 64 dividing it, top_k <= 32. */
 int ft_hip_route_experts(ft_hip_ctx* ctx, void* stream, const float* logits, int64_t logits_stride,
                          const float* bias, const float* expert_scale, int score, int64_t n_groups,
                          int64_t top_groups, int group_rank, int renorm, float scale, int32_t* ids, float* wts,
@@ -295,9 +296,11 @@ int ft_hip_reduce_pairs_weighted(ft_hip_ctx* ctx, void* stream, const float* y,
  * in a fixed order, or whole numbers where many threads add to one (there right
  * to 1e-9 of a sum): the same call gives the same bits.
  * logits: [n] rows of logits_type (FT_TYPE_*) logits_stride values apart, read
- * only; tokens [n]; logprobs [n] or NULL; each aligned to its type. workspace: device scratch of
- * ft_hip_sample_tokens_workspace_bytes() bytes (0 for a bad shape), 16-byte
- * aligned, any content, for one call at a time. */
+ * only; tokens [n]; logprobs [n] or NULL; each aligned to its type. workspace:
+ * device scratch of ft_hip_sample_tokens_workspace_bytes() bytes (0 for a bad
+ * shape), 16-byte aligned, any content, for one call at a time. tokens or
+ * logprobs may be one of the settings' arrays; any other overlap of an output
+ * or the workspace with an input or each other is refused. */
 #define FT_SAMPLE_MAX_VOCAB 2097152
 #define FT_SAMPLE_MAX_ROWS 65535
 size_t ft_hip_sample_tokens_workspace_bytes(int64_t vocab, int64_t n);

@@ -109,3 +109,32 @@ def test_norm_of_rows_side_by_side(gemv):
     gemv.add_rmsnorm(xi, w, H, n, 1e-6, residual=ri, h=ri, y=xi, q8=qi)
     torch.cuda.synchronize()
     assert torch.equal(ri, h) and torch.equal(xi, y) and torch.equal(qi, q8)
+
+
+@pytest.mark.parametrize("V", [700, 20000])
+def test_draw_into_the_settings_arrays(gemv, V):
+    """tokens over top_k and logprobs over the random numbers: as into arrays of their own."""
+    n = 40
+    l, ws = rows(n, V, V, 3.0), torch.empty(gemv.sample_tokens_workspace_bytes(V, n), dtype=torch.uint8, device=DEV)
+    u, k = torch.linspace(0, 0.99, n, device=DEV), torch.arange(n, dtype=torch.int32, device=DEV) * 3
+    t = torch.linspace(0, 2, n, device=DEV)
+    tokens, lp = torch.zeros(n, dtype=torch.int32, device=DEV), torch.zeros(n, device=DEV)
+    gemv.sample_tokens(l, V, n, u, tokens, ws, temperature=t, top_k=k, logprobs=lp)
+    gemv.sample_tokens(l, V, n, u, k, ws, temperature=t, top_k=k, logprobs=u)
+    torch.cuda.synchronize()
+    assert torch.equal(k, tokens) and torch.equal(u, lp)
+
+
+def test_routing_into_the_gaps_between_rows(gemv):
+    """ids and weights where padded rows of logits leave room: no row is touched."""
+    E, k = 64, 4
+    one = torch.full((2, 256), 60.0, device=DEV)
+    one[:, :E] = rows(2, E, 2)
+    before = one[:, :E].clone()
+    ids, wts = one[0, 128:128 + 2 * k].view(torch.int32), one[0, 200:200 + 2 * k]
+    want = torch.zeros((2, k), dtype=torch.int32, device=DEV), torch.zeros((2, k), device=DEV)
+    gemv.route_experts(one[:, :E].contiguous(), *want, E, k, 2)
+    gemv.route_experts(one[:, :E], ids, wts, E, k, 2)
+    torch.cuda.synchronize()
+    assert torch.equal(ids.view(2, k), want[0]) and torch.equal(wts.view(2, k), want[1])
+    assert torch.equal(one[:, :E], before)

@@ -92,3 +92,44 @@ def test_add_rmsnorm_refuses_outputs_that_overlap(change):
     rc = ft_hip.lib().ft_hip_add_rmsnorm(*{**LAID, **change}.values())
     msg = ft_hip.lib().ft_hip_last_error().decode()
     assert rc == ft_hip.E_SHAPE and "overlap" in msg, msg
+
+
+def refused(name, usual, change):
+    """Message of a call that has to be refused as a bad shape; whole numbers in place of pointers."""
+    now = {k: ctypes.c_void_p(v) if isinstance(usual[k], ctypes.c_void_p) and isinstance(v, int) else v
+           for k, v in {**usual, **change}.items()}
+    rc = getattr(ft_hip.lib(), "ft_hip_" + name)(*now.values())
+    msg = ft_hip.lib().ft_hip_last_error().decode()
+    assert rc == ft_hip.E_SHAPE, msg
+    return msg
+
+
+# 3 rows of 128 f32 (512 bytes) a KiB apart; ids and weights of 3 x 8 (96 bytes)
+ROUTED = dict(ROUTE, ctx=CTX, logits=ctypes.c_void_p(0x10000), stride=256, bias=ctypes.c_void_p(0x20000),
+              expert_scale=ctypes.c_void_p(0x20200), ids=ctypes.c_void_p(0x20400), wts=ctypes.c_void_p(0x20460))
+
+
+@pytest.mark.parametrize("change", [
+    dict(ids=0x10000), dict(wts=0x10000), dict(ids=0x101fc), dict(wts=0x103a4), dict(ids=0x109fc), dict(ids=0x20000),
+    dict(wts=0x201fc), dict(ids=0x203fc), dict(wts=0x201a4), dict(wts=0x20400), dict(wts=0x2045c), dict(ids=0x204bc),
+])
+def test_route_experts_refuses_outputs_that_overlap(change):
+    assert "overlap" in refused("route_experts", ROUTED, change)
+
+
+# 4 rows of 9000 logits (f32) 9216 apart, settings and outputs of 16 bytes each, the workspace behind
+SAMPLED = dict(SAMPLE, ctx=CTX, logits=ctypes.c_void_p(0x100000), stride=9216, vocab=9000,
+               temperature=ctypes.c_void_p(0x200000), top_k=ctypes.c_void_p(0x200010), top_p=ctypes.c_void_p(0x200020),
+               min_p=ctypes.c_void_p(0x200030), u=ctypes.c_void_p(0x200040), tokens=ctypes.c_void_p(0x200050),
+               logprobs=ctypes.c_void_p(0x200060), workspace=ctypes.c_void_p(0x300000))
+
+
+@pytest.mark.parametrize("change", [
+    dict(tokens=0x100000), dict(logprobs=0x108c9c), dict(tokens=0x109000 - 0x4), dict(logprobs=0x200050),
+    dict(logprobs=0x200044, u=0x200080), dict(logprobs=0x20005c), dict(workspace=0x100000), dict(workspace=0x108c90),
+    dict(workspace=0x200000), dict(workspace=0x1ffff0), dict(workspace=0x200040), dict(workspace=0x200050),
+    dict(workspace=0x200060), dict(tokens=0x200004), dict(tokens=0x200014), dict(logprobs=0x20001c),
+    dict(logprobs=0x200024), dict(tokens=0x200034), dict(tokens=0x20003c), dict(logprobs=0x200044),
+])
+def test_sample_tokens_refuses_memory_that_overlaps(change):
+    assert "overlap" in refused("sample_tokens", SAMPLED, change)
