@@ -286,7 +286,9 @@ extern "C" int ft_hip_add_rmsnorm(ft_hip_ctx* ctx, void* stream, const void* x, 
     if (!aligned(x, size) || !aligned(x_w, 4) || !aligned(residual, 4) || !aligned(h, 4) || !aligned(w, 4) ||
         !aligned(y, 4) || !aligned(q8, 4))
         return fail(FT_HIP_E_SHAPE, "add_rmsnorm: a pointer is not aligned to its type (q8: 4 bytes)");
-    if (!ctx || !x) return fail(FT_HIP_E_INVALID, "add_rmsnorm: null argument");
+    if (!ctx) return fail(FT_HIP_E_INVALID, "add_rmsnorm: null argument");
+    if (n == 0) return FT_HIP_OK;  // an empty tensor has no address
+    if (!x) return fail(FT_HIP_E_INVALID, "add_rmsnorm: null argument");
     if (!h && !y && !q8) return fail(FT_HIP_E_INVALID, "add_rmsnorm: no output (h, y and q8 are null)");
     // A thread writes the places that it has read, and no others: h or y may lie on an input's rows, on all of them with
     // the same stride; any other overlap would mix rows, or blocks with what they are made of.
@@ -302,7 +304,6 @@ extern "C" int ft_hip_add_rmsnorm(ft_hip_ctx* ctx, void* stream, const void* x, 
     if (overlap(sh, sy)) return fail(FT_HIP_E_SHAPE, "add_rmsnorm: h and y overlap");
     if (overlap(sq, sx) || overlap(sq, sr) || overlap(sq, sw) || overlap(sq, sxw))
         return fail(FT_HIP_E_SHAPE, "add_rmsnorm: q8 overlaps an input");
-    if (n == 0) return FT_HIP_OK;
     const NormArgs a{x, x_stride, x_w, residual, residual_stride, h, h_stride, w, y, y_stride,
                      static_cast<uint8_t*>(q8), (int)hidden, (double)eps, 1.0 / (double)hidden};
     // vectors of 4 where every row starts on one; else value by value

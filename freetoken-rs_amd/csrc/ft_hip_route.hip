@@ -369,14 +369,15 @@ extern "C" int ft_hip_route_experts(ft_hip_ctx* ctx, void* stream, const float* 
         return fail(FT_HIP_E_SHAPE, "route_experts: logits_stride out of range");
     if (!aligned(logits, 4) || !aligned(bias, 4) || !aligned(expert_scale, 4) || !aligned(ids, 4) || !aligned(wts, 4))
         return fail(FT_HIP_E_SHAPE, "route_experts: a pointer is not aligned to 4 bytes");
-    if (!ctx || !logits || !ids || !wts) return fail(FT_HIP_E_INVALID, "route_experts: null argument");
+    if (!ctx) return fail(FT_HIP_E_INVALID, "route_experts: null argument");
+    if (n_seqs == 0) return FT_HIP_OK;  // an empty tensor has no address
+    if (!logits || !ids || !wts) return fail(FT_HIP_E_INVALID, "route_experts: null argument");
     const Span in_l{logits, n_seqs, logits_stride * 4, E * 4}, in_b{bias, 1, 0, E * 4}, in_s{expert_scale, 1, 0, E * 4},
         out_i{ids, 1, 0, n_seqs * top_k * 4}, out_w{wts, 1, 0, n_seqs * top_k * 4};
     for (const Span& out : {out_i, out_w})
         if (overlap(out, in_l) || overlap(out, in_b) || overlap(out, in_s))
             return fail(FT_HIP_E_SHAPE, "route_experts: ids or wts overlap an input");
     if (overlap(out_i, out_w)) return fail(FT_HIP_E_SHAPE, "route_experts: ids and wts overlap");
-    if (n_seqs == 0) return FT_HIP_OK;
     const RouteArgs a{logits, logits_stride, bias, expert_scale, ids, wts, score == FT_SCORE_SIGMOID, (int)G,
                       (int)(E / G), (int)top_groups, group_rank, renorm, (double)scale, (int)E, (int)top_k, (int)n_seqs,
                       aligned(logits, 16) && logits_stride % 4 == 0 && E % 4 == 0};

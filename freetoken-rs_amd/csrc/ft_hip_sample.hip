@@ -1307,7 +1307,9 @@ extern "C" int ft_hip_sample_tokens(ft_hip_ctx* ctx, void* stream, const void* l
     const size_t need = ft_hip_sample_tokens_workspace_bytes(vocab, n);
     if (workspace_bytes < need)
         return fail(FT_HIP_E_SHAPE, "sample_tokens: workspace of %zu bytes, %zu needed", workspace_bytes, need);
-    if (!ctx || !logits || !u || !tokens || !workspace) return fail(FT_HIP_E_INVALID, "sample_tokens: null argument");
+    if (!ctx) return fail(FT_HIP_E_INVALID, "sample_tokens: null argument");
+    if (n == 0) return FT_HIP_OK;  // an empty tensor has no address
+    if (!logits || !u || !tokens || !workspace) return fail(FT_HIP_E_INVALID, "sample_tokens: null argument");
     // a row's settings are read before its outputs are written, and no other row's are: an output may be one of them
     const int64_t size = logits_type == FT_TYPE_F32 ? 4 : 2;
     const auto row4 = [&](const void* p) { return Span{p, 1, 0, n * 4}; };
@@ -1321,7 +1323,6 @@ extern "C" int ft_hip_sample_tokens(ft_hip_ctx* ctx, void* stream, const void* l
     for (const Span& in : settings)
         if (overlap(ws, in) || (overlap(tok, in) && tok.at != in.at) || (overlap(lp, in) && lp.at != in.at))
             return fail(FT_HIP_E_SHAPE, "sample_tokens: the workspace or an output overlaps a row's settings");
-    if (n == 0) return FT_HIP_OK;
     const int given = (temperature ? HAS_T : 0) | (top_k ? HAS_K : 0) | (top_p ? HAS_P : 0) | (min_p ? HAS_M : 0);
     const SampleArgs a{logits, logits_stride, (int)vocab, temperature ? temperature : u,
                        top_k ? top_k : reinterpret_cast<const int32_t*>(u), top_p ? top_p : u, min_p ? min_p : u, u,

@@ -111,7 +111,8 @@ int ft_hip_quantize_q8(ft_hip_ctx* ctx, void* stream, const float* x, int64_t x_
  * all three outputs); q8: [n][hidden/32] blocks or NULL, 4-byte aligned. h
  * or y may be residual itself, or x itself where that is f32 (same stride);
  * any other overlap of an output with an input or the other outputs is refused
- * (rows side by side in one buffer overlap nowhere). hidden <= 16384, a multiple of 32 where
+ * (rows side by side in one buffer overlap nowhere). n 0: nothing is done, and
+ * the rows' pointers may be NULL. hidden <= 16384, a multiple of 32 where
  * q8 is written; rows that all start on 4 values (16 bytes of f32) are read
  * four values at a time. */
 int ft_hip_add_rmsnorm(ft_hip_ctx* ctx, void* stream, const void* x, int x_type, int64_t x_stride, const float* x_w,
@@ -263,7 +264,8 @@ int ft_hip_topk_router(ft_hip_ctx* ctx, void* stream, const float* logits,
  * pairs stay inside the bank and add nothing.
  * logits: [n_seqs] rows logits_stride values apart; ids/wts [n_seqs][top_k];
  * all pointers 4-byte aligned; ids and wts that overlap each other or an input
- * are refused. n_experts <= 1024, n_groups <= 64 dividing it, top_k <= 32. */
+ * are refused. n_seqs 0: nothing is done, and the rows' pointers may be NULL.
+ * n_experts <= 1024, n_groups <= 64 dividing it, top_k <= 32. */
 int ft_hip_route_experts(ft_hip_ctx* ctx, void* stream, const float* logits, int64_t logits_stride,
                          const float* bias, const float* expert_scale, int score, int64_t n_groups,
                          int64_t top_groups, int group_rank, int renorm, float scale, int32_t* ids, float* wts,
@@ -300,7 +302,8 @@ int ft_hip_reduce_pairs_weighted(ft_hip_ctx* ctx, void* stream, const float* y,
  * device scratch of ft_hip_sample_tokens_workspace_bytes() bytes (0 for a bad
  * shape), 16-byte aligned, any content, for one call at a time. tokens or
  * logprobs may be one of the settings' arrays; any other overlap of an output
- * or the workspace with an input or each other is refused. */
+ * or the workspace with an input or each other is refused. n 0: nothing is
+ * done, and the pointers may be NULL. */
 #define FT_SAMPLE_MAX_VOCAB 2097152
 #define FT_SAMPLE_MAX_ROWS 65535
 size_t ft_hip_sample_tokens_workspace_bytes(int64_t vocab, int64_t n);

@@ -138,3 +138,17 @@ def test_routing_into_the_gaps_between_rows(gemv):
     torch.cuda.synchronize()
     assert torch.equal(ids.view(2, k), want[0]) and torch.equal(wts.view(2, k), want[1])
     assert torch.equal(one[:, :E], before)
+
+
+def test_an_empty_batch(gemv):
+    """Tensors without rows, as slices of a batch of none: nothing is done, nothing refused."""
+    f, i = torch.empty((0, 64), device=DEV), torch.empty((0, 4), dtype=torch.int32, device=DEV)
+    gemv.add_rmsnorm(f, None, 64, 0, 1e-6, residual=f, h=torch.empty_like(f), y=torch.empty_like(f),
+                     q8=torch.empty(0, dtype=torch.uint8, device=DEV))
+    gemv.add_rmsnorm(torch.empty((0, 1, 72), dtype=torch.float16, device=DEV), None, 64, 0, 1e-6, h=f)
+    gemv.route_experts(f, i, f[:, :4].contiguous(), 64, 4, 0)
+    for V in (64, 9000):
+        ws = torch.empty(gemv.sample_tokens_workspace_bytes(V, 0), dtype=torch.uint8, device=DEV)
+        none = torch.empty(0, device=DEV)
+        gemv.sample_tokens(torch.empty((0, V), device=DEV), V, 0, none, none.int(), ws, temperature=none, logprobs=none)
+    torch.cuda.synchronize()

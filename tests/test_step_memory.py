@@ -133,3 +133,18 @@ SAMPLED = dict(SAMPLE, ctx=CTX, logits=ctypes.c_void_p(0x100000), stride=9216, v
 ])
 def test_sample_tokens_refuses_memory_that_overlaps(change):
     assert "overlap" in refused("sample_tokens", SAMPLED, change)
+
+
+@pytest.mark.parametrize("name,change", [
+    ("add_rmsnorm", dict(x=None, residual=None, h=None, y=None, q8=None, n=0)), ("add_rmsnorm", dict(n=0)),
+    ("route_experts", dict(logits=None, ids=None, wts=None, n_seqs=0)), ("route_experts", dict(n_seqs=0)),
+    ("sample_tokens", dict(logits=None, u=None, tokens=None, workspace=None, n=0)), ("sample_tokens", dict(n=0)),
+])
+def test_no_rows(name, change):
+    """Nothing to do, also where an empty batch has no address; what is wrong of a shape or a handle stays refused."""
+    rc, msg = call(name, ctx=CTX, **change)
+    assert rc == ft_hip.OK, msg
+    rc, msg = call(name, **change)
+    assert rc == ft_hip.E_INVALID and "null" in msg, msg
+    bad = dict(add_rmsnorm=dict(hidden=0), route_experts=dict(top_k=0), sample_tokens=dict(vocab=0))[name]
+    assert call(name, ctx=CTX, **{**change, **bad})[0] == ft_hip.E_SHAPE
