@@ -9,10 +9,12 @@
 // The quants are those of u, before the row's scale: 127 u / a is the same
 // quotient for y, and taken from u it depends on 32 values instead of on the
 // last bit of a sum over the row. The quotient is rounded as the real number:
-// u and a have 24 bits, so 127 u / a is either a half exactly or further than
-// 2^-26 from one. It is taken as u times 127 / a * (1 + 2^-44), in f64 off by
-// less than 2^-45 of itself besides: a half comes out above the half, any
-// other stays on its side, and the nearest whole number is the one sought.
+// with u = U 2^i and a = A 2^j of 24-bit whole U and A, i <= j, it differs from
+// a half by |254 U - odd A 2^(j-i)| / (2 A 2^(j-i)): not at all, or by at least
+// 1 / (2 A 2^(j-i)), which is the quotient over 254 U and so over 2^-32 of it.
+// It is taken as u times 127 / a * (1 + 2^-44), in f64 off by less than 2^-45
+// of itself besides: a half comes out above the half, any other stays on its
+// side, and the nearest whole number is the one sought.
 //
 // Bound by memory: x, the residual, h, y and the blocks each move once; the
 // row stays in registers between its sum and its outputs. Sums and scales are
