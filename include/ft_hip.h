@@ -295,8 +295,10 @@ int ft_hip_reduce_pairs_weighted(ft_hip_ctx* ctx, void* stream, const float* y,
  * u: [n], in [0, 1); less or NaN as 0, 1 and more as the last kept index.
  * Logits of NaN and -inf are never drawn; +inf ones share the draw; a row
  * without any other gets token -1 and logprob NaN. Weights are f64 and sums f64
- * in a fixed order, or whole numbers where many threads add to one (there right
- * to 1e-9 of a sum): the same call gives the same bits.
+ * in a fixed order, or whole numbers where many threads add to one: there right
+ * to 1e-9 of a sum, and to vocab * 2^-43 of it (2.4e-7 at most) in a row whose
+ * cut lies among more values than a workgroup lists (over 8192). The same call
+ * gives the same bits.
  * logits: [n] rows of logits_type (FT_TYPE_*) logits_stride values apart, read
  * only; tokens [n]; logprobs [n] or NULL; each aligned to its type. workspace:
  * device scratch of ft_hip_sample_tokens_workspace_bytes() bytes (0 for a bad
