@@ -523,10 +523,11 @@ __device__ __forceinline__ void waves_before(const int* counts, int& before, int
 // A value that at least k of the row's values reach, from the maxima of parts
 // of it (lowest: the smallest of these above -inf, or less): k parts have one
 // each. -inf if fewer than k parts hold any. Counted in 256 pieces of the key
-// range, and again in the piece that reaches k while that holds many more: a
-// range that goes below 0 has pieces of whole binades. l.n is 0 on entry.
+// range, and again in the piece that reaches k while that holds many more, or
+// more than `most`: a range that goes below 0 has pieces of whole binades. l.n
+// is 0 on entry.
 template <typename PARTS>
-__device__ __forceinline__ float reached_by(int k, const PARTS& parts, float lowest, float M, RowLds& l) {
+__device__ __forceinline__ float reached_by(int k, int most, const PARTS& parts, float lowest, float M, RowLds& l) {
     const int lane = threadIdx.x & 63;
     uint32_t hi = key_of(M), lo = key_of(lowest);
     int base = 0;
@@ -560,7 +561,7 @@ __device__ __forceinline__ float reached_by(int k, const PARTS& parts, float low
         const uint64_t under = (((uint64_t)b + 1) << shift) - 1;
         lo = under >= width ? lo : hi - (uint32_t)under;
         hi -= (uint32_t)b << shift;
-        if (shift == 0 || through <= k + k / 2 + 32 || counts == l.n + 768) return of_key(lo);
+        if (shift == 0 || through <= min(k + k / 2 + 32, most) || counts == l.n + 768) return of_key(lo);
     }
 }
 
@@ -619,7 +620,7 @@ __global__ __launch_bounds__(ROW_THREADS) void k_sample_rows(SampleArgs a) {
     }
     const bool by_k = s.k < a.V, by_p = s.p < 1.0;
     float from = -INFINITY;
-    if (by_k && s.k <= ROW_THREADS) from = reached_by(s.k, Part{top}, lowest, M, l);
+    if (by_k && s.k <= ROW_THREADS) from = reached_by(s.k, ROW_THREADS, Part{top}, lowest, M, l);
     if (by_p && !by_k) {  // those of less than (1 - p) z / V are together less than the (1 - p) z that top_p leaves out
         double z = 0.0;
 #pragma unroll
@@ -669,6 +670,8 @@ struct Scan {
     char* base;
     int64_t row_bytes;
     int chunk, chunks, segs;
+    int most_k;        // the largest top-k that the segments' maxima decide
+    int most_reached;  // and how many of them the value that bounds it may leave
     __host__ __device__ static int64_t up16(int64_t v) { return (v + 15) / 16 * 16; }
     __host__ __device__ int64_t at_info() const { return up16((int64_t)segs * 4); }
     __host__ __device__ int64_t at_bins() const { return at_info() + up16((int64_t)chunks * sizeof(Chunk)); }
@@ -679,8 +682,8 @@ struct Scan {
 };
 
 // Whether a row is decided by its segments' maxima: the largest value alone,
-// or a top-k that the segments bound.
-__device__ __forceinline__ bool by_maxima(const Row& s, int segs) { return s.greedy || s.k <= segs; }
+// or a top-k that they bound by a list that fits (else the scan fills the bins).
+__device__ __forceinline__ bool by_maxima(const Row& s, const Scan& w) { return s.greedy || s.k <= w.most_k; }
 
 // A value's place in steps of e (per_unit: the step of 2^(1/8) per unit of the
 // logit), and its step, the nearest whole number: by the sum with MAGIC, whose
@@ -764,7 +767,7 @@ __global__ __launch_bounds__(1024) void k_sample_scan(SampleArgs a, Scan w, int6
         if ((lane & 15) == 0 && at < w.segs) seg[at] = x;
         m = fmaxf(m, x);
     }
-    if (by_maxima(s, w.segs)) return;
+    if (by_maxima(s, w)) return;
     m = wave_max(m);
     if (lane == 0) part[wave] = m;
     for (int b = t; b < BINS; b += T) bins[b] = 0;
@@ -1048,20 +1051,23 @@ __device__ __forceinline__ int run_end(const int* v, int n, int x) {
 }
 
 // The rest of a row after the scan, by one workgroup:
-//  - top_k up to the number of segments: the values that k segments' maxima
-//    reach are few and contain the top k; they go into the list, which decides
-//    alone.
+//  - top_k up to Scan::most_k: the values that k segments' maxima reach are a
+//    little more than k and contain the top k; they go into the list, which
+//    decides alone.
 //  - else the bins say on which step of e the order is cut. If all from there
 //    up fit the list, it decides alone; if not, the list holds the steps on
 //    which the cut lies, the bins what is above, and the token's chunk is read
 //    again for the draw.
-//  - where neither fits the list (thousands of equal values, say), or top_k of
-//    more than the list meets top_p, the row is streamed.
+//  - where neither fits the list, the row is streamed: more than LIST values on
+//    the step of the cut (equal ones, or a flat row: 262144 normal values of sd
+//    1 put 8806 on the step of top-p 0.9), top_k with top_p where more than LIST
+//    reach top_k's step, a top_k by maxima that lie in an order (the largest in
+//    few of the segments).
 // Bound by the chain of one workgroup's steps: about 4 us until the first data
 // is there, then the list's making and its cuts. A row of 262144: 14.5 us with
 // top-k 64 and top-p; 57 with top-p alone where the cut lies among thousands
 // (64 rows 71, 256 rows 87), of which reading its open segments again is 25 to
-// 36; streamed about 1 ms.
+// 36; streamed 0.3 to 1.4 ms, a row of 2^21 3 to 10.
 template <int TYPE>
 __global__ __launch_bounds__(ROW_THREADS) void k_sample_finish(SampleArgs a, Scan w, int64_t row0) {
     __shared__ RowLds l;
@@ -1101,8 +1107,8 @@ __global__ __launch_bounds__(ROW_THREADS) void k_sample_finish(SampleArgs a, Sca
     double rest = 0.0, goal = 0.0;
     const double unit = per_unit(s), g = step_of(M, unit), ref = over_step(M, g, unit);
     const uint64_t* bins = w.bins(blockIdx.x);
-    if (by_maxima(s, w.segs)) {
-        from = reached_by(s.k, segs, lowest, M, l);
+    if (by_maxima(s, w)) {
+        from = reached_by(s.k, w.most_reached, segs, lowest, M, l);
         if (s.m > 0.0 && !by_p) from = fmaxf(from, value_below(s.m, s, M));  // without top_p no sum needs the others
     } else {
         double far = 0.0;
@@ -1247,12 +1253,28 @@ constexpr int SCAN_ROWS = 512;  // rows whose scan the workspace holds
 // against 71.
 bool wide_scan(int64_t vocab, int64_t n) { return vocab * n < (int64_t)1024 * 8192; }
 
+// Where values lie in no order, those that k of the segments' maxima reach are -segs ln(1 - k / segs) in number: the k
+// for which they take a share of the list (a list that overflows is streamed).
+int parts_for(int segs, double share) { return (int)(segs * (1.0 - exp(-share * LIST / segs))); }
+
+// The largest top-k that the maxima decide takes 5/6 of the list, and is 7/8 of the segments at most: from there on the
+// list is far longer than k. Scan and finish, logits of sd 2.5, by maxima against by bins: 64 rows of 262144 (limit
+// 3322), top-k 64 28.9 us against 47.1, 3000 64 against 73; 256 rows, 3000 101 against 125, and past the limit 3481 392
+// against 134; a row of 2^21 (limit 6162), 6000 99 against 124, 8192 3126 against 162; 64 rows of 131072 (limit 1792),
+// 1740 46.5 against 52.0, 2048 248 against 56.
+int most_k_of(int segs) {
+    const int fits = parts_for(segs, 5.0 / 6.0), most = segs / 8 * 7;
+    return fits < most ? fits : most;
+}
+
 Scan scan_of(int64_t vocab, int64_t n, void* workspace) {
     Scan w;
     w.base = static_cast<char*>(workspace);
     w.chunk = 8192;
     w.chunks = (int)((vocab + w.chunk - 1) / w.chunk);
     w.segs = (int)((vocab + SEG - 1) / SEG);
+    w.most_k = most_k_of(w.segs);
+    w.most_reached = parts_for(w.segs, 0.95);
     w.row_bytes = Scan::up16(w.bytes());
     return w;
 }
