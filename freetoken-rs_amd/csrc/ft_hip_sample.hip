@@ -31,14 +31,20 @@ namespace {
 
 constexpr int ROW_THREADS = 1024, ROW_WAVES = ROW_THREADS / 64;
 constexpr int FIX = 42;     // fraction bits of a weight <= 1: 2^21 of them stay below 2^63
-constexpr int LIST = 8192;  // values of a row that a workgroup keeps in LDS
-constexpr int FEW = 256;    // values that are ranked by comparing all with all
+// values of a row that a workgroup keeps in LDS: the most, with what a finish keeps beside them, that its 160 KB hold
+// (one workgroup a CU). With 4096 64 rows of 8000 go through scan and finish, top-k 64 with top-p 18.2 us against 10.8,
+// neither 21.5 against 12.7, while 64 rows of 262144 with top-p take 91 against 97.
+constexpr int LIST = 8192;
+// values that are ranked by comparing all with all, four a lane of the wave that sums them: a row of 262144 with top-k
+// 64 and top-p 18.5 us, by counting as longer lists 23.9; where nothing but min_p cuts, 9.4 against 8.1 (64 rows of 2000)
+constexpr int FEW = 256;
 constexpr int SEG = 64;     // values whose maximum the scan leaves
 constexpr int MAX_SEGS = FT_SAMPLE_MAX_VOCAB / SEG;
 constexpr int MAX_CHUNKS = FT_SAMPLE_MAX_VOCAB / 8192;
 
 // e is counted in steps of 2^(1/8): BINS of them reach 2^-64 below a chunk's
-// largest. A value's e over its step's middle is in [2^-1/16, 2^1/16); a bin's
+// largest, beyond which 2^21 values weigh less than 2^-43 of it (more of them
+// would not fit the finish's LDS). A value's e over its step's middle is in [2^-1/16, 2^1/16); a bin's
 // word holds the number of values above bit 47 and below it their sum over
 // OFFSET in units of 2^-FRAC (8192 times 0.107 * 2^35 is far below 2^47). The
 // chunk's largest value itself is in no bin: how often it occurs is counted
@@ -1244,7 +1250,9 @@ __global__ __launch_bounds__(ROW_THREADS) void k_sample_finish(SampleArgs a, Sca
     draw(a, r, WholeRow<TYPE>{row, V}, c * w.chunk, min(w.chunk, V - c * w.chunk), before, total, cut, s, M, l);
 }
 
-constexpr int SCAN_ROWS = 512;  // rows whose scan the workspace holds
+// Rows whose scan the workspace holds, 148 KB each at 262144: two to a CU in the finish. 1024 rows of 32003 with top-k 64
+// and top-p 103 us; with 256 rows at a time 116, with all 1024 93 and twice the workspace.
+constexpr int SCAN_ROWS = 512;
 
 // A chunk of 8192 values by 1024 threads, where all chunks at once leave the
 // device half empty, or by 256 threads with four times the values each, which

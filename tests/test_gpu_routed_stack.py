@@ -7,7 +7,7 @@ import torch
 import ft_hip
 import moe_synth
 from test_gpu_norm import check_q8, host
-from test_gpu_step import SMALL, batch
+from test_gpu_step import SMALL, VOCAB, batch, head_of, settings, stack_of
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -65,3 +65,31 @@ def test_two_of_many_experts_carry_a_zipf_model(gemv, monkeypatch):
         popular = moe_synth.zipf_ranks(SMALL, m.L)[0] <= SMALL.top_k
         share.append(popular[host(r.ids)].mean())
     assert share[1] > share[0]
+
+
+def test_a_step_on_a_stream_that_is_not_current(gemv):
+    """All of a step on the given stream, behind what that stream already holds."""
+    n, H = 6, SMALL.hidden
+    r, head = stack_of(gemv, n), head_of(gemv, H, VOCAB, n)
+    x, s = batch(n, H, 70), settings(n, 70)
+    want = [t.clone() for t in (*head.run(*r.run(x, n), n, **s), r.branch, r.h)]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            r.branch.fill_(7.0)
+            r.h.fill_(7.0)
+        tokens, logprobs = head.run(*r.run(x, n, stream=side), n, stream=side, **s)
+        side.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip((tokens, logprobs, r.branch, r.h), want))
+    assert torch.cuda.current_stream() != side
+
+
+def test_a_step_of_no_sequences(gemv):
+    r, head = stack_of(gemv, 2), head_of(gemv, SMALL.hidden, VOCAB, 2)
+    none = torch.empty((0, SMALL.hidden), device=DEV)
+    before = [t.clone() for t in (r.h, r.ids, head.tokens)]
+    tokens, logprobs = head.run(*r.run(none, 0), 0, torch.empty(0, device=DEV))
+    torch.cuda.synchronize()
+    assert tokens.shape == logprobs.shape == (0,)
+    assert all(torch.equal(a.view(torch.int32), t.view(torch.int32)) for a, t in zip(before, (r.h, r.ids, head.tokens)))
