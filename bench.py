@@ -1,7 +1,7 @@
 #!/usr/bin/env python3
 """Benchmark of the MoE expert-FFN decode section on one MI355X.
 
-Workload (BASELINE.json configs[1]): the 30-layer Gemma-4-26B-A4B-shaped
+Workload: the 30-layer Gemma-4-26B-A4B-shaped
 expert section (H 2816, I 704, 128 experts, top-8, q4_0 banks of seeded
 Irwin-Hall(4) weights of sd 0.02, f32 routers of the same), decoding tokens at batch 1
 with the residual chain x <- x + MoE_l(rmsnorm(x)) between layers (attention
@@ -16,7 +16,7 @@ HBM GB/s over the algorithmic expert bytes (802,897,920 B/token), the
 roofline of the dominant kernel, and a CPU baseline (the oracle's restatement
 of ft-core's AVX2 path, timed on this host's cores on a bounded sample).
 
---config picks one of BASELINE.json's other configurations instead (cfg3 Zipf
+--config picks one of the other configurations instead (cfg3 Zipf
 routing, cfg4 batched decode at 16/64 tokens, cfg5 the large-expert shape at
 batch 1 and 32). One step is then one batch of B tokens through all layers;
 value stays us/token (step time / B) and GB/s counts each step's unique
@@ -47,7 +47,7 @@ MEASURED_TRAFFIC = {
     "large1": 132272406,     # k_gemv_gu_long, one launch (algorithmic 132,120,576 B)
 }
 METRIC = "MoE expert-FFN µs/token at batch 1 + achieved HBM GB/s (% of MI355X peak)"
-# name -> (shape, tokens per step, Zipf exponent of the router bias, BASELINE.json config)
+# name -> (shape, tokens per step, Zipf exponent of the router bias, number of the configuration)
 CONFIGS = {
     "gemma30": ("GEMMA", 1, None, 2),
     "zipf": ("GEMMA", 1, 1.1, 3),
@@ -775,7 +775,7 @@ def main():
     cpu = None
     chain = None
     if not args.no_cpu:
-        # the GPU box's CPU share for one GPU (OMP_NUM_THREADS there), else every logical CPU
+        # the CPU share given to one GPU (OMP_NUM_THREADS), else every logical CPU
         threads = int(os.environ.get("OMP_NUM_THREADS") or 0) or (os.cpu_count() or 1)
         cpu_name, n_logical = host_cpu()
         hid = hidden.view(n_steps * B, H).cpu().numpy()

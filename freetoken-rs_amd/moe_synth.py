@@ -40,7 +40,7 @@ class Shape:
     cfg_id: int
 
 
-# G (configs 1-4) and X (config 5).
+# Gemma's expert section (configurations 1-4) and the large experts (5).
 GEMMA = Shape("gemma4-26b-a4b-moe", 2816, 704, 128, 8, 30, 1)
 LARGE = Shape("large-expert-h4096-i14336", 4096, 14336, 8, 2, 32, 5)
 
