@@ -44,11 +44,12 @@ constexpr int MAX_CHUNKS = FT_SAMPLE_MAX_VOCAB / 8192;
 
 // e is counted in steps of 2^(1/8): BINS of them reach 2^-64 below a chunk's
 // largest, beyond which 2^21 values weigh less than 2^-43 of it (more of them
-// would not fit the finish's LDS). A value's e over its step's middle is in [2^-1/16, 2^1/16); a bin's
-// word holds the number of values above bit 47 and below it their sum over
-// OFFSET in units of 2^-FRAC (8192 times 0.107 * 2^35 is far below 2^47). The
-// chunk's largest value itself is in no bin: how often it occurs is counted
-// apart, so that equal largest logits weigh the same whole number everywhere.
+// would not fit the finish's LDS). A value's e over its step's middle is in
+// [2^-1/16, 2^1/16); a bin's word holds the number of values above bit 47 and
+// below it their sum over OFFSET in units of 2^-FRAC (8192 times 0.107 * 2^35
+// is far below 2^47). The chunk's largest value itself is in no bin: how often
+// it occurs is counted apart, so that equal largest logits weigh the same whole
+// number everywhere.
 constexpr int BINS = 512, FRAC = 35;
 constexpr double OFFSET = 0.9375;
 
@@ -743,8 +744,8 @@ __device__ __forceinline__ bool vec_row(const void* row) {
 
 // Workgroup (c, row): chunk c of the row in registers, VECS times four values
 // a thread; one pass over memory. With bins to fill it is bound by instructions,
-// about 36 a value, most in f64, and an LDS atomic: 256 rows of 262144 take 71 us
-// (3.8 TB/s), 64 rows 25, one 6.2. Where the segments' maxima decide, by memory:
+// about 33 a value, most in f64, and an LDS atomic: 256 rows of 262144 take 72 us
+// (3.7 TB/s), 64 rows 25, one 6.2. Where the segments' maxima decide, by memory:
 // 64 rows 11.7 us (5.7 TB/s, in part from the caches), one 3.2.
 template <int TYPE, int VECS>
 __global__ __launch_bounds__(1024) void k_sample_scan(SampleArgs a, Scan w, int64_t row0) {
@@ -1069,11 +1070,12 @@ __device__ __forceinline__ int run_end(const int* v, int n, int x) {
 //    1 put 8806 on the step of top-p 0.9), top_k with top_p where more than LIST
 //    reach top_k's step, a top_k by maxima that lie in an order (the largest in
 //    few of the segments).
-// Bound by the chain of one workgroup's steps: about 4 us until the first data
-// is there, then the list's making and its cuts. A row of 262144: 14.5 us with
-// top-k 64 and top-p; 57 with top-p alone where the cut lies among thousands
-// (64 rows 71, 256 rows 87), of which reading its open segments again is 25 to
-// 36; streamed 0.3 to 1.4 ms, a row of 2^21 3 to 10.
+// Bound by the chain of one workgroup's steps (its 162 KB of LDS leave a CU one):
+// about 4 us until the first data is there, then the list's making and its cuts.
+// A row of 262144: 14.7 us with top-k 64 and top-p; 57 with top-p alone where
+// the cut lies among thousands (64 rows 71, 256 rows 76 to 84), of which reading
+// its open segments again is 25 to 36; streamed 0.3 to 1.4 ms, a row of 2^21 3
+// to 10.
 template <int TYPE>
 __global__ __launch_bounds__(ROW_THREADS) void k_sample_finish(SampleArgs a, Scan w, int64_t row0) {
     __shared__ RowLds l;
