@@ -1067,7 +1067,7 @@ __device__ __forceinline__ int run_end(const int* v, int n, int x) {
 //    again for the draw.
 //  - where neither fits the list, the row is streamed: more than LIST values on
 //    the step of the cut (equal ones, or a flat row: 262144 normal values of sd
-//    1 put 8806 on the step of top-p 0.9), top_k with top_p where more than LIST
+//    1 put some 8750 on the step of top-p 0.9), top_k with top_p where more than LIST
 //    reach top_k's step, a top_k by maxima that lie in an order (the largest in
 //    few of the segments).
 // Bound by the chain of one workgroup's steps (its 162 KB of LDS leave a CU one):
