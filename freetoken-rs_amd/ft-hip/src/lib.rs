@@ -87,6 +87,53 @@ pub struct Route {
     pub scale: f32,
 }
 
+/// How a key-value cache holds its values (8 bits each, a scale a row).
+#[derive(Clone, Copy, Debug, PartialEq, Eq)]
+pub enum KvType {
+    I8,
+    E4m3,
+}
+
+/// A quantised key-value cache in device memory: `n_pages` pages of
+/// `page_tokens` tokens, `n_heads` key heads of `head_dim` (see the header).
+#[derive(Clone, Copy, Debug)]
+pub struct KvCache {
+    pub data: DevPtr,
+    pub kind: KvType,
+    pub n_pages: usize,
+    pub page_tokens: usize,
+    pub n_heads: usize,
+    pub head_dim: usize,
+}
+impl KvCache {
+    fn raw(self) -> i32 {
+        match self.kind {
+            KvType::I8 => ffi::FT_KV_I8,
+            KvType::E4m3 => ffi::FT_KV_E4M3,
+        }
+    }
+    /// Bytes of a page, None for sizes that are refused.
+    pub fn page_bytes(page_tokens: usize, n_heads: usize, head_dim: usize) -> Option<usize> {
+        let b = unsafe { ffi::ft_hip_kv_page_bytes(page_tokens as i64, n_heads as i64, head_dim as i64) };
+        usize::try_from(b).ok()
+    }
+}
+
+/// Lists of whole numbers, one a sequence: the address, the numbers from one
+/// list to the next and how many of them count.
+#[derive(Clone, Copy, Debug)]
+pub struct Lists(pub DevPtr, pub usize, pub usize);
+
+/// The penalties of `adjust_logits`, an array a row each, None: off.
+#[derive(Clone, Copy, Debug, Default)]
+pub struct Penalties {
+    pub history: Option<Lists>,
+    pub history_len: Option<DevPtr>,
+    pub repetition: Option<DevPtr>,
+    pub presence: Option<DevPtr>,
+    pub frequency: Option<DevPtr>,
+}
+
 /// Bytes per 32-element q8 activation block.
 pub const Q8_BLK: usize = ffi::FT_Q8_BLK;
 
@@ -304,6 +351,75 @@ impl Q4Gemv {
             ffi::ft_hip_sample_tokens(self.ctx, s.0, p(logits.0), logits_type.raw(), logits.1 as i64, vocab as i64,
                                       n as i64, opt(temperature), opt(top_k), opt(top_p), opt(min_p), p(u),
                                       pm(tokens), pm(logprobs.unwrap_or(0)), pm(workspace), workspace_bytes)
+        })
+    }
+
+    /// Penalties, biases (`bias`: ids and values, `n_bias` a row) and a mask on rows
+    /// of logits in front of `sample_tokens` (see the header).
+    #[allow(clippy::too_many_arguments)]
+    pub fn adjust_logits(&self, s: Stream, logits: Rows, logits_type: Type, vocab: usize, n: usize,
+                         penalties: Penalties, bias: Option<(DevPtr, DevPtr)>, n_bias: usize, mask: Option<Rows>,
+                         out: Rows) -> Result<()> {
+        let h = penalties.history.unwrap_or(Lists(0, 0, 0));
+        let m = mask.unwrap_or(Rows(0, 0));
+        let (ids, add) = bias.unwrap_or((0, 0));
+        check(unsafe {
+            ffi::ft_hip_adjust_logits(self.ctx, s.0, p(logits.0), logits_type.raw(), logits.1 as i64, vocab as i64,
+                                      n as i64, p(h.0), h.1 as i64, h.2 as i64, opt(penalties.history_len),
+                                      opt(penalties.repetition), opt(penalties.presence), opt(penalties.frequency),
+                                      p(ids), p(add), if bias.is_some() { n_bias as i64 } else { 0 }, p(m.0),
+                                      m.1 as i64, pm(out.0), out.1 as i64)
+        })
+    }
+
+    /// Rows of keys and values quantised into the cache's `slots` (the reference's
+    /// `kv_append`, ft-cuda/src/q4.cu:996-1012, keeps f32; see the header).
+    #[allow(clippy::too_many_arguments)]
+    pub fn kv_write(&self, s: Stream, k: Rows, v: Rows, kind: Type, slots: DevPtr, c: KvCache, n: usize)
+                    -> Result<()> {
+        check(unsafe {
+            ffi::ft_hip_kv_write(self.ctx, s.0, p(k.0), k.1 as i64, p(v.0), v.1 as i64, kind.raw(), p(slots),
+                                 pm(c.data), c.raw(), c.n_pages as i64, c.page_tokens as i64, c.n_heads as i64,
+                                 c.head_dim as i64, n as i64)
+        })
+    }
+
+    /// The reverse: rows of the tokens in `slots`.
+    #[allow(clippy::too_many_arguments)]
+    pub fn kv_read(&self, s: Stream, c: KvCache, slots: DevPtr, k: Rows, v: Rows, kind: Type, n: usize)
+                   -> Result<()> {
+        check(unsafe {
+            ffi::ft_hip_kv_read(self.ctx, s.0, p(c.data), c.raw(), c.n_pages as i64, c.page_tokens as i64,
+                                c.n_heads as i64, c.head_dim as i64, p(slots), pm(k.0), k.1 as i64, pm(v.0),
+                                v.1 as i64, kind.raw(), n as i64)
+        })
+    }
+
+    /// Bytes of `attention`'s workspace (0: a shape it refuses).
+    pub fn attention_workspace_bytes(n_seqs: usize, n_q: usize, n_heads: usize, n_kv_heads: usize, head_dim: usize)
+                                     -> usize {
+        unsafe {
+            ffi::ft_hip_attention_workspace_bytes(n_seqs as i64, n_q as i64, n_heads as i64, n_kv_heads as i64,
+                                                  head_dim as i64)
+        }
+    }
+
+    /// Attention of a batch's newest tokens over the cache (the reference's
+    /// `attn_decode_batch`, ft-cuda/src/q4.cu:732-829): each sequence over its own
+    /// pages in `tables`, `lens` tokens, behind `prefix` (its pages, how many, and
+    /// the device address of its tokens' number), which all share (see the header).
+    #[allow(clippy::too_many_arguments)]
+    pub fn attention(&self, s: Stream, q: Rows, kind: Type, c: KvCache, tables: Lists, lens: DevPtr,
+                     prefix: Option<(DevPtr, usize, DevPtr)>, n_seqs: usize, n_q: usize, n_heads: usize, scale: f32,
+                     window: usize, out: Rows, lse: Option<DevPtr>, workspace: DevPtr, workspace_bytes: usize)
+                     -> Result<()> {
+        let (pages, n, len) = prefix.unwrap_or((0, 0, 0));
+        check(unsafe {
+            ffi::ft_hip_attention(self.ctx, s.0, p(q.0), q.1 as i64, kind.raw(), p(c.data), c.raw(),
+                                  c.n_pages as i64, c.page_tokens as i64, c.n_heads as i64, c.head_dim as i64,
+                                  p(tables.0), tables.1 as i64, tables.2 as i64, p(lens), p(pages), n as i64, p(len),
+                                  n_seqs as i64, n_q as i64, n_heads as i64, scale, window as i64, pm(out.0),
+                                  out.1 as i64, pm(lse.unwrap_or(0)), pm(workspace), workspace_bytes)
         })
     }
 

@@ -22,6 +22,7 @@ Q8_BLK = 40
 LAYOUT_Q4_0, LAYOUT_Q4R = 0, 1
 TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+KV_I8, KV_E4M3 = 0, 1
 
 _lib = None
 
@@ -54,6 +55,14 @@ SIGNATURES = {
     "ft_hip_reduce_pairs_weighted": (_I, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64]),
     "ft_hip_sample_tokens_workspace_bytes": (_SZ, [_I64, _I64]),
     "ft_hip_sample_tokens": (_I, [_P, _P, _P, _I, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _SZ]),
+    "ft_hip_adjust_logits": (_I, [_P, _P, _P, _I, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _I64, _P,
+                                  _I64, _P, _I64]),
+    "ft_hip_kv_page_bytes": (_I64, [_I64, _I64, _I64]),
+    "ft_hip_kv_write": (_I, [_P, _P, _P, _I64, _P, _I64, _I, _P, _P, _I, _I64, _I64, _I64, _I64, _I64]),
+    "ft_hip_kv_read": (_I, [_P, _P, _P, _I, _I64, _I64, _I64, _I64, _P, _P, _I64, _P, _I64, _I, _I64]),
+    "ft_hip_attention_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I64]),
+    "ft_hip_attention": (_I, [_P, _P, _P, _I64, _I, _P, _I, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _P,
+                              _I64, _I64, _I64, _F, _I64, _P, _I64, _P, _P, _SZ]),
     "ft_hip_repack_rows": (_I, [_P, _P, _P, _I, _P, _I, _I64, _I64]),
     "ft_hip_gen_values": (_I, [_P, _P, _U64, _I64, _I64, _F, _P]),
     "ft_hip_gen_q4_rows": (_I, [_P, _P, _U64, _I64, _I64, _I64, _F, _P, _I]),
@@ -213,6 +222,30 @@ def _rows(t, n, width, size, what, device):
     if not ok and n > 0:
         raise FtHipError(E_SHAPE, f"{what}: {tuple(shape)} does not hold {n} rows of {width} consecutive values")
     return t.data_ptr(), stride
+
+
+def _values(t, n, whole, what, device):
+    """Pointer of n contiguous 4-byte values, whole numbers or f32; None: NULL."""
+    if t is None:
+        return None
+    if (t.get_device() != device or t.element_size() != 4 or t.dtype.is_floating_point is whole or not t.is_contiguous()
+            or t.numel() < n):
+        raise FtHipError(E_SHAPE, f"{what} does not hold {n} values of its 4-byte type on device {device}")
+    return t.data_ptr()
+
+
+def _lists(t, n, what, device):
+    """(pointer, row stride, width) of n rows of 4-byte whole numbers in a [rows, width] tensor; (NULL, 0, 0) for
+    None."""
+    if t is None:
+        return None, 0, 0
+    if t.get_device() != device:
+        raise FtHipError(E_INVALID, f"{what}: on {t.device}, the handle's device is {device}")
+    if t.element_size() != 4 or t.dtype.is_floating_point:
+        raise FtHipError(E_INVALID, f"{what}: {t.dtype} is no whole number of 4 bytes")
+    if t.dim() != 2 or t.shape[0] < n or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        raise FtHipError(E_SHAPE, f"{what}: {tuple(t.shape)} of strides {t.stride()} does not hold {n} rows")
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1], t.shape[1]
 
 
 class Q4Gemv:
@@ -401,6 +434,99 @@ class Q4Gemv:
             raise FtHipError(E_SHAPE, f"sample_tokens: workspace of strides {workspace.stride()} is not contiguous")
         check(lib().ft_hip_sample_tokens(self._ctx, self._on(stream), lp, _type(logits), ls, vocab, n, *ptrs,
                                          _ptr(workspace), workspace.numel() * workspace.element_size()))
+
+    # -- no reference counterpart: what a request's settings make of its logits, in front of the draw --
+    def adjust_logits(self, logits, out, vocab, n, history=None, history_len=None, repetition=None, presence=None,
+                      frequency=None, bias_ids=None, bias=None, mask=None, stream=None):
+        """out (f32 rows, or the f32 logits themselves) = rows of logits with penalties for the tokens of
+        history [n, width] (history_len [n] of them), biases [n, count] on bias_ids, and -inf where a mask's bit
+        ([n, words] of 32 tokens) is 0 (see the header)."""
+        lp, ls = _rows(logits, n, vocab, logits.element_size(), "adjust_logits: logits", self.device)
+        op, os_ = _rows(out, n, vocab, 4, "adjust_logits: out", self.device)
+        hp, hs, hm = _lists(history, n, "adjust_logits: history", self.device)
+        mp, ms, mw = _lists(mask, n, "adjust_logits: mask", self.device)
+        if mask is not None and mw < (vocab + 31) // 32:
+            raise FtHipError(E_SHAPE, f"adjust_logits: mask of {mw} words a row does not hold {vocab} bits")
+        if (bias is None) is not (bias_ids is None) or (bias is not None and bias.shape != bias_ids.shape):
+            raise FtHipError(E_SHAPE, "adjust_logits: bias and bias_ids are not of one shape")
+        if bias is not None and (bias.dim() != 2 or bias.shape[0] < n):
+            raise FtHipError(E_SHAPE, f"adjust_logits: bias of {tuple(bias.shape)} does not hold {n} rows")
+        nb = 0 if bias is None else bias.shape[1]
+        bp = _values(bias, n * nb, False, "adjust_logits: bias", self.device)
+        ip = _values(bias_ids, n * nb, True, "adjust_logits: bias_ids", self.device)
+        hl = _values(history_len, n, True, "adjust_logits: history_len", self.device)
+        per = [_values(t, n, False, f"adjust_logits: {what}", self.device)
+               for t, what in ((repetition, "repetition"), (presence, "presence"), (frequency, "frequency"))]
+        check(lib().ft_hip_adjust_logits(self._ctx, self._on(stream), lp, _type(logits), ls, vocab, n, hp, hs, hm, hl,
+                                         *per, ip, bp, nb, mp, ms, op, os_))
+
+    # -- ft-cuda/src/q4.cu:996-1012 (kv_append), quantised and in pages --
+    @staticmethod
+    def kv_page_bytes(page_tokens, n_heads, head_dim):
+        return lib().ft_hip_kv_page_bytes(page_tokens, n_heads, head_dim)
+
+    def _cache(self, cache, page_tokens, n_heads, head_dim, what):
+        """(pointer, pages) of a cache tensor."""
+        page = lib().ft_hip_kv_page_bytes(page_tokens, n_heads, head_dim)
+        if cache.get_device() != self.device or not cache.is_contiguous():
+            raise FtHipError(E_SHAPE, f"{what}: cache on {cache.device} of strides {cache.stride()} is not contiguous on "
+                                      f"device {self.device}")
+        # sizes without a page are the library's to refuse
+        return cache.data_ptr(), cache.numel() * cache.element_size() // page if page > 0 else 1
+
+    def kv_write(self, k, v, slots, cache, n, n_heads, head_dim, page_tokens, cache_type=KV_I8, stream=None):
+        """n rows of keys and values (f32, f16 or bf16, heads side by side) quantised into slots[n] of the cache
+        (a byte tensor of whole pages; see the header)."""
+        size = k.element_size()
+        if v.dtype != k.dtype:
+            raise FtHipError(E_INVALID, f"kv_write: keys of {k.dtype}, values of {v.dtype}")
+        kp, ks = _rows(k, n, n_heads * head_dim, size, "kv_write: k", self.device)
+        vp, vs = _rows(v, n, n_heads * head_dim, size, "kv_write: v", self.device)
+        sp = _values(slots, n, True, "kv_write: slots", self.device)
+        cp, pages = self._cache(cache, page_tokens, n_heads, head_dim, "kv_write")
+        check(lib().ft_hip_kv_write(self._ctx, self._on(stream), kp, ks, vp, vs, _type(k), sp, cp, cache_type, pages,
+                                    page_tokens, n_heads, head_dim, n))
+
+    def kv_read(self, cache, slots, k, v, n, n_heads, head_dim, page_tokens, cache_type=KV_I8, stream=None):
+        """The reverse: rows k and v of the tokens in slots[n]."""
+        size = k.element_size()
+        if v.dtype != k.dtype:
+            raise FtHipError(E_INVALID, f"kv_read: keys of {k.dtype}, values of {v.dtype}")
+        kp, ks = _rows(k, n, n_heads * head_dim, size, "kv_read: k", self.device)
+        vp, vs = _rows(v, n, n_heads * head_dim, size, "kv_read: v", self.device)
+        sp = _values(slots, n, True, "kv_read: slots", self.device)
+        cp, pages = self._cache(cache, page_tokens, n_heads, head_dim, "kv_read")
+        check(lib().ft_hip_kv_read(self._ctx, self._on(stream), cp, cache_type, pages, page_tokens, n_heads, head_dim,
+                                   sp, kp, ks, vp, vs, _type(k), n))
+
+    # -- ft-cuda/src/q4.cu:732-896 (attn_decode_batch), over the quantised cache, with a shared prefix --
+    @staticmethod
+    def attention_workspace_bytes(n_seqs, n_q, n_heads, n_kv_heads, head_dim):
+        return lib().ft_hip_attention_workspace_bytes(n_seqs, n_q, n_heads, n_kv_heads, head_dim)
+
+    def attention(self, q, cache, tables, lens, out, workspace, n_seqs, n_heads, n_kv_heads, head_dim, page_tokens,
+                  scale, n_q=1, window=0, prefix=None, prefix_len=None, lse=None, cache_type=KV_I8, stream=None):
+        """out = attention of the newest n_q tokens of n_seqs sequences (rows q, heads side by side) over the
+        prefix_len[0] tokens in the pages prefix[...] and their own lens[i] in tables[i, ...]; lse
+        [n_seqs * n_q, n_heads] or None (see the header)."""
+        rows, width = n_seqs * n_q, n_heads * head_dim
+        if out.dtype != q.dtype:
+            raise FtHipError(E_INVALID, f"attention: queries of {q.dtype}, out of {out.dtype}")
+        qp, qs = _rows(q, rows, width, q.element_size(), "attention: q", self.device)
+        op, os_ = _rows(out, rows, width, q.element_size(), "attention: out", self.device)
+        tp, ts, tw = _lists(tables, n_seqs, "attention: tables", self.device)
+        lp = _values(lens, n_seqs, True, "attention: lens", self.device)
+        pn = 0 if prefix is None else prefix.numel()
+        pp = _values(prefix, pn, True, "attention: prefix", self.device)
+        pl = _values(prefix_len, 1, True, "attention: prefix_len", self.device)
+        sp = _values(lse, rows * n_heads, False, "attention: lse", self.device)
+        cp, pages = self._cache(cache, page_tokens, n_kv_heads, head_dim, "attention")
+        if workspace.get_device() != self.device or not workspace.is_contiguous():
+            raise FtHipError(E_SHAPE, f"attention: workspace on {workspace.device} of strides {workspace.stride()} is not "
+                                      f"contiguous on device {self.device}")
+        check(lib().ft_hip_attention(self._ctx, self._on(stream), qp, qs, _type(q), cp, cache_type, pages, page_tokens,
+                                     n_kv_heads, head_dim, tp, ts, tw, lp, pp, pn, pl, n_seqs, n_q, n_heads, scale,
+                                     window, op, os_, sp, _ptr(workspace), workspace.numel() * workspace.element_size()))
 
     # -- setup: ft-core/src/q4_0.rs:248-258 on the device --
     def repack_rows(self, src, src_layout, dst, dst_layout, n_rows, k, stream=None):

@@ -64,6 +64,10 @@ extern "C" {
 #define FT_SCORE_SOFTMAX 0
 #define FT_SCORE_SIGMOID 1
 
+/* how a key-value cache holds its values (8 bits each, a scale a row) */
+#define FT_KV_I8 0
+#define FT_KV_E4M3 1
+
 typedef struct ft_hip_ctx ft_hip_ctx;
 
 /* Library version (major*10000 + minor*100 + patch). */
@@ -118,6 +122,75 @@ int ft_hip_quantize_q8(ft_hip_ctx* ctx, void* stream, const float* x, int64_t x_
 int ft_hip_add_rmsnorm(ft_hip_ctx* ctx, void* stream, const void* x, int x_type, int64_t x_stride, const float* x_w,
                        const float* residual, int64_t residual_stride, float* h, int64_t h_stride, const float* w,
                        float eps, float* y, int64_t y_stride, void* q8, int64_t hidden, int64_t n);
+
+/* A quantised key-value cache, written and read back (the reference's kv_append,
+ * ft-cuda/src/q4.cu:996-1012, keeps f32 rows).
+ * A cache is n_pages pages of page_tokens tokens (16, 32, 64, 128 or 256); slot
+ * p * page_tokens + o is place o of page p. A page holds for each of n_heads key
+ * heads, one after the other, with D = head_dim (64, 128 or 256):
+ *   keys    page_tokens x D bytes, [tiles of 16 tokens][D/16][16 tokens][16 dims]
+ *   values  page_tokens x D bytes, [tiles][D/64][4 groups][64 dims][4 tokens]
+ *   page_tokens f32 scales of the keys, then of the values
+ * ft_hip_kv_page_bytes: a page's bytes, n_heads * page_tokens * (2 D + 8), or -1
+ * for sizes that are refused. A value is its 8 bits' number times its row's
+ * scale d. With a = max |x| of the D values of a token and head:
+ *   FT_KV_I8    d = f32(a / 127), q = round half away from zero of 127 x / a
+ *               (the real quotient's), the byte is q + 128
+ *   FT_KV_E4M3  d = 2^e, the smallest with a / d <= 448 (e >= -126), the code is
+ *               the e4m3 value nearest to x / d, halves to even
+ * A row of zeros has d = 0; one with a NaN or an infinity d = NaN, all q 0.
+ *
+ * ft_hip_kv_write: k and v are n rows (k_stride, v_stride values apart, heads
+ * side by side: columns of a row of projections will do) of `type`; row i goes to
+ * slots[i]. A slot that is negative or behind the last is passed over, what no
+ * slot names stays as it was; equal slots leave one of their rows or a mixture.
+ * ft_hip_kv_read: the reverse; f32(q * d) rounded to `type`; the rows of slots
+ * that are passed over stay as they were.
+ * cache is 16-byte aligned, slots 4-byte, rows to their type; rows that start on
+ * four values are read four at a time. The cache, and read's rows, may not
+ * overlap any other argument. n 0: nothing is done, and the pointers may be
+ * NULL. n <= 2^24; n_heads <= 256; n_pages * page_tokens < 2^31. */
+int64_t ft_hip_kv_page_bytes(int64_t page_tokens, int64_t n_heads, int64_t head_dim);
+int ft_hip_kv_write(ft_hip_ctx* ctx, void* stream, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                    int type, const int32_t* slots, void* cache, int cache_type, int64_t n_pages, int64_t page_tokens,
+                    int64_t n_heads, int64_t head_dim, int64_t n);
+int ft_hip_kv_read(ft_hip_ctx* ctx, void* stream, const void* cache, int cache_type, int64_t n_pages,
+                   int64_t page_tokens, int64_t n_heads, int64_t head_dim, const int32_t* slots, void* k,
+                   int64_t k_stride, void* v, int64_t v_stride, int type, int64_t n);
+
+/* Attention of a batch's newest tokens over a quantised cache, with a prefix
+ * that all sequences share computed once for all (the reference's attn_decode
+ * and attn_decode_batch, ft-cuda/src/q4.cu:732-896, without pages or a prefix).
+ * Sequence i has lens[i] tokens of its own in the pages tables[i][0..table_pages)
+ * (its newest n_q included: they are written first) behind prefix_len[0] tokens
+ * in the pages prefix[0..prefix_pages) (prefix NULL: none). Its query t of n_q
+ * is its own token o = lens[i] - n_q + t; with o < 0 it is padding: out 0, lse
+ * -inf. It sees the prefix and its own tokens up to o, with a window w > 0 only
+ * the last w of them; per head h, on key head h / (n_heads / n_kv_heads):
+ *   s_j = scale * q . k_j,  out = sum_j exp(s_j) v_j / sum_j exp(s_j),
+ *   lse = log sum_j exp(s_j)
+ * lens and prefix_len are read on the device and taken as at least 0 and at most
+ * what their pages hold; tokens in a page that is not in the cache (negative
+ * or >= n_pages) count as not seen. A row that sees nothing has out 0 and lse
+ * -inf. q, out: n_seqs * n_q rows of `type`, heads side by side; lse:
+ * [n_seqs * n_q][n_heads] or NULL. Products are exact in their 8 bits and, for
+ * q and the weights, 11 bits where `type` is f16 or bf16 (q itself exact) and 22
+ * where it is f32, but not below 2^-32 of the largest weight times the largest
+ * scale of the values that a row's piece has met; sums are f32. The same call
+ * gives the same bits.
+ * workspace: device scratch of ft_hip_attention_workspace_bytes() bytes (0 for a
+ * bad shape), 16-byte aligned, any content, for one call at a time. out, lse and
+ * the workspace may not overlap an input or each other. n_seqs 0: nothing is
+ * done, and the pointers may be NULL. n_seqs <= FT_ATTN_MAX_SEQS, n_q <= 64. */
+#define FT_ATTN_MAX_SEQS 4096
+size_t ft_hip_attention_workspace_bytes(int64_t n_seqs, int64_t n_q, int64_t n_heads, int64_t n_kv_heads,
+                                        int64_t head_dim);
+int ft_hip_attention(ft_hip_ctx* ctx, void* stream, const void* q, int64_t q_stride, int type, const void* cache,
+                     int cache_type, int64_t n_pages, int64_t page_tokens, int64_t n_kv_heads, int64_t head_dim,
+                     const int32_t* tables, int64_t table_stride, int64_t table_pages, const int32_t* lens,
+                     const int32_t* prefix, int64_t prefix_pages, const int32_t* prefix_len, int64_t n_seqs,
+                     int64_t n_q, int64_t n_heads, float scale, int64_t window, void* out, int64_t out_stride,
+                     float* lse, void* workspace, size_t workspace_bytes);
 
 /* Grouped q4 x q8 GEMV over per-entry weight pointers. Replaces
  * gemv_grouped_q8_ptr (ft-cuda/src/lib.rs:593-623, layout q4_0) and
@@ -313,6 +386,30 @@ int ft_hip_sample_tokens(ft_hip_ctx* ctx, void* stream, const void* logits, int 
                          int64_t vocab, int64_t n, const float* temperature, const int32_t* top_k,
                          const float* top_p, const float* min_p, const float* u, int32_t* tokens, float* logprobs,
                          void* workspace, size_t workspace_bytes);
+
+/* Penalties for repeated tokens, biases and a grammar's mask on rows of logits,
+ * in front of ft_hip_sample_tokens (no reference counterpart). Per row and token
+ * v, c the times it is in the row's history:
+ *   x = l
+ *   c > 0: x = x > 0 ? x / repetition : x * repetition;
+ *          x = x - (presence + frequency * c)
+ *   x = x + b, b the sum of the row's biases for v, in their order
+ *   mask bit 0: x = -inf
+ * in f32, one rounding an operation. logits: [n] rows of logits_type; out: [n]
+ * f32 rows, or the logits themselves (f32, same stride). history: [n] rows of up
+ * to history_max tokens or NULL, history_len: [n] how many of them count (NULL:
+ * all); repetition, presence, frequency: [n] or NULL for 1, 0 and 0. bias_ids,
+ * bias: [n][n_bias]. Tokens of history and bias_ids outside [0, vocab) count
+ * nothing. mask: [n] rows of words, bit v % 32 of word v / 32 is 1 where v is
+ * allowed, or NULL. NaN stays NaN unless it is masked. Any other overlap of out
+ * with an input is refused. n 0: nothing is done, and the pointers may be NULL.
+ * vocab <= FT_SAMPLE_MAX_VOCAB, n <= FT_SAMPLE_MAX_ROWS, history_max <= 2^24. */
+#define FT_ADJUST_MAX_BIAS 1024
+int ft_hip_adjust_logits(ft_hip_ctx* ctx, void* stream, const void* logits, int logits_type, int64_t logits_stride,
+                         int64_t vocab, int64_t n, const int32_t* history, int64_t history_stride,
+                         int64_t history_max, const int32_t* history_len, const float* repetition,
+                         const float* presence, const float* frequency, const int32_t* bias_ids, const float* bias,
+                         int64_t n_bias, const uint32_t* mask, int64_t mask_stride, float* out, int64_t out_stride);
 
 /* Row layout conversion on the device (setup, not the hot path): the
  * reference repacks q4_0 banks to q4r at load (ft-model/src/lib.rs:570-609,
