@@ -42,6 +42,7 @@ namespace {
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float float2_ __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int STEP = 32;  // tokens of a step, two tiles
@@ -50,6 +51,8 @@ constexpr int MAX_SEQS = FT_ATTN_MAX_SEQS;
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.693147180559945309417f;
 
 enum { HALF, PACK, SPLIT };
+
+constexpr int BLOCKS = 512;  // workgroups at most, two on each CU
 
 // Where the parts of a call lie, in the workspace and else.
 struct AttnArgs {
@@ -67,12 +70,12 @@ struct AttnArgs {
     int prefix_pages, table_pages, n_pages, page_shift;
     int n_seqs, n_q, kv_heads, group, type;
     int row_tiles;   // tiles of a sequence's rows on a head
-    int pre_tiles;   // tiles of the batch's rows on a head
+    int pre_tiles, pre_nt;  // tiles of the batch's rows on a head, and of a wavefront's
     int window;
     float scale;     // times log2 e
     float pre_cost;  // of a prefix step, in own ones
     // workspace: a word of how many pieces the prefix is cut into, descriptors of the own items, pieces
-    int32_t* head;
+    int32_t* head;   // [0]: workgroups that the prefix is cut for
     int2* items;
     float* own;      // pieces of own rows: `piece` floats each
     float* pre;      // pieces of prefix rows: 16 rows each
@@ -83,6 +86,8 @@ struct AttnArgs {
 // Floats of a piece of `rows` rows: the rows' values, then their maxima and sums.
 __host__ __device__ __forceinline__ int64_t piece_floats(int rows, int D) { return (int64_t)rows * (D + 2); }
 
+// At the head of a branch that few waves take: keeps the compiler from doing its work always and choosing afterwards.
+__device__ __forceinline__ void rare() { asm volatile(""); }
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
@@ -122,6 +127,20 @@ __device__ __forceinline__ half8 widen8(uint32_t lo, uint32_t hi) {
     widen4<CT>(lo, a, b);
     widen4<CT>(hi, c, d);
     return half8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
+// Eight keys' dimensions. i8's byte q + 128 as it is makes a subnormal f16 of (q + 128) 2^-24, which the products take
+// exactly; what the 128 adds to a sum of products is the same for all keys, and the sum starts from less than 0 by it
+// (Attend::from). Values are not taken so: over many tokens their sum may be far smaller than the weights' times 128.
+template <int CT>
+__device__ __forceinline__ half8 widen_k(uint32_t lo, uint32_t hi) {
+    if constexpr (CT == FT_KV_I8) {
+        const u32x4 w = {__builtin_amdgcn_perm(0, lo, 0x0C010C00u), __builtin_amdgcn_perm(0, lo, 0x0C030C02u),
+                         __builtin_amdgcn_perm(0, hi, 0x0C010C00u), __builtin_amdgcn_perm(0, hi, 0x0C030C02u)};
+        return __builtin_bit_cast(half8, w);
+    } else {
+        return widen8<CT>(lo, hi);
+    }
 }
 
 __device__ __forceinline__ f32x4 mfma(half8 a, half8 b, f32x4 c) {
@@ -176,71 +195,110 @@ struct Column {
     bool live;         // there is such a row, and its query is no padding
 };
 
-// The pages of a run of tiles, 64 tiles at a time, a lane each; -1 for one that is not in the cache.
-struct Pages {
-    int first, now, next;  // first: the tile of lane 0
+// Where the tiles of a list of pages lie, 64 tiles at a time, a lane each.
+template <int D>
+struct Tiles64 {
+    int first, end;     // the tile of lane 0; the list's tiles end before this one
+    uint64_t in_cache;  // a bit for each lane whose tile is in the cache and before the end
+    int lo, hi;         // the lane's tile's address, a tile of page 0's in place of one that is not in the cache
+    int raw, raw_next;  // its page's number, and that of 64 tiles on
     const int32_t* ids;
     int n;
-    __device__ __forceinline__ int list(const AttnArgs& a, int from) const {
+    __device__ __forceinline__ int fetch(const AttnArgs& a, int from) const {
         const int at = (from + (int)(threadIdx.x & 63)) >> (a.page_shift - 4);
-        const int id = ids[at < n ? at : n - 1];
-        return (unsigned)id < (unsigned)a.n_pages ? id : -1;
+        return ids[at < n ? at : n - 1];
     }
-    __device__ __forceinline__ void open(const AttnArgs& a, const int32_t* pages, int count, int tile) {
-        ids = pages, n = count, first = tile;
-        now = list(a, tile), next = list(a, tile + 64);
+    // Has the pages' numbers fetched; settle() waits for them.
+    __device__ __forceinline__ void open(const AttnArgs& a, const int32_t* pages, int count, int tile, int end_) {
+        ids = pages, n = count, first = tile, end = end_;
+        raw = fetch(a, tile), raw_next = fetch(a, tile + 64);
+    }
+    __device__ __forceinline__ void settle(const AttnArgs& a, int head) {
+        const int tile = first + (threadIdx.x & 63), mask = (1 << (a.page_shift - 4)) - 1;
+        const bool good = (unsigned)raw < (unsigned)a.n_pages && tile < end;
+        const uint64_t at = reinterpret_cast<uint64_t>(a.cache) + (tile & mask) * (16 * D) +
+                            ((int64_t)(good ? raw : 0) * a.kv_heads + head) * kv_block_bytes((int64_t)1 << a.page_shift, D);
+        lo = (int)at, hi = (int)(at >> 32), in_cache = __ballot(good);
     }
     // To the tiles from `tile` on, which is an even number from the first.
-    __device__ __forceinline__ void reach(const AttnArgs& a, int tile) {
+    __device__ __forceinline__ void reach(const AttnArgs& a, int head, int tile) {
         if (tile - first < 64) return;
+        rare();
         first += 64;
-        now = next;
-        next = list(a, first + 64);
+        raw = raw_next;
+        raw_next = fetch(a, first + 64);
+        settle(a, head);
     }
-    __device__ __forceinline__ int page(int tile) const { return __builtin_amdgcn_readlane(now, tile - first); }
+    __device__ __forceinline__ const uint8_t* at(int tile) const {
+        const uint32_t l = __builtin_amdgcn_readlane(lo, tile - first), h = __builtin_amdgcn_readlane(hi, tile - first);
+        return reinterpret_cast<const uint8_t*>((uint64_t)h << 32 | l);
+    }
+    __device__ __forceinline__ bool has(int tile) const { return in_cache >> (tile - first) & 1; }
 };
+
+// From a tile's keys to its scales, or with D = 1 more than there is to its values' and theirs.
+__device__ __forceinline__ int64_t to_scales(const AttnArgs& a, int D, int tile) {
+    const int in = tile & ((1 << (a.page_shift - 4)) - 1);
+    return ((int64_t)(2 * D) << a.page_shift) - in * (16 * D - 64);
+}
 
 // Two tiles of a head's tokens, on their way.
 template <int ND>
 struct Step {
     static constexpr int D = 64 * ND;
+    static constexpr bool FAR = false;
+    static constexpr int BATCH = 2;  // operands that are taken at a time
     u32x4 k[2][ND], v[2][ND];
     f32x4 dk[2], dv[2];
 
-    // Where the tiles `tile` and `tile` + 1 of a list lie that ends before tile `end`.
+    // Where the tiles `tile` and `tile` + 1 of a list lie.
     struct Aim {
-        int page[2];
-        const uint8_t* block[2];
-        int in[2], lane16, lane64;
-        // some: there are such tiles; if not, what is loaded is of no use, and all lanes load the same
-        __device__ __forceinline__ void at(const AttnArgs& a, Pages& p, int head, int tile, int end, bool some) {
-            p.reach(a, tile);
-            const int mask = (1 << (a.page_shift - 4)) - 1, lane = threadIdx.x & 63;
-            page[0] = some ? p.page(tile) : -1, page[1] = some && tile + 1 < end ? p.page(tile + 1) : -1;
-            lane16 = some ? lane * 16 : 0, lane64 = some ? lane >> 4 << 4 : 0;
+        const uint8_t* at[2];
+        int64_t scales[2];
+        bool has[2];
+        int lane16, lane64;
+        __device__ __forceinline__ void to(const AttnArgs& a, Tiles64<D>& p, int head, int tile) {
+            p.reach(a, head, tile);
+            const int lane = threadIdx.x & 63;
+            lane16 = lane * 16, lane64 = lane >> 4 << 4;
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {  // instead of a page that is not there the first
-                block[x] = a.cache + ((int64_t)max(page[x], 0) * a.kv_heads + head) * kv_block_bytes((int64_t)1 << a.page_shift, D);
-                in[x] = (tile + x) & mask;
-            }
+            for (int x = 0; x < 2; ++x) at[x] = p.at(tile + x), has[x] = p.has(tile + x), scales[x] = to_scales(a, D, tile + x);
         }
+        // What is loaded next is of no use: all lanes load the same.
+        __device__ __forceinline__ void nowhere() { lane16 = lane64 = 0; }
     };
-    __device__ __forceinline__ void load_k(const AttnArgs& a, const Aim& m) {
+    // Operands of the products: keys 64 c + 16 g + 8 h on of tile x, values 64 c + 4 r + j of both tiles.
+    template <int CT>
+    __device__ __forceinline__ half8 key(int x, int c, int h) const { return widen_k<CT>(k[x][c][2 * h], k[x][c][2 * h + 1]); }
+    template <int CT>
+    __device__ __forceinline__ half8 value(int c, int j) const { return widen8<CT>(v[0][c][j], v[1][c][j]); }
+    __device__ __forceinline__ f32x4 key_scale(int x) const { return dk[x]; }
+    __device__ __forceinline__ f32x4 value_scale(int x) const { return dv[x]; }
+    // Tile x has tokens of the list in the bytes of `keep` alone: what the others hold may be codes and scales that are
+    // NaN, whose 0 fold is NaN.
+    __device__ __forceinline__ void clear(int x, uint32_t keep) {
+#pragma unroll
+        for (int c = 0; c < ND; ++c) v[x][c] &= keep;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (!(keep >> (8 * i) & 1)) dv[x][i] = 0.0f;
+    }
+
+    __device__ __forceinline__ void load_k(const Aim& m) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            const uint8_t* p = m.block[x] + m.in[x] * (16 * D);
 #pragma unroll
-            for (int c = 0; c < ND; ++c) k[x][c] = *reinterpret_cast<const u32x4*>(p + c * 1024 + m.lane16);
-            dk[x] = *reinterpret_cast<const f32x4*>(m.block[x] + ((int64_t)(2 * D) << a.page_shift) + m.in[x] * 64 + m.lane64);
+            for (int c = 0; c < ND; ++c) k[x][c] = *reinterpret_cast<const u32x4*>(m.at[x] + c * 1024 + m.lane16);
+            dk[x] = *reinterpret_cast<const f32x4*>(m.at[x] + m.scales[x] + m.lane64);
         }
     }
     __device__ __forceinline__ void load_v(const AttnArgs& a, const Aim& m) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            const uint8_t* p = m.block[x] + ((int64_t)D << a.page_shift) + m.in[x] * (16 * D);
+            const uint8_t* p = m.at[x] + ((int64_t)D << a.page_shift);
 #pragma unroll
             for (int c = 0; c < ND; ++c) v[x][c] = *reinterpret_cast<const u32x4*>(p + c * 1024 + m.lane16);
-            dv[x] = *reinterpret_cast<const f32x4*>(m.block[x] + ((int64_t)(2 * D + 4) << a.page_shift) + m.in[x] * 64 + m.lane64);
+            dv[x] = *reinterpret_cast<const f32x4*>(m.at[x] + m.scales[x] + (4 << a.page_shift) + m.lane64);
         }
     }
 };
@@ -253,106 +311,149 @@ struct Attend {
     static constexpr bool F32 = MODE != HALF;
     half8 q[NT][PARTS][2 * ND];
     f32x4 acc[NT][4 * ND];
-    float m[NT], base[NT], l[NT], fac[NT];
-    float unit, inv_unit;  // the weights' unit: the values' largest scale so far as a power of two, over 2^8
-    int lo[NT], hi[NT];    // tokens that the column sees
-    int all_lo, all_hi;    // that every column sees
-    int tokens;            // that the list of pages holds
+    float base[NT], l[NT];  // the maximum that weights are taken against, and their sum
+    float limit[NT];        // over the base: scores above it raise the base; -FLT_MAX while there is none
+    float from[NT];         // what a column's sums of products start from
+    float fac;              // of the products
+    float unit, inv_unit;   // the weights' unit: the values' largest scale so far as a power of two, over 2^8
+    int lo[NT], hi[NT];     // tokens that the column sees
+    int all_lo, all_hi;     // that every column sees
+    int tokens;             // that the list of pages holds
 
-    __device__ __forceinline__ void load(const AttnArgs& a, int n, const Column& c) {
+    // The columns' queries times scale, in units of a power of two that the largest of them all gives.
+    __device__ __forceinline__ void load(const AttnArgs& a, const Column (&c)[NT]) {
         const int g = (threadIdx.x & 63) >> 4;
         float x[2 * ND][8], top = 0.0f;
-        const int64_t at = ((int64_t)c.seq * a.n_q + c.t) * a.q_stride + (int64_t)c.head * D + 16 * g;
+        const auto fetch = [&](int n) {
+            const int64_t at = ((int64_t)c[n].seq * a.n_q + c[n].t) * a.q_stride + (int64_t)c[n].head * D + 16 * g;
 #pragma unroll
-        for (int i = 0; i < 2 * ND; ++i) load_q8<F32>(a.q, at + (i >> 1) * 64 + (i & 1) * 8, a.type == FT_TYPE_F16, x[i]);
+            for (int i = 0; i < 2 * ND; ++i) load_q8<F32>(a.q, at + (i >> 1) * 64 + (i & 1) * 8, a.type == FT_TYPE_F16, x[i]);
+        };
 #pragma unroll
-        for (int i = 0; i < 2 * ND; ++i)
+        for (int n = 0; n < NT; ++n) {
+            fetch(n);
+            float most = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[i][e]));
-        top = max_groups(top);
-        const int e2 = max(__float_as_int(top) >> 23, 10);
-        const float up = __int_as_float((263 - e2) << 23);  // the row's largest comes to lie in [2^9, 2^10)
-        fac[n] = a.scale * __int_as_float((e2 - 9) << 23);
-        const float second = MODE == PACK && (threadIdx.x & 8) ? 1.0f : 0.0f;
+            for (int i = 0; i < 2 * ND; ++i)
 #pragma unroll
-        for (int i = 0; i < 2 * ND; ++i)
+                for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[i][e]));
+            if (c[n].live) top = fmaxf(top, most);
+        }
+        top = wave_max(top);
+        const int e2 = clampi(__float_as_int(top) >> 23, 14, 254);
+        const float up = __int_as_float((267 - e2) << 23);  // the largest comes to lie in [2^13, 2^14)
+        fac = a.scale * __int_as_float((e2 - 13) << 23) * (CT == FT_KV_I8 ? 0x1p24f : 1.0f);
+        const float second = MODE == PACK && (threadIdx.x & 8) ? -1.0f : 0.0f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float v = x[i][e] * up;
-                const _Float16 h = (_Float16)v;
-                if constexpr (MODE == SPLIT) q[n][PARTS - 1][i][e] = (_Float16)(v - (float)h);
-                q[n][0][i][e] = MODE == PACK ? (_Float16)(v - second * (float)h) : h;
+        for (int n = 0; n < NT; ++n) {
+            if constexpr (NT > 1) {  // again, from the cache: all columns' at once would not fit the registers
+                asm volatile("" ::: "memory");
+                fetch(n);
             }
 #pragma unroll
-        for (int i = 0; i < 4 * ND; ++i) acc[n][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        m[n] = -INFINITY, base[n] = 0.0f, l[n] = 0.0f, unit = 0x1p-100f, inv_unit = 0x1p100f;
+            for (int i = 0; i < 2 * ND; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const float2_ v = {x[i][e] * up, x[i][e + 1] * up};
+                    const half2 h = __builtin_convertvector(v, half2);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        q[n][0][i][e + u] = MODE == PACK ? (_Float16)fmaf(second, (float)h[u], v[u]) : h[u];
+                        if constexpr (MODE == SPLIT) q[n][PARTS - 1][i][e + u] = (_Float16)fmaf(-1.0f, (float)h[u], v[u]);
+                    }
+                }
+            // keys come as (q + 128) 2^-24 (widen_k): what the 128 is worth, by products with it
+            f32x4 worth = {0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (CT == FT_KV_I8) {
+                const u32x4 k = {0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};  // f16 of -128 2^-24
+                const half8 minus = __builtin_bit_cast(half8, k);
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+                    for (int i = 0; i < 2 * ND; ++i) worth = mfma(minus, q[n][p][i], worth);
+            }
+            from[n] = worth[0];
+#pragma unroll
+            for (int i = 0; i < 4 * ND; ++i) acc[n][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            base[n] = 0.0f, l[n] = 0.0f, limit[n] = -FLT_MAX;
+        }
+        unit = 0x1p-100f, inv_unit = 0x1p100f;
     }
 
-    // The columns' scores of a step; the keys and their scales are free afterwards.
-    __device__ __forceinline__ void scores(const Step<ND>& t, f32x4 (&s)[NT][2]) const {
+    // The columns' scores of a step less their bases; the keys and their scales are free afterwards.
+    template <class Tiles>
+    __device__ __forceinline__ void scores(const Tiles& t, f32x4 (&s)[NT][2]) const {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = f32x4{from[n], from[n], from[n], from[n]};
 #pragma unroll
-        for (int c = 0; c < ND; ++c)
+        for (int i = 0; i < 4 * ND; i += Tiles::BATCH) {
+            constexpr int BATCH = Tiles::BATCH;
+            half8 k[BATCH];
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int u = 0; u < BATCH; ++u) k[u] = t.template key<CT>(i + u & 1, (i + u) >> 2, (i + u) >> 1 & 1);
+            if constexpr (Tiles::FAR) __builtin_amdgcn_sched_barrier(0);  // read together, not each where it is used
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const half8 k = widen8<CT>(t.k[x][c][2 * h], t.k[x][c][2 * h + 1]);
+            for (int u = 0; u < BATCH; ++u)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int p = 0; p < PARTS; ++p) s[n][x] = mfma(k, q[n][p][2 * c + h], s[n][x]);
-                }
+                    for (int p = 0; p < PARTS; ++p)
+                        s[n][i + u & 1] = mfma(k[u], q[n][p][(i + u) >> 1], s[n][i + u & 1]);
+        }
+        const f32x4 d[2] = {t.key_scale(0) * fac, t.key_scale(1) * fac};
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                if constexpr (MODE == PACK) {
+            for (int x = 0; x < 2; ++x)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s[n][x][i] += other8(s[n][x][i]);
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (MODE == PACK) s[n][x][i] += other8(s[n][x][i]);
+                    s[n][x][i] = fmaf(s[n][x][i], d[x][i], -base[n]);
                 }
-                s[n][x] *= t.dk[x] * fac[n];
-            }
     }
 
     // Weights of a step at token `at` from its scores, and their sums with the values.
-    __device__ __forceinline__ void weigh(Step<ND>& t, f32x4 (&s)[NT][2], const int (&page)[2], int at) {
+    template <class Tiles>
+    __device__ __forceinline__ void weigh(Tiles& t, f32x4 (&s)[NT][2], const bool (&has)[2], int at) {
         const int lane = threadIdx.x & 63, g = lane >> 4;
-        const bool whole = page[0] >= 0 && page[1] >= 0 && at >= all_lo && at + STEP <= all_hi;
-        half8 w[NT][PARTS];
-        float top[NT];
-        f32x4 dv[2] = {t.dv[0], t.dv[1]};
-        bool grows = false;
+        const bool whole = has[0] && has[1] && at >= all_lo && at + STEP <= all_hi;
+        constexpr int BATCH = Tiles::BATCH;
+        half8 w[NT][PARTS], v[BATCH];
+        if constexpr (Tiles::FAR) {  // the first values are on their way while the weights are made
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u) v[u] = t.template value<CT>(u >> 2, u & 3);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         if (!whole) {
+            rare();
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 uint32_t keep = 0;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int j = at + 16 * x + 4 * g + i;
-                    // tokens that the list does not hold may have codes and scales that are NaN, whose 0 fold is NaN
-                    const bool in = page[x] >= 0 && j < tokens;
+                    const bool in = has[x] && j < tokens;
                     if (in) keep |= 255u << (8 * i);
-                    if (!in) dv[x][i] = 0.0f;
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
                         if (!in || j < lo[n] || j >= hi[n]) s[n][x][i] = -INFINITY;
                 }
-#pragma unroll
-                for (int c = 0; c < ND; ++c) t.v[x][c] &= keep;
+                t.clear(x, keep);
             }
         }
+        f32x4 dv[2] = {t.value_scale(0), t.value_scale(1)};
+        // a lane's own scores say enough: the base is raised where any of them is far above it
+        float top[NT];
+        bool grows = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             top[n] = fmaxf(fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][0][2], s[n][0][3])),
                            fmaxf(fmaxf(s[n][1][0], s[n][1][1]), fmaxf(s[n][1][2], s[n][1][3])));
-            top[n] = max_groups(top[n]);
-            grows |= top[n] > m[n] + 6.0f;
+            grows |= top[n] > limit[n];
         }
         const float vt = fmaxf(fmaxf(fmaxf(dv[0][0], dv[0][1]), fmaxf(dv[0][2], dv[0][3])),
                                fmaxf(fmaxf(dv[1][0], dv[1][1]), fmaxf(dv[1][2], dv[1][3])));
-        if (__any(grows || vt > unit * 256.0f)) rescale(top, vt);
+        if (__any(grows || vt > unit * 256.0f)) rescale(s, top, vt);
 #pragma unroll
         for (int x = 0; x < 2; ++x) dv[x] *= inv_unit;
 #pragma unroll
@@ -361,31 +462,53 @@ struct Attend {
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float p = __builtin_amdgcn_exp2f(s[n][x][i] - base[n]);
-                    l[n] += p;
-                    float v = p * dv[x][i];
-                    // a scale that is NaN, of a token that the column does not see
-                    if (!whole && s[n][x][i] == -INFINITY) v = 0.0f;
-                    const _Float16 h = (_Float16)v;
-                    w[n][0][4 * x + i] = MODE == PACK ? (_Float16)(v - second * (float)h) : h;
-                    if constexpr (MODE == SPLIT) w[n][PARTS - 1][4 * x + i] = (_Float16)(v - (float)h);
+                for (int i = 0; i < 4; i += 2) {
+                    float2_ v;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float p = __builtin_amdgcn_exp2f(s[n][x][i + e]);
+                        l[n] += p;
+                        v[e] = p * dv[x][i + e];
+                    }
+                    const half2 h = __builtin_convertvector(v, half2);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        w[n][0][4 * x + i + e] = MODE == PACK ? (_Float16)fmaf(-second, (float)h[e], v[e]) : h[e];
+                        if constexpr (MODE == SPLIT) w[n][PARTS - 1][4 * x + i + e] = (_Float16)(v[e] - (float)h[e]);
+                    }
                 }
         }
+        if (!whole) {  // 0 times a scale that is NaN, of a token that the column does not see
+            rare();
 #pragma unroll
-        for (int c = 0; c < ND; ++c)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const half8 v = widen8<CT>(t.v[0][c][j], t.v[1][c][j]);
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (s[n][x][i] == -INFINITY) {
+#pragma unroll
+                            for (int p = 0; p < PARTS; ++p) w[n][p][4 * x + i] = (_Float16)0.0f;
+                        }
+        }
+#pragma unroll
+        for (int i = 0; i < 4 * ND; i += BATCH) {
+            if (!Tiles::FAR || i > 0) {
+#pragma unroll
+                for (int u = 0; u < BATCH; ++u) v[u] = t.template value<CT>((i + u) >> 2, (i + u) & 3);
+            }
+            if constexpr (Tiles::FAR) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u)
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int p = 0; p < PARTS; ++p) acc[n][4 * c + j] = mfma(v, w[n][p], acc[n][4 * c + j]);
-            }
+                    for (int p = 0; p < PARTS; ++p) acc[n][i + u] = mfma(v[u], w[n][p], acc[n][i + u]);
+        }
     }
 
     // A larger maximum, or a larger scale of values.
-    __device__ __forceinline__ void rescale(const float (&top)[NT], float vt) {
+    __device__ __forceinline__ void rescale(f32x4 (&s)[NT][2], float (&top)[NT], float vt) {
         float g = 1.0f;
         const float most = wave_max(vt);
         if (most > unit * 256.0f) {
@@ -398,16 +521,21 @@ struct Attend {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             float f = g;
-            if (top[n] > m[n]) {
-                const float d = __builtin_amdgcn_exp2f(m[n] - top[n]);
-                f *= d;
-                l[n] *= d;
-                m[n] = base[n] = top[n];
+            const float up = max_groups(top[n]);
+            if (up > fminf(limit[n], 0.0f)) {
+                const float d = __builtin_amdgcn_exp2f(-up);
+                if (limit[n] > 0.0f) f *= d, l[n] *= d;  // else there is nothing yet
+                limit[n] = 6.0f;
+                base[n] += up;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[n][0][i] -= up, s[n][1][i] -= up;
             }
 #pragma unroll
             for (int i = 0; i < 4 * ND; ++i) acc[n][i] *= f;
         }
     }
+    // The maximum that a column's sums are taken against.
+    __device__ __forceinline__ float top_of(int n) const { return limit[n] > 0.0f ? base[n] : -INFINITY; }
 
     // Sums over the lanes that share a column.
     __device__ __forceinline__ void finish(int n, bool live) {
@@ -432,7 +560,7 @@ struct Attend {
             for (int i = 0; i < 4; ++i)
                 *reinterpret_cast<f32x4*>(piece + (int64_t)col * D + 64 * c + 16 * g + 4 * i) = values(n, c, i, unit);
         if (g == 0) {
-            piece[(int64_t)rows * D + col] = m[n];
+            piece[(int64_t)rows * D + col] = top_of(n);
             piece[(int64_t)rows * D + rows + col] = l[n];
         }
     }
@@ -448,7 +576,7 @@ struct Attend {
                 store_out<F32>(a.out, row * a.out_stride + (int64_t)c.head * D + 64 * i + 16 * g + 4 * e, a.type == FT_TYPE_F16,
                                some ? values(n, i, e, f) : f32x4{0.0f, 0.0f, 0.0f, 0.0f});
         if (a.lse && g == 0)
-            a.lse[row * a.kv_heads * a.group + c.head] = some ? (m[n] + __builtin_amdgcn_logf(l[n])) * LN2 : -INFINITY;
+            a.lse[row * a.kv_heads * a.group + c.head] = some ? (top_of(n) + __builtin_amdgcn_logf(l[n])) * LN2 : -INFINITY;
     }
 };
 
@@ -495,8 +623,8 @@ struct Cuts {
 };
 
 // What the start and the end of an item cost a wavefront, in steps: each item counts as so many steps more, which come
-// first.
-constexpr int start_of(int nd) { return 4 / nd; }
+// first. 64 sequences of up to 4096 tokens 87 us, with 1 89 to 93, with 8 91; 256 of up to 300 28.5, 32 and 29.5.
+constexpr int START = 2;
 
 constexpr int MIN_STEPS = 2;  // of a wavefront's own steps, where there are more than FEW_STEPS in all
 constexpr int FEW_STEPS = 1024;
@@ -528,20 +656,92 @@ __device__ __forceinline__ int least_of_wave(int v) {
 }
 
 // Tiles of 16 rows that a wavefront takes of the prefix, as many as its registers hold.
-constexpr int pre_columns(int nd, bool f32) { return f32 ? (nd <= 2 ? 2 : 1) : 4 / nd; }
+constexpr int pre_columns(int nd, bool f32) { return nd == 4 ? 1 : nd == 2 ? 2 : f32 ? 2 : 4; }
 
-// Prefix rows: a wavefront takes a piece of the prefix for NT tiles of 16 rows.
+// Two tiles of the prefix in LDS, as the products take them.
+template <int ND>
+struct Wide {
+    static constexpr bool FAR = true;  // LDS: a batch of operands is read before the first is used
+    static constexpr int BATCH = ND == 1 ? 4 : 8;
+    half8 k[2][ND][2][64], v[ND][4][64];
+    f32x4 dk[2][4], dv[2][4];
+    int has[2];
+    template <int CT>
+    __device__ __forceinline__ half8 key(int x, int c, int h) const { return k[x][c][h][threadIdx.x & 63]; }
+    template <int CT>
+    __device__ __forceinline__ half8 value(int c, int j) const { return v[c][j][threadIdx.x & 63]; }
+    __device__ __forceinline__ f32x4 key_scale(int x) const { return dk[x][(threadIdx.x & 63) >> 4]; }
+    __device__ __forceinline__ f32x4 value_scale(int x) const { return dv[x][(threadIdx.x & 63) >> 4]; }
+    __device__ __forceinline__ void clear(int, uint32_t) const {}  // done where they were widened
+};
+
+// A wavefront's share of two tiles on their way: the keys (waves 0 and 1) or values (2 and 3) of one of them.
+template <int CT, int ND>
+struct Share {
+    static constexpr int D = 64 * ND;
+    u32x4 raw[ND];
+    float scale;
+    int tile;
+    bool has;
+    __device__ __forceinline__ void load(const AttnArgs& a, Tiles64<D>& p, int head, int at, bool some) {
+        const int wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63;
+        p.reach(a, head, at);
+        tile = at + (wave & 1);
+        has = some && p.has(tile);
+        const uint8_t* keys = p.at(tile);
+        const uint8_t* from = keys + ((int64_t)(wave >> 1) * D << a.page_shift) + (some ? lane * 16 : 0);
+#pragma unroll
+        for (int c = 0; c < ND; ++c) raw[c] = *reinterpret_cast<const u32x4*>(from + c * 1024);
+        scale = *reinterpret_cast<const float*>(keys + to_scales(a, D, tile) + ((wave >> 1) * 4 << a.page_shift) + (lane & 15) * 4);
+    }
+    __device__ __forceinline__ void widen(Wide<ND>& to, int tokens) {
+        const int wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63, x = wave & 1;
+        if (wave < 2) {
+#pragma unroll
+            for (int c = 0; c < ND; ++c)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) to.k[x][c][h][lane] = widen_k<CT>(raw[c][2 * h], raw[c][2 * h + 1]);
+            if (lane < 16) reinterpret_cast<float*>(to.dk[x])[lane] = scale;
+            if (lane == 0) to.has[x] = has;
+            return;
+        }
+        if (!has || tile * 16 + 16 > tokens) {  // Step::clear
+            rare();
+            uint32_t keep = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (has && tile * 16 + (lane >> 4) * 4 + i < tokens) keep |= 255u << (8 * i);
+#pragma unroll
+            for (int c = 0; c < ND; ++c) raw[c] &= keep;
+            if (!has || tile * 16 + (lane & 15) >= tokens) scale = 0.0f;
+        }
+#pragma unroll
+        for (int c = 0; c < ND; ++c)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                half2 w[2];
+                widen4<CT>(raw[c][j], w[0], w[1]);
+                reinterpret_cast<uint2*>(&to.v[c][j][lane])[x] = make_uint2(__builtin_bit_cast(uint32_t, w[0]), __builtin_bit_cast(uint32_t, w[1]));
+            }
+        if (lane < 16) reinterpret_cast<float*>(to.dv[x])[lane] = scale;
+    }
+};
+
+// Prefix rows: the lines of WAVES NT tiles of 16 rows on a head, one after the other, are cut into a piece for each
+// workgroup. Its wavefronts share the widening: each step's tiles lie in LDS while the next one's are widened beside them.
 template <int CT, int ND, int MODE, int NT>
-__device__ __forceinline__ void attend_prefix(const AttnArgs& a, const Prefix& pre, int cuts, int x0, int stride) {
-    const int lane = threadIdx.x & 63, col = lane & 15;
-    const int groups = (a.pre_tiles + NT - 1) / NT;
-    for (int x = x0; x < cuts * a.kv_heads * groups; x += stride) {
-        const int tile = uni(x % groups) * NT, seg = x / groups;
-        const int head = uni(seg / cuts), cut = uni(seg % cuts);
-        const Cuts by((unsigned)pre.steps, (unsigned)cuts);
-        int s0 = (int)by.begin(cut), s1 = (int)by.begin(cut + 1);
-        Pages pages;
-        pages.open(a, a.prefix, a.prefix_pages, pre.tile0 + 2 * s0);
+__device__ __forceinline__ void attend_prefix(const AttnArgs& a, const Prefix& pre, int b, int blocks, Wide<ND>* wide, int* part) {
+    const int lane = threadIdx.x & 63, col = lane & 15, wave = uni(threadIdx.x >> 6);
+    const int groups = (a.pre_tiles + NT * WAVES - 1) / (NT * WAVES);
+    const Cuts by((unsigned)pre.steps * (unsigned)(a.kv_heads * groups), (unsigned)blocks);
+    unsigned pos = by.begin(b);
+    const unsigned stop = by.begin(b + 1);
+    while (pos < stop) {
+        const int line = uni((int)(pos / (unsigned)pre.steps)), head = line / groups, tile = (line % groups * WAVES + wave) * NT;
+        int s0 = (int)pos - line * pre.steps, s1 = min(pre.steps, s0 + (int)(stop - pos));
+        pos += s1 - s0;
+        Tiles64<64 * ND> tiles;
+        tiles.open(a, a.prefix, a.prefix_pages, pre.tile0 + 2 * s0, (pre.len + 15) / 16);
         Attend<CT, ND, MODE, NT> w;
         Column c[NT];
         int least = pre.len, most_lo = 0;
@@ -557,43 +757,55 @@ __device__ __forceinline__ void attend_prefix(const AttnArgs& a, const Prefix& p
             w.lo[n] = c[n].live ? lo : INT32_MIN, w.hi[n] = pre.len;  // one without a query sees all, to no effect
             if (c[n].live) least = min(least, lo), most_lo = max(most_lo, lo);
         }
-        w.tokens = w.all_hi = pre.len, w.all_lo = -least_of_wave(-most_lo);
-        // the steps before the first column's first token are nobody's
-        const int skip = (least_of_wave(least) / 16 - pre.tile0) / 2;
-        if (skip > s0) s0 = min(skip, s1), pages.open(a, a.prefix, a.prefix_pages, pre.tile0 + 2 * s0);
-        Step<ND> t;
-        typename Step<ND>::Aim aim;
-        const int end = (pre.len + 15) / 16;
-        int at = pre.tile0 + 2 * s0;
-        aim.at(a, pages, head, at, end, s0 < s1);
-        t.load_k(a, aim);
-        t.load_v(a, aim);
+        w.tokens = w.all_hi = pre.len, w.all_lo = a.window ? -least_of_wave(-most_lo) : 0;
+        if (a.window) {  // the steps before the first column's first token are nobody's
+            least = least_of_wave(least);
+            __syncthreads();
+            if (lane == 0) part[wave] = least;
+            __syncthreads();
 #pragma unroll
-        for (int n = 0; n < NT; ++n) w.load(a, n, c[n]);
+            for (int v = 0; v < WAVES; ++v) least = min(least, part[v]);
+            const int skip = uni(clampi((least / 16 - pre.tile0) / 2, s0, s1));
+            if (skip > s0) s0 = skip, tiles.open(a, a.prefix, a.prefix_pages, pre.tile0 + 2 * s0, (pre.len + 15) / 16);
+        }
+        const int first = pre.tile0 + 2 * s0;
+        tiles.settle(a, head);
+        Share<CT, ND> share;
+        share.load(a, tiles, head, first, s0 < s1);
+        w.load(a, c);
+        __syncthreads();  // the last piece's tiles are done with
+        share.widen(wide[0], pre.len);
+        share.load(a, tiles, head, first + 2, s0 + 1 < s1);
+        const bool mine = tile < a.pre_tiles;
         for (int s = s0; s < s1; ++s) {
-            f32x4 sc[NT][2];
-            const int page[2] = {aim.page[0], aim.page[1]};
-            aim.at(a, pages, head, at + 2, end, s + 1 < s1);
-            w.scores(t, sc);
-            t.load_k(a, aim);
-            w.weigh(t, sc, page, at * 16);
-            t.load_v(a, aim);
-            at += 2;
+            const int at = pre.tile0 + 2 * s, now = (s - s0) & 1;
+            __syncthreads();
+            share.widen(wide[now ^ 1], pre.len);
+            share.load(a, tiles, head, at + 4, s + 2 < s1);
+            if (mine) {
+                const bool has[2] = {uni(wide[now].has[0]) != 0, uni(wide[now].has[1]) != 0};
+                f32x4 sc[NT][2];
+                w.scores(wide[now], sc);
+                w.weigh(wide[now], sc, has, at * 16);
+            }
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
+            if (tile + n >= a.pre_tiles) continue;
             w.finish(n, c[n].live);
-            if (tile + n < a.pre_tiles)
-                w.to_piece(n, a.pre + ((int64_t)seg * a.pre_tiles + tile + n) * piece_floats(16, 64 * ND), 16, col);
+            w.to_piece(n, a.pre + ((int64_t)(b + line) * (WAVES * NT) + wave * NT + n) * piece_floats(16, 64 * ND), 16, col);
         }
     }
 }
 
 template <int CT, int ND, int MODE, bool PRE>
 __global__ __launch_bounds__(THREADS, 2) void k_attn(AttnArgs a) {
-    constexpr int COLS = MODE == PACK ? 8 : 16, START = start_of(ND);
-    __shared__ int cum[MAX_SEQS + 1], lens[MAX_SEQS];
+    constexpr int COLS = MODE == PACK ? 8 : 16;
+    // the prefix's tiles lie where the lengths were
+    constexpr int LENS = (2 * MAX_SEQS + 1) * 4, POOL = PRE && (int)sizeof(Wide<ND>[2]) > LENS ? (int)sizeof(Wide<ND>[2]) : LENS;
+    __shared__ __attribute__((aligned(16))) char pool[POOL];
     __shared__ int part[WAVES];
+    int *const cum = reinterpret_cast<int*>(pool), *const lens = cum + MAX_SEQS + 1;
     const int t = threadIdx.x, lane = t & 63, col = lane & 15;
     // the steps before each sequence
     int before = 0;
@@ -609,22 +821,24 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn(AttnArgs a) {
     __syncthreads();
     const unsigned lines = a.kv_heads * a.row_tiles;  // items of a sequence
     const unsigned T = before * lines;
-    int n_own = (a.own_waves + WAVES - 1) / WAVES, cuts = 0;
+    int n_own = (a.own_waves + WAVES - 1) / WAVES;
+    bool alone = true;  // the own tokens are all that is seen
     if constexpr (PRE) {
         constexpr int NT = pre_columns(ND, MODE != HALF);
         const Prefix pre = prefix_of(a);
         if (pre.steps > 0) {
-            // the workgroups are dealt by the steps; a prefix step is worth PRE_COST own ones
-            const unsigned groups = a.kv_heads * ((a.pre_tiles + NT - 1) / NT);
+            alone = false;
+            // the workgroups are dealt by the steps; a prefix step is worth pre_cost own ones
+            const int blocks = gridDim.x, groups = a.kv_heads * ((a.pre_tiles + NT * WAVES - 1) / (NT * WAVES));
             const float work = (float)pre.steps * (float)groups * a.pre_cost, all = work + (float)T;
-            const int blocks = gridDim.x;
             n_own = min(n_own, clampi((int)((float)T / all * (float)blocks + 0.5f), 1, blocks - 1));
-            const int n_pre = blocks - n_own;
-            cuts = clampi((int)((unsigned)n_pre * WAVES / groups), 1, (pre.steps + MIN_STEPS - 1) / MIN_STEPS);
+            const int n_pre = min(blocks - n_own, (pre.steps + 1) / 2 * groups);
             if ((int)blockIdx.x >= n_own) {
-                if ((int)blockIdx.x == n_own && t == 0) a.head[0] = cuts;
-                const int b = near_block(blockIdx.x - n_own, n_pre);
-                attend_prefix<CT, ND, MODE == PACK ? SPLIT : MODE, NT>(a, pre, cuts, uni(b * WAVES + (t >> 6)), n_pre * WAVES);
+                const int b = near_block(blockIdx.x - n_own, blocks - n_own);
+                if (b == 0 && t == 0) a.head[0] = n_pre;
+                __syncthreads();
+                if (b < n_pre)
+                    attend_prefix<CT, ND, MODE == PACK ? SPLIT : MODE, NT>(a, pre, b, n_pre, reinterpret_cast<Wide<ND>*>(pool), part);
                 return;
             }
         } else if (blockIdx.x == 0 && t == 0) {
@@ -657,31 +871,32 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn(AttnArgs a) {
     if (pos >= end) return;
     s0 = max(s0, 0);
     Own o = own_of(a, uni(lens[seq]));
-    Pages pages;
-    pages.open(a, a.tables + seq * a.table_stride, a.table_pages, o.tile0 + 2 * s0);
+    Tiles64<64 * ND> tiles;
+    tiles.open(a, a.tables + seq * a.table_stride, a.table_pages, o.tile0 + 2 * s0, (o.len + 15) / 16);
+    tiles.settle(a, line % a.kv_heads);
     Step<ND> st;
     typename Step<ND>::Aim aim;
-    aim.at(a, pages, line % a.kv_heads, o.tile0 + 2 * s0, (o.len + 15) / 16, o.len > 0);
-    st.load_k(a, aim);
+    aim.to(a, tiles, line % a.kv_heads, o.tile0 + 2 * s0);
+    st.load_k(aim);
     st.load_v(a, aim);
     bool first = true;
     while (true) {
         const int head = line % a.kv_heads, tile = line / a.kv_heads;
-        const int s1 = min(o.steps, s0 + (int)(end - pos)), last = (o.len + 15) / 16;
+        const int s1 = min(o.steps, s0 + (int)(end - pos));
         // the item behind this one: its pages are on their way while this one is worked on
         const unsigned then = pos + (s1 - s0) + START;
         const bool follows = then < end;
         int seq2 = seq, line2 = line + 1;
         Own o2 = o;
-        Pages pages2 = pages;
+        Tiles64<64 * ND> tiles2 = tiles;
         if (follows) {
             if (line2 == (int)lines) {
                 seq2 = seq + 1, line2 = 0;
                 o2 = own_of(a, uni(lens[seq2]));
             }
-            pages2.open(a, a.tables + seq2 * a.table_stride, a.table_pages, o2.tile0);
+            tiles2.open(a, a.tables + seq2 * a.table_stride, a.table_pages, o2.tile0, (o2.len + 15) / 16);
         }
-        Column c;
+        Column cs[1], &c = cs[0];
         const int mine = MODE == PACK ? col & 7 : col;
         const int rows = a.n_q * a.group, r = tile * COLS + mine;
         const bool row = r < rows;
@@ -689,7 +904,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn(AttnArgs a) {
         const int place = o.len - a.n_q + c.t;
         c.live = row && place >= 0;
         Attend<CT, ND, MODE, 1> w;
-        w.load(a, 0, c);
+        w.load(a, cs);
         w.lo[0] = c.live && a.window ? max(0, place - a.window + 1) : 0;
         w.hi[0] = c.live ? place + 1 : o.len;  // one without a query sees all, to no effect
         w.tokens = o.len;
@@ -700,17 +915,20 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn(AttnArgs a) {
         }
         int at = o.tile0 + 2 * s0;
         for (int s = s0; s < s1; ++s) {
-            const int page[2] = {aim.page[0], aim.page[1]};
+            const bool has[2] = {aim.has[0], aim.has[1]};
             if (s + 1 < s1) {
-                aim.at(a, pages, head, at + 2, last, true);
+                aim.to(a, tiles, head, at + 2);
+            } else if (follows) {
+                tiles = tiles2;
+                tiles.settle(a, line2 % a.kv_heads);
+                aim.to(a, tiles, line2 % a.kv_heads, o2.tile0);
             } else {
-                pages = pages2;
-                aim.at(a, pages, line2 % a.kv_heads, follows ? o2.tile0 : pages.first, (o2.len + 15) / 16, follows && o2.len > 0);
+                aim.nowhere();
             }
             f32x4 sc[1][2];
-            w.scores(st, sc);
-            st.load_k(a, aim);
-            if (o.len > 0) w.weigh(st, sc, page, at * 16);
+            if (o.len > 0) w.scores(st, sc);
+            st.load_k(aim);
+            if (o.len > 0) w.weigh(st, sc, has, at * 16);
             st.load_v(a, aim);
             at += 2;
         }
@@ -718,7 +936,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn(AttnArgs a) {
         const unsigned item_at = cum[seq] * lines + line * (o.steps + START) + START;
         const int fw = (int)by.of(item_at), lw = (int)by.of(item_at + o.steps - 1);
         const int64_t id = (int64_t)seq * lines + line;
-        const bool direct = fw == lw && cuts == 0;
+        const bool direct = fw == lw && alone;
         // a piece is its wave's first (slot 2 w) or its last (2 w + 1); of a whole item with a prefix, the item's
         const int64_t slot = fw == lw ? 2 * (int64_t)a.own_waves + id : first ? 2 * (int64_t)me : 2 * (int64_t)me + 1;
         if (s0 == 0 && lane == 0)
@@ -752,7 +970,7 @@ __global__ __launch_bounds__(ALL ? 1024 : 256) void k_attn_merge(AttnArgs a, int
     const int64_t id = blockIdx.x;
     const int y = ALL ? blockIdx.y : blockIdx.y * MERGE_WAVES + wave;  // the row in its tile
     const int2 it = a.items[id];
-    const int cuts = a.prefix ? a.head[0] : 0;
+    const int n_pre = a.prefix ? a.head[0] : 0;
     const int own = it.y >> 16, fw = it.y & 0xFFFF;
     if (own == 0) return;  // written where it was made
     const int seq = (int)(id / lines), item = (int)(id % lines);
@@ -761,10 +979,21 @@ __global__ __launch_bounds__(ALL ? 1024 : 256) void k_attn_merge(AttnArgs a, int
     if (y >= a.rows || r >= a.n_q * a.group) return;
     const int all = (seq * a.n_q + r / a.group) * a.group + r % a.group;  // the row among the batch's
     const int64_t own_floats = piece_floats(a.rows, D), pre_floats = piece_floats(16, D);
-    const int n = own + cuts;
+    // the prefix's pieces of the row's line
+    int n = own;
+    const float* pre = nullptr;
+    const int width = WAVES * a.pre_nt;  // tiles of a line
+    if (n_pre > 0) {
+        const Prefix p = prefix_of(a);
+        const int groups = (a.pre_tiles + width - 1) / width, line = head * groups + (all >> 4) / width;
+        const Cuts by((unsigned)p.steps * (unsigned)(a.kv_heads * groups), (unsigned)n_pre);
+        const int first = (int)by.of((unsigned)line * p.steps);
+        n += (int)by.of((unsigned)line * p.steps + p.steps - 1) - first + 1;
+        pre = a.pre + ((int64_t)(first + line) * width + (all >> 4) % width) * pre_floats;
+    }
     const auto piece = [&](int i) {
         return i < own ? a.own + (i == 0 ? (int64_t)it.x : 2 * (int64_t)(fw + i)) * own_floats
-                       : a.pre + ((int64_t)(head * cuts + i - own) * a.pre_tiles + (all >> 4)) * pre_floats;
+                       : pre + (int64_t)(i - own) * width * pre_floats;
     };
     float* const fs = factor[ALL ? 0 : wave];
     // what is in a round of pieces joins what was before it: more rounds than one only where pieces are very many
@@ -855,12 +1084,10 @@ __global__ __launch_bounds__(ALL ? 1024 : 256) void k_attn_merge(AttnArgs a, int
 
 // What a call's sizes make of it.
 struct Sizes {
-    int cols, rows, row_tiles, pre_tiles;
-    int64_t items, lines_pre;
+    int cols, rows, row_tiles, pre_tiles, pre_nt, waves;
+    int64_t items;
     size_t at_items, at_own, at_pre, bytes;
 };
-// Workgroups: two on each CU.
-constexpr int BLOCKS = 512, OWN_WAVES = BLOCKS * WAVES;
 
 bool sizes_of(Sizes& z, bool f32, int64_t n_seqs, int64_t n_q, int64_t n_heads, int64_t kv_heads, int64_t D) {
     if (n_seqs < 0 || n_seqs > MAX_SEQS || n_q < 1 || n_q > 64 || kv_heads < 1 || kv_heads > 256 ||
@@ -872,16 +1099,17 @@ bool sizes_of(Sizes& z, bool f32, int64_t n_seqs, int64_t n_q, int64_t n_heads, 
     z.row_tiles = (int)((rows + z.cols - 1) / z.cols);
     const int64_t pre_tiles = (n_seqs * rows + 15) / 16;
     z.items = n_seqs * kv_heads * z.row_tiles;
-    z.lines_pre = kv_heads * pre_tiles;
-    if (z.items > 1 << 24 || z.lines_pre > 1 << 24) return false;
+    if (z.items > 1 << 24 || kv_heads * pre_tiles > 1 << 20) return false;
     z.pre_tiles = (int)pre_tiles;
+    z.waves = BLOCKS * WAVES;
+    z.pre_nt = pre_columns((int)D / 64, f32);
     const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
     z.at_items = 256;
     z.at_own = z.at_items + up((size_t)z.items * 8);
-    z.at_pre = z.at_own + up((size_t)(2 * OWN_WAVES + z.items) * piece_floats(z.rows, (int)D) * 4);
-    // pieces of the prefix: one for each of a wavefront's tiles, or for each line where there are more of those
-    const int64_t pieces = (int64_t)OWN_WAVES * pre_columns((int)D / 64, f32);
-    z.bytes = z.at_pre + up((size_t)(z.lines_pre > pieces ? z.lines_pre : pieces) * piece_floats(16, (int)D) * 4);
+    z.at_pre = z.at_own + up((size_t)(2 * z.waves + z.items) * piece_floats(z.rows, (int)D) * 4);
+    // pieces of the prefix: a line's for each workgroup, and one more wherever a line begins in one
+    const int64_t width = WAVES * z.pre_nt, lines = kv_heads * ((pre_tiles + width - 1) / width);
+    z.bytes = z.at_pre + up((size_t)(BLOCKS + lines) * width * piece_floats(16, (int)D) * 4);
     return true;
 }
 
@@ -959,7 +1187,7 @@ extern "C" int ft_hip_attention(ft_hip_ctx* ctx, void* stream, const void* q, in
                     (long long)n_q, (long long)n_heads);
     if (table_pages < 1 || table_pages > INT32_MAX / page_tokens)
         return fail(FT_HIP_E_SHAPE, "attention: table_pages=%lld not in [1, 2^31 tokens]", (long long)table_pages);
-    const int64_t cap_steps = z.items * (table_pages * page_tokens / STEP + 2 + start_of((int)head_dim / 64));
+    const int64_t cap_steps = z.items * (table_pages * page_tokens / STEP + 2 + START);
     if (cap_steps >= (int64_t)1 << 31)
         return fail(FT_HIP_E_SHAPE, "attention: n_seqs=%lld tables of table_pages=%lld are too many for one call", (long long)n_seqs,
                     (long long)table_pages);
@@ -968,6 +1196,9 @@ extern "C" int ft_hip_attention(ft_hip_ctx* ctx, void* stream, const void* q, in
     if (prefix_pages < 0 || prefix_pages > INT32_MAX / page_tokens || (prefix && prefix_pages < 1))
         return fail(FT_HIP_E_SHAPE, "attention: prefix_pages=%lld not in [1, 2^31 tokens]", (long long)prefix_pages);
     const int64_t tokens_most = (int64_t)(prefix ? prefix_pages : 0) + table_pages;
+    if (prefix && z.pre_tiles * n_kv_heads * (prefix_pages * page_tokens / STEP + 2) >= (int64_t)1 << 31)
+        return fail(FT_HIP_E_SHAPE, "attention: n_seqs=%lld behind prefix_pages=%lld are too many for one call", (long long)n_seqs,
+                    (long long)prefix_pages);
     if (tokens_most > INT32_MAX / page_tokens)
         return fail(FT_HIP_E_SHAPE, "attention: prefix_pages=%lld and table_pages=%lld pass 2^31 tokens", (long long)prefix_pages,
                     (long long)table_pages);
@@ -1008,12 +1239,12 @@ extern "C" int ft_hip_attention(ft_hip_ctx* ctx, void* stream, const void* q, in
     a.prefix = prefix, a.prefix_len = prefix_len, a.prefix_pages = (int)prefix_pages;
     a.table_pages = (int)table_pages, a.n_pages = (int)n_pages, a.page_shift = shift;
     a.n_seqs = (int)n_seqs, a.n_q = (int)n_q, a.kv_heads = (int)n_kv_heads, a.group = (int)(n_heads / n_kv_heads), a.type = type;
-    a.row_tiles = z.row_tiles, a.pre_tiles = z.pre_tiles, a.rows = z.rows, a.window = (int)window;
+    a.row_tiles = z.row_tiles, a.pre_tiles = z.pre_tiles, a.pre_nt = z.pre_nt, a.rows = z.rows, a.window = (int)window;
     a.scale = scale * LOG2E;
-    a.pre_cost = 1.0f;
+    a.pre_cost = 3.0f;
     a.head = reinterpret_cast<int32_t*>(ws), a.items = reinterpret_cast<int2*>(ws + z.at_items);
     a.own = reinterpret_cast<float*>(ws + z.at_own), a.pre = reinterpret_cast<float*>(ws + z.at_pre);
-    a.own_waves = (int)(cap_steps < OWN_WAVES ? cap_steps : OWN_WAVES);
+    a.own_waves = (int)(cap_steps < z.waves ? cap_steps : z.waves);
     DeviceGuard on(ctx->device);
     if (!on.ok) return fail(FT_HIP_E_DEVICE, "attention: device %d cannot be made current", ctx->device);
     if (cache_type == FT_KV_I8)

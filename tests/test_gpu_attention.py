@@ -454,9 +454,12 @@ def test_two_calls_at_once_with_a_workspace_each(gemv):
     want = [one.check(), two.check()]
     streams = [torch.cuda.Stream() for _ in range(2)]
     ws = [one.workspace(), two.workspace()]
-    torch.cuda.synchronize()
     for _ in range(5):
-        got = [b.run(workspace=w, stream=s) for b, w, s in zip((one, two), ws, streams)]
+        # made and filled before either call: that is the current stream's work
+        given = [dict(b.tensors(), out=torch.full_like(b.q, 9.0), lse=torch.full_like(w[1], 9.0))
+                 for b, w in zip((one, two), want)]
+        torch.cuda.synchronize()
+        got = [b.run(workspace=w, stream=s, **g) for b, w, s, g in zip((one, two), ws, streams, given)]
         torch.cuda.synchronize()
         for g, w in zip(got, want):
             assert torch.equal(g[0], w[0]) and torch.equal(g[1], w[1])
