@@ -1210,15 +1210,17 @@ extern "C" int ft_hip_attention(ft_hip_ctx* ctx, void* stream, const void* q, in
     if (!aligned(q, size) || !aligned(out, size) || !aligned(cache, 16) || !aligned(tables, 4) || !aligned(lens, 4) ||
         !aligned(prefix, 4) || !aligned(prefix_len, 4) || !aligned(lse, 4) || !aligned(workspace, 16))
         return fail(FT_HIP_E_SHAPE, "attention: a pointer is not aligned to its type (cache and workspace: 16 bytes)");
-    if (workspace_bytes < z.bytes)
-        return fail(FT_HIP_E_SHAPE, "attention: workspace of %zu bytes, %zu needed", workspace_bytes, z.bytes);
+    // one size for every type
+    const size_t need = ft_hip_attention_workspace_bytes(n_seqs, n_q, n_heads, n_kv_heads, head_dim);
+    if (need == 0 || workspace_bytes < need)
+        return fail(FT_HIP_E_SHAPE, "attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     if (!ctx) return fail(FT_HIP_E_INVALID, "attention: null argument");
     if (n_seqs == 0) return FT_HIP_OK;  // an empty tensor has no address
     if (!q || !cache || !tables || !lens || !out || !workspace || (prefix && !prefix_len))
         return fail(FT_HIP_E_INVALID, "attention: null argument");
     const int64_t rows = n_seqs * n_q;
     const Span sq{q, rows, q_stride * size, width * size}, so{out, rows, out_stride * size, width * size},
-        sl{lse, 1, 0, rows * n_heads * 4}, sw{workspace, 1, 0, (int64_t)z.bytes};
+        sl{lse, 1, 0, rows * n_heads * 4}, sw{workspace, 1, 0, (int64_t)need};
     const Span in[] = {sq,
                        {cache, 1, 0, n_pages * n_kv_heads * kv_block_bytes(page_tokens, head_dim)},
                        {tables, n_seqs, table_stride * 4, table_pages * 4},
