@@ -33,6 +33,8 @@ using namespace ft;
 
 namespace {
 
+constexpr int64_t MANY = 4096;  // tokens times heads
+
 struct KvArgs {
     const void *k, *v;  // rows to write, or to read into
     int64_t k_stride, v_stride;
@@ -42,23 +44,32 @@ struct KvArgs {
     unsigned n_slots;
 };
 
-__device__ __forceinline__ float4 load4(const void* base, int64_t at, int type, bool vec) {
-    if (type == FT_TYPE_F32) {
-        const float* p = static_cast<const float*>(base) + at;
-        if (vec) return *reinterpret_cast<const float4*>(p);
-        return make_float4(p[0], p[1], p[2], p[3]);
+// W values as they lie, and what they are.
+template <int TYPE, int W>
+struct Some {
+    static constexpr int WORDS = TYPE == FT_TYPE_F32 ? W : W / 2;
+    uint32_t w[WORDS];
+    __device__ __forceinline__ void load(const void* base, int64_t at, bool vec) {
+        if (vec) {
+            typedef uint32_t vector __attribute__((ext_vector_type(WORDS)));
+            const vector a = *reinterpret_cast<const vector*>(static_cast<const char*>(base) + at * (TYPE == FT_TYPE_F32 ? 4 : 2));
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) w[i] = a[i];
+        } else if constexpr (TYPE == FT_TYPE_F32) {
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) w[i] = static_cast<const uint32_t*>(base)[at + i];
+        } else {
+            const uint16_t* p = static_cast<const uint16_t*>(base) + at;
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) w[i] = p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+        }
     }
-    const uint16_t* p = static_cast<const uint16_t*>(base) + at;
-    uint16_t b[4];
-    if (vec) {
-        const uint2 a = *reinterpret_cast<const uint2*>(p);
-        b[0] = (uint16_t)a.x, b[1] = (uint16_t)(a.x >> 16), b[2] = (uint16_t)a.y, b[3] = (uint16_t)(a.y >> 16);
-    } else {
-        b[0] = p[0], b[1] = p[1], b[2] = p[2], b[3] = p[3];
+    __device__ __forceinline__ float value(int i) const {
+        if constexpr (TYPE == FT_TYPE_F32) return __uint_as_float(w[i]);
+        const uint16_t b = (uint16_t)(w[i >> 1] >> (i & 1) * 16);
+        return TYPE == FT_TYPE_F16 ? h2f(b) : __uint_as_float((uint32_t)b << 16);
     }
-    const auto wide = [&](uint16_t v) { return type == FT_TYPE_F16 ? h2f(v) : __uint_as_float((uint32_t)v << 16); };
-    return make_float4(wide(b[0]), wide(b[1]), wide(b[2]), wide(b[3]));
-}
+};
 
 __device__ __forceinline__ uint16_t narrow(float v, int type) {
     if (type == FT_TYPE_F16) return f2h(v);
@@ -67,24 +78,33 @@ __device__ __forceinline__ uint16_t narrow(float v, int type) {
     return (uint16_t)((b + 0x7FFF + (b >> 16 & 1)) >> 16);
 }
 
-__device__ __forceinline__ void store4(void* base, int64_t at, int type, bool vec, const float* v) {
-    if (type == FT_TYPE_F32) {
-        float* p = static_cast<float*>(base) + at;
-        if (vec) {
-            *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-            return;
-        }
-        for (int i = 0; i < 4; ++i) p[i] = v[i];
-        return;
+template <int TYPE, int W>
+__device__ __forceinline__ void store_some(void* base, int64_t at, bool vec, const float* v) {
+    constexpr int WORDS = Some<TYPE, W>::WORDS;
+    uint32_t w[WORDS];
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) {
+        if constexpr (TYPE == FT_TYPE_F32)
+            w[i] = __float_as_uint(v[i]);
+        else
+            w[i] = narrow(v[2 * i], TYPE) | (uint32_t)narrow(v[2 * i + 1], TYPE) << 16;
     }
-    uint16_t* p = static_cast<uint16_t*>(base) + at;
-    uint16_t b[4];
-    for (int i = 0; i < 4; ++i) b[i] = narrow(v[i], type);
+    char* const p = static_cast<char*>(base) + at * (TYPE == FT_TYPE_F32 ? 4 : 2);
     if (vec) {
-        *reinterpret_cast<uint2*>(p) = make_uint2(b[0] | (uint32_t)b[1] << 16, b[2] | (uint32_t)b[3] << 16);
-        return;
+        typedef uint32_t vector __attribute__((ext_vector_type(WORDS)));
+        vector a;
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) a[i] = w[i];
+        *reinterpret_cast<vector*>(p) = a;
+    } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            if constexpr (TYPE == FT_TYPE_F32)
+                reinterpret_cast<uint32_t*>(p)[i] = w[i];
+            else
+                reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)(w[i >> 1] >> (i & 1) * 16);
+        }
     }
-    for (int i = 0; i < 4; ++i) p[i] = b[i];
 }
 
 // Lane (token g, r) holds four values' bytes of token g; afterwards lane (g, r)
@@ -101,12 +121,12 @@ struct Place {
     int idx;        // the token's index in the call
     int slot;       // its place in the cache, or -1
     bool together;  // the four stand in one group of the cache, in order
-    uint8_t* block; // its head's block
+    int64_t page;   // where its page begins
     int o;          // its place in the page
 };
 
 // The groups of four are laid so that those of the first token's run meet the cache's.
-__device__ __forceinline__ Place place_of(const KvArgs& a, int group, int head, int dim, int g) {
+__device__ __forceinline__ Place place_of(const KvArgs& a, int group, int dim, int g) {
     const int first = a.slots[0];
     Place p;
     p.idx = 4 * group - (first > 0 ? first & 3 : 0) + g;
@@ -114,144 +134,228 @@ __device__ __forceinline__ Place place_of(const KvArgs& a, int group, int head, 
     p.slot = (unsigned)slot < a.n_slots ? slot : -1;
     const int at0 = __builtin_amdgcn_readfirstlane(p.slot);  // of token 0
     p.together = at0 >= 0 && (at0 & 3) == 0 && __all(p.slot == at0 + g);
-    const int page = p.slot >> a.page_shift;
+    p.page = (int64_t)(p.slot >> a.page_shift) * a.heads * kv_block_bytes((int64_t)1 << a.page_shift, dim);
     p.o = p.slot & ((1 << a.page_shift) - 1);
-    p.block = a.cache + ((int64_t)page * a.heads + head) * kv_block_bytes((int64_t)1 << a.page_shift, dim);
     return p;
 }
 
-// A value's word or byte (token t of its group) in a block's keys or values.
+// Where in a block's keys dimension `dim` of the token at `o` lies, and in its values.
 template <int ND>
-__device__ __forceinline__ int key_at(int o, int i, int r) {
-    return (o >> 4) * (1024 * ND) + (4 * i + (r >> 2)) * 256 + (o & 15) * 16 + (r & 3) * 4;
+__device__ __forceinline__ int key_at(int o, int dim) {
+    return (o >> 4) * (1024 * ND) + (dim >> 4) * 256 + (o & 15) * 16 + (dim & 15);
 }
 template <int ND>
-__device__ __forceinline__ int value_at(int o, int i, int dim) {
-    return (o >> 4) * (1024 * ND) + i * 1024 + (o >> 2 & 3) * 256 + dim * 4 + (o & 3);
+__device__ __forceinline__ int value_at(int o, int dim) {
+    return (o >> 4) * (1024 * ND) + (dim >> 6) * 1024 + (o >> 2 & 3) * 256 + (dim & 63) * 4 + (o & 3);
 }
 
-// grid: (groups of 16 tokens, 2 * heads); a wavefront per group of four
-template <int CT, int TYPE, int ND>
+// A lane's W values' bytes, words of four. Values of four tokens side by side change places over the lanes: lane g then
+// holds the four tokens' bytes of W / 4 of the values, those from its g's on.
+template <int W>
+__device__ __forceinline__ void spread(uint32_t (&w)[W / 4], int g) {
+    if constexpr (W == 8) {  // even and odd values apart
+        const uint32_t even = __builtin_amdgcn_perm(w[1], w[0], 0x06040200), odd = __builtin_amdgcn_perm(w[1], w[0], 0x07050301);
+        w[0] = swap_tokens(even, g), w[1] = swap_tokens(odd, g);
+    } else {
+        w[0] = swap_tokens(w[0], g);
+    }
+}
+template <int W>
+__device__ __forceinline__ void gather(uint32_t (&w)[W / 4], int g) {
+    if constexpr (W == 8) {
+        const uint32_t even = swap_tokens(w[0], g), odd = swap_tokens(w[1], g);
+        w[0] = __builtin_amdgcn_perm(odd, even, 0x05010400), w[1] = __builtin_amdgcn_perm(odd, even, 0x07030602);
+    } else {
+        w[0] = swap_tokens(w[0], g);
+    }
+}
+template <int W>
+__device__ __forceinline__ void put(uint8_t* p, const uint32_t (&w)[W / 4]) {
+    if constexpr (W == 8)
+        *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else
+        *reinterpret_cast<uint32_t*>(p) = w[0];
+}
+template <int W>
+__device__ __forceinline__ void take(const uint8_t* p, uint32_t (&w)[W / 4]) {
+    if constexpr (W == 8) {
+        const uint2 a = *reinterpret_cast<const uint2*>(p);
+        w[0] = a.x, w[1] = a.y;
+    } else {
+        w[0] = *reinterpret_cast<const uint32_t*>(p);
+    }
+}
+
+// A wavefront per group of four tokens and R of the 2 * heads parts, a head's keys or values each, which are all on
+// their way before the first is worked on; 16 lanes a token, W values a lane in each round. Four groups make a workgroup;
+// the workgroups of one group's parts follow each other, so that those running at once touch whole rows and all of the
+// memory's channels (32768 tokens of 8 heads of 256 read 107 us with the tokens first, 85 so).
+template <int CT, int TYPE, int ND, int R, int W>
 __global__ __launch_bounds__(256) void k_kv_write(KvArgs a, bool vec) {
-    constexpr int D = 64 * ND;
+    constexpr int D = 64 * ND, NR = D / (16 * W);
     const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
-    const int head = blockIdx.y >> 1;
-    const bool value = blockIdx.y & 1;
-    const Place p = place_of(a, blockIdx.x * 4 + (threadIdx.x >> 6), head, D, g);
+    const int parts = (2 * a.heads + R - 1) / R, group = blockIdx.x / parts, part0 = (blockIdx.x - group * parts) * R;
+    const Place p = place_of(a, group * 4 + (threadIdx.x >> 6), D, g);
     const bool live = p.slot >= 0;
-    float4 x[ND];
-    float top = 0.0f;
-    const int64_t from = (int64_t)p.idx * (value ? a.v_stride : a.k_stride) + head * D + 4 * r;
+    Some<TYPE, W> raw[R][NR];
 #pragma unroll
-    for (int i = 0; i < ND; ++i) {
-        x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (live) x[i] = load4(value ? a.v : a.k, from + 64 * i, TYPE, vec);
-        // NaN counts as inf: the maximum then says that the row is no numbers
-        const auto size = [](float v) { return fabsf(v) <= FLT_MAX ? fabsf(v) : INFINITY; };
-        top = fmaxf(fmaxf(fmaxf(top, size(x[i].x)), fmaxf(size(x[i].y), size(x[i].z))), size(x[i].w));
-    }
-    top = row_max16(top);
-    const bool bad = top == INFINITY;
-    float d = 0.0f;
-    uint32_t word[ND];
-    if constexpr (CT == FT_KV_I8) {
-        const double of = top > 0.0f && !bad ? 127.0 / (double)top * (1.0 + 0x1p-44) : 0.0;
-        d = (float)((double)top / 127.0);
+    for (int u = 0; u < R; ++u) {
+        const int part = part0 + u;
+        if (R > 1 && part >= 2 * a.heads) break;
+        const int64_t from = (int64_t)p.idx * (part & 1 ? a.v_stride : a.k_stride) + (part >> 1) * D + W * r;
 #pragma unroll
-        for (int i = 0; i < ND; ++i) {
-            // the sum's last bit is 1: its low half is the nearest whole number
-            const auto q = [&](float v) { return (uint32_t)(int)__double_as_longlong(fma((double)(bad ? 0.0f : v), of, 0x1.8p52 + 128.0)); };
-            word[i] = (q(x[i].x) & 255) | (q(x[i].y) & 255) << 8 | (q(x[i].z) & 255) << 16 | q(x[i].w) << 24;
-        }
-    } else {
-        const int bits = __float_as_int(top);
-        const int e = max((bits >> 23) - 127 - 8 + ((bits & 0x7FFFFF) > 0x600000 ? 1 : 0), -126);
-        const float inv = __int_as_float((127 - e) << 23);
-        if (top > 0.0f) d = __int_as_float((127 + e) << 23);
-#pragma unroll
-        for (int i = 0; i < ND; ++i) {
-            const auto y = [&](float v) { return bad ? 0.0f : v * inv; };
-            int w = __builtin_amdgcn_cvt_pk_fp8_f32(y(x[i].x), y(x[i].y), 0, false);
-            word[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y(x[i].z), y(x[i].w), w, true);
+        for (int i = 0; i < NR; ++i) {
+            raw[u][i] = Some<TYPE, W>{};
+            if (live) raw[u][i].load(part & 1 ? a.v : a.k, from + 16 * W * i, vec);
         }
     }
-    if (bad) d = __int_as_float(0x7FC00000);
-    uint8_t* const rows = p.block + (value ? (int64_t)D << a.page_shift : 0);
-    if (live && r == 0) reinterpret_cast<float*>(p.block + ((int64_t)(2 * D) << a.page_shift))[(value ? 1 << a.page_shift : 0) + p.o] = d;
-    if (!value) {
-        if (!live) return;
 #pragma unroll
-        for (int i = 0; i < ND; ++i) *reinterpret_cast<uint32_t*>(rows + key_at<ND>(p.o, i, r)) = word[i];
-    } else if (p.together) {
+    for (int u = 0; u < R; ++u) {
+        const int part = part0 + u, head = part >> 1;
+        const bool value = part & 1;
+        if (R > 1 && part >= 2 * a.heads) break;
+        float x[NR][W], top = 0.0f;
 #pragma unroll
-        for (int i = 0; i < ND; ++i)
-            *reinterpret_cast<uint32_t*>(rows + value_at<ND>(p.o & ~3, i, 4 * r + g)) = swap_tokens(word[i], g);
-    } else if (live) {
+        for (int i = 0; i < NR; ++i)
 #pragma unroll
-        for (int i = 0; i < ND; ++i)
+            for (int e = 0; e < W; ++e) {
+                x[i][e] = raw[u][i].value(e);
+                // NaN counts as inf: the maximum then says that the row is no numbers
+                top = fmaxf(top, fabsf(x[i][e]) <= FLT_MAX ? fabsf(x[i][e]) : INFINITY);
+            }
+        top = row_max16(top);
+        const bool bad = top == INFINITY;
+        float d = 0.0f;
+        uint32_t word[NR][W / 4];
+        if constexpr (CT == FT_KV_I8) {
+            const double of = top > 0.0f && !bad ? 127.0 / (double)top * (1.0 + 0x1p-44) : 0.0;
+            d = (float)((double)top / 127.0);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) rows[value_at<ND>(p.o, i, 4 * r + e)] = (uint8_t)(word[i] >> (8 * e));
+            for (int i = 0; i < NR; ++i)
+#pragma unroll
+                for (int e = 0; e < W; e += 4) {
+                    // the sum's last bit is 1: its low half is the nearest whole number
+                    const auto q = [&](float v) { return (uint32_t)(int)__double_as_longlong(fma((double)(bad ? 0.0f : v), of, 0x1.8p52 + 128.0)); };
+                    word[i][e / 4] = (q(x[i][e]) & 255) | (q(x[i][e + 1]) & 255) << 8 | (q(x[i][e + 2]) & 255) << 16 | q(x[i][e + 3]) << 24;
+                }
+        } else {
+            const int bits = __float_as_int(top);
+            const int e2 = max((bits >> 23) - 127 - 8 + ((bits & 0x7FFFFF) > 0x600000 ? 1 : 0), -126);
+            const float inv = __int_as_float((127 - e2) << 23);
+            if (top > 0.0f) d = __int_as_float((127 + e2) << 23);
+#pragma unroll
+            for (int i = 0; i < NR; ++i)
+#pragma unroll
+                for (int e = 0; e < W; e += 4) {
+                    const auto y = [&](float v) { return bad ? 0.0f : v * inv; };
+                    const int w = __builtin_amdgcn_cvt_pk_fp8_f32(y(x[i][e]), y(x[i][e + 1]), 0, false);
+                    word[i][e / 4] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y(x[i][e + 2]), y(x[i][e + 3]), w, true);
+                }
+        }
+        if (bad) d = __int_as_float(0x7FC00000);
+        uint8_t* const block = a.cache + p.page + head * kv_block_bytes((int64_t)1 << a.page_shift, D);
+        uint8_t* const rows = block + (value ? (int64_t)D << a.page_shift : 0);
+        if (live && r == 0)
+            reinterpret_cast<float*>(block + ((int64_t)(2 * D) << a.page_shift))[(value ? 1 << a.page_shift : 0) + p.o] = d;
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+            const int dim = 16 * W * i + W * r;
+            if (!value) {
+                if (live) put<W>(rows + key_at<ND>(p.o, dim), word[i]);
+            } else if (p.together) {
+                spread<W>(word[i], g);
+                put<W>(rows + value_at<ND>(p.o & ~3, dim + W / 4 * g), word[i]);
+            } else if (live) {
+#pragma unroll
+                for (int e = 0; e < W; ++e) rows[value_at<ND>(p.o, dim + e)] = (uint8_t)(word[i][e >> 2] >> (8 * (e & 3)));
+            }
+        }
     }
 }
 
-template <int CT, int TYPE, int ND>
+template <int CT, int TYPE, int ND, int R, int W>
 __global__ __launch_bounds__(256) void k_kv_read(KvArgs a, bool vec) {
-    constexpr int D = 64 * ND;
+    constexpr int D = 64 * ND, NR = D / (16 * W);
     const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
-    const int head = blockIdx.y >> 1;
-    const bool value = blockIdx.y & 1;
-    const Place p = place_of(a, blockIdx.x * 4 + (threadIdx.x >> 6), head, D, g);
+    const int parts = (2 * a.heads + R - 1) / R, group = blockIdx.x / parts, part0 = (blockIdx.x - group * parts) * R;
+    const Place p = place_of(a, group * 4 + (threadIdx.x >> 6), D, g);
     const bool live = p.slot >= 0;
-    const uint8_t* const rows = p.block + (value ? (int64_t)D << a.page_shift : 0);
-    uint32_t word[ND];
-    float d = 0.0f;
-    if (live) d = reinterpret_cast<const float*>(p.block + ((int64_t)(2 * D) << a.page_shift))[(value ? 1 << a.page_shift : 0) + p.o];
-    if (!value) {
-        if (!live) return;
+    uint32_t word[R][NR][W / 4];
+    float d[R];
 #pragma unroll
-        for (int i = 0; i < ND; ++i) word[i] = *reinterpret_cast<const uint32_t*>(rows + key_at<ND>(p.o, i, r));
-    } else if (p.together) {
+    for (int u = 0; u < R; ++u) {
+        const int part = part0 + u;
+        const bool value = part & 1;
+        if (R > 1 && part >= 2 * a.heads) break;
+        const uint8_t* const block = a.cache + p.page + (part >> 1) * kv_block_bytes((int64_t)1 << a.page_shift, D);
+        const uint8_t* const rows = block + (value ? (int64_t)D << a.page_shift : 0);
+        d[u] = 0.0f;
+        if (live) d[u] = reinterpret_cast<const float*>(block + ((int64_t)(2 * D) << a.page_shift))[(value ? 1 << a.page_shift : 0) + p.o];
 #pragma unroll
-        for (int i = 0; i < ND; ++i) word[i] = *reinterpret_cast<const uint32_t*>(rows + value_at<ND>(p.o & ~3, i, 4 * r + g));
+        for (int i = 0; i < NR; ++i) {
+            const int dim = 16 * W * i + W * r;
 #pragma unroll
-        for (int i = 0; i < ND; ++i) word[i] = swap_tokens(word[i], g);
-    } else {
-        if (!live) return;
+            for (int e = 0; e < W / 4; ++e) word[u][i][e] = 0;
+            if (!live) continue;
+            if (!value) {
+                take<W>(rows + key_at<ND>(p.o, dim), word[u][i]);
+            } else if (p.together) {
+                take<W>(rows + value_at<ND>(p.o & ~3, dim + W / 4 * g), word[u][i]);
+            } else {
 #pragma unroll
-        for (int i = 0; i < ND; ++i) {
-            word[i] = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) word[i] |= (uint32_t)rows[value_at<ND>(p.o, i, 4 * r + e)] << (8 * e);
+                for (int e = 0; e < W; ++e) word[u][i][e >> 2] |= (uint32_t)rows[value_at<ND>(p.o, dim + e)] << (8 * (e & 3));
+            }
         }
     }
-    const int64_t to = (int64_t)p.idx * (value ? a.v_stride : a.k_stride) + head * D + 4 * r;
 #pragma unroll
-    for (int i = 0; i < ND; ++i) {
-        float v[4];
+    for (int u = 0; u < R; ++u) {
+        const int part = part0 + u;
+        const bool value = part & 1;
+        if (R > 1 && part >= 2 * a.heads) break;
+        const int64_t to = (int64_t)p.idx * (value ? a.v_stride : a.k_stride) + (part >> 1) * D + W * r;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            float q;
-            if constexpr (CT == FT_KV_I8)
-                q = (float)(int)(word[i] >> (8 * e) & 255) - 128.0f;
-            else
-                q = e == 0   ? __builtin_amdgcn_cvt_f32_fp8((int)word[i], 0)
-                    : e == 1 ? __builtin_amdgcn_cvt_f32_fp8((int)word[i], 1)
-                    : e == 2 ? __builtin_amdgcn_cvt_f32_fp8((int)word[i], 2)
-                             : __builtin_amdgcn_cvt_f32_fp8((int)word[i], 3);
-            v[e] = q * d;
+        for (int i = 0; i < NR; ++i) {
+            if (value && p.together) gather<W>(word[u][i], g);
+            float v[W];
+#pragma unroll
+            for (int e = 0; e < W; ++e) {
+                const uint32_t w = word[u][i][e >> 2];
+                float q;
+                if constexpr (CT == FT_KV_I8)
+                    q = (float)(int)(w >> (8 * (e & 3)) & 255) - 128.0f;
+                else
+                    q = (e & 3) == 0   ? __builtin_amdgcn_cvt_f32_fp8((int)w, 0)
+                        : (e & 3) == 1 ? __builtin_amdgcn_cvt_f32_fp8((int)w, 1)
+                        : (e & 3) == 2 ? __builtin_amdgcn_cvt_f32_fp8((int)w, 2)
+                                       : __builtin_amdgcn_cvt_f32_fp8((int)w, 3);
+                v[e] = q * d[u];
+            }
+            if (live) store_some<TYPE, W>(const_cast<void*>(value ? a.v : a.k), to + 16 * W * i, vec, v);
         }
-        store4(const_cast<void*>(value ? a.v : a.k), to + 64 * i, TYPE, vec, v);
     }
+}
+
+template <bool WRITE, int CT, int TYPE, int ND, int R>
+void launch_parts(const KvArgs& a, bool vec, hipStream_t s) {
+    // a group more than the tokens need: the first may begin up to three tokens before the first token
+    const dim3 grid((unsigned)(((int64_t)a.n + 3 + 15) / 16 * ((2 * a.heads + R - 1) / R)));
+    // 16 bytes of a row a lane, as far as the heads have them
+    constexpr int W = TYPE == FT_TYPE_F32 || ND == 1 ? 4 : 8;
+    if (WRITE)
+        hipLaunchKernelGGL((k_kv_write<CT, TYPE, ND, R, W>), grid, dim3(256), 0, s, a, vec);
+    else
+        hipLaunchKernelGGL((k_kv_read<CT, TYPE, ND, R, W>), grid, dim3(256), 0, s, a, vec);
 }
 
 template <bool WRITE, int CT, int TYPE>
-void launch_nd(const KvArgs& a, int nd, bool vec, dim3 grid, hipStream_t s) {
+void launch_nd(const KvArgs& a, int nd, bool vec, hipStream_t s) {
     const auto go = [&](auto ND) {
         constexpr int N = decltype(ND)::value;
-        if (WRITE)
-            hipLaunchKernelGGL((k_kv_write<CT, TYPE, N>), grid, dim3(256), 0, s, a, vec);
+        // many tokens: several parts a wavefront
+        if ((int64_t)a.n * a.heads >= MANY)
+            launch_parts<WRITE, CT, TYPE, N, 4>(a, vec, s);
         else
-            hipLaunchKernelGGL((k_kv_read<CT, TYPE, N>), grid, dim3(256), 0, s, a, vec);
+            launch_parts<WRITE, CT, TYPE, N, 1>(a, vec, s);
     };
     if (nd == 1)
         go(std::integral_constant<int, 1>{});
@@ -262,24 +366,21 @@ void launch_nd(const KvArgs& a, int nd, bool vec, dim3 grid, hipStream_t s) {
 }
 
 template <bool WRITE>
-void launch_kv(const KvArgs& a, int cache_type, int type, int head_dim, bool vec, hipStream_t s) {
-    // a group more than the tokens need: the first may begin up to three tokens before the first token
-    const dim3 grid((unsigned)(((int64_t)a.n + 3 + 15) / 16), (unsigned)(2 * a.heads));
-    const int nd = head_dim / 64;
+void launch_kv(const KvArgs& a, int cache_type, int type, int nd, bool vec, hipStream_t s) {
     if (cache_type == FT_KV_I8) {
         if (type == FT_TYPE_F32)
-            launch_nd<WRITE, FT_KV_I8, FT_TYPE_F32>(a, nd, vec, grid, s);
+            launch_nd<WRITE, FT_KV_I8, FT_TYPE_F32>(a, nd, vec, s);
         else if (type == FT_TYPE_F16)
-            launch_nd<WRITE, FT_KV_I8, FT_TYPE_F16>(a, nd, vec, grid, s);
+            launch_nd<WRITE, FT_KV_I8, FT_TYPE_F16>(a, nd, vec, s);
         else
-            launch_nd<WRITE, FT_KV_I8, FT_TYPE_BF16>(a, nd, vec, grid, s);
+            launch_nd<WRITE, FT_KV_I8, FT_TYPE_BF16>(a, nd, vec, s);
     } else {
         if (type == FT_TYPE_F32)
-            launch_nd<WRITE, FT_KV_E4M3, FT_TYPE_F32>(a, nd, vec, grid, s);
+            launch_nd<WRITE, FT_KV_E4M3, FT_TYPE_F32>(a, nd, vec, s);
         else if (type == FT_TYPE_F16)
-            launch_nd<WRITE, FT_KV_E4M3, FT_TYPE_F16>(a, nd, vec, grid, s);
+            launch_nd<WRITE, FT_KV_E4M3, FT_TYPE_F16>(a, nd, vec, s);
         else
-            launch_nd<WRITE, FT_KV_E4M3, FT_TYPE_BF16>(a, nd, vec, grid, s);
+            launch_nd<WRITE, FT_KV_E4M3, FT_TYPE_BF16>(a, nd, vec, s);
     }
 }
 
@@ -294,7 +395,7 @@ int kv_call(const char* what, ft_hip_ctx* ctx, void* stream, const void* k, int6
                     what, (long long)page_tokens, (long long)n_heads, (long long)head_dim);
     if (!kv_pages_fit(n_pages, page_tokens))
         return fail(FT_HIP_E_SHAPE, "%s: n_pages=%lld not in [1, 2^31 tokens]", what, (long long)n_pages);
-    if (n < 0 || n > 1 << 24) return fail(FT_HIP_E_SHAPE, "%s: n=%lld not in [0, 2^24]", what, (long long)n);
+    if (n < 0 || n > 1 << 20) return fail(FT_HIP_E_SHAPE, "%s: n=%lld not in [0, 2^20]", what, (long long)n);
     if (type != FT_TYPE_F32 && type != FT_TYPE_F16 && type != FT_TYPE_BF16)
         return fail(FT_HIP_E_INVALID, "%s: type=%d is no FT_TYPE", what, type);
     if (cache_type != FT_KV_I8 && cache_type != FT_KV_E4M3)
@@ -318,11 +419,11 @@ int kv_call(const char* what, ft_hip_ctx* ctx, void* stream, const void* k, int6
     while (1 << shift < page_tokens) ++shift;
     const KvArgs a{k, v, k_stride, v_stride, slots, static_cast<uint8_t*>(const_cast<void*>(cache)), (int)n,
                    (int)n_heads, shift, (unsigned)(n_pages * page_tokens)};
-    // four values at a time where every row starts on them
-    const bool vec = aligned(k, 4 * size) && aligned(v, 4 * size) && k_stride % 4 == 0 && v_stride % 4 == 0;
+    // 16 bytes of a row at a time where every row starts on them
+    const bool vec = aligned(k, 16) && aligned(v, 16) && k_stride * size % 16 == 0 && v_stride * size % 16 == 0;
     DeviceGuard on(ctx->device);
     if (!on.ok) return fail(FT_HIP_E_DEVICE, "%s: device %d cannot be made current", what, ctx->device);
-    launch_kv<WRITE>(a, cache_type, type, (int)head_dim, vec, static_cast<hipStream_t>(stream));
+    launch_kv<WRITE>(a, cache_type, type, (int)head_dim / 64, vec, static_cast<hipStream_t>(stream));
     return launch_status(what);
 }
 

@@ -69,10 +69,14 @@ __device__ __forceinline__ float4 four(const LogitArgs& a, int64_t row, int v) {
 template <int TYPE, int CHUNK, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_adjust(LogitArgs a) {
     constexpr int EACH = CHUNK / 4 / THREADS;
-    __shared__ uint32_t count[CHUNK], biased[CHUNK / 32];
-    __shared__ int list_at[MAX_BIAS];
-    __shared__ float list_add[MAX_BIAS];
-    __shared__ int listed;
+    // what is not given takes no LDS: more workgroups on a CU
+    extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
+    uint32_t* const count = lds;
+    uint32_t* const biased = lds + (a.history ? CHUNK : 0);
+    int* const list_at = reinterpret_cast<int*>(biased + CHUNK / 32);
+    int* const list_i = list_at + a.n_bias;
+    float* const list_add = reinterpret_cast<float*>(list_i + a.n_bias);
+    __shared__ int listed, again;
     const int t = threadIdx.x, v0 = blockIdx.x * CHUNK;
     const int64_t row = blockIdx.y;
     float4 x[EACH];
@@ -84,36 +88,84 @@ __global__ __launch_bounds__(THREADS) void k_adjust(LogitArgs a) {
         bits[i] = 15;
         if (a.mask && v < a.V) bits[i] = a.mask[row * a.mask_stride + (v >> 5)] >> (v & 31);
     }
+    // the lists' first entries are on their way as well
+    const int32_t* const h = a.history + row * a.h_stride;
+    const int32_t* const ids = a.bias_ids + row * a.n_bias;
+    const float* const adds = a.bias + row * a.n_bias;
+    int len = 0, id[8], bias_id = -1;
+    float bias = 0.0f;
     if (a.history) {
+        len = a.h_len ? a.h_len[row] : a.h_max;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) id[u] = u * THREADS + t < a.h_max ? h[u * THREADS + t] : -1;
         for (int i = t; i < CHUNK / 4; i += THREADS) reinterpret_cast<uint4*>(count)[i] = make_uint4(0, 0, 0, 0);
-        __syncthreads();
-        int len = a.h_len ? a.h_len[row] : a.h_max;
+    }
+    if (a.n_bias) {
+        if (t < a.n_bias) bias_id = ids[t], bias = adds[t];
+        for (int i = t; i < CHUNK / 32; i += THREADS) biased[i] = 0;
+        if (t == 0) listed = 0, again = 0;
+    }
+    __syncthreads();
+    if (a.history) {
         len = len < a.h_max ? len : a.h_max;
-        const int32_t* h = a.history + row * a.h_stride;
-        for (int i = t; i < len; i += THREADS) {
-            const unsigned at = (unsigned)h[i] - (unsigned)v0;
-            if (at < CHUNK) atomicAdd(&count[at], 1u);
+        for (int i0 = 0; i0 < len; i0 += 8 * THREADS) {
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const unsigned at = (unsigned)id[u] - (unsigned)v0;
+                if (i0 + u * THREADS + t < len && at < CHUNK && id[u] >= 0) atomicAdd(&count[at], 1u);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int i = i0 + (8 + u) * THREADS + t;
+                id[u] = i < len ? h[i] : -1;
+            }
         }
     }
     if (a.n_bias) {
-        for (int i = t; i < CHUNK / 32; i += THREADS) biased[i] = 0;
-        if (t == 0) listed = 0;
-        __syncthreads();
-        const int32_t* ids = a.bias_ids + row * a.n_bias;
-        const float* add = a.bias + row * a.n_bias;
         for (int i = t; i < a.n_bias; i += THREADS) {
-            const int id = ids[i];
-            const unsigned at = (unsigned)id - (unsigned)v0;
-            if (at >= CHUNK || id < 0) continue;
-            bool first = true;  // the token's first entry adds them all, in their order
-            for (int j = 0; j < i && first; ++j) first = ids[j] != id;
-            if (!first) continue;
-            float s = add[i];
-            for (int j = i + 1; j < a.n_bias; ++j)
-                if (ids[j] == id) s += add[j];
-            const int k = atomicAdd(&listed, 1);
-            list_at[k] = (int)at, list_add[k] = s;
-            atomicOr(&biased[at >> 5], 1u << (at & 31));
+            const unsigned at = (unsigned)bias_id - (unsigned)v0;
+            if (at < CHUNK && bias_id >= 0) {
+                const int k = atomicAdd(&listed, 1);
+                list_at[k] = (int)at, list_add[k] = bias, list_i[k] = i;
+                if (atomicOr(&biased[at >> 5], 1u << (at & 31)) >> (at & 31) & 1) again = 1;
+            }
+            if (i + THREADS < a.n_bias) bias_id = ids[i + THREADS], bias = adds[i + THREADS];
+        }
+        __syncthreads();
+        if (again) {  // a token more than once: its first entry adds them all, in their order
+            constexpr int OWN = MAX_BIAS / THREADS;
+            float sum[OWN];
+            bool first[OWN];
+#pragma unroll
+            for (int u = 0; u < OWN; ++u) {
+                const int k = t + u * THREADS;
+                first[u] = false, sum[u] = 0.0f;
+                if (k >= listed) continue;
+                const int at = list_at[k];
+                int last = -1;
+                while (true) {  // the token's entries by rising index, a look through the list for each
+                    int best = -1;
+                    for (int j = 0; j < listed; ++j)
+                        if (list_at[j] == at && list_i[j] > last && (best < 0 || list_i[j] < list_i[best])) best = j;
+                    if (best < 0) break;
+                    if (last < 0) {
+                        first[u] = best == k;
+                        if (!first[u]) break;
+                        sum[u] = list_add[best];
+                    } else {
+                        sum[u] += list_add[best];
+                    }
+                    last = list_i[best];
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < OWN; ++u) {
+                const int k = t + u * THREADS;
+                if (k >= listed) continue;
+                list_add[k] = sum[u];
+                if (!first[u]) list_at[k] = -1;
+            }
         }
     }
     __syncthreads();
@@ -160,13 +212,23 @@ __global__ __launch_bounds__(THREADS) void k_adjust(LogitArgs a) {
     }
 }
 
+template <int TYPE, int CHUNK, int THREADS>
+void launch_chunks(const LogitArgs& a, int64_t n, hipStream_t s) {
+    const size_t lds = (a.history ? CHUNK * 4 : 0) + (a.n_bias ? CHUNK / 8 + a.n_bias * 12 : 0);
+    hipLaunchKernelGGL((k_adjust<TYPE, CHUNK, THREADS>), dim3((unsigned)((a.V + CHUNK - 1) / CHUNK), (unsigned)n), dim3(THREADS), lds, s, a);
+}
+
+// Chunks as long as there are enough of them: each goes through the whole history. 64 rows of 262144 with 6000 tokens and
+// 100 biases 32.1 us, in chunks of 8192 37.2 and of 4096 37.5; 12 rows 11.3, 10.0 and 9.8.
 template <int TYPE>
-void launch_adjust(const LogitArgs& a, int64_t n, int cus, hipStream_t s) {
-    // small chunks while they do not fill the device
-    if ((int64_t)a.V * n < (int64_t)cus * 8192)
-        hipLaunchKernelGGL((k_adjust<TYPE, 2048, 256>), dim3((unsigned)((a.V + 2047) / 2048), (unsigned)n), dim3(256), 0, s, a);
+void launch_adjust(const LogitArgs& a, int64_t n, hipStream_t s) {
+    const int64_t values = (int64_t)a.V * n;
+    if (values < 1 << 20)
+        launch_chunks<TYPE, 2048, 256>(a, n, s);
+    else if (values < 1 << 23)
+        launch_chunks<TYPE, 4096, 512>(a, n, s);
     else
-        hipLaunchKernelGGL((k_adjust<TYPE, 8192, 512>), dim3((unsigned)((a.V + 8191) / 8192), (unsigned)n), dim3(512), 0, s, a);
+        launch_chunks<TYPE, 16384, 1024>(a, n, s);
 }
 
 }  // namespace
@@ -222,10 +284,10 @@ extern "C" int ft_hip_adjust_logits(ft_hip_ctx* ctx, void* stream, const void* l
     if (!on.ok) return fail(FT_HIP_E_DEVICE, "adjust_logits: device %d cannot be made current", ctx->device);
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (logits_type == FT_TYPE_F32)
-        launch_adjust<FT_TYPE_F32>(a, n, ctx->num_cus, s);
+        launch_adjust<FT_TYPE_F32>(a, n, s);
     else if (logits_type == FT_TYPE_F16)
-        launch_adjust<FT_TYPE_F16>(a, n, ctx->num_cus, s);
+        launch_adjust<FT_TYPE_F16>(a, n, s);
     else
-        launch_adjust<FT_TYPE_BF16>(a, n, ctx->num_cus, s);
+        launch_adjust<FT_TYPE_BF16>(a, n, s);
     return launch_status("adjust_logits");
 }

@@ -147,9 +147,9 @@ int ft_hip_add_rmsnorm(ft_hip_ctx* ctx, void* stream, const void* x, int x_type,
  * ft_hip_kv_read: the reverse; f32(q * d) rounded to `type`; the rows of slots
  * that are passed over stay as they were.
  * cache is 16-byte aligned, slots 4-byte, rows to their type; rows that start on
- * four values are read four at a time. The cache, and read's rows, may not
+ * 16 bytes are read and written 16 at a time. The cache, and read's rows, may not
  * overlap any other argument. n 0: nothing is done, and the pointers may be
- * NULL. n <= 2^24; n_heads <= 256; n_pages * page_tokens < 2^31. */
+ * NULL. n <= 2^20; n_heads <= 256; n_pages * page_tokens < 2^31. */
 int64_t ft_hip_kv_page_bytes(int64_t page_tokens, int64_t n_heads, int64_t head_dim);
 int ft_hip_kv_write(ft_hip_ctx* ctx, void* stream, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
                     int type, const int32_t* slots, void* cache, int cache_type, int64_t n_pages, int64_t page_tokens,

@@ -50,7 +50,7 @@ CACHE = [(dict(page_tokens=0), "SHAPE", "page_tokens"), (dict(page_tokens=8), "S
          (dict(cache_type=2), "INVALID", "cache_type"), (dict(cache_type=-1), "INVALID", "cache_type"),
          (dict(type=3), "INVALID", "type"), (dict(cache=0x30008), "SHAPE", "aligned"), (dict(cache=None), "INVALID", "null")]
 ROWS = CACHE + [(dict(n_heads=0), "SHAPE", "n_heads"), (dict(n_heads=257), "SHAPE", "n_heads"),
-                (dict(n=-1), "SHAPE", "n="), (dict(n=(1 << 24) + 1), "SHAPE", "n="), (dict(n=BIG), "SHAPE", "n="),
+                (dict(n=-1), "SHAPE", "n="), (dict(n=(1 << 20) + 1), "SHAPE", "n="), (dict(n=BIG), "SHAPE", "n="),
                 (dict(k_stride=127), "SHAPE", "k_stride"), (dict(v_stride=0), "SHAPE", "v_stride"),
                 (dict(k_stride=BIG), "SHAPE", "k_stride"), (dict(k=0x10002), "SHAPE", "aligned"),
                 (dict(type=1, v=0x10201), "SHAPE", "aligned"), (dict(slots=0x20002), "SHAPE", "aligned"),

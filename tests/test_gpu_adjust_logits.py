@@ -78,7 +78,7 @@ def check(gemv, x, s, vocab, out=None, place=None):
 @pytest.mark.parametrize("n,vocab,history,bias,mask", [
     (1, 1, 1, 1, True), (1, 31, 5, 0, True), (3, 33, 0, 4, False), (2, 2047, 100, 3, True), (5, 2048, 1, 1, False),
     (4, 2049, 3000, 0, False), (2, 8193, 50, 1024, True), (300, 8191, 40, 5, True), (64, 50021, 700, 30, True),
-    (9, 262144, 2000, 17, False), (1, 262144, 20000, 300, True), (3, 5000, 0, 0, True), (2, 5000, 0, 0, False)])
+    (9, 262144, 2000, 17, False), (1, 262144, 20000, 300, True), (33, 262144, 20000, 1024, True), (40, 262143, 0, 0, True), (3, 5000, 0, 0, True), (2, 5000, 0, 0, False)])
 def test_against_the_formula(gemv, dtype, n, vocab, history, bias, mask):
     x, s = inputs(np.random.default_rng(n * 7 + vocab), n, vocab, history, bias, mask, dtype)
     check(gemv, x, s, vocab)
