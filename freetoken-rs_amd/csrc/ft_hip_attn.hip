@@ -953,15 +953,15 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn(AttnArgs a) {
     }
 }
 
-// Joins the pieces of the own items' rows: a wavefront a row, or with ALL the
-// whole workgroup. First the pieces' maxima and sums, a lane each, then their
-// values, several pieces at a time.
-template <int ND, bool ALL>
-__global__ __launch_bounds__(ALL ? 1024 : 256) void k_attn_merge(AttnArgs a, int cols) {
+// Joins the pieces of the own items' rows, TEAM threads a row. The pieces' maxima and sums, a lane each, and the first
+// eight pieces' values for each thread are on their way together.
+template <int ND, int TEAM>
+__global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void k_attn_merge(AttnArgs a, int cols) {
+    constexpr bool ALL = TEAM >= 256;          // the workgroup's one row
     constexpr int D = 64 * ND, LANES = D / 4;  // lanes that hold a piece's values
-    constexpr int MERGE_WAVES = ALL ? 16 : 4;
+    constexpr int MERGE_WAVES = ALL ? TEAM / 64 : 4;
     constexpr int MOST = ALL ? 1024 : 256;  // pieces of a round
-    constexpr int TEAM = ALL ? 1024 : 64, SLICES = TEAM / LANES;
+    constexpr int SLICES = TEAM / LANES;
     __shared__ float factor[ALL ? 1 : MERGE_WAVES][MOST];
     __shared__ f32x4 sums[ALL ? TEAM : 1];
     __shared__ float red[2][MERGE_WAVES];
@@ -1001,7 +1001,16 @@ __global__ __launch_bounds__(ALL ? 1024 : 256) void k_attn_merge(AttnArgs a, int
     f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int i0 = 0; i0 < n; i0 += MOST) {
         if (ALL && i0) __syncthreads();
-        const int k = min(n - i0, MOST);
+        const int k = min(n - i0, MOST), at = (t % LANES) * 4;
+        const auto fetch = [&](f32x4 (&v)[8], int from) {  // eight pieces at once
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int j = min(from + u * SLICES, k - 1);
+                v[u] = *reinterpret_cast<const f32x4*>(piece(i0 + j) + (int64_t)(i0 + j < own ? y : all & 15) * D + at);
+            }
+        };
+        f32x4 v[8];
+        fetch(v, t / LANES);
         float top = M;
         for (int i = t; i < k; i += TEAM) {
             const float* p = piece(i0 + i);
@@ -1040,14 +1049,8 @@ __global__ __launch_bounds__(ALL ? 1024 : 256) void k_attn_merge(AttnArgs a, int
         L = L * f + sum;
         x *= f;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the lanes read each other's factors
-        const int at = (t % LANES) * 4;
-        for (int i = t / LANES; i < k; i += 8 * SLICES) {  // eight pieces at once on their way
-            f32x4 v[8];
-#pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const int j = min(i + u * SLICES, k - 1);
-                v[u] = *reinterpret_cast<const f32x4*>(piece(i0 + j) + (int64_t)(i0 + j < own ? y : all & 15) * D + at);
-            }
+        for (int i = t / LANES; i < k; i += 8 * SLICES) {
+            if (i >= 8 * SLICES) fetch(v, i);
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
                 const int j = i + u * SLICES;
@@ -1081,6 +1084,8 @@ __global__ __launch_bounds__(ALL ? 1024 : 256) void k_attn_merge(AttnArgs a, int
         store_out<false>(a.out, to, a.type == FT_TYPE_F16, v);
     if (a.lse && t == 0) a.lse[token * a.kv_heads * a.group + qh] = some ? (M + __builtin_amdgcn_logf(L)) * LN2 : -INFINITY;
 }
+
+constexpr int PER_WAVE = 8;  // pieces that a wavefront joins as fast as four do
 
 // What a call's sizes make of it.
 struct Sizes {
@@ -1120,11 +1125,15 @@ void launch_attn(const AttnArgs& a, const Sizes& z, hipStream_t s) {
         hipLaunchKernelGGL((k_attn<CT, ND, MODE, true>), dim3(BLOCKS), dim3(THREADS), 0, s, a);
     else
         hipLaunchKernelGGL((k_attn<CT, ND, MODE, false>), dim3(own), dim3(THREADS), 0, s, a);
-    if (z.items * z.rows > 256)  // rows enough for a wavefront each
-        hipLaunchKernelGGL((k_attn_merge<ND, false>), dim3((unsigned)z.items, (unsigned)((z.rows + 3) / 4)), dim3(256), 0, s, a,
-                           z.cols);
-    else
-        hipLaunchKernelGGL((k_attn_merge<ND, true>), dim3((unsigned)z.items, (unsigned)z.rows), dim3(1024), 0, s, a, z.cols);
+    // a row's pieces at most, where they are dealt evenly
+    const int64_t pieces = a.own_waves / z.items + (a.prefix ? 2 * BLOCKS * z.pre_nt * WAVES / (a.kv_heads * z.pre_tiles) : 0) + 2;
+    const auto rows = dim3((unsigned)z.items, (unsigned)z.rows);
+    if (pieces > 64 && z.items * z.rows <= 256)
+        hipLaunchKernelGGL((k_attn_merge<ND, 1024>), rows, dim3(1024), 0, s, a, z.cols);
+    else if (pieces > PER_WAVE && z.items * z.rows <= 2048)
+        hipLaunchKernelGGL((k_attn_merge<ND, 256>), rows, dim3(256), 0, s, a, z.cols);
+    else  // rows enough for a wavefront each, or little to join
+        hipLaunchKernelGGL((k_attn_merge<ND, 64>), dim3((unsigned)z.items, (unsigned)((z.rows + 3) / 4)), dim3(256), 0, s, a, z.cols);
 }
 
 template <int CT, int ND>
