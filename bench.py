@@ -205,7 +205,10 @@ def bench_dense(args, g):
     GEMV with the q8 of that in its launch) (config.shared_mlp_chain_us; the
     token with the fastest chain: config.us_per_token_with_shared_chain), and
     the chain behind the last layer: its norm with the q8 of the result, lm_head
-    and the draw of a token (config.head_chain_us)."""
+    and the draw of a token (config.head_chain_us). config.attention_chain_us:
+    one new token behind 4096 others from qkv to o_proj: the qkv GEMV, its keys
+    and values into the quantised cache, attention over it, q8 and o_proj, on
+    rotating weights and caches."""
     import numpy as np
     import torch
     import ft_hip
@@ -323,6 +326,54 @@ def bench_dense(args, g):
     torch.cuda.synchronize()
     floor_us = ev0.elapsed_time(ev1) * 1000.0 / args.steps
     log(f"[dense] launch floor (1 x 32 matrix): {floor_us:.2f} us/launch")
+    # from the normed row to o_proj's output: moe_synth.CachedAttention between the two projections, one token of one
+    # sequence of 4097, 16 query heads on 8 key heads of 256
+    heads, kv, dim, page, ctx = 16, 8, 256, 64, 4097
+    (qr, H), (_, ok) = moe_synth.DENSE["qkv"], moe_synth.DENSE["o_proj"]
+    qb, ob = qr * ft_hip.row_bytes(H, ft_hip.LAYOUT_Q4R), H * ft_hip.row_bytes(ok, ft_hip.LAYOUT_Q4R)
+    n_copies = max(2, -(-1_500_000_000 // (qb + ob)))
+    Wq = moe_synth.dense_weights(g, "qkv", copies=n_copies, device=dev)
+    Wo = moe_synth.dense_weights(g, "o_proj", copies=n_copies, device=dev)
+    pages = -(-ctx // page)
+    layers = [moe_synth.CachedAttention(g, heads, kv, dim, pages, page, 1, device=dev) for _ in range(16)]
+    past = torch.from_numpy(np.random.default_rng(13).standard_normal((ctx - 1, qr)).astype(np.float32)).to(dev)
+    where = torch.from_numpy(np.random.default_rng(14).permutation(pages).astype(np.int32)).to(dev)
+    at = torch.arange(ctx, device=dev)
+    slots_all = (where.long()[at // page] * page + at % page).int()
+    for a in layers:
+        a.write(past, slots_all, ctx - 1)
+    lens = torch.full((1,), ctx, dtype=torch.int32, device=dev)
+    last, table = slots_all[-1:].clone(), where.view(1, -1)
+    xq = torch.from_numpy(np.random.default_rng(15).standard_normal(H).astype(np.float32)).to(dev)
+    q8x = torch.zeros(H // 32 * 40, dtype=torch.uint8, device=dev)
+    q8o = torch.zeros(ok // 32 * 40, dtype=torch.uint8, device=dev)
+    qkv, yo = torch.zeros((1, qr), device=dev), torch.zeros(H, device=dev)
+    torch.cuda.synchronize()
+
+    def attend(n):
+        for i in range(n):
+            c, a = i % n_copies, layers[i % len(layers)]
+            g.quantize_q8(xq, 0, q8x, H, 1, stream=stream)
+            g.gemv_grouped_slots(Wq[c * qb:(c + 1) * qb], 0, 0, slots, None, 1, q8x, 0, qkv, qr, qr, H, stream=stream)
+            row = a.run(qkv, last, table, lens, 1, stream=stream)
+            g.quantize_q8(row, 0, q8o, ok, 1, stream=stream)
+            g.gemv_grouped_slots(Wo[c * ob:(c + 1) * ob], 0, 0, slots, None, 1, q8o, 0, yo, H, H, ok, stream=stream)
+
+    with torch.cuda.stream(stream):
+        attend(args.warmup)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            attend(args.steps)
+        graph.replay()
+        ev0, ev1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        ev0.record(stream)
+        graph.replay()
+        ev1.record(stream)
+    torch.cuda.synchronize()
+    attention_us = ev0.elapsed_time(ev1) * 1000.0 / args.steps
+    log(f"[dense] qkv, cache, attention over {ctx} tokens, o_proj: {attention_us:.2f} us")
+    del Wq, Wo, layers, past, graph
+    torch.cuda.empty_cache()
     # from the residual stream to the next token: the last norm with its q8, lm_head, the draw (top-k 64, top-p 0.95)
     V, H = moe_synth.DENSE["lm_head"]
     head = moe_synth.VocabHead(g, moe_synth.dense_weights(g, "lm_head", device=dev), torch.ones(H, device=dev), V, H, 1)
@@ -363,7 +414,7 @@ def bench_dense(args, g):
         "config": {"workload": "dense q4r GEMVs of the Gemma-4-26B-A4B-shaped decode step, batch 1",
                    "name": "dense", "gemvs": per, "layers": L, "gemv_lanes": args.gemv_lanes or "auto",
                    "launch_floor_us": round(floor_us, 3), "shared_mlp_chain_us": chains,
-                   "head_chain_us": round(head_us, 2),
+                   "head_chain_us": round(head_us, 2), "attention_chain_us": round(attention_us, 2),
                    "us_per_token_with_shared_chain": round(tok_chain_us, 2)},
         "achieved_GBps": round(tok_bytes / (tok_us * 1e-6) / 1e9, 1),
         "hbm_frac": round(tok_bytes / (tok_us * 1e-6) / 1e9 / HBM_PEAK_GBPS, 4),

@@ -363,10 +363,44 @@ def _current(g, stream):
     return torch.cuda.stream(torch.cuda.current_stream(g.device) if stream is None else stream)
 
 
+class CachedAttention:
+    """What stands between the dense projections qkv and o_proj: the new tokens' keys and values go into a quantised
+    cache, and their queries attend over it. The cache has n_pages pages of page_tokens tokens; which pages a sequence
+    has is the caller's to say. Up to max_seqs sequences with n_q new tokens each."""
+
+    def __init__(self, gemv, heads, kv_heads, head_dim, n_pages, page_tokens, max_seqs, n_q=1,
+                 cache_type=ft_hip.KV_I8, window=0, device="cuda"):
+        self.g, self.heads, self.kv_heads, self.head_dim, self.n_q = gemv, heads, kv_heads, head_dim, n_q
+        self.page_tokens, self.cache_type, self.window = page_tokens, cache_type, window
+        self.cache = torch.zeros((n_pages, gemv.kv_page_bytes(page_tokens, kv_heads, head_dim)), dtype=torch.uint8,
+                                 device=device)
+        self.out = torch.empty((max_seqs * n_q, heads * head_dim), dtype=torch.float32, device=device)
+        self.ws = torch.empty(gemv.attention_workspace_bytes(max_seqs, n_q, heads, kv_heads, head_dim),
+                              dtype=torch.uint8, device=device)
+
+    def write(self, qkv, slots, n, stream=None):
+        """Keys and values of n rows of projections [n, (heads + 2 kv_heads) head_dim] into slots[n]."""
+        q, kv = self.heads * self.head_dim, self.kv_heads * self.head_dim
+        self.g.kv_write(qkv[:, q:q + kv], qkv[:, q + kv:q + 2 * kv], slots, self.cache, n, self.kv_heads, self.head_dim,
+                        self.page_tokens, self.cache_type, stream=stream)
+
+    def run(self, qkv, slots, tables, lens, n_seqs, prefix=None, prefix_len=None, stream=None):
+        """Attention of n_seqs sequences' newest tokens, whose rows of projections are qkv: they are written first;
+        lens counts them. f32 rows [n_seqs n_q, heads head_dim]."""
+        with _current(self.g, stream):
+            self.write(qkv, slots, n_seqs * self.n_q)
+            self.g.attention(qkv[:, :self.heads * self.head_dim], self.cache, tables, lens, self.out, self.ws, n_seqs,
+                             self.heads, self.kv_heads, self.head_dim, self.page_tokens, self.head_dim ** -0.5,
+                             n_q=self.n_q, window=self.window, prefix=prefix, prefix_len=prefix_len,
+                             cache_type=self.cache_type)
+        return self.out[:n_seqs * self.n_q]
+
+
 class VocabHead:
     """From the residual stream to the next tokens: the last norm with its q8
-    blocks, the vocabulary head's q4r GEMV (one row set for every sequence) and
-    the draw, for up to max_seqs sequences. weights: [vocab] q4r rows of hidden."""
+    blocks, the vocabulary head's q4r GEMV (one row set for every sequence),
+    on request the requests' rules (adjust_logits), and the draw, for up to
+    max_seqs sequences. weights: [vocab] q4r rows of hidden."""
 
     def __init__(self, gemv, weights, norm_w, vocab, hidden, max_seqs, eps=1e-6):
         self.g, self.weights, self.norm_w, self.vocab, self.H, self.eps = gemv, weights, norm_w, vocab, hidden, eps
@@ -378,12 +412,16 @@ class VocabHead:
         self.logprobs = torch.empty(max_seqs, dtype=torch.float32, device=dev)
         self.ws = torch.empty(gemv.sample_tokens_workspace_bytes(vocab, max_seqs), dtype=torch.uint8, device=dev)
 
-    def run(self, branch, residual, n_seqs, u, temperature=None, top_k=None, top_p=None, min_p=None, stream=None):
-        """tokens (and log probabilities) of n_seqs sequences from residual + branch (residual None: branch alone)."""
+    def run(self, branch, residual, n_seqs, u, temperature=None, top_k=None, top_p=None, min_p=None, stream=None,
+            rules=None):
+        """tokens (and log probabilities) of n_seqs sequences from residual + branch (residual None: branch alone).
+        rules: keyword arguments of adjust_logits, applied in place to the logits."""
         with _current(self.g, stream):
             self.g.add_rmsnorm(branch, self.norm_w, self.H, n_seqs, self.eps, residual=residual, q8=self.q8)
             self.g.gemv_q4r_idx(self.weights, 0, 0, self.slots, None, n_seqs, self.q8, self.H // 32, self.logits,
                                 self.vocab, self.vocab, self.H)
+            if rules:
+                self.g.adjust_logits(self.logits, self.logits, self.vocab, n_seqs, **rules)
             self.g.sample_tokens(self.logits, self.vocab, n_seqs, u, self.tokens, self.ws, temperature, top_k, top_p,
                                  min_p, self.logprobs)
         return self.tokens[:n_seqs], self.logprobs[:n_seqs]
