@@ -314,42 +314,31 @@ struct Attend {
     float base[NT], l[NT];  // the maximum that weights are taken against, and their sum
     float limit[NT];        // over the base: scores above it raise the base; -FLT_MAX while there is none
     float from[NT];         // what a column's sums of products start from
-    float fac;              // of the products
+    float fac[NT];          // of a column's products
     float unit, inv_unit;   // the weights' unit: the values' largest scale so far as a power of two, over 2^8
     int lo[NT], hi[NT];     // tokens that the column sees
     int all_lo, all_hi;     // that every column sees
     int tokens;             // that the list of pages holds
 
-    // The columns' queries times scale, in units of a power of two that the largest of them all gives.
+    // The columns' queries, each in units of a power of two that its largest value gives: one that is no number, or far
+    // larger, is no other's concern.
     __device__ __forceinline__ void load(const AttnArgs& a, const Column (&c)[NT]) {
         const int g = (threadIdx.x & 63) >> 4;
-        float x[2 * ND][8], top = 0.0f;
-        const auto fetch = [&](int n) {
-            const int64_t at = ((int64_t)c[n].seq * a.n_q + c[n].t) * a.q_stride + (int64_t)c[n].head * D + 16 * g;
-#pragma unroll
-            for (int i = 0; i < 2 * ND; ++i) load_q8<F32>(a.q, at + (i >> 1) * 64 + (i & 1) * 8, a.type == FT_TYPE_F16, x[i]);
-        };
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            fetch(n);
-            float most = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 2 * ND; ++i)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[i][e]));
-            if (c[n].live) top = fmaxf(top, most);
-        }
-        top = wave_max(top);
-        const int e2 = clampi(__float_as_int(top) >> 23, 14, 254);
-        const float up = __int_as_float((267 - e2) << 23);  // the largest comes to lie in [2^13, 2^14)
-        fac = a.scale * __int_as_float((e2 - 13) << 23) * (CT == FT_KV_I8 ? 0x1p24f : 1.0f);
         const float second = MODE == PACK && (threadIdx.x & 8) ? -1.0f : 0.0f;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            if constexpr (NT > 1) {  // again, from the cache: all columns' at once would not fit the registers
-                asm volatile("" ::: "memory");
-                fetch(n);
-            }
+            const int64_t at = ((int64_t)c[n].seq * a.n_q + c[n].t) * a.q_stride + (int64_t)c[n].head * D + 16 * g;
+            float x[2 * ND][8], top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 2 * ND; ++i) load_q8<F32>(a.q, at + (i >> 1) * 64 + (i & 1) * 8, a.type == FT_TYPE_F16, x[i]);
+#pragma unroll
+            for (int i = 0; i < 2 * ND; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[i][e]));
+            top = max_groups(top);
+            const int e2 = clampi(__float_as_int(top) >> 23, 14, 254);
+            const float up = __int_as_float((267 - e2) << 23);  // the largest comes to lie in [2^13, 2^14)
+            fac[n] = a.scale * __int_as_float((e2 - 13) << 23) * (CT == FT_KV_I8 ? 0x1p24f : 1.0f);
 #pragma unroll
             for (int i = 0; i < 2 * ND; ++i)
 #pragma unroll
@@ -400,16 +389,18 @@ struct Attend {
                     for (int p = 0; p < PARTS; ++p)
                         s[n][i + u & 1] = mfma(k[u], q[n][p][(i + u) >> 1], s[n][i + u & 1]);
         }
-        const f32x4 d[2] = {t.key_scale(0) * fac, t.key_scale(1) * fac};
+        const f32x4 dk[2] = {t.key_scale(0), t.key_scale(1)};
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
+            for (int x = 0; x < 2; ++x) {
+                const f32x4 d = dk[x] * fac[n];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     if constexpr (MODE == PACK) s[n][x][i] += other8(s[n][x][i]);
-                    s[n][x][i] = fmaf(s[n][x][i], d[x][i], -base[n]);
+                    s[n][x][i] = fmaf(s[n][x][i], d[i], -base[n]);
                 }
+            }
     }
 
     // Weights of a step at token `at` from its scores, and their sums with the values.
@@ -522,7 +513,7 @@ struct Attend {
         for (int n = 0; n < NT; ++n) {
             float f = g;
             const float up = max_groups(top[n]);
-            if (up > fminf(limit[n], 0.0f)) {
+            if (up > limit[n]) {  // by its own scores alone: a row's bits are the same whatever its neighbours are
                 const float d = __builtin_amdgcn_exp2f(-up);
                 if (limit[n] > 0.0f) f *= d, l[n] *= d;  // else there is nothing yet
                 limit[n] = 6.0f;

@@ -303,6 +303,28 @@ def test_large_and_small_queries(gemv, dtype):
     b.check()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n_q,prefix", [(1, 0), (1, 100), (4, 100), (4, 0)])
+def test_rows_of_other_sizes_do_not_reach_each_other(gemv, dtype, n_q, prefix):
+    """Queries far smaller and far larger than their neighbours', and rows that are no numbers: the others' results are
+    what they were, bit for bit."""
+    b = Batch(gemv, [60, 9, 100, 33, 20], 16, 2, 2, 64, I8, dtype, prefix=prefix, n_q=n_q, seed=40)
+    want, lse = b.check()
+    big = 6e4 if dtype == torch.float16 else 1e30
+    q = b.q.clone()
+    b.q[n_q] *= 1e-4 if dtype == torch.float16 else 1e-25
+    b.q[2 * n_q, 5] = big
+    b.q[3 * n_q] = float("inf")
+    b.q[4 * n_q, 130] = float("-inf")
+    out, got = b.run()
+    torch.cuda.synchronize()
+    same = [i for i in range(5 * n_q) if i not in (n_q, 2 * n_q, 3 * n_q, 4 * n_q)]
+    assert torch.equal(out[same], want[same]) and torch.equal(got[same], lse[same])
+    o, tol, _, _ = b.want()
+    assert np.all(np.abs(host(out.float())[n_q] - o[n_q]) <= tol[n_q])
+    assert torch.equal(out[4 * n_q, :128], want[4 * n_q, :128]) and torch.equal(q[0], b.q[0])
+
+
 def test_nan_and_infinities_reach_those_who_see_them_alone(gemv):
     """Rows of NaN in the cache (what a NaN leaves there) in front of a window, behind a query, and in sight."""
     b = Batch(gemv, [100, 100, 100], 16, 1, 2, 64, E4M3, torch.float32, n_q=3, seed=9)
