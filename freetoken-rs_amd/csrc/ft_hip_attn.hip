@@ -129,12 +129,13 @@ __device__ __forceinline__ half8 widen8(uint32_t lo, uint32_t hi) {
     return half8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
-// Eight keys' dimensions. i8's byte q + 128 as it is makes a subnormal f16 of (q + 128) 2^-24, which the products take
-// exactly; what the 128 adds to a sum of products is the same for all keys, and the sum starts from less than 0 by it
-// (Attend::from). Values are not taken so: over many tokens their sum may be far smaller than the weights' times 128.
-template <int CT>
+// Eight keys' dimensions. Where q is of 16 bits, i8's byte q + 128 as it is makes a subnormal f16 of (q + 128) 2^-24,
+// which the products take exactly; what the 128 adds to a sum of products is the same for all keys, and the sum starts
+// from less than 0 by it (Attend::from). The sum is larger for it and its roundings are: f32 rows would lose half a digit
+// (64 sequences of up to 4096 tokens 3.0e-6 off against 0.4e-6), and over many tokens values would lose more.
+template <int CT, bool F32>
 __device__ __forceinline__ half8 widen_k(uint32_t lo, uint32_t hi) {
-    if constexpr (CT == FT_KV_I8) {
+    if constexpr (CT == FT_KV_I8 && !F32) {
         const u32x4 w = {__builtin_amdgcn_perm(0, lo, 0x0C010C00u), __builtin_amdgcn_perm(0, lo, 0x0C030C02u),
                          __builtin_amdgcn_perm(0, hi, 0x0C010C00u), __builtin_amdgcn_perm(0, hi, 0x0C030C02u)};
         return __builtin_bit_cast(half8, w);
@@ -268,8 +269,8 @@ struct Step {
         __device__ __forceinline__ void nowhere() { lane16 = lane64 = 0; }
     };
     // Operands of the products: keys 64 c + 16 g + 8 h on of tile x, values 64 c + 4 r + j of both tiles.
-    template <int CT>
-    __device__ __forceinline__ half8 key(int x, int c, int h) const { return widen_k<CT>(k[x][c][2 * h], k[x][c][2 * h + 1]); }
+    template <int CT, bool F32>
+    __device__ __forceinline__ half8 key(int x, int c, int h) const { return widen_k<CT, F32>(k[x][c][2 * h], k[x][c][2 * h + 1]); }
     template <int CT>
     __device__ __forceinline__ half8 value(int c, int j) const { return widen8<CT>(v[0][c][j], v[1][c][j]); }
     __device__ __forceinline__ f32x4 key_scale(int x) const { return dk[x]; }
@@ -338,7 +339,7 @@ struct Attend {
             top = max_groups(top);
             const int e2 = clampi(__float_as_int(top) >> 23, 14, 254);
             const float up = __int_as_float((267 - e2) << 23);  // the largest comes to lie in [2^13, 2^14)
-            fac[n] = a.scale * __int_as_float((e2 - 13) << 23) * (CT == FT_KV_I8 ? 0x1p24f : 1.0f);
+            fac[n] = a.scale * __int_as_float((e2 - 13) << 23) * (CT == FT_KV_I8 && !F32 ? 0x1p24f : 1.0f);
 #pragma unroll
             for (int i = 0; i < 2 * ND; ++i)
 #pragma unroll
@@ -353,7 +354,7 @@ struct Attend {
                 }
             // keys come as (q + 128) 2^-24 (widen_k): what the 128 is worth, by products with it
             f32x4 worth = {0.0f, 0.0f, 0.0f, 0.0f};
-            if constexpr (CT == FT_KV_I8) {
+            if constexpr (CT == FT_KV_I8 && !F32) {
                 const u32x4 k = {0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};  // f16 of -128 2^-24
                 const half8 minus = __builtin_bit_cast(half8, k);
 #pragma unroll
@@ -379,7 +380,7 @@ struct Attend {
             constexpr int BATCH = Tiles::BATCH;
             half8 k[BATCH];
 #pragma unroll
-            for (int u = 0; u < BATCH; ++u) k[u] = t.template key<CT>(i + u & 1, (i + u) >> 2, (i + u) >> 1 & 1);
+            for (int u = 0; u < BATCH; ++u) k[u] = t.template key<CT, F32>(i + u & 1, (i + u) >> 2, (i + u) >> 1 & 1);
             if constexpr (Tiles::FAR) __builtin_amdgcn_sched_barrier(0);  // read together, not each where it is used
 #pragma unroll
             for (int u = 0; u < BATCH; ++u)
@@ -460,6 +461,8 @@ struct Attend {
                         const float p = __builtin_amdgcn_exp2f(s[n][x][i + e]);
                         l[n] += p;
                         v[e] = p * dv[x][i + e];
+                        // the product as rounded, or hi would round it once and lo be the rest of another hi
+                        if constexpr (F32) asm("" : "+v"(v[e]));
                     }
                     const half2 h = __builtin_convertvector(v, half2);
 #pragma unroll
@@ -657,7 +660,7 @@ struct Wide {
     half8 k[2][ND][2][64], v[ND][4][64];
     f32x4 dk[2][4], dv[2][4];
     int has[2];
-    template <int CT>
+    template <int CT, bool F32>
     __device__ __forceinline__ half8 key(int x, int c, int h) const { return k[x][c][h][threadIdx.x & 63]; }
     template <int CT>
     __device__ __forceinline__ half8 value(int c, int j) const { return v[c][j][threadIdx.x & 63]; }
@@ -667,7 +670,7 @@ struct Wide {
 };
 
 // A wavefront's share of two tiles on their way: the keys (waves 0 and 1) or values (2 and 3) of one of them.
-template <int CT, int ND>
+template <int CT, int ND, bool F32>
 struct Share {
     static constexpr int D = 64 * ND;
     u32x4 raw[ND];
@@ -691,7 +694,7 @@ struct Share {
 #pragma unroll
             for (int c = 0; c < ND; ++c)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) to.k[x][c][h][lane] = widen_k<CT>(raw[c][2 * h], raw[c][2 * h + 1]);
+                for (int h = 0; h < 2; ++h) to.k[x][c][h][lane] = widen_k<CT, F32>(raw[c][2 * h], raw[c][2 * h + 1]);
             if (lane < 16) reinterpret_cast<float*>(to.dk[x])[lane] = scale;
             if (lane == 0) to.has[x] = has;
             return;
@@ -761,7 +764,7 @@ __device__ __forceinline__ void attend_prefix(const AttnArgs& a, const Prefix& p
         }
         const int first = pre.tile0 + 2 * s0;
         tiles.settle(a, head);
-        Share<CT, ND> share;
+        Share<CT, ND, MODE != HALF> share;
         share.load(a, tiles, head, first, s0 < s1);
         w.load(a, c);
         __syncthreads();  // the last piece's tiles are done with

@@ -329,6 +329,7 @@ __global__ __launch_bounds__(256) void k_kv_read(KvArgs a, bool vec) {
                         : (e & 3) == 2 ? __builtin_amdgcn_cvt_f32_fp8((int)w, 2)
                                        : __builtin_amdgcn_cvt_f32_fp8((int)w, 3);
                 v[e] = q * d[u];
+                if constexpr (TYPE == FT_TYPE_F16) asm("" : "+v"(v[e]));  // as rounded to f32, not once to f16 in an instruction
             }
             if (live) store_some<TYPE, W>(const_cast<void*>(value ? a.v : a.k), to + 16 * W * i, vec, v);
         }

@@ -303,6 +303,26 @@ def test_large_and_small_queries(gemv, dtype):
     b.check()
 
 
+@pytest.mark.parametrize("kind", [I8, E4M3])
+@pytest.mark.parametrize("n,group,prefix", [(200, 4, 0), (100, 20, 0), (150, 6, 60)])
+def test_each_weight_of_f32_queries(gemv, kind, n, group, prefix):
+    """Values of one number at a dimension of their own, so that each output is a single token's weight: with a small
+    scale the bound is a few 2^-16 of it, and a weight that loses its second half in one of thousands shows."""
+    lens = [4] * n if prefix else [60 + i % 5 for i in range(n)]
+    b = Batch(gemv, lens, 16, 1, group, 64, kind, torch.float32, prefix=prefix, seed=60)
+    rng = np.random.default_rng(61)
+    rows = [(b.places(b.tables[i], x), np.arange(x) + prefix) for i, x in enumerate(lens)]
+    if prefix:
+        rows.append((b.places(b.prefix, prefix), np.arange(prefix)))
+    slots = np.concatenate([r[0] for r in rows]).astype(np.int32)
+    v = np.zeros((len(slots), 64), np.float32)
+    v[np.arange(len(slots)), np.concatenate([r[1] for r in rows]) % 64] = rng.uniform(0.5, 2.0, len(slots))
+    k = rng.standard_normal((len(slots), 64)).astype(np.float32)
+    t = lambda a: torch.from_numpy(a).to(DEV)  # noqa: E731
+    gemv.kv_write(t(k), t(v), t(slots), b.cache, len(slots), 1, 64, 16, kind)
+    b.check(scale=2.0 ** -6)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n_q,prefix", [(1, 0), (1, 100), (4, 100), (4, 0)])
 def test_rows_of_other_sizes_do_not_reach_each_other(gemv, dtype, n_q, prefix):

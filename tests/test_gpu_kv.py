@@ -345,6 +345,22 @@ def test_replayed_on_new_tokens_and_on_another_stream(gemv):
             assert np.array_equal(host(got).reshape(n, heads, dim), x)
 
 
+@pytest.mark.parametrize("kind", [I8, E4M3])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_narrow_rows_are_rounded_from_f32(gemv, kind, dtype):
+    """f32(q d) and then the type, where one rounding of q d would now and then be another number."""
+    n, heads, dim = 5000, 4, 64
+    x = (torch.randn(2, n, heads * dim, generator=torch.Generator().manual_seed(5)) * 3.0).to(DEV)
+    layout, slots = Layout(16, heads, dim), torch.arange(n, dtype=torch.int32, device=DEV)
+    cache = torch.zeros(313 * heads * layout.block, dtype=torch.uint8, device=DEV)
+    gemv.kv_write(x[0], x[1], slots, cache, n, heads, dim, 16, kind)
+    out = [torch.empty_like(x[0], dtype=dtype) for _ in range(2)]
+    gemv.kv_read(cache, slots, *out, n, heads, dim, 16, kind)
+    torch.cuda.synchronize()
+    for got, want in zip(out, layout.get(host(cache), np.arange(n), kind)):  # 8 bits times 24: exact in 64 bits
+        assert torch.equal(got.cpu(), torch.from_numpy(want.reshape(n, -1).astype(np.float32)).to(dtype))
+
+
 def test_no_tokens(gemv):
     cache = torch.full((2 * 16 * 136,), 9, dtype=torch.uint8, device=DEV)
     none = torch.empty((0, 64), device=DEV)
