@@ -22,9 +22,21 @@
 // head by head, cut into equal lengths, one a wavefront: no sequence is longer
 // than another for it, and a single long one is worked on by the whole device.
 // What it leaves of a row that it has not seen whole goes to the workspace and
-// k_attn_merge joins the pieces. The prefix is a line of its own, of which a
-// wavefront takes a piece for 16 rows, whichever sequence they belong to: read
-// once per 16 rows of the batch, and by neighbours at the same time.
+// k_attn_merge joins the pieces. The prefix is a line of its own, cut likewise
+// into a piece for each workgroup that the own tokens leave: its four wavefronts
+// take 16 rows or more each, whichever sequence they belong to, on tiles that they
+// widen once for all of them in LDS. By wavefronts alone, each widening for itself,
+// 64 queries behind 32768 tokens took 167 us for 118.
+//
+// What bounds it, own and joining kernels in turn (an MI355X that copies 5.1 TB/s
+// and multiplies 1110 TFLOP/s in f16): one sequence of 131071 tokens on 8 heads of
+// 128, 277 MB, 54 + 9 us, 5.2 TB/s in the first: the cache's bytes, then the
+// joining of 256 pieces a row. 64 sequences of up to 4096 on 8 heads of 256, f32:
+// 75 + 6 us, bytes and the widening beside them. One of 777: 9 + 4.5 us, the time
+// of two launches and of three dependent reads (length, page, tokens) in each.
+// 256 queries of 64 heads of 128 behind 16390: 247 + 18 us, where the products
+// alone are 125: the softmax's vector instructions, which a wavefront's products
+// do not hide, and rows of a few hundred own tokens.
 
 #include "ft_device.hpp"
 #include "ft_kv.hpp"
@@ -52,7 +64,7 @@ constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.693147180559945309417f;
 
 enum { HALF, PACK, SPLIT };
 
-constexpr int BLOCKS = 512;  // workgroups at most, two on each CU
+constexpr int BLOCKS = 512;  // workgroups at most, two on each CU; a third costs registers that do not fit (spills)
 
 // Where the parts of a call lie, in the workspace and else.
 struct AttnArgs {
@@ -73,7 +85,6 @@ struct AttnArgs {
     int pre_tiles, pre_nt;  // tiles of the batch's rows on a head, and of a wavefront's
     int window;
     float scale;     // times log2 e
-    float pre_cost;  // of a prefix step, in own ones
     // workspace: a word of how many pieces the prefix is cut into, descriptors of the own items, pieces
     int32_t* head;   // [0]: workgroups that the prefix is cut for
     int2* items;
@@ -131,8 +142,9 @@ __device__ __forceinline__ half8 widen8(uint32_t lo, uint32_t hi) {
 
 // Eight keys' dimensions. Where q is of 16 bits, i8's byte q + 128 as it is makes a subnormal f16 of (q + 128) 2^-24,
 // which the products take exactly; what the 128 adds to a sum of products is the same for all keys, and the sum starts
-// from less than 0 by it (Attend::from). The sum is larger for it and its roundings are: f32 rows would lose half a digit
-// (64 sequences of up to 4096 tokens 3.0e-6 off against 0.4e-6), and over many tokens values would lose more.
+// from less than 0 by it (Attend::from). f32 queries take the keys without the 128: its part of a sum is several times the
+// rest and so are the roundings, and their first halves' and second halves' products leave time for the widening (64
+// sequences of up to 4096 tokens 82 us with the 128, 75 without).
 template <int CT, bool F32>
 __device__ __forceinline__ half8 widen_k(uint32_t lo, uint32_t hi) {
     if constexpr (CT == FT_KV_I8 && !F32) {
@@ -620,8 +632,15 @@ struct Cuts {
 // first. 64 sequences of up to 4096 tokens 87 us, with 1 89 to 93, with 8 91; 256 of up to 300 28.5, 32 and 29.5.
 constexpr int START = 2;
 
-constexpr int MIN_STEPS = 2;  // of a wavefront's own steps, where there are more than FEW_STEPS in all
+// A wavefront's own steps at least, where there are more than FEW_STEPS in all. One sequence of 4096 tokens on 8 heads 17.0
+// us, with 1 step 19.1, with 4 19.4; 8 of up to 4096 23.3, 26.1 and 21.9. One of 777 12.6, with 2 steps 13.9.
+constexpr int MIN_STEPS = 2;
 constexpr int FEW_STEPS = 1024;
+
+// A prefix step of a workgroup in steps of a wavefront, by which the workgroups are dealt. 64 queries' 16 heads behind 8192
+// tokens 55.2 us, at 3 56.5, at 6 60.2; 32 queries' 64 heads behind 16390 with 2000 own tokens 63.4, 66.5 and 69.5; 16 behind
+// 32768 59.8, 59.9 and 69.2. 256 queries of 64 heads: 248, 250, 333.
+constexpr float PRE_COST = 4.0f;
 
 // The prefix as the batch sees it: its tokens, its first tile that a query may see and the steps from there.
 struct Prefix {
@@ -822,9 +841,9 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn(AttnArgs a) {
         const Prefix pre = prefix_of(a);
         if (pre.steps > 0) {
             alone = false;
-            // the workgroups are dealt by the steps; a prefix step is worth pre_cost own ones
+            // the workgroups are dealt by the steps; a prefix step is worth PRE_COST own ones
             const int blocks = gridDim.x, groups = a.kv_heads * ((a.pre_tiles + NT * WAVES - 1) / (NT * WAVES));
-            const float work = (float)pre.steps * (float)groups * a.pre_cost, all = work + (float)T;
+            const float work = (float)pre.steps * (float)groups * PRE_COST, all = work + (float)T;
             n_own = min(n_own, clampi((int)((float)T / all * (float)blocks + 0.5f), 1, blocks - 1));
             const int n_pre = min(blocks - n_own, (pre.steps + 1) / 2 * groups);
             if ((int)blockIdx.x >= n_own) {
@@ -1079,7 +1098,13 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void k_attn_merge(AttnArgs
     if (a.lse && t == 0) a.lse[token * a.kv_heads * a.group + qh] = some ? (M + __builtin_amdgcn_logf(L)) * LN2 : -INFINITY;
 }
 
-constexpr int PER_WAVE = 8;  // pieces that a wavefront joins as fast as four do
+// Threads that join a row: a wavefront where the rows fill the device or have few pieces, four where the device would be
+// empty (one sequence of 777 tokens 12.6 us of both kernels, by a wavefront 15.8; 8 of up to 4096 23.1 and 30.0; but 2048 rows
+// behind 16390 tokens 66.5 and 64.3, and one sequence of 97, of few pieces, 12.3 and 12.0), sixteen for a handful of rows of
+// many pieces (one sequence of 20000 30.7, by four 36.9; 16 rows of 32 pieces 13.5 by sixteen and 12.6 by
+// four; 1024 rows of over 64 67.0 and 56.5).
+constexpr int PER_WAVE = 16, PER_FOUR = 64;        // pieces
+constexpr int ROWS_FOUR = 1024, ROWS_SIXTEEN = 256;
 
 // What a call's sizes make of it.
 struct Sizes {
@@ -1122,11 +1147,11 @@ void launch_attn(const AttnArgs& a, const Sizes& z, hipStream_t s) {
     // a row's pieces at most, where they are dealt evenly
     const int64_t pieces = a.own_waves / z.items + (a.prefix ? 2 * BLOCKS * z.pre_nt * WAVES / (a.kv_heads * z.pre_tiles) : 0) + 2;
     const auto rows = dim3((unsigned)z.items, (unsigned)z.rows);
-    if (pieces > 64 && z.items * z.rows <= 256)
+    if (pieces > PER_FOUR && z.items * z.rows <= ROWS_SIXTEEN)
         hipLaunchKernelGGL((k_attn_merge<ND, 1024>), rows, dim3(1024), 0, s, a, z.cols);
-    else if (pieces > PER_WAVE && z.items * z.rows <= 2048)
+    else if (pieces > PER_WAVE && z.items * z.rows <= ROWS_FOUR)
         hipLaunchKernelGGL((k_attn_merge<ND, 256>), rows, dim3(256), 0, s, a, z.cols);
-    else  // rows enough for a wavefront each, or little to join
+    else
         hipLaunchKernelGGL((k_attn_merge<ND, 64>), dim3((unsigned)z.items, (unsigned)((z.rows + 3) / 4)), dim3(256), 0, s, a, z.cols);
 }
 
@@ -1246,7 +1271,6 @@ extern "C" int ft_hip_attention(ft_hip_ctx* ctx, void* stream, const void* q, in
     a.n_seqs = (int)n_seqs, a.n_q = (int)n_q, a.kv_heads = (int)n_kv_heads, a.group = (int)(n_heads / n_kv_heads), a.type = type;
     a.row_tiles = z.row_tiles, a.pre_tiles = z.pre_tiles, a.pre_nt = z.pre_nt, a.rows = z.rows, a.window = (int)window;
     a.scale = scale * LOG2E;
-    a.pre_cost = 3.0f;
     a.head = reinterpret_cast<int32_t*>(ws), a.items = reinterpret_cast<int2*>(ws + z.at_items);
     a.own = reinterpret_cast<float*>(ws + z.at_own), a.pre = reinterpret_cast<float*>(ws + z.at_pre);
     a.own_waves = (int)(cap_steps < z.waves ? cap_steps : z.waves);

@@ -141,22 +141,14 @@ __global__ __launch_bounds__(THREADS) void k_adjust(LogitArgs a) {
                 const int k = t + u * THREADS;
                 first[u] = false, sum[u] = 0.0f;
                 if (k >= listed) continue;
-                const int at = list_at[k];
-                int last = -1;
-                while (true) {  // the token's entries by rising index, a look through the list for each
-                    int best = -1;
-                    for (int j = 0; j < listed; ++j)
-                        if (list_at[j] == at && list_i[j] > last && (best < 0 || list_i[j] < list_i[best])) best = j;
-                    if (best < 0) break;
-                    if (last < 0) {
-                        first[u] = best == k;
-                        if (!first[u]) break;
-                        sum[u] = list_add[best];
-                    } else {
-                        sum[u] += list_add[best];
-                    }
-                    last = list_i[best];
-                }
+                const int at = list_at[k], i0 = list_i[k];
+                first[u] = true;
+                for (int j = 0; j < listed; ++j)
+                    if (list_at[j] == at && list_i[j] < i0) first[u] = false;
+                if (!first[u]) continue;
+                sum[u] = list_add[k];
+                for (int i = i0 + 1; i < a.n_bias; ++i)
+                    if (ids[i] == v0 + at) sum[u] += adds[i];
             }
             __syncthreads();
 #pragma unroll

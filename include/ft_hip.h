@@ -176,8 +176,10 @@ int ft_hip_kv_read(ft_hip_ctx* ctx, void* stream, const void* cache, int cache_t
  * [n_seqs * n_q][n_heads] or NULL. Products are exact in their 8 bits and, for
  * q and the weights, 11 bits where `type` is f16 or bf16 (q itself exact) and 22
  * where it is f32, but not below 2^-32 of the largest weight times the largest
- * scale of the values that a row's piece has met; sums are f32. The same call
- * gives the same bits.
+ * scale of the values that a row's piece has met; sums are f32. |scale| times a
+ * row's largest |q| is to lie between 2^-100 and 2^100 (or be 0): beyond, its
+ * factors may leave f32's range before its scores do. The same call gives the
+ * same bits.
  * workspace: device scratch of ft_hip_attention_workspace_bytes() bytes (0 for a
  * bad shape), 16-byte aligned, any content, for one call at a time. out, lse and
  * the workspace may not overlap an input or each other. n_seqs 0: nothing is

@@ -156,6 +156,28 @@ def test_write_and_read(gemv, kind, dtype, page, heads, dim, n):
         assert np.all(np.abs(got - x) <= lost * (1 + 2.0 ** -20) + (half + 2.0 ** -23) * np.abs(x) + least)
 
 
+@pytest.mark.parametrize("dim,dtype,kind", [(64, torch.float32, E4M3), (64, torch.float16, I8), (64, torch.bfloat16, E4M3),
+                                            (128, torch.float16, E4M3), (128, torch.float32, I8), (256, torch.bfloat16, I8)])
+def test_many_rows_with_parts_left_over(gemv, dim, dtype, kind):
+    """65604 rows: four of a token's 142 parts a wavefront, and two at its end."""
+    rng = np.random.default_rng(dim)
+    page, heads, n = 32, 71, 924
+    pages = n // page + 2
+    order = rng.permutation(pages)
+    at = np.arange(2, n + 2)
+    slots = (order[at // page] * page + at % page).astype(np.int32)
+    slots[[5, 100, 101]] = -1, pages * page, 2 ** 31 - 1
+    k, v = rows_of(rng, n, heads * dim, dtype), rows_of(rng, n, heads * dim, dtype)
+    cache = check_write(gemv, k, v, slots, page, heads, dim, kind, pages)
+    ko, vo = torch.full_like(k, 9.0), torch.full_like(v, 9.0)
+    gemv.kv_read(cache, torch.from_numpy(slots).to(DEV), ko, vo, n, heads, dim, page, kind)
+    torch.cuda.synchronize()
+    live = (slots >= 0) & (slots < pages * page)
+    for got, want in zip((ko, vo), Layout(page, heads, dim).get(host(cache), slots[live], kind)):
+        exact = torch.from_numpy(want.reshape(int(live.sum()), -1).astype(np.float32)).to(dtype)
+        assert torch.equal(got.cpu()[live], exact) and bool((got.cpu()[~live] == 9.0).all())
+
+
 @pytest.mark.parametrize("kind", [I8, E4M3])
 def test_scattered_skipped_and_out_of_range_slots(gemv, kind):
     rng = np.random.default_rng(4)
