@@ -1186,7 +1186,7 @@ extern "C" size_t ft_hip_attention_workspace_bytes(int64_t n_seqs, int64_t n_q, 
     return f.bytes > h.bytes ? f.bytes : h.bytes;
 }
 
-extern "C" int ft_hip_attention(ft_hip_ctx* ctx, void* stream, const void* q, int64_t q_stride, int type,
+extern "C" int ft_hip_attention(ft_hip_ctx* ctx, void* stream, const void* q, int64_t q_stride, int q_type,
                                 const void* cache, int cache_type, int64_t n_pages, int64_t page_tokens,
                                 int64_t n_kv_heads, int64_t head_dim, const int32_t* tables, int64_t table_stride,
                                 int64_t table_pages, const int32_t* lens, const int32_t* prefix, int64_t prefix_pages,
@@ -1199,8 +1199,8 @@ extern "C" int ft_hip_attention(ft_hip_ctx* ctx, void* stream, const void* q, in
                     (long long)page_tokens, (long long)n_kv_heads, (long long)head_dim);
     if (!kv_pages_fit(n_pages, page_tokens))
         return fail(FT_HIP_E_SHAPE, "attention: n_pages=%lld not in [1, 2^31 tokens]", (long long)n_pages);
-    if (type != FT_TYPE_F32 && type != FT_TYPE_F16 && type != FT_TYPE_BF16)
-        return fail(FT_HIP_E_INVALID, "attention: type=%d is no FT_TYPE", type);
+    if (q_type != FT_TYPE_F32 && q_type != FT_TYPE_F16 && q_type != FT_TYPE_BF16)
+        return fail(FT_HIP_E_INVALID, "attention: q_type=%d is no FT_TYPE", q_type);
     if (cache_type != FT_KV_I8 && cache_type != FT_KV_E4M3)
         return fail(FT_HIP_E_INVALID, "attention: cache_type=%d is no FT_KV", cache_type);
     if (n_seqs < 0 || n_seqs > MAX_SEQS)
@@ -1210,7 +1210,7 @@ extern "C" int ft_hip_attention(ft_hip_ctx* ctx, void* stream, const void* q, in
         return fail(FT_HIP_E_SHAPE, "attention: n_heads=%lld not in [1, 4096] or no multiple of n_kv_heads=%lld", (long long)n_heads,
                     (long long)n_kv_heads);
     Sizes z;
-    if (!sizes_of(z, type == FT_TYPE_F32, n_seqs, n_q, n_heads, n_kv_heads, head_dim))
+    if (!sizes_of(z, q_type == FT_TYPE_F32, n_seqs, n_q, n_heads, n_kv_heads, head_dim))
         return fail(FT_HIP_E_SHAPE, "attention: n_seqs=%lld of n_q=%lld queries on n_heads=%lld are too many for one call", (long long)n_seqs,
                     (long long)n_q, (long long)n_heads);
     if (table_pages < 1 || table_pages > INT32_MAX / page_tokens)
@@ -1232,7 +1232,7 @@ extern "C" int ft_hip_attention(ft_hip_ctx* ctx, void* stream, const void* q, in
                     (long long)table_pages);
     if (window < 0 || window > INT32_MAX) return fail(FT_HIP_E_SHAPE, "attention: window=%lld not in [0, 2^31)", (long long)window);
     if (!std::isfinite(scale)) return fail(FT_HIP_E_SHAPE, "attention: scale is not finite");
-    const int64_t width = n_heads * head_dim, size = type == FT_TYPE_F32 ? 4 : 2;
+    const int64_t width = n_heads * head_dim, size = q_type == FT_TYPE_F32 ? 4 : 2;
     if (q_stride < width || q_stride > (int64_t)1 << 36 || out_stride < width || out_stride > (int64_t)1 << 36)
         return fail(FT_HIP_E_SHAPE, "attention: q_stride or out_stride out of range");
     if (!aligned(q, size) || !aligned(out, size) || !aligned(cache, 16) || !aligned(tables, 4) || !aligned(lens, 4) ||
@@ -1268,7 +1268,7 @@ extern "C" int ft_hip_attention(ft_hip_ctx* ctx, void* stream, const void* q, in
     a.cache = static_cast<const uint8_t*>(cache), a.tables = tables, a.table_stride = table_stride, a.lens = lens;
     a.prefix = prefix, a.prefix_len = prefix_len, a.prefix_pages = (int)prefix_pages;
     a.table_pages = (int)table_pages, a.n_pages = (int)n_pages, a.page_shift = shift;
-    a.n_seqs = (int)n_seqs, a.n_q = (int)n_q, a.kv_heads = (int)n_kv_heads, a.group = (int)(n_heads / n_kv_heads), a.type = type;
+    a.n_seqs = (int)n_seqs, a.n_q = (int)n_q, a.kv_heads = (int)n_kv_heads, a.group = (int)(n_heads / n_kv_heads), a.type = q_type;
     a.row_tiles = z.row_tiles, a.pre_tiles = z.pre_tiles, a.pre_nt = z.pre_nt, a.rows = z.rows, a.window = (int)window;
     a.scale = scale * LOG2E;
     a.head = reinterpret_cast<int32_t*>(ws), a.items = reinterpret_cast<int2*>(ws + z.at_items);

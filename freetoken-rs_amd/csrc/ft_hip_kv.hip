@@ -396,7 +396,7 @@ void launch_kv(const KvArgs& a, int cache_type, int type, int nd, bool vec, hipS
 // What both entry points check and do; rows: the tensors beside the cache.
 template <bool WRITE>
 int kv_call(const char* what, ft_hip_ctx* ctx, void* stream, const void* k, int64_t k_stride, const void* v,
-            int64_t v_stride, int type, const int32_t* slots, const void* cache, int cache_type, int64_t n_pages,
+            int64_t v_stride, int row_type, const int32_t* slots, const void* cache, int cache_type, int64_t n_pages,
             int64_t page_tokens, int64_t n_heads, int64_t head_dim, int64_t n) {
     clear_error();
     if (!kv_dims_fit(page_tokens, n_heads, head_dim))
@@ -405,14 +405,14 @@ int kv_call(const char* what, ft_hip_ctx* ctx, void* stream, const void* k, int6
     if (!kv_pages_fit(n_pages, page_tokens))
         return fail(FT_HIP_E_SHAPE, "%s: n_pages=%lld not in [1, 2^31 tokens]", what, (long long)n_pages);
     if (n < 0 || n > 1 << 20) return fail(FT_HIP_E_SHAPE, "%s: n=%lld not in [0, 2^20]", what, (long long)n);
-    if (type != FT_TYPE_F32 && type != FT_TYPE_F16 && type != FT_TYPE_BF16)
-        return fail(FT_HIP_E_INVALID, "%s: type=%d is no FT_TYPE", what, type);
+    if (row_type != FT_TYPE_F32 && row_type != FT_TYPE_F16 && row_type != FT_TYPE_BF16)
+        return fail(FT_HIP_E_INVALID, "%s: row_type=%d is no FT_TYPE", what, row_type);
     if (cache_type != FT_KV_I8 && cache_type != FT_KV_E4M3)
         return fail(FT_HIP_E_INVALID, "%s: cache_type=%d is no FT_KV", what, cache_type);
     const int64_t width = n_heads * head_dim, most = (int64_t)1 << 36;
     if (k_stride < width || k_stride > most || v_stride < width || v_stride > most)
         return fail(FT_HIP_E_SHAPE, "%s: k_stride or v_stride out of range", what);
-    const int64_t size = type == FT_TYPE_F32 ? 4 : 2;
+    const int64_t size = row_type == FT_TYPE_F32 ? 4 : 2;
     if (!aligned(k, size) || !aligned(v, size) || !aligned(slots, 4) || !aligned(cache, 16))
         return fail(FT_HIP_E_SHAPE, "%s: a pointer is not aligned to its type (cache: 16 bytes)", what);
     if (!ctx) return fail(FT_HIP_E_INVALID, "%s: null argument", what);
@@ -432,7 +432,7 @@ int kv_call(const char* what, ft_hip_ctx* ctx, void* stream, const void* k, int6
     const bool vec = aligned(k, 16) && aligned(v, 16) && k_stride * size % 16 == 0 && v_stride * size % 16 == 0;
     DeviceGuard on(ctx->device);
     if (!on.ok) return fail(FT_HIP_E_DEVICE, "%s: device %d cannot be made current", what, ctx->device);
-    launch_kv<WRITE>(a, cache_type, type, (int)head_dim / 64, vec, static_cast<hipStream_t>(stream));
+    launch_kv<WRITE>(a, cache_type, row_type, (int)head_dim / 64, vec, static_cast<hipStream_t>(stream));
     return launch_status(what);
 }
 
@@ -443,15 +443,15 @@ extern "C" int64_t ft_hip_kv_page_bytes(int64_t page_tokens, int64_t n_heads, in
 }
 
 extern "C" int ft_hip_kv_write(ft_hip_ctx* ctx, void* stream, const void* k, int64_t k_stride, const void* v,
-                               int64_t v_stride, int type, const int32_t* slots, void* cache, int cache_type,
+                               int64_t v_stride, int row_type, const int32_t* slots, void* cache, int cache_type,
                                int64_t n_pages, int64_t page_tokens, int64_t n_heads, int64_t head_dim, int64_t n) {
-    return kv_call<true>("kv_write", ctx, stream, k, k_stride, v, v_stride, type, slots, cache, cache_type, n_pages,
+    return kv_call<true>("kv_write", ctx, stream, k, k_stride, v, v_stride, row_type, slots, cache, cache_type, n_pages,
                          page_tokens, n_heads, head_dim, n);
 }
 
 extern "C" int ft_hip_kv_read(ft_hip_ctx* ctx, void* stream, const void* cache, int cache_type, int64_t n_pages,
                               int64_t page_tokens, int64_t n_heads, int64_t head_dim, const int32_t* slots, void* k,
-                              int64_t k_stride, void* v, int64_t v_stride, int type, int64_t n) {
-    return kv_call<false>("kv_read", ctx, stream, k, k_stride, v, v_stride, type, slots, cache, cache_type, n_pages,
+                              int64_t k_stride, void* v, int64_t v_stride, int row_type, int64_t n) {
+    return kv_call<false>("kv_read", ctx, stream, k, k_stride, v, v_stride, row_type, slots, cache, cache_type, n_pages,
                           page_tokens, n_heads, head_dim, n);
 }

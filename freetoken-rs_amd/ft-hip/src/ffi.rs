@@ -70,10 +70,10 @@ extern "C" {
     pub fn ft_hip_sample_tokens_workspace_bytes(vocab: i64, n: i64) -> usize;
     pub fn ft_hip_sample_tokens(ctx: *mut FtHipCtx, stream: *mut c_void, logits: *const c_void, logits_type: c_int, logits_stride: i64, vocab: i64, n: i64, temperature: *const f32, top_k: *const i32, top_p: *const f32, min_p: *const f32, u: *const f32, tokens: *mut i32, logprobs: *mut f32, workspace: *mut c_void, workspace_bytes: usize) -> c_int;
     pub fn ft_hip_kv_page_bytes(page_tokens: i64, n_heads: i64, head_dim: i64) -> i64;
-    pub fn ft_hip_kv_write(ctx: *mut FtHipCtx, stream: *mut c_void, k: *const c_void, k_stride: i64, v: *const c_void, v_stride: i64, type: c_int, slots: *const i32, cache: *mut c_void, cache_type: c_int, n_pages: i64, page_tokens: i64, n_heads: i64, head_dim: i64, n: i64) -> c_int;
-    pub fn ft_hip_kv_read(ctx: *mut FtHipCtx, stream: *mut c_void, cache: *const c_void, cache_type: c_int, n_pages: i64, page_tokens: i64, n_heads: i64, head_dim: i64, slots: *const i32, k: *mut c_void, k_stride: i64, v: *mut c_void, v_stride: i64, type: c_int, n: i64) -> c_int;
+    pub fn ft_hip_kv_write(ctx: *mut FtHipCtx, stream: *mut c_void, k: *const c_void, k_stride: i64, v: *const c_void, v_stride: i64, row_type: c_int, slots: *const i32, cache: *mut c_void, cache_type: c_int, n_pages: i64, page_tokens: i64, n_heads: i64, head_dim: i64, n: i64) -> c_int;
+    pub fn ft_hip_kv_read(ctx: *mut FtHipCtx, stream: *mut c_void, cache: *const c_void, cache_type: c_int, n_pages: i64, page_tokens: i64, n_heads: i64, head_dim: i64, slots: *const i32, k: *mut c_void, k_stride: i64, v: *mut c_void, v_stride: i64, row_type: c_int, n: i64) -> c_int;
     pub fn ft_hip_attention_workspace_bytes(n_seqs: i64, n_q: i64, n_heads: i64, n_kv_heads: i64, head_dim: i64) -> usize;
-    pub fn ft_hip_attention(ctx: *mut FtHipCtx, stream: *mut c_void, q: *const c_void, q_stride: i64, type: c_int, cache: *const c_void, cache_type: c_int, n_pages: i64, page_tokens: i64, n_kv_heads: i64, head_dim: i64, tables: *const i32, table_stride: i64, table_pages: i64, lens: *const i32, prefix: *const i32, prefix_pages: i64, prefix_len: *const i32, n_seqs: i64, n_q: i64, n_heads: i64, scale: f32, window: i64, out: *mut c_void, out_stride: i64, lse: *mut f32, workspace: *mut c_void, workspace_bytes: usize) -> c_int;
+    pub fn ft_hip_attention(ctx: *mut FtHipCtx, stream: *mut c_void, q: *const c_void, q_stride: i64, q_type: c_int, cache: *const c_void, cache_type: c_int, n_pages: i64, page_tokens: i64, n_kv_heads: i64, head_dim: i64, tables: *const i32, table_stride: i64, table_pages: i64, lens: *const i32, prefix: *const i32, prefix_pages: i64, prefix_len: *const i32, n_seqs: i64, n_q: i64, n_heads: i64, scale: f32, window: i64, out: *mut c_void, out_stride: i64, lse: *mut f32, workspace: *mut c_void, workspace_bytes: usize) -> c_int;
     pub fn ft_hip_adjust_logits(ctx: *mut FtHipCtx, stream: *mut c_void, logits: *const c_void, logits_type: c_int, logits_stride: i64, vocab: i64, n: i64, history: *const i32, history_stride: i64, history_max: i64, history_len: *const i32, repetition: *const f32, presence: *const f32, frequency: *const f32, bias_ids: *const i32, bias: *const f32, n_bias: i64, mask: *const u32, mask_stride: i64, out: *mut f32, out_stride: i64) -> c_int;
     pub fn ft_hip_repack_rows(ctx: *mut FtHipCtx, stream: *mut c_void, src: *const c_void, src_layout: c_int, dst: *mut c_void, dst_layout: c_int, n_rows: i64, k: i64) -> c_int;
     pub fn ft_hip_gen_values(ctx: *mut FtHipCtx, stream: *mut c_void, key: u64, start: i64, n: i64, scale: f32, out: *mut f32) -> c_int;

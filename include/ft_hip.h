@@ -141,10 +141,10 @@ int ft_hip_add_rmsnorm(ft_hip_ctx* ctx, void* stream, const void* x, int x_type,
  * A row of zeros has d = 0; one with a NaN or an infinity d = NaN, all q 0.
  *
  * ft_hip_kv_write: k and v are n rows (k_stride, v_stride values apart, heads
- * side by side: columns of a row of projections will do) of `type`; row i goes to
+ * side by side: columns of a row of projections will do) of row_type; row i goes to
  * slots[i]. A slot that is negative or behind the last is passed over, what no
  * slot names stays as it was; equal slots leave one of their rows or a mixture.
- * ft_hip_kv_read: the reverse; f32(q * d) rounded to `type`; the rows of slots
+ * ft_hip_kv_read: the reverse; f32(q * d) rounded to row_type; the rows of slots
  * that are passed over stay as they were.
  * cache is 16-byte aligned, slots 4-byte, rows to their type; rows that start on
  * 16 bytes are read and written 16 at a time. The cache, and read's rows, may not
@@ -152,11 +152,11 @@ int ft_hip_add_rmsnorm(ft_hip_ctx* ctx, void* stream, const void* x, int x_type,
  * NULL. n <= 2^20; n_heads <= 256; n_pages * page_tokens < 2^31. */
 int64_t ft_hip_kv_page_bytes(int64_t page_tokens, int64_t n_heads, int64_t head_dim);
 int ft_hip_kv_write(ft_hip_ctx* ctx, void* stream, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
-                    int type, const int32_t* slots, void* cache, int cache_type, int64_t n_pages, int64_t page_tokens,
+                    int row_type, const int32_t* slots, void* cache, int cache_type, int64_t n_pages, int64_t page_tokens,
                     int64_t n_heads, int64_t head_dim, int64_t n);
 int ft_hip_kv_read(ft_hip_ctx* ctx, void* stream, const void* cache, int cache_type, int64_t n_pages,
                    int64_t page_tokens, int64_t n_heads, int64_t head_dim, const int32_t* slots, void* k,
-                   int64_t k_stride, void* v, int64_t v_stride, int type, int64_t n);
+                   int64_t k_stride, void* v, int64_t v_stride, int row_type, int64_t n);
 
 /* Attention of a batch's newest tokens over a quantised cache, with a prefix
  * that all sequences share computed once for all (the reference's attn_decode
@@ -172,9 +172,9 @@ int ft_hip_kv_read(ft_hip_ctx* ctx, void* stream, const void* cache, int cache_t
  * lens and prefix_len are read on the device and taken as at least 0 and at most
  * what their pages hold; tokens in a page that is not in the cache (negative
  * or >= n_pages) count as not seen. A row that sees nothing has out 0 and lse
- * -inf. q, out: n_seqs * n_q rows of `type`, heads side by side; lse:
+ * -inf. q, out: n_seqs * n_q rows of q_type, heads side by side; lse:
  * [n_seqs * n_q][n_heads] or NULL. Products are exact in their 8 bits and, for
- * q and the weights, 11 bits where `type` is f16 or bf16 (q itself exact) and 22
+ * q and the weights, 11 bits where q_type is f16 or bf16 (q itself exact) and 22
  * where it is f32, but not below 2^-32 of the largest weight times the largest
  * scale of the values that a row's piece has met; sums are f32. |scale| times a
  * row's largest |q| is to lie between 2^-100 and 2^100 (or be 0): beyond, its
@@ -187,7 +187,7 @@ int ft_hip_kv_read(ft_hip_ctx* ctx, void* stream, const void* cache, int cache_t
 #define FT_ATTN_MAX_SEQS 4096
 size_t ft_hip_attention_workspace_bytes(int64_t n_seqs, int64_t n_q, int64_t n_heads, int64_t n_kv_heads,
                                         int64_t head_dim);
-int ft_hip_attention(ft_hip_ctx* ctx, void* stream, const void* q, int64_t q_stride, int type, const void* cache,
+int ft_hip_attention(ft_hip_ctx* ctx, void* stream, const void* q, int64_t q_stride, int q_type, const void* cache,
                      int cache_type, int64_t n_pages, int64_t page_tokens, int64_t n_kv_heads, int64_t head_dim,
                      const int32_t* tables, int64_t table_stride, int64_t table_pages, const int32_t* lens,
                      const int32_t* prefix, int64_t prefix_pages, const int32_t* prefix_len, int64_t n_seqs,

@@ -92,3 +92,25 @@ def test_build_script_builds_and_links_the_library():
     assert "build.py" in b and "rustc-link-lib=dylib=fthip" in b
     toml = open(os.path.join(CRATE, "Cargo.toml")).read()
     assert 'name = "ft-hip"' in toml
+
+
+# strict and reserved words of every edition; a raw identifier (r#type) would be another name than the header's
+KEYWORDS = set("""as break const continue crate else enum extern false fn for if impl in let loop match mod move mut pub
+    ref return self Self static struct super trait true type unsafe use where while async await dyn abstract become box
+    do final macro override priv try typeof unsized virtual yield gen""".split())
+
+
+def test_no_parameter_is_a_rust_keyword():
+    """Neither of the header, whose names the crate takes, nor of the crate's items and wrappers."""
+    for name, (params, _) in list(header_protos().items()) + list(rust_decls().items()):
+        assert not KEYWORDS & {p for p, _ in params}, (name, params)
+    lib = re.sub(r"//[^\n]*", "", open(os.path.join(CRATE, "src", "lib.rs")).read())
+    wrappers = 0
+    for m in re.finditer(r"\bfn (\w+)[^(]*\(", lib):
+        at = end = m.end()
+        while lib[at:end].count(")") <= lib[at:end].count("("):
+            end += 1
+        names = re.findall(r"(?:^|[,(])\s*(?:mut\s+)?(\w+)\s*:(?!:)", lib[at:end])
+        assert not KEYWORDS & {m.group(1), *names}, (m.group(1), names)
+        wrappers += 1
+    assert wrappers >= 40
