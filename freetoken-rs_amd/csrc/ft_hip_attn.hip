@@ -94,7 +94,7 @@ struct AttnArgs {
     int rows;        // of an own piece
 };
 
-// Floats of a piece of `rows` rows: the rows' values, then their maxima and sums.
+// Floats of a piece of `rows` rows: the rows' averages, then their maxima and sums.
 __host__ __device__ __forceinline__ int64_t piece_floats(int rows, int D) { return (int64_t)rows * (D + 2); }
 
 // At the head of a branch that few waves take: keeps the compiler from doing its work always and choosing afterwards.
@@ -558,13 +558,15 @@ struct Attend {
     __device__ __forceinline__ f32x4 values(int n, int c, int i, float f) const {
         return f32x4{acc[n][4 * c][i], acc[n][4 * c + 1][i], acc[n][4 * c + 2][i], acc[n][4 * c + 3][i]} * f;
     }
+    // A piece is an average, which is no larger than the values: their sum may leave f32's range.
     __device__ __forceinline__ void to_piece(int n, float* piece, int rows, int col) const {
         const int g = (threadIdx.x & 63) >> 4;
+        const float f = l[n] == 0.0f ? 0.0f : unit * __builtin_amdgcn_rcpf(l[n]);  // within 2^-23
 #pragma unroll
         for (int c = 0; c < ND; ++c)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<f32x4*>(piece + (int64_t)col * D + 64 * c + 16 * g + 4 * i) = values(n, c, i, unit);
+                *reinterpret_cast<f32x4*>(piece + (int64_t)col * D + 64 * c + 16 * g + 4 * i) = values(n, c, i, f);
         if (g == 0) {
             piece[(int64_t)rows * D + col] = top_of(n);
             piece[(int64_t)rows * D + rows + col] = l[n];
@@ -1047,9 +1049,9 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void k_attn_merge(AttnArgs
             const float* p = piece(i0 + i);
             const int rows = i0 + i < own ? a.rows : 16, row = i0 + i < own ? y : all & 15;
             const float l = p[(int64_t)rows * D + rows + row];
-            const float e = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(fs[i] - M);
+            const float e = l == 0.0f ? 0.0f : l * __builtin_amdgcn_exp2f(fs[i] - M);
             fs[i] = e;
-            sum += l * e;
+            sum += e;
         }
         sum = (float)wave_sum((double)sum);
         if (ALL) {
@@ -1059,15 +1061,18 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void k_attn_merge(AttnArgs
 #pragma unroll
             for (int w = 0; w < MERGE_WAVES; ++w) sum += red[1][w];
         }
-        L = L * f + sum;
-        x *= f;
+        // x is the average of what was joined so far
+        const float was = L * f;
+        L = was + sum;
+        const float part = L == 0.0f ? 0.0f : 1.0f / L;
+        x *= was * part;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the lanes read each other's factors
         for (int i = t / LANES; i < k; i += 8 * SLICES) {
             if (i >= 8 * SLICES) fetch(v, i);
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
                 const int j = i + u * SLICES;
-                const float e = j < k ? fs[j] : 0.0f;
+                const float e = j < k ? fs[j] * part : 0.0f;
                 if (e != 0.0f) x += v[u] * e;  // what was seen by nobody may be no number
             }
         }
@@ -1089,7 +1094,7 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void k_attn_merge(AttnArgs
     const bool some = L > 0.0f || L != L;
     const int64_t token = (int64_t)seq * a.n_q + r / a.group;
     const int qh = head * a.group + r % a.group;
-    const f32x4 v = some ? x * (1.0f / L) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const f32x4 v = some ? x : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     const int64_t to = token * a.out_stride + (int64_t)qh * D + 4 * (t % LANES);
     if (a.type == FT_TYPE_F32)
         store_out<true>(a.out, to, false, v);
