@@ -379,7 +379,7 @@ struct Attend {
             for (int i = 0; i < 4 * ND; ++i) acc[n][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             base[n] = 0.0f, l[n] = 0.0f, limit[n] = -FLT_MAX;
         }
-        unit = 0x1p-100f, inv_unit = 0x1p100f;
+        unit = 0x1p-126f, inv_unit = 0x1p126f;  // p dv is exact to 2^-151 at least: f32 itself has no finer steps than 2^-149
     }
 
     // The columns' scores of a step less their bases; the keys and their scales are free afterwards.
@@ -518,7 +518,7 @@ struct Attend {
         float g = 1.0f;
         const float most = wave_max(vt);
         if (most > unit * 256.0f) {
-            const int e = clampi((__float_as_int(most) >> 23) + 1, 30, 254);
+            const int e = min((__float_as_int(most) >> 23) + 1, 254);
             const float to = __int_as_float((e - 8) << 23);
             inv_unit = __int_as_float((254 - (e - 8)) << 23);
             g = unit * inv_unit;

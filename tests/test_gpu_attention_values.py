@@ -1,4 +1,9 @@
 """ft_hip_attention on values of every size: the definition and tolerances are test_gpu_attention's.
+
+What those leave out: numbers below the smallest normal one. A piece of a row leaves its average and the pieces are
+joined in f32, each rounded to half of the type's smallest step at most: (pieces + 2) 2^-150 beside the rest, and a
+piece has at least one token. A weight times a scale is held to 2^-151 at least, which a value's 8 bits multiply:
+n 2^-151 max |q|.
 """
 import numpy as np
 import pytest
@@ -31,6 +36,24 @@ def close(b, out, want, subnormal=0.0):
     got = host(out.float()).astype(np.float64)
     off = np.abs(got - o)
     assert np.all(off <= tol + subnormal), (float(np.nanmax(off / (tol + subnormal))), np.argwhere(~(off <= tol + subnormal))[:4].tolist())
+
+
+@pytest.mark.parametrize("kind", [I8, E4M3])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("prefix", [0, 100])
+@pytest.mark.parametrize("size", [1e-24, 1e-27, 1e-30, 1e-33, 1e-36, 1e-38, 1e-41])
+def test_small_values(gemv, kind, dtype, prefix, size):
+    """Down to scales that are no normal numbers: no less exact than others, as far as outputs have the bits."""
+    b = Batch(gemv, [100, 40, 700, 1], 16, 1, 4, 64, kind, dtype, prefix=prefix, seed=70)
+    slots = all_slots(b)
+    rng = np.random.default_rng(71)
+    put(b, slots, v=size * (rng.uniform(0.5, 1.5, (len(slots), 64)) * rng.choice([-1.0, 1.0, 1.0], (len(slots), 64))))
+    out, _ = b.run()
+    torch.cuda.synchronize()
+    want = b.want()
+    assert np.abs(want[0]).max() > size / 8
+    codes = 127.0 if kind == I8 else min(448.0, 1.1 * (1.5 * size * 2.0 ** 126 + 2.0 ** -9))  # |v| / d, d at least 2^-126
+    close(b, out, want, (700 + prefix + 2) * 2.0 ** -150 + (700 + prefix) * 2.0 ** -151 * codes)
 
 
 @pytest.mark.parametrize("kind", [I8, E4M3])
