@@ -316,19 +316,22 @@ struct Step {
     }
 };
 
-// A wavefront's NT times 16 columns (PACK: 8 rows).
-template <int CT, int ND, int MODE, int NT>
+// A wavefront's NT times 16 columns (PACK: 8 rows). EACH: a lane's columns may see different tokens, and each has a unit of
+// its own, so that values that one does not see cost it no bits. With one for all, which the prefix takes where there is no
+// window, 256 queries behind 16390 tokens are 253 us, with one each 262.
+template <int CT, int ND, int MODE, int NT, bool EACH>
 struct Attend {
     static constexpr int D = 64 * ND;
     static constexpr int PARTS = MODE == SPLIT ? 2 : 1;
     static constexpr bool F32 = MODE != HALF;
+    static constexpr int UNITS = EACH ? NT : 1;
     half8 q[NT][PARTS][2 * ND];
     f32x4 acc[NT][4 * ND];
     float base[NT], l[NT];  // the maximum that weights are taken against, and their sum
     float limit[NT];        // over the base: scores above it raise the base; -FLT_MAX while there is none
     float from[NT];         // what a column's sums of products start from
     float fac[NT];          // of a column's products
-    float unit, inv_unit;   // the weights' unit: the values' largest scale so far as a power of two, over 2^8
+    float unit[UNITS];      // the weights' unit: the values' largest scale so far as a power of two, over 2^8
     int lo[NT], hi[NT];     // tokens that the column sees
     int all_lo, all_hi;     // that every column sees
     int tokens;             // that the list of pages holds
@@ -379,7 +382,8 @@ struct Attend {
             for (int i = 0; i < 4 * ND; ++i) acc[n][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             base[n] = 0.0f, l[n] = 0.0f, limit[n] = -FLT_MAX;
         }
-        unit = 0x1p-126f, inv_unit = 0x1p126f;  // p dv is exact to 2^-151 at least: f32 itself has no finer steps than 2^-149
+#pragma unroll
+        for (int n = 0; n < UNITS; ++n) unit[n] = 0x1p-126f;  // p dv is exact to 2^-151 at least: f32 itself has no finer steps than 2^-149
     }
 
     // The columns' scores of a step less their bases; the keys and their scales are free afterwards.
@@ -423,6 +427,7 @@ struct Attend {
         const bool whole = has[0] && has[1] && at >= all_lo && at + STEP <= all_hi;
         constexpr int BATCH = Tiles::BATCH;
         half8 w[NT][PARTS], v[BATCH];
+        float vt[UNITS];  // the largest scale of values that a lane's columns see of its tokens
         if constexpr (Tiles::FAR) {  // the first values are on their way while the weights are made
 #pragma unroll
             for (int u = 0; u < BATCH; ++u) v[u] = t.template value<CT>(u >> 2, u & 3);
@@ -444,25 +449,41 @@ struct Attend {
                 }
                 t.clear(x, keep);
             }
+#pragma unroll
+            for (int n = 0; n < (EACH ? NT : 0); ++n) {
+                vt[n] = 0.0f;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const f32x4 d = t.value_scale(x);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (s[n][x][i] != -INFINITY) vt[n] = fmaxf(vt[n], d[i]);
+                }
+            }
         }
-        f32x4 dv[2] = {t.value_scale(0), t.value_scale(1)};
+        const f32x4 dv[2] = {t.value_scale(0), t.value_scale(1)};
         // a lane's own scores say enough: the base is raised where any of them is far above it
         float top[NT];
         bool grows = false;
+        const float largest = fmaxf(fmaxf(fmaxf(dv[0][0], dv[0][1]), fmaxf(dv[0][2], dv[0][3])),
+                                    fmaxf(fmaxf(dv[1][0], dv[1][1]), fmaxf(dv[1][2], dv[1][3])));
+        if (whole || !EACH) {
+#pragma unroll
+            for (int n = 0; n < UNITS; ++n) vt[n] = largest;
+        }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             top[n] = fmaxf(fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][0][2], s[n][0][3])),
                            fmaxf(fmaxf(s[n][1][0], s[n][1][1]), fmaxf(s[n][1][2], s[n][1][3])));
             grows |= top[n] > limit[n];
+            if (n < UNITS) grows |= vt[n] > unit[n] * 256.0f;
         }
-        const float vt = fmaxf(fmaxf(fmaxf(dv[0][0], dv[0][1]), fmaxf(dv[0][2], dv[0][3])),
-                               fmaxf(fmaxf(dv[1][0], dv[1][1]), fmaxf(dv[1][2], dv[1][3])));
-        if (__any(grows || vt > unit * 256.0f)) rescale(s, top, vt);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) dv[x] *= inv_unit;
+        if (__any(grows)) rescale(s, top, vt);
+        f32x4 in_units[2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const float second = MODE == PACK && (lane & 8) ? 1.0f : 0.0f;
+            if (n < UNITS) in_units[0] = dv[0] * inverse(unit[n]), in_units[1] = dv[1] * inverse(unit[n]);
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -472,7 +493,7 @@ struct Attend {
                     for (int e = 0; e < 2; ++e) {
                         const float p = __builtin_amdgcn_exp2f(s[n][x][i + e]);
                         l[n] += p;
-                        v[e] = p * dv[x][i + e];
+                        v[e] = p * in_units[x][i + e];
                         // the product as rounded, or hi would round it once and lo be the rest of another hi
                         if constexpr (F32) asm("" : "+v"(v[e]));
                     }
@@ -514,18 +535,19 @@ struct Attend {
     }
 
     // A larger maximum, or a larger scale of values.
-    __device__ __forceinline__ void rescale(f32x4 (&s)[NT][2], float (&top)[NT], float vt) {
+    __device__ __forceinline__ void rescale(f32x4 (&s)[NT][2], const float (&top)[NT], const float (&vt)[UNITS]) {
         float g = 1.0f;
-        const float most = wave_max(vt);
-        if (most > unit * 256.0f) {
-            const int e = min((__float_as_int(most) >> 23) + 1, 254);
-            const float to = __int_as_float((e - 8) << 23);
-            inv_unit = __int_as_float((254 - (e - 8)) << 23);
-            g = unit * inv_unit;
-            unit = to;
-        }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
+            if (n < UNITS) {
+                const float most = max_groups(vt[n]);
+                g = 1.0f;
+                if (most > unit[n] * 256.0f) {
+                    const float to = __int_as_float((min((__float_as_int(most) >> 23) + 1, 254) - 8) << 23);
+                    g = unit[n] * inverse(to);
+                    unit[n] = to;
+                }
+            }
             float f = g;
             const float up = max_groups(top[n]);
             if (up > limit[n]) {  // by its own scores alone: a row's bits are the same whatever its neighbours are
@@ -540,6 +562,9 @@ struct Attend {
             for (int i = 0; i < 4 * ND; ++i) acc[n][i] *= f;
         }
     }
+    __device__ __forceinline__ float unit_of(int n) const { return unit[n < UNITS ? n : 0]; }
+    // 1 / v of a power of two from 2^-126 to 2^126.
+    __device__ __forceinline__ static float inverse(float v) { return __int_as_float(0x7F000000 - __float_as_int(v)); }
     // The maximum that a column's sums are taken against.
     __device__ __forceinline__ float top_of(int n) const { return limit[n] > 0.0f ? base[n] : -INFINITY; }
 
@@ -561,7 +586,7 @@ struct Attend {
     // A piece is an average, which is no larger than the values: their sum may leave f32's range.
     __device__ __forceinline__ void to_piece(int n, float* piece, int rows, int col) const {
         const int g = (threadIdx.x & 63) >> 4;
-        const float f = l[n] == 0.0f ? 0.0f : unit * __builtin_amdgcn_rcpf(l[n]);  // within 2^-23
+        const float f = unit_of(n) * __builtin_amdgcn_rcpf(l[n]);  // within 2^-23; no number where nothing is seen, which is passed over
 #pragma unroll
         for (int c = 0; c < ND; ++c)
 #pragma unroll
@@ -576,7 +601,7 @@ struct Attend {
         const int g = (threadIdx.x & 63) >> 4;
         const int64_t row = (int64_t)c.seq * a.n_q + c.t;
         const bool some = l[n] > 0.0f || l[n] != l[n];
-        const float f = some ? unit / l[n] : 0.0f;
+        const float f = some ? unit_of(n) / l[n] : 0.0f;
 #pragma unroll
         for (int i = 0; i < ND; ++i)
 #pragma unroll
@@ -744,7 +769,7 @@ struct Share {
 
 // Prefix rows: the lines of WAVES NT tiles of 16 rows on a head, one after the other, are cut into a piece for each
 // workgroup. Its wavefronts share the widening: each step's tiles lie in LDS while the next one's are widened beside them.
-template <int CT, int ND, int MODE, int NT>
+template <int CT, int ND, int MODE, int NT, bool EACH>
 __device__ __forceinline__ void attend_prefix(const AttnArgs& a, const Prefix& pre, int b, int blocks, Wide<ND>* wide, int* part) {
     const int lane = threadIdx.x & 63, col = lane & 15, wave = uni(threadIdx.x >> 6);
     const int groups = (a.pre_tiles + NT * WAVES - 1) / (NT * WAVES);
@@ -757,7 +782,7 @@ __device__ __forceinline__ void attend_prefix(const AttnArgs& a, const Prefix& p
         pos += s1 - s0;
         Tiles64<64 * ND> tiles;
         tiles.open(a, a.prefix, a.prefix_pages, pre.tile0 + 2 * s0, (pre.len + 15) / 16);
-        Attend<CT, ND, MODE, NT> w;
+        Attend<CT, ND, MODE, NT, EACH> w;
         Column c[NT];
         int least = pre.len, most_lo = 0;
 #pragma unroll
@@ -768,12 +793,12 @@ __device__ __forceinline__ void attend_prefix(const AttnArgs& a, const Prefix& p
             c[n].seq = token / a.n_q, c[n].t = token % a.n_q, c[n].head = head * a.group + (row ? r % a.group : 0);
             const int at = own_of(a, a.lens[c[n].seq]).len - a.n_q + c[n].t;
             c[n].live = row && at >= 0;
-            const int lo = a.window ? max(0, pre.len + at - a.window + 1) : 0;
+            const int lo = EACH && a.window ? max(0, pre.len + at - a.window + 1) : 0;
             w.lo[n] = c[n].live ? lo : INT32_MIN, w.hi[n] = pre.len;  // one without a query sees all, to no effect
             if (c[n].live) least = min(least, lo), most_lo = max(most_lo, lo);
         }
-        w.tokens = w.all_hi = pre.len, w.all_lo = a.window ? -least_of_wave(-most_lo) : 0;
-        if (a.window) {  // the steps before the first column's first token are nobody's
+        w.tokens = w.all_hi = pre.len, w.all_lo = EACH && a.window ? -least_of_wave(-most_lo) : 0;
+        if (EACH && a.window) {  // the steps before the first column's first token are nobody's
             least = least_of_wave(least);
             __syncthreads();
             if (lane == 0) part[wave] = least;
@@ -852,8 +877,13 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn(AttnArgs a) {
                 const int b = near_block(blockIdx.x - n_own, blocks - n_own);
                 if (b == 0 && t == 0) a.head[0] = n_pre;
                 __syncthreads();
-                if (b < n_pre)
-                    attend_prefix<CT, ND, MODE == PACK ? SPLIT : MODE, NT>(a, pre, b, n_pre, reinterpret_cast<Wide<ND>*>(pool), part);
+                if (b >= n_pre) return;
+                constexpr int M = MODE == PACK ? SPLIT : MODE;
+                Wide<ND>* const wide = reinterpret_cast<Wide<ND>*>(pool);
+                if (NT > 1 && a.window)
+                    attend_prefix<CT, ND, M, NT, true>(a, pre, b, n_pre, wide, part);
+                else
+                    attend_prefix<CT, ND, M, NT, NT == 1>(a, pre, b, n_pre, wide, part);
                 return;
             }
         } else if (blockIdx.x == 0 && t == 0) {
@@ -918,7 +948,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn(AttnArgs a) {
         c.seq = seq, c.t = row ? r / a.group : 0, c.head = head * a.group + (row ? r % a.group : 0);
         const int place = o.len - a.n_q + c.t;
         c.live = row && place >= 0;
-        Attend<CT, ND, MODE, 1> w;
+        Attend<CT, ND, MODE, 1, true> w;
         w.load(a, cs);
         w.lo[0] = c.live && a.window ? max(0, place - a.window + 1) : 0;
         w.hi[0] = c.live ? place + 1 : o.len;  // one without a query sees all, to no effect

@@ -176,8 +176,8 @@ int ft_hip_kv_read(ft_hip_ctx* ctx, void* stream, const void* cache, int cache_t
  * [n_seqs * n_q][n_heads] or NULL. Products are exact in their 8 bits and, for
  * q and the weights, 11 bits where q_type is f16 or bf16 (q itself exact) and 22
  * where it is f32, but not below 2^-32 of the largest weight times the largest
- * scale of the values that a row's piece has met, nor below 2^-151 (f32 itself
- * has no steps finer than 2^-149); sums are f32. |scale| times a
+ * scale of the values that the row sees, nor below 2^-151 (f32 itself has no
+ * steps finer than 2^-149); sums are f32. |scale| times a
  * row's largest |q| is to lie between 2^-100 and 2^100 (or be 0): beyond, its
  * factors may leave f32's range before its scores do. The same call gives the
  * same bits.

@@ -68,3 +68,64 @@ def test_the_largest_values(gemv, kind, dtype, n, prefix):
     out, _ = b.run()
     torch.cuda.synchronize()
     close(b, out, b.want())
+
+
+@pytest.mark.parametrize("kind", [I8, E4M3])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n_q,window,prefix", [(4, 0, 0), (4, 50, 0), (1, 50, 0), (3, 0, 64), (2, 90, 64), (1, 90, 64)])
+def test_scales_of_tokens_that_a_query_does_not_see(gemv, kind, dtype, n_q, window, prefix):
+    """Values far larger than the rest, behind a query or before its window: nothing of them reaches it, not in its
+    last bit."""
+    lens = [100, 77, 60, 20]
+    b = Batch(gemv, lens, 16, 1, 2, 64, kind, dtype, prefix=prefix, n_q=n_q, seed=74)
+    put(b, all_slots(b))
+    plain, lse = b.check(window=window)
+    # of each sequence: its newest token, if several are new, and the last one that its last query's window leaves out
+    big, before = [], []
+    for i, x in enumerate(lens):
+        at = prefix + x - window - 1 if window else -1  # among prefix and own tokens
+        for place in ([x - 1] if n_q > 1 else []) + ([at - prefix] if at >= prefix else []):
+            big.append(b.places(b.tables[i], x)[place])
+        before.append(at if window else -1)
+    shared = [at for at in before if 0 <= at < prefix]
+    if shared:  # the prefix's token that the shortest window end leaves out, and others still see
+        big.append(b.places(b.prefix, prefix)[min(shared)])
+    put(b, big, v=np.full((len(big), b.kv * 64), 1e30))
+    out, got = b.run(window=window)
+    torch.cuda.synchronize()
+    out, plain = host(out.float()).reshape(4, n_q, -1), host(plain.float()).reshape(4, n_q, -1)
+    checked = 0
+    for i, x in enumerate(lens):
+        for t in range(n_q):
+            place = prefix + x - n_q + t
+            lo = max(0, place + 1 - window) if window else 0
+            sees = [prefix + x - 1] if n_q > 1 else []
+            if before[i] >= prefix:
+                sees.append(before[i])
+            if shared:
+                sees.append(min(shared))
+            if not any(lo <= s <= place for s in sees):
+                assert np.array_equal(out[i, t], plain[i, t]), (i, t)
+                checked += 1
+    assert checked
+    assert torch.equal(got, lse)  # what a query sees of keys is the same
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kind", [I8, E4M3])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf")])
+def test_a_query_of_infinities_beside_large_values(gemv, dtype, kind, bad):
+    """Its scores are no numbers or infinities; whichever values they fall on, the other rows' results are what they
+    were. Rows enough that a lane holds several, a prefix that ends inside a step."""
+    b = Batch(gemv, [5] * 40, 16, 1, 2, 64, kind, dtype, prefix=75, seed=76)
+    put(b, all_slots(b))
+    put(b, b.places(b.prefix, 75)[-1:], v=np.full((1, 64), 1e30))
+    want, lse = b.check()
+    for row in (0, 33):  # q k is minus or plus infinity by the key's sign
+        q = b.q.clone()
+        q[row] = 0.0
+        q[row, ::64] = bad
+        out, got = b.run(q=q)
+        torch.cuda.synchronize()
+        same = [i for i in range(40) if i != row]
+        assert torch.equal(out[same], want[same]) and torch.equal(got[same], lse[same])
