@@ -129,3 +129,17 @@ def test_a_query_of_infinities_beside_large_values(gemv, dtype, kind, bad):
         torch.cuda.synchronize()
         same = [i for i in range(40) if i != row]
         assert torch.equal(out[same], want[same]) and torch.equal(got[same], lse[same])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("lens", [[131071], [70001], [40000] + [20] * 300, [131071] + [9] * 19])
+def test_more_pieces_than_are_joined_at_once(gemv, dtype, lens):
+    """One key head, so that all wavefronts have a piece of the long row; its largest scores are first or late: what was
+    joined before is scaled, or what comes after."""
+    group = 16 if len(lens) == 20 else 2
+    b = Batch(gemv, lens, 64, 1, group, 64, I8, dtype, seed=75)
+    q = host(b.q.float())[0].reshape(group, 64)
+    places = b.places(b.tables[0], lens[0])
+    for at, score in ((7, 16.0), (lens[0] - 100, 24.0), (lens[0] // 2, 40.0)):
+        put(b, [places[at]], k=(8.0 * score / float(q[0] @ q[0]) * q[0])[None], v=np.full((1, 64), 3.0))
+        b.check()
