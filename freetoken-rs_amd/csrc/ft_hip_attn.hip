@@ -1079,9 +1079,9 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void k_attn_merge(AttnArgs
             const float* p = piece(i0 + i);
             const int rows = i0 + i < own ? a.rows : 16, row = i0 + i < own ? y : all & 15;
             const float l = p[(int64_t)rows * D + rows + row];
-            const float e = l == 0.0f ? 0.0f : l * __builtin_amdgcn_exp2f(fs[i] - M);
-            fs[i] = e;
-            sum += e;
+            const float e = l * __builtin_amdgcn_exp2f(fs[i] - M);
+            fs[i] = l == 0.0f ? -1.0f : e;  // nothing seen: its average may be no number, which is nobody's
+            if (l != 0.0f) sum += e;
         }
         sum = (float)wave_sum((double)sum);
         if (ALL) {
@@ -1102,8 +1102,8 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void k_attn_merge(AttnArgs
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
                 const int j = i + u * SLICES;
-                const float e = j < k ? fs[j] * part : 0.0f;
-                if (e != 0.0f) x += v[u] * e;  // what was seen by nobody may be no number
+                const float e = j < k ? fs[j] * part : -1.0f;
+                if (!(e < 0.0f)) x += v[u] * e;  // a weight of 0 too: no number among what is seen shows, whatever its weight
             }
         }
     }

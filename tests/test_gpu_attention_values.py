@@ -143,3 +143,19 @@ def test_more_pieces_than_are_joined_at_once(gemv, dtype, lens):
     for at, score in ((7, 16.0), (lens[0] - 100, 24.0), (lens[0] // 2, 40.0)):
         put(b, [places[at]], k=(8.0 * score / float(q[0] @ q[0]) * q[0])[None], v=np.full((1, 64), 3.0))
         b.check()
+
+
+@pytest.mark.parametrize("lens,prefix", [([40], 0), ([5000], 0), ([90], 700), ([40000] + [20] * 300, 0)])
+def test_no_number_shows_whatever_its_weight(gemv, lens, prefix):
+    """A value that is NaN, seen with a weight that is 0 in f32 as all weights of its piece are."""
+    b = Batch(gemv, lens, 16, 1, 2, 64, E4M3, torch.float32, prefix=prefix, seed=77)
+    top = b.places(b.tables[0], lens[0])[-1]
+    q = host(b.q)[0].reshape(2, 64)
+    put(b, [top], k=(1000.0 * q.sum(0) / float(q[0] @ q[0]))[None])  # first among its row's by far
+    out, lse = b.check(scale=50.0)
+    first = b.places(b.prefix, prefix) if prefix else b.places(b.tables[0], lens[0])
+    put(b, first[:1], v=np.full((1, 64), np.nan))
+    got, same = b.run(scale=50.0)
+    torch.cuda.synchronize()
+    assert torch.isnan(got[0]).all() and torch.equal(same, lse)
+    assert torch.equal(got[1:].isnan().all(1), torch.full((len(lens) - 1,), bool(prefix), device=DEV))
