@@ -188,3 +188,10 @@ def test_no_rows(gemv):
     none = torch.empty((0, 100), device=DEV)
     gemv.adjust_logits(none, none, 100, 0)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("n,vocab", [(8400, 1000), (65535, 129), (1025, 8192), (513, 16385)])
+def test_many_rows_of_a_small_vocabulary(gemv, n, vocab):
+    """Values enough for the longest chunks, rows that fill a part of one or a little more."""
+    x, s = inputs(np.random.default_rng(n), n, vocab, 30, 7, True)
+    check(gemv, x, s, vocab)
