@@ -159,3 +159,30 @@ def test_no_number_shows_whatever_its_weight(gemv, lens, prefix):
     torch.cuda.synchronize()
     assert torch.isnan(got[0]).all() and torch.equal(same, lse)
     assert torch.equal(got[1:].isnan().all(1), torch.full((len(lens) - 1,), bool(prefix), device=DEV))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kind", [I8, E4M3])
+@pytest.mark.parametrize("lens,prefix", [([50], 0), ([2000], 0), ([60, 3], 500)])
+def test_keys_as_large_as_scores_allow(gemv, dtype, kind, lens, prefix):
+    """The scale times the largest query and key just under 2^120: each row's largest score is alone, and its value the output."""
+    b = Batch(gemv, lens, 16, 1, 2, 64, kind, dtype, prefix=prefix, seed=78)
+    slots = all_slots(b)
+    rng = np.random.default_rng(79)
+    q = host(b.q.float()).astype(np.float64).reshape(len(lens), 2, 64)
+    size = 2.0 ** 119 / (np.abs(q).max() / 8.0)
+    put(b, slots, k=size * rng.uniform(-1, 1, (len(slots), 64)))
+    out, lse = b.run()
+    torch.cuda.synchronize()
+    shared, pv = b.layout.get(host(b.cache), b.places(b.prefix, prefix), kind) if prefix else (np.zeros((0, 1, 64)),) * 2
+    for i, n in enumerate(lens):
+        k, v = b.layout.get(host(b.cache), b.places(b.tables[i], n), kind)
+        k, v = np.concatenate([shared, k])[:, 0], np.concatenate([pv, v])[:, 0]
+        for h in range(2):
+            s = k @ q[i, h] / 8.0
+            first = np.argsort(s)[::-1][:2]
+            assert s[first[0]] - s[first[1]] > 1e-5 * s[first[0]]  # or its rounding might choose
+            want = torch.from_numpy(v[first[0]]).to(dtype).double().numpy()
+            got = host(out.double()).reshape(len(lens), 2, 64)[i, h]
+            assert np.all(np.abs(got - want) <= (2.0 ** -21 + torch.finfo(dtype).eps) * np.abs(want))
+            assert abs(host(lse)[i, h] / s[first[0]] - 1) < 1e-5
