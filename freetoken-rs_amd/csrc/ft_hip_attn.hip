@@ -28,15 +28,18 @@
 // widen once for all of them in LDS. By wavefronts alone, each widening for itself,
 // 64 queries behind 32768 tokens took 167 us for 118.
 //
-// What bounds it, own and joining kernels in turn (an MI355X that copies 5.1 TB/s
-// and multiplies 1110 TFLOP/s in f16): one sequence of 131071 tokens on 8 heads of
-// 128, 277 MB, 54 + 9 us, 5.2 TB/s in the first: the cache's bytes, then the
-// joining of 256 pieces a row. 64 sequences of up to 4096 on 8 heads of 256, f32:
-// 75 + 6 us, bytes and the widening beside them. One of 777: 9 + 4.5 us, the time
-// of two launches and of three dependent reads (length, page, tokens) in each.
-// 256 queries of 64 heads of 128 behind 16390: 247 + 18 us, where the products
-// alone are 125: the softmax's vector instructions, which a wavefront's products
-// do not hide, and rows of a few hundred own tokens.
+// What bounds it (an MI355X that copies 5.1 TB/s and multiplies 1110 TFLOP/s in
+// f16), in us a call, and of the own and joining kernels in a profiled run:
+// one sequence of 131071 tokens on 8 heads of 128, 277 MB, 62 (53 + 8.4): the
+// cache's bytes, 5.2 TB/s in the first, then the joining of 256 pieces a row.
+// 64 sequences of up to 4096 on 8 heads of 256, f32, 82 (75 + 6): bytes and the
+// widening beside them. One of 777, 12.6 (9.7 + 4.7): two launches, and in each
+// reads that wait for each other (lengths, pages, tokens, queries). 64 queries of
+// 16 heads of 256 behind 8192, f32, 54 (48 + 8.8): 34 of it do not grow with the
+// prefix (21 for each further 8192 tokens), starts, pieces and their joining.
+// 256 queries of 64 heads of 128 behind 16390, 252 (265 + 19 at a profiled run's
+// clock), where the products alone are 125: the softmax's vector instructions,
+// which a wavefront's products do not hide, and rows of a few hundred own tokens.
 
 #include "ft_device.hpp"
 #include "ft_kv.hpp"
@@ -64,7 +67,10 @@ constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.693147180559945309417f;
 
 enum { HALF, PACK, SPLIT };
 
-constexpr int BLOCKS = 512;  // workgroups at most, two on each CU; a third costs registers that do not fit (spills)
+// Workgroups at most, two on each CU: a third leaves 168 registers, and the prefix's loop spills (256 queries behind 16390 283
+// us for 261). With two, forms that are not among the timed ones spill as well: f32 heads of 256 with more than 8 rows (43 to
+// 53 registers), 16-bit heads of 64 behind a prefix (24, i8 60) and f32 heads of 128 behind one (22 to 28).
+constexpr int BLOCKS = 512;
 
 // Where the parts of a call lie, in the workspace and else.
 struct AttnArgs {

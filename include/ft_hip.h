@@ -158,9 +158,10 @@ int ft_hip_kv_read(ft_hip_ctx* ctx, void* stream, const void* cache, int cache_t
                    int64_t page_tokens, int64_t n_heads, int64_t head_dim, const int32_t* slots, void* k,
                    int64_t k_stride, void* v, int64_t v_stride, int row_type, int64_t n);
 
-/* Attention of a batch's newest tokens over a quantised cache, with a prefix
- * that all sequences share computed once for all (the reference's attn_decode
- * and attn_decode_batch, ft-cuda/src/q4.cu:732-896, without pages or a prefix).
+/* Attention of a batch's newest tokens over a quantised cache, behind a prefix
+ * that all sequences share, each of its tiles taken for many sequences' rows at
+ * once (the reference's attn_decode and attn_decode_batch,
+ * ft-cuda/src/q4.cu:732-896, without pages or a prefix).
  * Sequence i has lens[i] tokens of its own in the pages tables[i][0..table_pages)
  * (its newest n_q included: they are written first) behind prefix_len[0] tokens
  * in the pages prefix[0..prefix_pages) (prefix NULL: none). Its query t of n_q
@@ -174,13 +175,15 @@ int ft_hip_kv_read(ft_hip_ctx* ctx, void* stream, const void* cache, int cache_t
  * or >= n_pages) count as not seen. A row that sees nothing has out 0 and lse
  * -inf. q, out: n_seqs * n_q rows of q_type, heads side by side; lse:
  * [n_seqs * n_q][n_heads] or NULL. Products are exact in their 8 bits and, for
- * q and the weights, 11 bits where q_type is f16 or bf16 (q itself exact) and 22
- * where it is f32, but not below 2^-32 of the largest weight times the largest
- * scale of the values that the row sees, nor below 2^-151 (f32 itself has no
- * steps finer than 2^-149); sums are f32. |scale| times a
- * row's largest |q| is to lie between 2^-100 and 2^100 (or be 0): beyond, its
- * factors may leave f32's range before its scores do. The same call gives the
- * same bits.
+ * q and the weights, 11 bits where q_type is f16 or bf16 and 22 where it is f32.
+ * q has those bits down to 2^-38 of its row's largest, the weights times their
+ * values' scales down to 2^-32 of the largest weight times the largest scale of
+ * the values that the row sees, and to 2^-151 (f32 itself has no steps finer than
+ * 2^-149); sums are f32. |scale| times a row's largest |q| is to lie between
+ * 2^-100 and 2^100 (or be 0), and that times the largest |k| it sees below 2^120:
+ * beyond, factors may leave f32's range before the scores do. A NaN among the
+ * values that a row sees makes its output NaN, whatever its weight. The same call
+ * gives the same bits.
  * workspace: device scratch of ft_hip_attention_workspace_bytes() bytes (0 for a
  * bad shape), 16-byte aligned, any content, for one call at a time. out, lse and
  * the workspace may not overlap an input or each other. n_seqs 0: nothing is
@@ -401,8 +404,10 @@ int ft_hip_sample_tokens(ft_hip_ctx* ctx, void* stream, const void* logits, int 
  * in f32, one rounding an operation. logits: [n] rows of logits_type; out: [n]
  * f32 rows, or the logits themselves (f32, same stride). history: [n] rows of up
  * to history_max tokens or NULL, history_len: [n] how many of them count (NULL:
- * all); repetition, presence, frequency: [n] or NULL for 1, 0 and 0. bias_ids,
- * bias: [n][n_bias]. Tokens of history and bias_ids outside [0, vocab) count
+ * all); repetition, presence, frequency: [n] or NULL for 1, 0 and 0, of one and
+ * the same history: where repetition counts the prompt and the answer and the
+ * others the answer alone, call with the first, then with the others, in place.
+ * bias_ids, bias: [n][n_bias]. Tokens of history and bias_ids outside [0, vocab) count
  * nothing. mask: [n] rows of words, bit v % 32 of word v / 32 is 1 where v is
  * allowed, or NULL. NaN stays NaN unless it is masked. Any other overlap of out
  * with an input is refused. n 0: nothing is done, and the pointers may be NULL.
