@@ -100,7 +100,8 @@ struct AttnArgs {
     int rows;        // of an own piece
 };
 
-// Floats of a piece of `rows` rows: the rows' averages, then their maxima and sums.
+// Floats of a piece of `rows` rows: the rows' averages, then their maxima and sums. An odd number of rows leaves the next piece
+// between two vectors' places.
 __host__ __device__ __forceinline__ int64_t piece_floats(int rows, int D) { return (int64_t)rows * (D + 2); }
 
 // At the head of a branch that few waves take: keeps the compiler from doing its work always and choosing afterwards.
@@ -597,7 +598,7 @@ struct Attend {
         for (int c = 0; c < ND; ++c)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<f32x4*>(piece + (int64_t)col * D + 64 * c + 16 * g + 4 * i) = values(n, c, i, f);
+                *reinterpret_cast<f32x4_any*>(piece + (int64_t)col * D + 64 * c + 16 * g + 4 * i) = values(n, c, i, f);
         if (g == 0) {
             piece[(int64_t)rows * D + col] = top_of(n);
             piece[(int64_t)rows * D + rows + col] = l[n];
@@ -1057,7 +1058,7 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void k_attn_merge(AttnArgs
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
                 const int j = min(from + u * SLICES, k - 1);
-                v[u] = *reinterpret_cast<const f32x4*>(piece(i0 + j) + (int64_t)(i0 + j < own ? y : all & 15) * D + at);
+                v[u] = *reinterpret_cast<const f32x4_any*>(piece(i0 + j) + (int64_t)(i0 + j < own ? y : all & 15) * D + at);
             }
         };
         f32x4 v[8];
